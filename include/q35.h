@@ -426,6 +426,127 @@ typedef struct q35_attn_prefill_args {
 uint64_t q35_attn_prefill_workspace_bytes(const q35_attn_prefill_args *args);
 q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
 
+/* ------------------------------------------------------------------------------------ */
+/* a batch of continuations of one prompt                                                */
+/* ------------------------------------------------------------------------------------ */
+/* The mixers of one step for a batch of sequences that may share a prompt (the reference runs
+ * one sequence; these have no counterpart in it). Arrays marked "device" are int32 arrays in
+ * device memory, read by the kernels, so one captured graph serves every step. Calls that
+ * overlap in time need a workspace each. The stream belongs to the current device. */
+
+/* Gated GQA attention for one token per sequence: sequence b attends to the prefix_len rows
+ * of the shared prefix (a prompt's cache, read once for all sequences), to the rows of its
+ * own cache and to its new token, whose row is appended to the own cache. The arithmetic of
+ * q35_attn_decode otherwise (q_norm + RoPE on q, k_norm + RoPE on the new key, softmax,
+ * times sigmoid(gate)); the RoPE position is given apart from the cache's slot, so a cache
+ * from which rows were evicted stays usable.
+ *   qg [batch][NQ][2*HD] (per head: q then gate), k_new, v_new [batch][NKV][HD]
+ *   k_prefix, v_prefix [NKV][prefix_capacity][HD] (not read, may be NULL, with prefix_len 0)
+ *   k_own, v_own [batch][NKV][own_capacity][HD]; rows from own_len[b] on are not read
+ *   own_len (device) [batch]: rows in the own cache before this call; the new row goes to slot
+ *     own_len[b] (the array itself is left as it is: it serves every layer). A negative entry
+ *     marks an empty place: nothing of it is read or written. An entry at or above
+ *     own_capacity is a caller's mistake: nothing is appended and its out rows are NaN.
+ *   pos (device) [batch]: RoPE position of the new token
+ *   own_score [batch][NKV][own_capacity], may be NULL: the softmax weight that each own row
+ *     received, summed over the query heads of its kv head, is added to the row's entry; the
+ *     new row's entry is set to its weight (q35_kv_evict's order)
+ *   own_pos [batch][NKV][own_capacity], may be NULL: receives pos[b] at the new slot
+ *   out [batch][NQ][HD]
+ * workspace (16-byte aligned): q35_attn_batch_workspace_bytes() bytes; its size depends on
+ * sizes alone, never on the lengths. Requires HD == 256, NQ / NKV at most 16, an even
+ * rotary_dim, and 16-byte aligned fp32 rows and caches. */
+typedef struct q35_attn_batch_args {
+    int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;
+    int32_t kv_dtype;      /* elements of both caches: 0 = fp32, 1 = bf16 (appended rows rounded to nearest even) */
+    int64_t prefix_len, prefix_capacity, own_capacity;
+    double rope_theta;
+    float eps;
+    const int32_t *own_len, *pos;
+    const float *qg, *k_new, *v_new, *q_norm, *k_norm;
+    const void *k_prefix, *v_prefix;
+    void *k_own, *v_own;
+    float *own_score;
+    int32_t *own_pos;
+    float *out;
+    void *workspace;
+    uint64_t workspace_bytes;
+} q35_attn_batch_args;
+uint64_t q35_attn_batch_workspace_bytes(const q35_attn_batch_args *args);
+q35_status q35_attn_batch(const q35_attn_batch_args *args, q35_stream s);
+
+/* Eviction by accumulated attention weight: every own cache with more than `keep` rows is cut
+ * to `keep`, each kv head choosing for itself. Rows whose position is below n_sink or at
+ * least next_pos[b] - n_recent stay whatever their weight, then the rows of the largest
+ * scores; of equal ones the lower slot stays (and of protected rows, should positions occur
+ * twice and leave more than `keep`), and a NaN counts as below every number. Rows that
+ * stay in slots below `keep` do not move; the others move, in ascending order, into the slots
+ * below `keep` that evicted rows leave, in ascending order (attention does not depend on the
+ * order of the rows, and this moves the fewest).
+ *   len (device) [batch]: rows of each cache. A sequence with at most `keep` rows keeps its
+ *     rows where they are; a negative entry marks an empty place and is left alone, and so is
+ *     an entry above capacity (a caller's mistake): nothing of the caches is read or written.
+ *   next_pos (device) [batch]: the position of each sequence's next token
+ *   k, v [batch][NKV][capacity][HD], in place: only slots below `keep` change
+ *   score, pos [batch][NKV][capacity]; score_out, pos_out the same shape, each the same array
+ *     as its input or one that does not overlap it: entries [0, new length) receive the scores
+ *     and positions of the rows now there
+ *   new_len (device) [batch], may be the same array as len: min(len, keep) (len as it is for
+ *     entries that are left alone)
+ * keep is at least 1 and n_sink + n_recent at most keep. workspace (16-byte aligned):
+ * q35_kv_evict_workspace_bytes() bytes. Requires HD == 256 and 16-byte aligned caches. */
+typedef struct q35_kv_evict_args {
+    int32_t batch, kv_heads, head_dim;
+    int32_t kv_dtype;      /* cache elements: 0 = fp32, 1 = bf16 */
+    int32_t keep, n_sink, n_recent, reserved;
+    int64_t capacity;
+    const int32_t *len, *next_pos;
+    const float *score;
+    const int32_t *pos;
+    void *k, *v;
+    float *score_out;
+    int32_t *pos_out;
+    int32_t *new_len;
+    void *workspace;
+    uint64_t workspace_bytes;
+} q35_kv_evict_args;
+uint64_t q35_kv_evict_workspace_bytes(const q35_kv_evict_args *args);
+q35_status q35_kv_evict(const q35_kv_evict_args *args, q35_stream s);
+
+/* The gated delta rule, recurrent, for a batch: each sequence has its own state and conv ring
+ * and brings one token or a few (drafted tokens to verify); q35_gdn_prefill is the faster
+ * form for many. The arithmetic of q35_gdn_decode.
+ *   row0 (device) [batch + 1], may be NULL: sequence b's tokens are rows row0[b] ..
+ *     row0[b+1] - 1 of the token-major inputs; NULL: row b. Rows beyond `rows` are not read or
+ *     written, nor are rows of no sequence. A sequence may have no token.
+ *   pos (device) [batch]: position of each sequence's first token (selects the ring slots). A
+ *     negative entry marks an empty place: nothing of it is read or written.
+ *   qkv [rows][ld_qkv] (CONV pre-conv channels), z [rows][ld_z] (VD), b, a [rows][ld_ba] (VH each)
+ *   conv_w, A_log, dt_bias, norm_w as for q35_gdn_decode
+ *   conv_ring [KER][CONV] and state [VH][DK][DV] of sequence b at b * stride_ring, b *
+ *     stride_state (elements), written
+ *   conv_ring_in, state_in: where they are read. NULL: from the same place (in place). Else
+ *     sequence b reads at b * stride_ring_in, b * stride_state_in, and stride 0 reads one
+ *     prompt's for all: the batch is forked from it (a sequence without tokens gets a copy).
+ *     Both or neither are given, and what is read must not overlap what is written.
+ *   out [rows][VD]: with norm_w != NULL the gated-rmsnorm output, else the raw readout
+ * Requires DK == DV == 128, KER == 4, 16-byte aligned conv_w, rings, states and strides
+ * of the states that are multiples of 4. */
+typedef struct q35_gdn_batch_args {
+    int32_t batch, rows, k_heads, v_heads, head_dim_k, head_dim_v, conv_kernel;
+    float eps;
+    const int32_t *row0, *pos;
+    const float *qkv, *z, *b, *a;
+    int64_t ld_qkv, ld_z, ld_ba;
+    const float *conv_w, *A_log, *dt_bias, *norm_w;
+    const float *conv_ring_in, *state_in;
+    int64_t stride_ring_in, stride_state_in;
+    float *conv_ring, *state;
+    int64_t stride_ring, stride_state;
+    float *out;
+} q35_gdn_batch_args;
+q35_status q35_gdn_batch(const q35_gdn_batch_args *args, q35_stream s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -287,6 +287,70 @@ hipError_t launch_attn_prefill(const AttnPrefillArgs& a, hipStream_t s);
 // hidden[t][:] = bf16 embed[ids[t]][:]
 hipError_t launch_embed_rows(const uint16_t* embed, const int* ids, float* hidden, int T, int H, hipStream_t s);
 
+// ---------------------------------------------------------------- a batch of continuations
+// Attention of one token per sequence over a shared prefix and each sequence's own cache.
+struct AttnBatchArgs {
+    int B, NQ, NKV, GRP, ROT, kv_bf16;  // HD = 256
+    int64_t P, prefix_cap, cap;         // prefix rows, rows allocated per kv head of the prefix / of an own cache
+    double theta;
+    float eps;
+    const int *own_len, *pos;           // device [B]; own_len < 0: an empty place
+    const float *qg, *k_new, *v_new, *q_norm, *k_norm;
+    const void *k_prefix, *v_prefix;
+    void *k_own, *v_own;
+    float* own_score;                   // may be null
+    int* own_pos;                       // may be null
+    float* out;
+    // set by attn_batch_carve
+    AttnBatchPlan plan;
+    float* Qa;                          // [NKV][B GRP][HD] normed, rotated queries
+    float* part_p;                      // [NKV][prefix pieces][B GRP][HD]
+    float2* ml_p;                       // [NKV][prefix pieces][B GRP] (max, sum)
+    float* part_o;                      // [B][NKV][own pieces][GRP][HD]
+    float2* ml_o;                       // [B][NKV][own pieces][GRP]
+    float* raw;                         // [B][NKV][GRP][cap] scores of the own rows (own_score)
+};
+int64_t attn_batch_workspace_floats(const AttnBatchArgs& a);
+void attn_batch_carve(AttnBatchArgs& a, float* ws);
+hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s);
+
+// Eviction by score: the select kernel chooses, the move kernel copies.
+struct KvEvictArgs {
+    int B, NKV, kv_bf16, keep, n_sink, n_recent;
+    int64_t cap;
+    const int *len, *next_pos;
+    const float* score;
+    const int* pos;
+    void *k, *v;
+    float* score_out;
+    int* pos_out;
+    int* new_len;
+    // set by kv_evict_carve: per (b, kv head) the new length and the rows to move, then the
+    // slots they go to and come from
+    int2* head;
+    int *to, *from;
+    int most;                           // rows that may have to move
+};
+int64_t kv_evict_workspace_ints(int B, int NKV, int64_t cap, int keep);
+void kv_evict_carve(KvEvictArgs& a, int* ws);
+hipError_t launch_kv_evict(const KvEvictArgs& a, hipStream_t s);
+
+// The recurrent delta rule for a batch of sequences with a few tokens each.
+struct GdnBatchArgs {
+    int B, rows, KH, VH;
+    float eps;
+    const int *row0, *pos;              // device; row0 may be null (one token each)
+    const float *qkv, *z, *b, *a;
+    int64_t ld_qkv, ld_z, ld_ba;
+    const float *conv_w, *A_log, *dt_bias, *norm_w;  // norm_w null: raw readout
+    const float *ring_in, *state_in;    // where the rings and states are read (the outputs: in place)
+    int64_t s_ring_in, s_state_in;
+    float *ring, *state;
+    int64_t s_ring, s_state;
+    float* out;
+};
+hipError_t launch_gdn_batch(const GdnBatchArgs& a, hipStream_t s);
+
 // ---------------------------------------------------------------- small kernels
 // y = W x with fp32 weights [rows][n], any n
 hipError_t launch_matvec_f32(const float* W, const float* x, float* y, int rows, int n, hipStream_t s);

@@ -200,4 +200,26 @@ inline bool gemm_small_plan(int M, int N, int K, bool swiglu, int path, int n_cu
 // kSmallCus - 1 more) or, per XCD, to a share of its units over the row tiles.
 inline int gemm_small_max_parts(int N) { return N / 16 + kSmallCus + 16; }
 
+// ---------------------------------------------------------------- batched attention
+// How the attention of a batch over a shared prefix and own caches is cut: pieces of pkeys
+// prefix rows, and pieces of okeys rows of each own cache. Depends on sizes alone.
+struct AttnBatchPlan {
+    int pieces, pkeys;  // of the prefix (0 pieces: none)
+    int own, okeys;     // of an own cache
+};
+inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
+    const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
+    AttnBatchPlan p{0, 0, 1, 32};
+    const int64_t want = 2 * n_cu;
+    if (P > 0) {
+        const int64_t n = std::min<int64_t>(up(P, 64), std::max<int64_t>(1, want / NKV));
+        p.pkeys = static_cast<int>(up(up(P, n), 32) * 32);
+        p.pieces = static_cast<int>(up(P, p.pkeys));
+    }
+    const int64_t n = std::min<int64_t>(up(cap, 64), std::max<int64_t>(1, want / (static_cast<int64_t>(B) * NKV)));
+    p.okeys = static_cast<int>(up(up(cap, n), 32) * 32);
+    p.own = static_cast<int>(up(cap, p.okeys));
+    return p;
+}
+
 }  // namespace q35k

@@ -97,6 +97,33 @@ class AttnPrefillArgs(C.Structure):
         ("workspace_bytes", C.c_uint64)]
 
 
+class AttnBatchArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "q_heads", "kv_heads", "head_dim", "rotary_dim", "kv_dtype")] + [
+        (n, C.c_int64) for n in ("prefix_len", "prefix_capacity", "own_capacity")] + [
+        ("rope_theta", C.c_double), ("eps", C.c_float)] + [
+        (n, C.c_void_p) for n in ("own_len", "pos", "qg", "k_new", "v_new", "q_norm", "k_norm", "k_prefix", "v_prefix",
+                                  "k_own", "v_own", "own_score", "own_pos", "out", "workspace")] + [
+        ("workspace_bytes", C.c_uint64)]
+
+
+class KvEvictArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "kv_heads", "head_dim", "kv_dtype", "keep", "n_sink", "n_recent",
+                                         "reserved")] + [("capacity", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("len", "next_pos", "score", "pos", "k", "v", "score_out", "pos_out", "new_len",
+                                  "workspace")] + [("workspace_bytes", C.c_uint64)]
+
+
+class GdnBatchArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "rows", "k_heads", "v_heads", "head_dim_k", "head_dim_v",
+                                         "conv_kernel")] + [("eps", C.c_float)] + [
+        (n, C.c_void_p) for n in ("row0", "pos", "qkv", "z", "b", "a")] + [
+        (n, C.c_int64) for n in ("ld_qkv", "ld_z", "ld_ba")] + [
+        (n, C.c_void_p) for n in ("conv_w", "A_log", "dt_bias", "norm_w", "conv_ring_in", "state_in")] + [
+        (n, C.c_int64) for n in ("stride_ring_in", "stride_state_in")] + [
+        (n, C.c_void_p) for n in ("conv_ring", "state")] + [
+        (n, C.c_int64) for n in ("stride_ring", "stride_state")] + [("out", C.c_void_p)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built: run __graft_entry__.build() "
@@ -171,6 +198,11 @@ def _load():
         "q35_gdn_prefill": (S, [C.POINTER(GdnPrefillArgs), P]),
         "q35_attn_prefill_workspace_bytes": (U64, [C.POINTER(AttnPrefillArgs)]),
         "q35_attn_prefill": (S, [C.POINTER(AttnPrefillArgs), P]),
+        "q35_attn_batch_workspace_bytes": (U64, [C.POINTER(AttnBatchArgs)]),
+        "q35_attn_batch": (S, [C.POINTER(AttnBatchArgs), P]),
+        "q35_kv_evict_workspace_bytes": (U64, [C.POINTER(KvEvictArgs)]),
+        "q35_kv_evict": (S, [C.POINTER(KvEvictArgs), P]),
+        "q35_gdn_batch": (S, [C.POINTER(GdnBatchArgs), P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
