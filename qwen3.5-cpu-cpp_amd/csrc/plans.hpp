@@ -207,7 +207,7 @@ struct AttnBatchPlan {
     int pieces, pkeys;  // of the prefix (0 pieces: none)
     int own, okeys;     // of an own cache
 };
-inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
+inline AttnBatchPlan attn_batch_plan(int B, int, int NKV, int64_t P, int64_t cap, bool, int n_cu) {
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
     AttnBatchPlan p{0, 0, 1, 32};
     const int64_t want = 2 * n_cu;
