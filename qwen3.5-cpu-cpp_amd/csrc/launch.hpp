@@ -308,7 +308,7 @@ struct AttnBatchArgs {
     float2* ml_p;                       // [NKV][prefix pieces][B GRP] (max, sum)
     float* part_o;                      // [B][NKV][own pieces][GRP][HD]
     float2* ml_o;                       // [B][NKV][own pieces][GRP]
-    float* raw;                         // [B][NKV][GRP][cap] scores of the own rows (own_score)
+    float* raw;                         // [B][NKV][GRP][cap rounded up to 32] scores of the own rows (own_score)
 };
 int64_t attn_batch_workspace_floats(const AttnBatchArgs& a);
 void attn_batch_carve(AttnBatchArgs& a, float* ws);

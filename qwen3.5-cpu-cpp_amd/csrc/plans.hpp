@@ -201,23 +201,30 @@ inline bool gemm_small_plan(int M, int N, int K, bool swiglu, int path, int n_cu
 inline int gemm_small_max_parts(int N) { return N / 16 + kSmallCus + 16; }
 
 // ---------------------------------------------------------------- batched attention
-// How the attention of a batch over a shared prefix and own caches is cut: pieces of pkeys
-// prefix rows, and pieces of okeys rows of each own cache. Depends on sizes alone.
+// How the attention of a batch over a shared prefix and own caches is cut: the prefix's query
+// rows (batch x heads of the group) into blocks of `block` rows and its keys into pieces of pkeys,
+// every own cache into pieces of okeys keys. Depends on sizes alone, never on lengths.
 struct AttnBatchPlan {
-    int pieces, pkeys;  // of the prefix (0 pieces: none)
-    int own, okeys;     // of an own cache
+    int block, nblk, pieces, pkeys;  // of the prefix (0 pieces: none)
+    int own, okeys;                  // of an own cache
 };
-inline AttnBatchPlan attn_batch_plan(int B, int, int NKV, int64_t P, int64_t cap, bool, int n_cu) {
+constexpr int kBatchNarrow = 16;                                              // query rows of one wave
+constexpr int batch_wide(bool kv_bf16) { return kv_bf16 ? 64 : 128; }         // query rows of a wide workgroup
+constexpr int batch_unit(bool kv_bf16) { return kv_bf16 ? 32 : 128; }         // keys pieces are multiples of
+constexpr int batch_most_narrow(bool kv_bf16) { return kv_bf16 ? 16 : 32; }   // rows still taken in blocks of 16
+inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
-    AttnBatchPlan p{0, 0, 1, 32};
-    const int64_t want = 2 * n_cu;
+    const int64_t rows = static_cast<int64_t>(B) * GRP, unit = batch_unit(kv_bf16), slots = n_cu * (kv_bf16 ? 2 : 1);
+    AttnBatchPlan p{0, 0, 0, 0, 1, 0};
     if (P > 0) {
-        const int64_t n = std::min<int64_t>(up(P, 64), std::max<int64_t>(1, want / NKV));
-        p.pkeys = static_cast<int>(up(up(P, n), 32) * 32);
+        p.block = rows <= batch_most_narrow(kv_bf16) ? kBatchNarrow : batch_wide(kv_bf16);
+        p.nblk = static_cast<int>(up(rows, p.block));
+        const int64_t n = std::min<int64_t>(up(P, 2 * unit), std::max<int64_t>(1, slots / (static_cast<int64_t>(NKV) * p.nblk)));
+        p.pkeys = static_cast<int>(up(up(P, n), unit) * unit);
         p.pieces = static_cast<int>(up(P, p.pkeys));
     }
-    const int64_t n = std::min<int64_t>(up(cap, 64), std::max<int64_t>(1, want / (static_cast<int64_t>(B) * NKV)));
-    p.okeys = static_cast<int>(up(up(cap, n), 32) * 32);
+    const int64_t n = std::min<int64_t>(up(cap, 2 * unit), std::max<int64_t>(1, slots / (static_cast<int64_t>(B) * NKV)));
+    p.okeys = static_cast<int>(up(up(cap, n), unit) * unit);
     p.own = static_cast<int>(up(cap, p.okeys));
     return p;
 }
