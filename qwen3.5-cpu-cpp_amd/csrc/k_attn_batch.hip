@@ -22,48 +22,63 @@ __device__ __forceinline__ int new_slot(const AttnBatchArgs& a, int b) {
 // stride of the rows of raw scores: whole tiles
 __host__ __device__ inline int64_t raw_stride(int64_t cap) { return (cap + 31) / 32 * 32; }
 
-// grid (B, NQ + NKV), one thread per dim: rmsnorm (1 + w) + RoPE of a query row -> Qa, or of
-// the new key row -> own cache, with its value row.
+// grid ((NQ + NKV) / 4, B), a wave per row: rmsnorm (1 + w) + RoPE of a query row -> Qa, or of the
+// new key row -> own cache, with its value row. Angles in double, one lane each.
 __global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a) {
-    const int b = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
-    __shared__ float buf[kHD];
-    __shared__ double red[4];
+    const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 4 + wave;
+    __shared__ __align__(16) float buf[4][kHD];
+    __shared__ float cs[2][kHD / 2];
     const int slot = new_slot(a, b);
-    const bool is_q = r < a.NQ;
-    const int kh = is_q ? r / a.GRP : r - a.NQ;
-    float* q = a.Qa + ((static_cast<int64_t>(kh) * a.B + b) * a.GRP + (r - kh * a.GRP)) * kHD + d;
+    const bool is_q = r < a.NQ, there = r < a.NQ + a.NKV;
+    const int kh = is_q ? r / a.GRP : min(r - a.NQ, a.NKV - 1);
+    float* q = a.Qa + ((static_cast<int64_t>(kh) * a.B + b) * a.GRP + (r - kh * a.GRP)) * kHD + 4 * lane;
     if (slot < 0) {
-        if (is_q) *q = 0.0f;
+        if (is_q) *reinterpret_cast<float4*>(q) = make_float4(0.f, 0.f, 0.f, 0.f);
         return;
     }
-    const float* src = is_q ? a.qg + (static_cast<int64_t>(b) * a.NQ + r) * 2 * kHD
-                            : a.k_new + (static_cast<int64_t>(b) * a.NKV + kh) * kHD;
-    const float x = src[d];
-    const double ss = block_sum(static_cast<double>(x) * x, red);
+    const int64_t bk = static_cast<int64_t>(b) * a.NKV + kh;
+    const float* src = is_q ? a.qg + (static_cast<int64_t>(b) * a.NQ + r) * 2 * kHD : a.k_new + bk * kHD;
+    const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
+    const float4 w = *reinterpret_cast<const float4*>((is_q ? a.q_norm : a.k_norm) + 4 * lane);
+    const float4 v = *reinterpret_cast<const float4*>(a.v_new + bk * kHD + 4 * lane);
+    const int half = a.ROT / 2, pos = a.pos[b];
+    for (int i = threadIdx.x; i < half; i += 256) {
+        const double ang = static_cast<double>(pos) * pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
+        double sn, cn;
+        sincos(ang, &sn, &cn);
+        cs[0][i] = static_cast<float>(cn);
+        cs[1][i] = static_cast<float>(sn);
+    }
+    const double ss = wave_sum(static_cast<double>(x.x) * x.x + static_cast<double>(x.y) * x.y + static_cast<double>(x.z) * x.z +
+                               static_cast<double>(x.w) * x.w);
     const float inv = 1.0f / sqrtf(static_cast<float>(ss / kHD) + a.eps);
-    float y = x * inv * (1.0f + (is_q ? a.q_norm : a.k_norm)[d]);
-    buf[d] = y;
+    float y[4] = {x.x * inv * (1.0f + w.x), x.y * inv * (1.0f + w.y), x.z * inv * (1.0f + w.z), x.w * inv * (1.0f + w.w)};
+    *reinterpret_cast<float4*>(&buf[wave][4 * lane]) = make_float4(y[0], y[1], y[2], y[3]);
     __syncthreads();
-    if (d < a.ROT) {
-        const int half = a.ROT / 2, i = d < half ? d : d - half;
-        const double ang = static_cast<double>(a.pos[b]) * pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
-        const float c = static_cast<float>(cos(ang)), s = static_cast<float>(sin(ang));
-        y = d < half ? buf[i] * c - buf[i + half] * s : buf[i + half] * c + buf[i] * s;
+    if (!there) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int d = 4 * lane + e;
+        if (d < a.ROT) {
+            const int i = d < half ? d : d - half;
+            const float c = cs[0][i], s = cs[1][i];
+            y[e] = d < half ? y[e] * c - buf[wave][i + half] * s : y[e] * c + buf[wave][i] * s;
+        }
     }
-    if (is_q) {
-        *q = y * 0.0625f;  // 1 / sqrt(HD), exact
+    if (is_q) {  // scaled by 1 / sqrt(HD), exact
+        *reinterpret_cast<float4*>(q) = make_float4(y[0] * 0.0625f, y[1] * 0.0625f, y[2] * 0.0625f, y[3] * 0.0625f);
         return;
     }
-    const int64_t row = (static_cast<int64_t>(b) * a.NKV + kh) * a.cap + slot;
-    const float v = a.v_new[(static_cast<int64_t>(b) * a.NKV + kh) * kHD + d];
+    const int64_t row = bk * a.cap + slot;
     if (a.kv_bf16) {
-        static_cast<uint16_t*>(a.k_own)[row * kHD + d] = to_bf16(y);
-        static_cast<uint16_t*>(a.v_own)[row * kHD + d] = to_bf16(v);
+        const auto pair = [](float lo, float hi) { return to_bf16(lo) | static_cast<uint32_t>(to_bf16(hi)) << 16; };
+        static_cast<uint2*>(a.k_own)[row * (kHD / 4) + lane] = make_uint2(pair(y[0], y[1]), pair(y[2], y[3]));
+        static_cast<uint2*>(a.v_own)[row * (kHD / 4) + lane] = make_uint2(pair(v.x, v.y), pair(v.z, v.w));
     } else {
-        static_cast<float*>(a.k_own)[row * kHD + d] = y;
-        static_cast<float*>(a.v_own)[row * kHD + d] = v;
+        static_cast<float4*>(a.k_own)[row * (kHD / 4) + lane] = make_float4(y[0], y[1], y[2], y[3]);
+        static_cast<float4*>(a.v_own)[row * (kHD / 4) + lane] = v;
     }
-    if (a.own_pos && d == 0) a.own_pos[row] = a.pos[b];
+    if (a.own_pos && lane == 0) a.own_pos[row] = pos;
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -214,30 +229,36 @@ __device__ __forceinline__ int v_off(int r16, int g4) {                         
     return row * 512 + ((((2 * row) & 15) + ((r16 & 3) >> 1)) << 4) + (r16 & 1) * 8;
 }
 
+// scores of keys past the last
+__device__ __forceinline__ void mask_tail(float (&s)[8], int k0, int hi, int g4) {
+    if (k0 + kKT <= hi) return;  // uniform
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k0 + 16 * (i >> 2) + 4 * g4 + (i & 3) >= hi) s[i] = -INFINITY;
+}
+
 // dims 16 t + r16 of keys 4 g4 .. + 3 of the tile's first half, then of its second
-__device__ __forceinline__ bf16x8 v_operand(const uint4* V, int off) {
+template <class X8>
+__device__ __forceinline__ X8 v_operand(const uint4* V, int off) {
     typedef __attribute__((address_space(3))) i16x4 lds4;
     const char* p = reinterpret_cast<const char*>(V) + off;
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
     const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * 512));
     const i16x8 x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(bf16x8, x);
+    return __builtin_bit_cast(X8, x);
 }
 
-// One 32-key tile for the 16 query rows of a wave, on v_mfma_f32_16x16x32_bf16. Every fp32
-// operand is the exact sum of three bf16 parts; with a bf16 cache K and V are one part each and
-// every product is exact, else the six part products of lowest order are summed (the others
-// are below 2^-23 of the product).
+// One 32-key tile of a bf16 cache for the 16 query rows of a wave, on v_mfma_f32_16x16x32_bf16.
+// Queries and weights are the exact sums of three bf16 parts, K and V one part as they are, so every
+// product is exact in fp32.
 //   S^T = K Q^T by 16-key halves: lane (r16, g4) ends with keys 4 g4 + v of both for query r16
 //   O += P V: those eight weights are the A operand as they lie, its k slots 8 g4 .. + 7 being
 //         keys 4 g4 .. + 3 of the first half and of the second, which transposed LDS reads give V too;
 //         lane (r16, g4) ends with dims 16 t + r16 of queries 4 g4 + v
 // T tiles of 16 dims from t0 on (a narrow workgroup's waves share the dims and each form all scores).
-template <int NP, int T>
-__device__ __forceinline__ void tile_products(const uint4 (&Kc)[NP][1024], const uint4 (&Vc)[NP][1024], const bf16x8 (&qp)[3][8],
-                                              int k0, int hi, int r16, int g4, int t0, float* raw, float& m, float& l,
-                                              floatx4 (&o)[T]) {
-    constexpr int lo_part[6] = {2, 1, 0, 1, 0, 0}, hi_part[6] = {0, 1, 2, 0, 1, 0};  // smallest products first
+template <int T>
+__device__ __forceinline__ void bf16_tile(const uint4 (&Kc)[1024], const uint4 (&Vc)[1024], const bf16x8 (&qp)[3][8], int k0,
+                                          int hi, int r16, int g4, int t0, float* raw, float& m, float& l, floatx4 (&o)[T]) {
     floatx4 St[2];
     int ko = k_off(r16, g4), vo = v_off(r16, g4);
     asm volatile("" : "+v"(ko), "+v"(vo));  // formed per tile: kept, the 24 addresses would spill
@@ -248,22 +269,10 @@ __device__ __forceinline__ void tile_products(const uint4 (&Kc)[NP][1024], const
         for (int e = 0; e < 2; ++e) sa[e] = sb[e] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            bf16x8 kop[NP];
-#pragma unroll
-            for (int p = 0; p < NP; ++p)
-                kop[p] = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(&Kc[p][0]) + hf * 16 * 512 + (ko ^ (c << 6)));
-            floatx4& b = sb[c & 1];
-            if constexpr (NP == 1) {
-                b = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[0], qp[2][c], b, 0, 0, 0);
-                b = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[0], qp[1][c], b, 0, 0, 0);
-                sa[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[0], qp[0][c], sa[c & 1], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 6; ++i) {
-                    floatx4& s = i < 5 ? b : sa[c & 1];
-                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[lo_part[i] % NP], qp[hi_part[i]][c], s, 0, 0, 0);
-                }
-            }
+            const bf16x8 k = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(Kc) + hf * 16 * 512 + (ko ^ (c << 6)));
+            sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[2][c], sb[c & 1], 0, 0, 0);
+            sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[1][c], sb[c & 1], 0, 0, 0);
+            sa[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[0][c], sa[c & 1], 0, 0, 0);
         }
         St[hf] = (sb[0] + sb[1]) + (sa[0] + sa[1]);
     }
@@ -274,28 +283,16 @@ __device__ __forceinline__ void tile_products(const uint4 (&Kc)[NP][1024], const
         *reinterpret_cast<floatx4*>(raw + k0 + 4 * g4) = St[0];
         *reinterpret_cast<floatx4*>(raw + k0 + 16 + 4 * g4) = St[1];
     }
-    if (k0 + kKT > hi) {  // uniform
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (k0 + 16 * (i >> 2) + 4 * g4 + (i & 3) >= hi) p[i] = -INFINITY;
-    }
+    mask_tail(p, k0, hi, g4);
     const float f = softmax_step(p, m, l);
     rescale(f, g4, o);
     bf16x8 pa[3];
     split3_8(p, pa);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-        bf16x8 vb[NP];
+        const bf16x8 v = v_operand<bf16x8>(Vc, vo ^ ((t0 + t) << 5));
 #pragma unroll
-        for (int q = 0; q < NP; ++q) vb[q] = v_operand(&Vc[q][0], vo ^ ((t0 + t) << 5));
-        if constexpr (NP == 1) {
-#pragma unroll
-            for (int q = 2; q >= 0; --q) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[q], vb[0], o[t], 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 6; ++i)
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[lo_part[i]], vb[hi_part[i] % NP], o[t], 0, 0, 0);
-        }
+        for (int q = 2; q >= 0; --q) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[q], v, o[t], 0, 0, 0);
     }
 }
 
@@ -323,7 +320,7 @@ __device__ __forceinline__ void store_part(const Item& it, int first, int r16, i
 __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a) {
     // (separate arrays: the compiler then knows that a copy into one need not be waited for
     // before reads of another)
-    __shared__ __align__(16) uint4 K0[1][1024], V0[1][1024], K1[1][1024], V1[1][1024];
+    __shared__ __align__(16) uint4 K0[1024], V0[1024], K1[1024], V1[1024];
     Item it;
     if (!item_of(a, it)) return;
     const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
@@ -343,7 +340,7 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
                 (__attribute__((address_space(3))) void*)(V + c), 16, 0, 0);
         }
     };
-    copy(it.lo, &K0[0][0], &V0[0][0]);
+    copy(it.lo, K0, V0);
     const int first = it.narrow ? it.row0 : it.row0 + 16 * wave;
     bf16x8 qp[3][8];
     load_query(it, first, r16, g4, qp);
@@ -351,15 +348,15 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
     auto walk = [&](auto& o, int t0, float* raw, bool live) {
 #pragma unroll
         for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
-        auto tile = [&](int k0, const uint4 (&Kc)[1][1024], const uint4 (&Vc)[1][1024], uint4* Kn, uint4* Vn) {
+        auto tile = [&](int k0, const uint4 (&Kc)[1024], const uint4 (&Vc)[1024], uint4* Kn, uint4* Vn) {
             __builtin_amdgcn_s_waitcnt(kWaitVm);  // this wave's share of the tile
             lds_barrier();                        // every share; every wave is done with the other buffer
             if (k0 + kKT < it.hi) copy(k0 + kKT, Kn, Vn);  // uniform
-            if (live) tile_products<1>(Kc, Vc, qp, k0, it.hi, r16, g4, t0, raw, m, l, o);
+            if (live) bf16_tile(Kc, Vc, qp, k0, it.hi, r16, g4, t0, raw, m, l, o);
         };
         for (int k0 = it.lo; k0 < it.hi; k0 += 2 * kKT) {
-            tile(k0, K0, V0, &K1[0][0], &V1[0][0]);
-            if (k0 + kKT < it.hi) tile(k0 + kKT, K1, V1, &K0[0][0], &V0[0][0]);
+            tile(k0, K0, V0, K1, V1);
+            if (k0 + kKT < it.hi) tile(k0 + kKT, K1, V1, K0, V0);
         }
     };
     if (it.narrow) {
@@ -374,65 +371,181 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
     }
 }
 
-// fp32 caches, wide: 128 query rows, 16 a wave. A tile's rows are loaded into registers under
-// the products of the one before, split into three bf16 parts and stored to LDS once for all
-// eight waves.
-__device__ __forceinline__ void f32_wide(const Item& it, uint4 (&Kc)[3][1024], uint4 (&Vc)[3][1024]) {
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+// 2^e
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+// eight floats times s as two fp16 parts h = fp16(x), l = fp16(x - h): |x - h - l| <= 2^-23 |x|
+__device__ __forceinline__ void split2_8(const float (&x)[8], float s, halfx8 (&part)[2]) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2h_pair(x[2 * e] * s, x[2 * e + 1] * s, h[e], l[e]);
+    part[0] = __builtin_bit_cast(halfx8, make_uint4(h[0], h[1], h[2], h[3]));
+    part[1] = __builtin_bit_cast(halfx8, make_uint4(l[0], l[1], l[2], l[3]));
+}
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+    float m = fabsf(x[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+    return m;
+}
+
+// fp32 caches, wide: 64 query rows, 16 a wave, 32-key tiles, on v_mfma_f32_16x16x32_f16. Every
+// operand row (a query, a key, a value row, a query's weights over the tile) is scaled by a power
+// of two that brings its largest entry into [2^14, 2^15) and split into two fp16 parts; the three
+// part products of lowest order are summed (the fourth is below 2^-22 of the product) and the
+// scales undone exactly: a key's in the scores, a value row's in the weights before their own
+// scaling, and that one as the tile's products, summed from zero, are added to the output. So
+// nothing is lost relative to the largest weight times value row of the tile, whatever rows lie
+// beside it.
+// A tile's rows come through registers and are split once for the four waves: K of the next tile
+// while V is multiplied, V while K is.
+__device__ __forceinline__ void f32_wide(const Item& it, uint4 (*Kc)[1024], uint4 (*Vc)[1024], float* kscale, float* vscale) {
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = it.row0 + 16 * wave;
-    float4 kst[4], vst[4];
-    auto load = [&](int k0) {
+    const bool live = first < it.rows;  // uniform per wave
+    float4 st[8];
+    auto load = [&](const void* cache, int k0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = (tid >> 5) + 16 * i;
-            const int64_t at = static_cast<int64_t>(min(k0 + row, it.hi - 1)) * kHD + 8 * (tid & 31);
-            const float4 *ks = reinterpret_cast<const float4*>(static_cast<const float*>(it.K) + at),
-                         *vs = reinterpret_cast<const float4*>(static_cast<const float*>(it.V) + at);
-            kst[2 * i] = ks[0], kst[2 * i + 1] = ks[1];
-            vst[2 * i] = vs[0], vst[2 * i + 1] = vs[1];
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = static_cast<int64_t>(min(k0 + (tid >> 5) + 8 * i, it.hi - 1)) * kHD + 8 * (tid & 31);
+            const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(cache) + at);
+            st[2 * i] = s[0], st[2 * i + 1] = s[1];
         }
     };
-    auto store = [&]() {
+    auto store = [&](uint4 (*dst)[1024], float* scale, int mul) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = (tid >> 5) + 16 * i, c = tid & 31;
-            bf16x8 p[3];
-            const float k8[8] = {kst[2 * i].x, kst[2 * i].y, kst[2 * i].z, kst[2 * i].w,
-                                 kst[2 * i + 1].x, kst[2 * i + 1].y, kst[2 * i + 1].z, kst[2 * i + 1].w};
-            split3_8(k8, p);
+        for (int i = 0; i < 4; ++i) {
+            const int row = (tid >> 5) + 8 * i, c = tid & 31;
+            const float x[8] = {st[2 * i].x, st[2 * i].y, st[2 * i].z, st[2 * i].w,
+                                st[2 * i + 1].x, st[2 * i + 1].y, st[2 * i + 1].z, st[2 * i + 1].w};
+            float mx = max8(x);  // over the row: the 32 lanes of half a wave
+            mx = fmaxf(mx, dpp_f<0xB1>(mx));
+            mx = fmaxf(mx, dpp_f<0x4E>(mx));
+            mx = fmaxf(mx, dpp_f<0x141>(mx));
+            mx = fmaxf(mx, dpp_f<0x140>(mx));
+            mx = fmaxf(mx, swz16_f(mx));
+            const int e = split_row_exp(mx);
+            halfx8 p[2];
+            split2_8(x, pow2(e), p);
 #pragma unroll
-            for (int q = 0; q < 3; ++q) Kc[q][32 * row + (c ^ (row & 15))] = __builtin_bit_cast(uint4, p[q]);
-            const float v8[8] = {vst[2 * i].x, vst[2 * i].y, vst[2 * i].z, vst[2 * i].w,
-                                 vst[2 * i + 1].x, vst[2 * i + 1].y, vst[2 * i + 1].z, vst[2 * i + 1].w};
-            split3_8(v8, p);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) Vc[q][32 * row + (c ^ ((2 * row) & 15))] = __builtin_bit_cast(uint4, p[q]);
+            for (int q = 0; q < 2; ++q) dst[q][32 * row + (c ^ ((mul * row) & 15))] = __builtin_bit_cast(uint4, p[q]);
+            if (c == 0) scale[row] = pow2(-e);
         }
     };
-    load(it.lo);
-    bf16x8 qp[3][8];
-    load_query(it, first, r16, g4, qp);
+    load(it.K, it.lo);
+    halfx8 qp[2][8];
+    float qscale;
+    {
+        const float* src = it.Q + static_cast<int64_t>(min(first + r16, it.rows - 1)) * kHD + 8 * g4;
+        float4 u[16];
+        float mx = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            u[2 * c] = *reinterpret_cast<const float4*>(src + 32 * c);
+            u[2 * c + 1] = *reinterpret_cast<const float4*>(src + 32 * c + 4);
+        }
+#pragma unroll
+        for (auto& x : u) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const int e = split_row_exp(mx);
+        qscale = pow2(-e);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float x[8] = {u[2 * c].x, u[2 * c].y, u[2 * c].z, u[2 * c].w,
+                                u[2 * c + 1].x, u[2 * c + 1].y, u[2 * c + 1].z, u[2 * c + 1].w};
+            halfx8 p[2];
+            split2_8(x, pow2(e), p);
+            qp[0][c] = p[0], qp[1][c] = p[1];
+        }
+    }
+    store(Kc, kscale, 1);
+    load(it.V, it.lo);
     float m = -INFINITY, l = 0.0f;
     floatx4 o[16];
 #pragma unroll
     for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
-    store();
+    store(Vc, vscale, 2);
     lds_barrier();
     for (int k0 = it.lo; k0 < it.hi; k0 += kKT) {
-        load(min(k0 + kKT, it.hi - 1));
-        if (first < it.rows) tile_products<3>(Kc, Vc, qp, k0, it.hi, r16, g4, 0, nullptr, m, l, o);  // uniform per wave
-        lds_barrier();  // every wave is done with this tile
-        if (k0 + kKT < it.hi) {
-            store();
-            lds_barrier();
+        const bool more = k0 + kKT < it.hi;  // uniform
+        if (more) load(it.K, k0 + kKT);
+        int ko = k_off(r16, g4), vo = v_off(r16, g4);
+        asm volatile("" : "+v"(ko), "+v"(vo));  // formed per tile: kept, the 24 addresses would spill
+        float p[8], f = 1.0f;
+        if (live) {
+            floatx4 St[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                floatx4 sa[2], sb[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) sa[e] = sb[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    halfx8 k[2];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+                        k[q] = *reinterpret_cast<const halfx8*>(reinterpret_cast<const char*>(Kc[q]) + hf * 16 * 512 + (ko ^ (c << 6)));
+                    sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1], qp[0][c], sb[c & 1], 0, 0, 0);
+                    sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0], qp[1][c], sb[c & 1], 0, 0, 0);
+                    sa[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0], qp[0][c], sa[c & 1], 0, 0, 0);
+                }
+                St[hf] = (sb[0] + sb[1]) + (sa[0] + sa[1]);
+            }
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const floatx4 ks = *reinterpret_cast<const floatx4*>(kscale + 16 * hf + 4 * g4);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) p[4 * hf + v] = (St[hf][v] * qscale) * ks[v];
+            }
+            mask_tail(p, k0, it.hi, g4);
+            f = softmax_step(p, m, l);
         }
+        lds_barrier();  // every wave is done with K, every share of V is in
+        if (more) {
+            store(Kc, kscale, 1);
+            load(it.V, k0 + kKT);
+        }
+        if (live) {
+            rescale(f, g4, o);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const floatx4 vs = *reinterpret_cast<const floatx4*>(vscale + 16 * hf + 4 * g4);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) p[4 * hf + v] *= vs[v];
+            }
+            float mx = max8(p);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const int e = split_row_exp(mx);
+            halfx8 pp[2];
+            split2_8(p, pow2(e), pp);
+            const float undo = pow2(-e);
+            float er[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) er[v] = __shfl(undo, 4 * g4 + v);
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const halfx8 v0 = v_operand<halfx8>(Vc[0], vo ^ (t << 5)), v1 = v_operand<halfx8>(Vc[1], vo ^ (t << 5));
+                floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp[1], v0, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp[0], v1, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp[0], v0, x, 0, 0, 0);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) o[t][v] += x[v] * er[v];
+            }
+        }
+        lds_barrier();  // every wave is done with V, every share of the next K is in
+        if (more) store(Vc, vscale, 2);
     }
     store_part(it, first, r16, g4, 0, o, m, l, true);
 }
 
 // fp32 caches, narrow: 16 query rows on v_mfma_f32_16x16x4_f32 with K and V straight from memory
-// as its operands, no LDS and no barrier in the loop; the eight waves take 16 keys in turn and are
+// as its operands, no LDS and no barrier in the loop; the four waves take 16 keys in turn and are
 // merged at the end.
 //   S^T = K Q^T: lane (r16, g4) loads dims 16 u + 4 g4 .. + 3 of key r16; the k slot g4 of product
 //         (u, e) is dim 16 u + 4 g4 + e on both sides
@@ -452,7 +565,7 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
     floatx4 o[16];
 #pragma unroll
     for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = it.lo + 16 * wave; k0 < it.hi; k0 += 128) {
+    for (int k0 = it.lo + 16 * wave; k0 < it.hi; k0 += 64) {
         floatx4 s[4];
 #pragma unroll
         for (auto& x : s) x = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -492,119 +605,140 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
                 o[4 * t + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[v], vv[v][t].w, o[4 * t + 3], 0, 0, 0);
             }
     }
-    // merge of the waves, eight rows at a time; a wave without keys has maximum -inf and weight 0
+    // merge of the waves; one without keys has maximum -inf and weight 0
     if (g4 == 0) {
         ms[wave][r16] = m;
         ls[wave][r16] = l;
     }
     lds_barrier();
-    float top = ms[0][r16];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, ms[w][r16]);
+    const float top = fmaxf(fmaxf(ms[0][r16], ms[1][r16]), fmaxf(ms[2][r16], ms[3][r16]));
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * kLog2e);
     rescale(f, g4, o);
     const int n = min(16, it.rows - it.row0);
     if (wave == 0 && g4 == 0 && r16 < n) {
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
+        for (int w = 0; w < 4; ++w)
             if (ms[w][r16] != -INFINITY) sum += ls[w][r16] * __builtin_amdgcn_exp2f((ms[w][r16] - top) * kLog2e);
         it.ml[it.row0 + r16] = make_float2(top, sum);
     }
-    for (int r0 = 0; r0 < n; r0 += 8) {
-        if (r0) lds_barrier();
-        if (g4 >> 1 == r0 >> 3) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < 4; ++v)
+        if (4 * g4 + v < n) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    *reinterpret_cast<float4*>(buf + (wave * 8 + 4 * (g4 & 1) + v) * kHD + 64 * t + 4 * r16) =
-                        make_float4(o[4 * t][v], o[4 * t + 1][v], o[4 * t + 2][v], o[4 * t + 3][v]);
+            for (int t = 0; t < 4; ++t)
+                *reinterpret_cast<float4*>(buf + (wave * 16 + 4 * g4 + v) * kHD + 64 * t + 4 * r16) =
+                    make_float4(o[4 * t][v], o[4 * t + 1][v], o[4 * t + 2][v], o[4 * t + 3][v]);
         }
-        lds_barrier();
-        const int r = tid >> 6;
-        if (r0 + r < n) {
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    lds_barrier();
+    for (int r = wave; r < n; r += 4) {
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                const float4 x = *reinterpret_cast<const float4*>(buf + (w * 8 + r) * kHD + 4 * lane);
-                y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
-            }
-            *reinterpret_cast<float4*>(it.part + static_cast<int64_t>(it.row0 + r0 + r) * kHD + 4 * lane) = y;
+        for (int w = 0; w < 4; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(buf + (w * 16 + r) * kHD + 4 * lane);
+            y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
         }
+        *reinterpret_cast<float4*>(it.part + static_cast<int64_t>(it.row0 + r) * kHD + 4 * lane) = y;
     }
 }
 
-__global__ __launch_bounds__(512, 1) void attn_batch_f32_kernel(AttnBatchArgs a) {
-    __shared__ __align__(16) uint4 lds[2][3][1024];
+// fp32 caches: four waves, two workgroups per compute unit.
+__global__ __launch_bounds__(256, 2) void attn_batch_f32_kernel(AttnBatchArgs a) {
+    __shared__ __align__(16) uint4 lds[2][2][1024];
+    __shared__ __align__(16) float small[2][4][16];
     Item it;
     if (!item_of(a, it)) return;
-    if (it.narrow) {
-        float(*ms)[16] = reinterpret_cast<float(*)[16]>(&lds[1][2][0]);  // behind 64 KB of rows
-        f32_narrow(it, reinterpret_cast<float*>(lds), ms, ms + 8);
-    } else {
-        f32_wide(it, lds[0], lds[1]);
-    }
+    if (it.narrow) f32_narrow(it, reinterpret_cast<float*>(lds), small[0], small[1]);
+    else f32_wide(it, lds[0], lds[1], &small[0][0][0], &small[1][0][0]);
 }
 
-// The (max, sum) of row g of (b, kh) over all its pieces; f(i, m, l) for each.
-template <class F>
-__device__ __forceinline__ void pieces_of(const AttnBatchArgs& a, int b, int kh, int g, int n_own, F&& f) {
-    for (int i = 0; i < a.plan.pieces; ++i) {
-        const int64_t row = (static_cast<int64_t>(kh) * a.plan.pieces + i) * a.B * a.GRP + b * a.GRP + g;
-        f(a.part_p + row * kHD, a.ml_p[row]);
+constexpr int kCombWaves = 8;
+
+// The (max, sum) of piece i of row g of (b, kh): the prefix's pieces, then the own cache's.
+__device__ __forceinline__ int64_t piece_row(const AttnBatchArgs& a, int b, int kh, int g, int i) {
+    return i < a.plan.pieces
+               ? (static_cast<int64_t>(kh) * a.plan.pieces + i) * a.B * a.GRP + b * a.GRP + g
+               : ((static_cast<int64_t>(b) * a.NKV + kh) * a.plan.own + i - a.plan.pieces) * a.GRP + g;
+}
+__device__ __forceinline__ float2 piece_ml(const AttnBatchArgs& a, int b, int kh, int g, int i) {
+    return (i < a.plan.pieces ? a.ml_p : a.ml_o)[piece_row(a, b, kh, g, i)];
+}
+// (max, sum) over n pieces, by the lanes of a wave
+__device__ __forceinline__ float2 merge_ml(const AttnBatchArgs& a, int b, int kh, int g, int n, int lane) {
+    float m = -INFINITY, l = 0.0f;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, piece_ml(a, b, kh, g, i).x);
+    m = wave_max(m);
+    for (int i = lane; i < n; i += 64) {
+        const float2 x = piece_ml(a, b, kh, g, i);
+        l += x.y * __builtin_amdgcn_exp2f((x.x - m) * kLog2e);
     }
-    for (int i = 0; i < n_own; ++i) {
-        const int64_t row = ((static_cast<int64_t>(b) * a.NKV + kh) * a.plan.own + i) * a.GRP + g;
-        f(a.part_o + row * kHD, a.ml_o[row]);
-    }
+    return make_float2(m, wave_sum(l));
 }
 
-// grid (NQ, B), one thread per dim: merges the pieces, divides, gates.
-__global__ __launch_bounds__(256) void attn_batch_combine_kernel(AttnBatchArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-    const int n = a.own_len[b];
-    if (n < 0) return;
-    float* out = a.out + (static_cast<int64_t>(b) * a.NQ + h) * kHD + d;
-    if (n >= a.cap) {
-        *out = NAN;
+// Workgroups [0, B NQ): one output row each. The pieces' factors e^(their maximum - the row's) / sum
+// first, into LDS, so that the partial outputs stream with nothing between their loads: a wave
+// takes every eighth piece, a lane four dims. Then the gate.
+// The others (with own_score): 512 own rows of a (sequence, kv head) each: their weights, summed
+// over the heads of the group in order, into the scores.
+__global__ __launch_bounds__(kCombWaves * 64) void attn_batch_combine_kernel(AttnBatchArgs a) {
+    extern __shared__ __align__(16) float fac[];  // a factor per piece
+    __shared__ __align__(16) float part[kCombWaves][kHD];
+    __shared__ float ms[16], ls[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int rows = a.B * a.NQ;
+    if (static_cast<int>(blockIdx.x) >= rows) {
+        const int chunks = static_cast<int>((a.cap + 511) / 512);
+        const int64_t bk = (blockIdx.x - rows) / chunks;
+        const int chunk = (blockIdx.x - rows) % chunks;
+        const int b = static_cast<int>(bk / a.NKV), kh = static_cast<int>(bk % a.NKV);
+        const int slot = new_slot(a, b);
+        if (slot < 0 || chunk * 512LL > slot) return;
+        const int n = a.plan.pieces + slot / a.plan.okeys + 1;
+        for (int g = wave; g < a.GRP; g += kCombWaves) {
+            const float2 x = merge_ml(a, b, kh, g, n, lane);
+            if (lane == 0) ms[g] = x.x, ls[g] = 1.0f / x.y;
+        }
+        __syncthreads();
+        const int64_t t = chunk * 512LL + tid;
+        if (t > slot) return;
+        float w = 0.0f;
+        for (int g = 0; g < a.GRP; ++g)
+            w += __builtin_amdgcn_exp2f((a.raw[(bk * a.GRP + g) * raw_stride(a.cap) + t] - ms[g]) * kLog2e) * ls[g];
+        float* sc = a.own_score + bk * a.cap + t;
+        *sc = t == slot ? w : *sc + w;
         return;
     }
-    const int kh = h / a.GRP, g = h - kh * a.GRP, n_own = n / a.plan.okeys + 1;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    pieces_of(a, b, kh, g, n_own, [&](const float*, float2 ml) { m = fmaxf(m, ml.x); });
-    pieces_of(a, b, kh, g, n_own, [&](const float* po, float2 ml) {
-        const float f = expf(ml.x - m);
-        l += ml.y * f;
-        o += po[d] * f;
-    });
-    const float gate = a.qg[(static_cast<int64_t>(b) * a.NQ + h) * 2 * kHD + kHD + d];
-    *out = (o / l) * sigmoid_f(gate);
-}
-
-// grid (cap / 256, NKV, B): the weights of the own rows, summed over the heads of the group
-// in their order, into the scores.
-__global__ __launch_bounds__(256) void attn_batch_score_kernel(AttnBatchArgs a) {
-    const int kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-    const int slot = new_slot(a, b);
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + tid;
-    if (slot < 0 || blockIdx.x * 256LL > slot) return;
-    __shared__ float ms[16], ls[16];
-    if (tid < a.GRP) {
-        float m = -INFINITY, l = 0.0f;
-        const int n_own = slot / a.plan.okeys + 1;
-        pieces_of(a, b, kh, tid, n_own, [&](const float*, float2 ml) { m = fmaxf(m, ml.x); });
-        pieces_of(a, b, kh, tid, n_own, [&](const float*, float2 ml) { l += ml.y * expf(ml.x - m); });
-        ms[tid] = m;
-        ls[tid] = l;
+    const int h = blockIdx.x % a.NQ, b = blockIdx.x / a.NQ;
+    const int len = a.own_len[b];
+    if (len < 0) return;
+    float* out = a.out + (static_cast<int64_t>(b) * a.NQ + h) * kHD + 4 * lane;
+    if (len >= a.cap) {
+        if (wave == 0) *reinterpret_cast<float4*>(out) = make_float4(NAN, NAN, NAN, NAN);
+        return;
     }
+    const int kh = h / a.GRP, g = h - kh * a.GRP, n = a.plan.pieces + len / a.plan.okeys + 1;
+    const float4 gate = *reinterpret_cast<const float4*>(a.qg + (static_cast<int64_t>(b) * a.NQ + h) * 2 * kHD + kHD + 4 * lane);
+    const float2 all = merge_ml(a, b, kh, g, n, lane);  // every wave the same
+    for (int i = tid; i < n; i += kCombWaves * 64)
+        fac[i] = __builtin_amdgcn_exp2f((piece_ml(a, b, kh, g, i).x - all.x) * kLog2e);
     __syncthreads();
-    if (t > slot) return;
-    const int64_t bk = static_cast<int64_t>(b) * a.NKV + kh;
-    float w = 0.0f;
-    for (int g = 0; g < a.GRP; ++g) w += expf(a.raw[(bk * a.GRP + g) * raw_stride(a.cap) + t] - ms[g]) / ls[g];
-    float* sc = a.own_score + bk * a.cap + t;
-    *sc = t == slot ? w : *sc + w;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = wave; i < n; i += kCombWaves) {
+        const float4 x = *reinterpret_cast<const float4*>((i < a.plan.pieces ? a.part_p : a.part_o) + piece_row(a, b, kh, g, i) * kHD + 4 * lane);
+        const float f = fac[i];
+        y.x += x.x * f, y.y += x.y * f, y.z += x.z * f, y.w += x.w * f;
+    }
+    *reinterpret_cast<float4*>(&part[wave][4 * lane]) = y;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < kCombWaves; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(&part[w][4 * lane]);
+        y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+    }
+    *reinterpret_cast<float4*>(out) = make_float4((y.x / all.y) * sigmoid_f(gate.x), (y.y / all.y) * sigmoid_f(gate.y),
+                                                  (y.z / all.y) * sigmoid_f(gate.z), (y.w / all.y) * sigmoid_f(gate.w));
 }
 
 struct Carve {
@@ -641,13 +775,12 @@ void attn_batch_carve(AttnBatchArgs& a, float* ws) {
 }
 
 hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s) {
-    klaunch(attn_batch_prep_kernel, dim3(a.B, a.NQ + a.NKV), 256, 0, s, a);
+    klaunch(attn_batch_prep_kernel, dim3((a.NQ + a.NKV + 3) / 4, a.B), 256, 0, s, a);
     const uint32_t prefix = (a.plan.pieces * a.NKV + 7) / 8 * 8 * a.plan.nblk, own = a.B * a.NKV * a.plan.own;
     if (a.kv_bf16) klaunch(attn_batch_bf16_kernel, dim3(prefix + own), 256, 0, s, a);
-    else klaunch(attn_batch_f32_kernel, dim3(prefix + own), 512, 0, s, a);
-    klaunch(attn_batch_combine_kernel, dim3(a.NQ, a.B), 256, 0, s, a);
-    if (a.own_score)
-        klaunch(attn_batch_score_kernel, dim3(static_cast<uint32_t>((a.cap + 255) / 256), a.NKV, a.B), 256, 0, s, a);
+    else klaunch(attn_batch_f32_kernel, dim3(prefix + own), 256, 0, s, a);
+    const uint32_t scores = a.own_score ? static_cast<uint32_t>((a.cap + 511) / 512) * a.B * a.NKV : 0;
+    klaunch(attn_batch_combine_kernel, dim3(a.B * a.NQ + scores), kCombWaves * 64, (a.plan.pieces + a.plan.own) * 4, s, a);
     return hipGetLastError();
 }
 
