@@ -326,10 +326,14 @@ struct KvEvictArgs {
     int* pos_out;
     int* new_len;
     // set by kv_evict_carve: per (b, kv head) the new length and the rows to move, then the
-    // slots they go to and come from
+    // slots they go to and come from; for long caches the rows' keys, the keys in the bin of the
+    // last one that stays, counts and a histogram per slice of rows, and that bin
     int2* head;
     int *to, *from;
     int most;                           // rows that may have to move
+    uint32_t *keys, *cand, *hist;
+    uint4* slice;
+    uint2* limit;
 };
 int64_t kv_evict_workspace_ints(int B, int NKV, int64_t cap, int keep);
 void kv_evict_carve(KvEvictArgs& a, int* ws);

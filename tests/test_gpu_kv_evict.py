@@ -113,6 +113,24 @@ def test_long(hip, cap, keep, bf16):
     run(hip, x, keep, min(4, keep // 2), min(64, keep // 2), bf16=bf16)
 
 
+@pytest.mark.parametrize("kind", ["ties", "same", "close", "bits"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_long_with_equal_scores(hip, kind, in_place):
+    """More equal keys than the selection holds in LDS, and lengths that end within a slice."""
+    cap = 40961
+    x = make(3, 2, cap, [cap, 20000, 33000], seed=len(kind), bf16=True, kind=kind)
+    for keep in (30000, 1):
+        run(hip, x, keep, min(3, keep // 2), min(100, keep // 2), bf16=True, in_place=in_place)
+
+
+@pytest.mark.parametrize("cap", [4096, 4097, 16384, 16385])
+def test_around_the_forms_of_the_selection(hip, cap):
+    lens = [cap, cap - 1, 2049, 2048, 2047, 0, -1, cap + 1]
+    run(hip, make(len(lens), 1, cap, lens, seed=cap, bf16=True), 2048, 4, 64, bf16=True)
+    run(hip, make(len(lens), 1, cap, lens, seed=cap, bf16=True, kind="close"), cap - 1, 4, 64, bf16=True, in_place=True)
+    run(hip, make(2, 1, cap, [cap, 5], seed=cap, bf16=True), cap + 5, bf16=True)
+
+
 def test_many_sequences(hip):
     rng = np.random.default_rng(4)
     x = make(64, 2, 96, rng.integers(-1, 98, 64), seed=4, bf16=True)
