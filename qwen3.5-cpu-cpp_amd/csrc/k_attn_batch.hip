@@ -92,6 +92,7 @@ constexpr int kWaitVm = 0x0f70; // s_waitcnt: vector memory, nothing outstanding
 // What one workgroup does: rows [row0, rows) of one list of query rows over keys [lo, hi) of one
 // cache, and where its partial result goes.
 struct Item {
+
     const float* Q;         // query rows [rows][HD]
     int rows, row0;
     int lo, hi;
@@ -103,13 +104,13 @@ struct Item {
     bool narrow;            // at most 16 rows, shared by the workgroup's waves
 };
 
-// Workgroups [0, prefix) are (piece, kv head, row block) of the prefix, the others (piece, kv
+// Items [0, prefix_items) are (piece, kv head, row block) of the prefix, the others (piece, kv
 // head, sequence) of the own caches. Workgroups go to the 8 XCDs in turn: the row blocks that
 // read one piece get numbers 8 apart, so that one L2 fetches it for all of them.
-__device__ __forceinline__ bool item_of(const AttnBatchArgs& a, Item& it) {
-    const int pairs = a.plan.pieces * a.NKV, groups = (pairs + 7) / 8;
-    const int prefix = groups * 8 * a.plan.nblk;
-    int i = blockIdx.x;
+__host__ __device__ inline int prefix_items(const AttnBatchPlan& p, int NKV) { return (p.pieces * NKV + 7) / 8 * 8 * p.nblk; }
+__device__ __forceinline__ bool item_of(const AttnBatchArgs& a, int i, Item& it) {
+    const int pairs = a.plan.pieces * a.NKV, prefix = prefix_items(a.plan, a.NKV);
+
     const int64_t row_bytes = a.kv_bf16 ? kHD * 2 : kHD * 4;
     if (i < prefix) {
         const int blk = (i >> 3) % a.plan.nblk, pair = (i >> 3) / a.plan.nblk * 8 + (i & 7);
@@ -131,8 +132,10 @@ __device__ __forceinline__ bool item_of(const AttnBatchArgs& a, Item& it) {
         return true;
     }
     i -= prefix;
-    const int piece = i % a.plan.own;
-    i /= a.plan.own;
+    // first pieces first: later ones may be empty, and would leave whole XCDs idle side by side
+    const int piece = i / (a.B * a.NKV);
+    if (piece >= a.plan.own) return false;
+    i -= piece * (a.B * a.NKV);
     const int kh = i % a.NKV, b = i / a.NKV;
     const int slot = new_slot(a, b);
     const int64_t lo = static_cast<int64_t>(piece) * a.plan.okeys;
@@ -178,6 +181,21 @@ __device__ __forceinline__ void load_query(const Item& it, int first, int r16, i
     }
 }
 
+// max and sum over the four lanes r16 + 16 g of a query (the 16- and 32-lane swaps of gfx950)
+template <class F>
+__device__ __forceinline__ float over_query(float v, F&& f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    v = f(__builtin_bit_cast(float, static_cast<int>(r[0])), __builtin_bit_cast(float, static_cast<int>(r[1])));
+    r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return f(__builtin_bit_cast(float, static_cast<int>(r[0])), __builtin_bit_cast(float, static_cast<int>(r[1])));
+}
+__device__ __forceinline__ float query_max(float v) {
+    return over_query(v, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ float query_sum(float v) {
+    return over_query(v, [](float x, float y) { return x + y; });
+}
+
 // Online softmax of N scores of the lane's query (four lanes r16 + 16 g share it): s becomes
 // weights, (m, l) the query's running maximum and sum. Returns the factor of the output so
 // far. The reference maximum moves only when a score exceeds it by more than 8; a query without
@@ -188,8 +206,7 @@ __device__ __forceinline__ float softmax_step(float (&s)[N], float& m, float& l)
     float tm = s[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) tm = fmaxf(tm, s[i]);
-    tm = fmaxf(tm, __shfl_xor(tm, 16));
-    tm = fmaxf(tm, __shfl_xor(tm, 32));
+    tm = query_max(tm);
     const float m_new = tm > m + 8.0f ? tm : m;
     const bool live = m_new != -INFINITY;
     const float f = live ? __builtin_amdgcn_exp2f((m - m_new) * kLog2e) : 1.0f;
@@ -199,24 +216,17 @@ __device__ __forceinline__ float softmax_step(float (&s)[N], float& m, float& l)
         s[i] = live ? __builtin_amdgcn_exp2f((s[i] - m_new) * kLog2e) : 0.0f;
         ps += s[i];
     }
-    ps += __shfl_xor(ps, 16);
-    ps += __shfl_xor(ps, 32);
-    l = l * f + ps;
+    l = l * f + query_sum(ps);
     m = m_new;
     return f;
 }
 
-// o[.][v] (query rows 4 g4 + v) times the factors of lanes 4 g4 + v
+// the lane's outputs times its query's factor, which is mostly 1
 template <int N>
-__device__ __forceinline__ void rescale(float f, int g4, floatx4 (&o)[N]) {
+__device__ __forceinline__ void rescale(float f, floatx4 (&o)[N]) {
     if (!__any(f != 1.0f)) return;
-    float fr[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) fr[v] = __shfl(f, 4 * g4 + v);
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o[t][v] *= fr[v];
+    for (int t = 0; t < N; ++t) o[t] *= f;
 }
 
 // The 16-byte chunk (dims 8 c ..) of row r of a 32-key tile of bf16 lies in LDS at chunk
@@ -227,6 +237,20 @@ __device__ __forceinline__ int k_off(int r16, int g4) { return r16 * 512 + ((g4 
 __device__ __forceinline__ int v_off(int r16, int g4) {                                            // ^ (t << 5)
     const int row = 4 * g4 + (r16 >> 2);
     return row * 512 + ((((2 * row) & 15) + ((r16 & 3) >> 1)) << 4) + (r16 & 1) * 8;
+}
+
+// Order of a run of STEPS steps of READS LDS reads and PRODUCTS matrix products on what they
+// return: the reads of two steps first, then those of each next step under the products of one
+// (left alone, the compiler reads and waits step by step, 100 to 200 cycles each).
+template <int STEPS, int READS, int PRODUCTS>
+__device__ __forceinline__ void reads_ahead() {
+    constexpr int kRead = 0x100, kProduct = 0x8, kAhead = STEPS < 2 ? STEPS : 2;
+    __builtin_amdgcn_sched_group_barrier(kRead, kAhead * READS, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kProduct, PRODUCTS, 0);
+        if (i + kAhead < STEPS) __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
+    }
 }
 
 // scores of keys past the last
@@ -252,9 +276,10 @@ __device__ __forceinline__ X8 v_operand(const uint4* V, int off) {
 // Queries and weights are the exact sums of three bf16 parts, K and V one part as they are, so every
 // product is exact in fp32.
 //   S^T = K Q^T by 16-key halves: lane (r16, g4) ends with keys 4 g4 + v of both for query r16
-//   O += P V: those eight weights are the A operand as they lie, its k slots 8 g4 .. + 7 being
-//         keys 4 g4 .. + 3 of the first half and of the second, which transposed LDS reads give V too;
-//         lane (r16, g4) ends with dims 16 t + r16 of queries 4 g4 + v
+//   O^T += V^T P^T: those eight weights are the B operand as they lie, its k slots 8 g4 .. + 7
+//         being keys 4 g4 .. + 3 of the first half and of the second, which transposed LDS reads
+//         give V too; lane (r16, g4) ends with dims 16 t + 4 g4 + v of query r16, so that a
+//         query's factors stay in its lanes
 // T tiles of 16 dims from t0 on (a narrow workgroup's waves share the dims and each form all scores).
 template <int T>
 __device__ __forceinline__ void bf16_tile(const uint4 (&Kc)[1024], const uint4 (&Vc)[1024], const bf16x8 (&qp)[3][8], int k0,
@@ -268,14 +293,21 @@ __device__ __forceinline__ void bf16_tile(const uint4 (&Kc)[1024], const uint4 (
 #pragma unroll
         for (int e = 0; e < 2; ++e) sa[e] = sb[e] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const bf16x8 k = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(Kc) + hf * 16 * 512 + (ko ^ (c << 6)));
-            sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[2][c], sb[c & 1], 0, 0, 0);
-            sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[1][c], sb[c & 1], 0, 0, 0);
-            sa[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[0][c], sa[c & 1], 0, 0, 0);
+        for (int c = 0; c < 8; c += 2) {
+            bf16x8 k[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                k[e] = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(Kc) + hf * 16 * 512 + (ko ^ ((c + e) << 6)));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sb[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[e], qp[2][c + e], sb[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sa[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[e], qp[0][c + e], sa[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sb[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[e], qp[1][c + e], sb[e], 0, 0, 0);
         }
         St[hf] = (sb[0] + sb[1]) + (sa[0] + sa[1]);
     }
+    reads_ahead<8, 2, 6>();
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = St[i >> 2][i & 3];
@@ -285,32 +317,40 @@ __device__ __forceinline__ void bf16_tile(const uint4 (&Kc)[1024], const uint4 (
     }
     mask_tail(p, k0, hi, g4);
     const float f = softmax_step(p, m, l);
-    rescale(f, g4, o);
+    rescale(f, o);
     bf16x8 pa[3];
     split3_8(p, pa);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const bf16x8 v = v_operand<bf16x8>(Vc, vo ^ ((t0 + t) << 5));
+    for (int t = 0; t < T; t += 2) {
+        bf16x8 v[2];
 #pragma unroll
-        for (int q = 2; q >= 0; --q) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[q], v, o[t], 0, 0, 0);
+        for (int e = 0; e < 2; ++e) v[e] = v_operand<bf16x8>(Vc, vo ^ ((t0 + t + e) << 5));
+#pragma unroll
+        for (int q = 2; q >= 0; --q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) o[t + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[e], pa[q], o[t + e], 0, 0, 0);
     }
+    reads_ahead<T / 2, 4, 6>();
 }
 
-// A wave's unnormalised output (dims 16 (t0 + t) + r16 of rows first + 4 g4 + v) and, from the
+// A wave's unnormalised output (dims 16 (t0 + t) + 4 g4 + v of row first + r16) and, from the
 // wave that is asked, the rows' (max, sum).
 template <int T>
 __device__ __forceinline__ void store_part(const Item& it, int first, int r16, int g4, int t0, const floatx4 (&o)[T], float m,
                                            float l, bool with_ml) {
+    const int row = first + r16;
+    if (row >= it.rows) return;
+    float* dst = it.part + static_cast<int64_t>(row) * kHD + 16 * t0 + 4 * g4;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        const int row = first + 4 * g4 + v;
-        if (row < it.rows) {
-            float* dst = it.part + static_cast<int64_t>(row) * kHD + 16 * t0 + r16;
-#pragma unroll
-            for (int t = 0; t < T; ++t) dst[16 * t] = o[t][v];
-        }
-    }
-    if (with_ml && g4 == 0 && first + r16 < it.rows) it.ml[first + r16] = make_float2(m, l);
+    for (int t = 0; t < T; ++t) *reinterpret_cast<floatx4*>(dst + 16 * t) = o[t];
+    if (with_ml && g4 == 0) it.ml[row] = make_float2(m, l);
+}
+
+// 16 bytes a lane from memory straight into LDS: lane i's go to dst + i.
+__device__ __forceinline__ void copy_16(const uint4* src, uint4* dst) {
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
 // bf16 caches: four waves, two workgroups per compute unit. Tiles are copied from memory
@@ -322,7 +362,7 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
     // before reads of another)
     __shared__ __align__(16) uint4 K0[1024], V0[1024], K1[1024], V1[1024];
     Item it;
-    if (!item_of(a, it)) return;
+    if (!item_of(a, blockIdx.x, it)) return;
     const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto copy = [&](int k0, uint4* K, uint4* V) {
@@ -332,12 +372,8 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
             const int64_t at = static_cast<int64_t>(min(k0 + row, it.hi - 1)) * 32;
             const uint4* ks = static_cast<const uint4*>(it.K) + at + (pos ^ (row & 15));
             const uint4* vs = static_cast<const uint4*>(it.V) + at + (pos ^ ((2 * row) & 15));
-            __builtin_amdgcn_global_load_lds(
-                reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(ks)),
-                (__attribute__((address_space(3))) void*)(K + c), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(
-                reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(vs)),
-                (__attribute__((address_space(3))) void*)(V + c), 16, 0, 0);
+            copy_16(ks, K + c);
+            copy_16(vs, V + c);
         }
     };
     copy(it.lo, K0, V0);
@@ -380,240 +416,325 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 __device__ __forceinline__ void split2_8(const float (&x)[8], float s, halfx8 (&part)[2]) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split2h_pair(x[2 * e] * s, x[2 * e + 1] * s, h[e], l[e]);
+    for (int e = 0; e < 4; ++e) {  // (the mixed-precision fused multiply-adds round straight to fp16)
+        const float a = x[2 * e], b = x[2 * e + 1];
+        const _Float16 ha = static_cast<_Float16>(__builtin_fmaf(a, s, 0.0f)), hb = static_cast<_Float16>(__builtin_fmaf(b, s, 0.0f));
+        const _Float16 la = static_cast<_Float16>(__builtin_fmaf(a, s, -static_cast<float>(ha)));
+        const _Float16 lb = static_cast<_Float16>(__builtin_fmaf(b, s, -static_cast<float>(hb)));
+        h[e] = __builtin_bit_cast(uint32_t, split_h2_t{ha, hb});
+        l[e] = __builtin_bit_cast(uint32_t, split_h2_t{la, lb});
+    }
     part[0] = __builtin_bit_cast(halfx8, make_uint4(h[0], h[1], h[2], h[3]));
     part[1] = __builtin_bit_cast(halfx8, make_uint4(l[0], l[1], l[2], l[3]));
 }
+// largest |x| (in instructions: the compiler would first quieten each operand)
 __device__ __forceinline__ float max8(const float (&x)[8]) {
-    float m = fabsf(x[0]);
+    float m;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(m) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[3]), "v"(x[4]));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[5]), "v"(x[6]));
+    return fmaxf(m, fabsf(x[7]));
+}
+// the power of two that brings a largest magnitude (its bits) into [2^14, 2^15), as far as 2^+-100
+__device__ __forceinline__ int row_exp(uint32_t bits) { return min(max(141 - static_cast<int>(bits >> 23), -100), 100); }
+
+// A tile of an fp32 cache in LDS: two fp16 parts of K and of V, and what undoes their rows' scales.
+//
+// fp32 caches run on v_mfma_f32_16x16x32_f16. Every operand row (a query, a key, a value row, a
+// query's weights over the tile) is scaled by a power of two that brings its largest entry into
+// [2^14, 2^15) and split into two fp16 parts; the three part products of lowest order are summed
+// (the fourth is below 2^-22 of the product) and the scales undone exactly: a key's in the scores,
+// a value row's in the weights before their own scaling, and that one as the tile's products,
+// summed from zero, are added to the output. So nothing is lost relative to the largest weight
+// times value row of the tile, whatever rows lie beside it.
+struct F32Tile {
+    uint4 K[2][1024], V[2][1024];
+    float kscale[kKT], vscale[kKT];
+};
+struct F32Query {
+    halfx8 p[2][8];  // row first + r16, dims 32 c + 8 g4 .. + 7
+    float scale;
+};
+
+__device__ __forceinline__ void f32_query(const Item& it, int first, int r16, int g4, F32Query& q) {
+    const float* src = it.Q + static_cast<int64_t>(min(first + r16, it.rows - 1)) * kHD + 8 * g4;
+    float4 u[16];
+    float mx = 0.0f;
 #pragma unroll
-    for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
-    return m;
+    for (int c = 0; c < 8; ++c) {
+        u[2 * c] = *reinterpret_cast<const float4*>(src + 32 * c);
+        u[2 * c + 1] = *reinterpret_cast<const float4*>(src + 32 * c + 4);
+    }
+#pragma unroll
+    for (auto& x : u) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+    const int e = row_exp(__float_as_uint(query_max(mx)));
+    q.scale = pow2(-e);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const float x[8] = {u[2 * c].x, u[2 * c].y, u[2 * c].z, u[2 * c].w,
+                            u[2 * c + 1].x, u[2 * c + 1].y, u[2 * c + 1].z, u[2 * c + 1].w};
+        halfx8 p[2];
+        split2_8(x, pow2(e), p);
+        q.p[0][c] = p[0], q.p[1][c] = p[1];
+    }
 }
 
-// fp32 caches, wide: 64 query rows, 16 a wave, 32-key tiles, on v_mfma_f32_16x16x32_f16. Every
-// operand row (a query, a key, a value row, a query's weights over the tile) is scaled by a power
-// of two that brings its largest entry into [2^14, 2^15) and split into two fp16 parts; the three
-// part products of lowest order are summed (the fourth is below 2^-22 of the product) and the
-// scales undone exactly: a key's in the scores, a value row's in the weights before their own
-// scaling, and that one as the tile's products, summed from zero, are added to the output. So
-// nothing is lost relative to the largest weight times value row of the tile, whatever rows lie
-// beside it.
-// A tile's rows come through registers and are split once for the four waves: K of the next tile
-// while V is multiplied, V while K is.
-__device__ __forceinline__ void f32_wide(const Item& it, uint4 (*Kc)[1024], uint4 (*Vc)[1024], float* kscale, float* vscale) {
+// Dims 8 c .. + 7 (lo, hi) of row `row` of a tile's K or V: the 32 lanes of half a wave hold the row.
+__device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c, floatx4 lo, floatx4 hi) {
+    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    uint32_t mx = __float_as_uint(max8(x));
+    mx = max(mx, static_cast<uint32_t>(dpp_i<0xB1>(mx)));
+    mx = max(mx, static_cast<uint32_t>(dpp_i<0x4E>(mx)));
+    mx = max(mx, static_cast<uint32_t>(dpp_i<0x141>(mx)));
+    mx = max(mx, static_cast<uint32_t>(dpp_i<0x140>(mx)));
+    const auto r = __builtin_amdgcn_permlane16_swap(mx, mx, false, false);
+    const int e = row_exp(max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1])));
+    halfx8 p[2];
+    split2_8(x, pow2(e), p);
+    const int at = 32 * row + (c ^ ((v ? 2 * row : row) & 15));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) (v ? tile.V : tile.K)[q][at] = __builtin_bit_cast(uint4, p[q]);
+    if (c == 0) (v ? tile.vscale : tile.kscale)[row] = pow2(-e);
+}
+
+// Scores of query r16 of the wave: keys 4 g4 + v of the tile's first half, then of its second.
+__device__ __forceinline__ void f32_scores(const F32Tile& tile, const F32Query& q, int r16, int g4, float (&p)[8]) {
+    int ko = k_off(r16, g4);
+    asm volatile("" : "+v"(ko));  // addresses formed per tile: kept, they would spill
+    floatx4 St[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+        floatx4 sa[2], sb[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sa[e] = sb[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+            halfx8 k[2][2];
+#pragma unroll
+            for (int h = 1; h >= 0; --h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    k[h][e] = *reinterpret_cast<const halfx8*>(reinterpret_cast<const char*>(tile.K[h]) + hf * 16 * 512 + (ko ^ ((c + e) << 6)));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sb[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][e], q.p[0][c + e], sb[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sa[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][e], q.p[0][c + e], sa[e], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sb[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][e], q.p[1][c + e], sb[e], 0, 0, 0);
+        }
+        St[hf] = (sb[0] + sb[1]) + (sa[0] + sa[1]);
+    }
+    reads_ahead<8, 4, 6>();
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+        const floatx4 ks = *reinterpret_cast<const floatx4*>(tile.kscale + 16 * hf + 4 * g4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) p[4 * hf + v] = (St[hf][v] * q.scale) * ks[v];
+    }
+}
+
+// O^T += V^T P^T for T tiles of 16 dims from t0 on.
+template <int T>
+__device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], int r16, int g4, int t0, floatx4 (&o)[T]) {
+    int vo = v_off(r16, g4);
+    asm volatile("" : "+v"(vo));
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+        const floatx4 vs = *reinterpret_cast<const floatx4*>(tile.vscale + 16 * hf + 4 * g4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) p[4 * hf + v] *= vs[v];
+    }
+    const int e = row_exp(__float_as_uint(query_max(max8(p))));
+    halfx8 pp[2];
+    split2_8(p, pow2(e), pp);
+    const float undo = pow2(-e);
+    // steps of 32 dims: the next but one's reads and the last one's sums go with this one's products
+    constexpr int kAhead = 2, kSteps = T / 2;
+    halfx8 v[kAhead + 1][2][2];
+    floatx4 x[2][2];
+    const auto read = [&](int u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) v[u % (kAhead + 1)][h][d] = v_operand<halfx8>(tile.V[h], vo ^ ((t0 + 2 * u + d) << 5));
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) read(u);
+#pragma unroll
+    for (int u = 0; u <= kSteps; ++u) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (u + kAhead < kSteps) read(u + kAhead);
+        if (u < kSteps) {
+            const halfx8(&w)[2][2] = v[u % (kAhead + 1)];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) x[u & 1][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][d], pp[1], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) x[u & 1][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[1][d], pp[0], x[u & 1][d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) x[u & 1][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][d], pp[0], x[u & 1][d], 0, 0, 0);
+        }
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+            if (u) o[2 * u - 2 + d] += x[u & 1 ^ 1][d] * undo;
+    }
+}
+
+// Wide: 128 query rows, 16 a wave. Tiles come through registers and are split once for all waves
+// into the other of two buffers, one barrier a tile. Of the two waves that share a matrix core one
+// stages before its products with K and the other after, so that one's vector work runs under the
+// other's products.
+__device__ __forceinline__ void f32_wide(const Item& it, F32Tile* tiles) {
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = it.row0 + 16 * wave;
     const bool live = first < it.rows;  // uniform per wave
-    float4 st[8];
-    auto load = [&](const void* cache, int k0) {
+    floatx4 st[8];
+    const auto load = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t at = static_cast<int64_t>(min(k0 + (tid >> 5) + 8 * i, it.hi - 1)) * kHD + 8 * (tid & 31);
-            const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(cache) + at);
-            st[2 * i] = s[0], st[2 * i + 1] = s[1];
+        for (int i = 0; i < 2; ++i) {
+            const int64_t at = static_cast<int64_t>(min(k0 + (tid >> 5) + 16 * i, it.hi - 1)) * kHD + 8 * (tid & 31);
+            const floatx4 *k = reinterpret_cast<const floatx4*>(static_cast<const float*>(it.K) + at),
+                          *v = reinterpret_cast<const floatx4*>(static_cast<const float*>(it.V) + at);
+            st[2 * i] = k[0], st[2 * i + 1] = k[1];
+            st[4 + 2 * i] = v[0], st[5 + 2 * i] = v[1];
         }
     };
-    auto store = [&](uint4 (*dst)[1024], float* scale, int mul) {
+    const auto stage = [&](F32Tile& dst) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = (tid >> 5) + 8 * i, c = tid & 31;
-            const float x[8] = {st[2 * i].x, st[2 * i].y, st[2 * i].z, st[2 * i].w,
-                                st[2 * i + 1].x, st[2 * i + 1].y, st[2 * i + 1].z, st[2 * i + 1].w};
-            float mx = max8(x);  // over the row: the 32 lanes of half a wave
-            mx = fmaxf(mx, dpp_f<0xB1>(mx));
-            mx = fmaxf(mx, dpp_f<0x4E>(mx));
-            mx = fmaxf(mx, dpp_f<0x141>(mx));
-            mx = fmaxf(mx, dpp_f<0x140>(mx));
-            mx = fmaxf(mx, swz16_f(mx));
-            const int e = split_row_exp(mx);
-            halfx8 p[2];
-            split2_8(x, pow2(e), p);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) dst[q][32 * row + (c ^ ((mul * row) & 15))] = __builtin_bit_cast(uint4, p[q]);
-            if (c == 0) scale[row] = pow2(-e);
-        }
+        for (int i = 0; i < 4; ++i) f32_stage(dst, i >= 2, (tid >> 5) + 16 * (i & 1), tid & 31, st[2 * i], st[2 * i + 1]);
     };
-    load(it.K, it.lo);
-    halfx8 qp[2][8];
-    float qscale;
-    {
-        const float* src = it.Q + static_cast<int64_t>(min(first + r16, it.rows - 1)) * kHD + 8 * g4;
-        float4 u[16];
-        float mx = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            u[2 * c] = *reinterpret_cast<const float4*>(src + 32 * c);
-            u[2 * c + 1] = *reinterpret_cast<const float4*>(src + 32 * c + 4);
-        }
-#pragma unroll
-        for (auto& x : u) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int e = split_row_exp(mx);
-        qscale = pow2(-e);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float x[8] = {u[2 * c].x, u[2 * c].y, u[2 * c].z, u[2 * c].w,
-                                u[2 * c + 1].x, u[2 * c + 1].y, u[2 * c + 1].z, u[2 * c + 1].w};
-            halfx8 p[2];
-            split2_8(x, pow2(e), p);
-            qp[0][c] = p[0], qp[1][c] = p[1];
-        }
-    }
-    store(Kc, kscale, 1);
-    load(it.V, it.lo);
+    load(it.lo);
+    F32Query q;
+    f32_query(it, first, r16, g4, q);
+    stage(tiles[0]);
+    load(it.lo + kKT);  // (past the end: the last row again)
     float m = -INFINITY, l = 0.0f;
     floatx4 o[16];
 #pragma unroll
     for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
-    store(Vc, vscale, 2);
     lds_barrier();
+    int cur = 0;
     for (int k0 = it.lo; k0 < it.hi; k0 += kKT) {
         const bool more = k0 + kKT < it.hi;  // uniform
-        if (more) load(it.K, k0 + kKT);
-        int ko = k_off(r16, g4), vo = v_off(r16, g4);
-        asm volatile("" : "+v"(ko), "+v"(vo));  // formed per tile: kept, the 24 addresses would spill
+        const auto next = [&]() {
+            if (!more) return;
+            stage(tiles[cur ^ 1]);
+            load(k0 + 2 * kKT);
+        };
+        if (wave < 4) next();
         float p[8], f = 1.0f;
         if (live) {
-            floatx4 St[2];
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                floatx4 sa[2], sb[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) sa[e] = sb[e] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    halfx8 k[2];
-#pragma unroll
-                    for (int q = 0; q < 2; ++q)
-                        k[q] = *reinterpret_cast<const halfx8*>(reinterpret_cast<const char*>(Kc[q]) + hf * 16 * 512 + (ko ^ (c << 6)));
-                    sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1], qp[0][c], sb[c & 1], 0, 0, 0);
-                    sb[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0], qp[1][c], sb[c & 1], 0, 0, 0);
-                    sa[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0], qp[0][c], sa[c & 1], 0, 0, 0);
-                }
-                St[hf] = (sb[0] + sb[1]) + (sa[0] + sa[1]);
-            }
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const floatx4 ks = *reinterpret_cast<const floatx4*>(kscale + 16 * hf + 4 * g4);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) p[4 * hf + v] = (St[hf][v] * qscale) * ks[v];
-            }
+            f32_scores(tiles[cur], q, r16, g4, p);
             mask_tail(p, k0, it.hi, g4);
             f = softmax_step(p, m, l);
         }
-        lds_barrier();  // every wave is done with K, every share of V is in
-        if (more) {
-            store(Kc, kscale, 1);
-            load(it.V, k0 + kKT);
-        }
+        if (wave >= 4) next();
         if (live) {
-            rescale(f, g4, o);
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const floatx4 vs = *reinterpret_cast<const floatx4*>(vscale + 16 * hf + 4 * g4);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) p[4 * hf + v] *= vs[v];
-            }
-            float mx = max8(p);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const int e = split_row_exp(mx);
-            halfx8 pp[2];
-            split2_8(p, pow2(e), pp);
-            const float undo = pow2(-e);
-            float er[4];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) er[v] = __shfl(undo, 4 * g4 + v);
-#pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const halfx8 v0 = v_operand<halfx8>(Vc[0], vo ^ (t << 5)), v1 = v_operand<halfx8>(Vc[1], vo ^ (t << 5));
-                floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
-                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp[1], v0, x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp[0], v1, x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp[0], v0, x, 0, 0, 0);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) o[t][v] += x[v] * er[v];
-            }
+            rescale(f, o);
+            f32_output(tiles[cur], p, r16, g4, 0, o);
         }
-        lds_barrier();  // every wave is done with V, every share of the next K is in
-        if (more) store(Vc, vscale, 2);
+        cur ^= 1;
+        lds_barrier();  // every wave is done with this tile, every share of the next one is in
     }
-    store_part(it, first, r16, g4, 0, o, m, l, true);
+    if (live) store_part(it, first, r16, g4, 0, o, m, l, true);
 }
 
-// fp32 caches, narrow: 16 query rows on v_mfma_f32_16x16x4_f32 with K and V straight from memory
-// as its operands, no LDS and no barrier in the loop; the four waves take 16 keys in turn and are
-// merged at the end.
+// Narrow: 16 query rows on v_mfma_f32_16x16x4_f32, K and V straight from memory as its operands, no
+// staging and no barrier in the loop (splitting a tile costs more vector work than its products
+// here: 2.4 us a tile against 1.4). Four waves take 16 keys in turn and are merged at the end; a
+// workgroup's halves have an item each (one without rows only meets the barriers).
 //   S^T = K Q^T: lane (r16, g4) loads dims 16 u + 4 g4 .. + 3 of key r16; the k slot g4 of product
 //         (u, e) is dim 16 u + 4 g4 + e on both sides
-//   O += P V: product (v, t, e) takes the weights of keys 4 g4 + v as they lie and dims
-//         64 t + 4 r16 + e of those keys; lane (r16, g4) ends with dims 64 t + 4 r16 + e of rows 4 g4 + .
+//   O^T += V^T P^T: product (v, t, e) takes the weights of keys 4 g4 + v as they lie and dims
+//         64 t + 4 r16 + e of those keys; lane (r16, g4) ends with dims 64 t + 16 g4 + 4 i + e of
+//         query r16 in o[4 t + e][i]
+// K and V of the wave's next 16 keys are on their way while this 16's products run; the queries are
+// read from LDS as they are needed, which is what leaves registers for both.
 __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*ms)[16], float (*ls)[16]) {
-    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4, wave = tid >> 6;
-    float4 q[16];
-    {
-        const float* src = it.Q + static_cast<int64_t>(min(it.row0 + r16, it.rows - 1)) * kHD + 4 * g4;
-#pragma unroll
-        for (int u = 0; u < 16; ++u) q[u] = *reinterpret_cast<const float4*>(src + 16 * u);
+    const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4, wave = threadIdx.x >> 6 & 3;
+    if (!it.rows) {
+        lds_barrier();
+        lds_barrier();
+        lds_barrier();
+        return;
     }
     const float *K = static_cast<const float*>(it.K), *V = static_cast<const float*>(it.V);
-    float* raw = it.raw && r16 < it.rows ? it.raw + r16 * it.raw_stride : nullptr;
-    float m = -INFINITY, l = 0.0f;
-    floatx4 o[16];
-#pragma unroll
-    for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = it.lo + 16 * wave; k0 < it.hi; k0 += 64) {
-        floatx4 s[4];
-#pragma unroll
-        for (auto& x : s) x = floatx4{0.f, 0.f, 0.f, 0.f};
-        float4 k[16];
+    float4 k[16], vv[4][4];
+    const auto load_k = [&](int k0) {  // keys past the last: it again
         const float* kr = K + static_cast<int64_t>(min(k0 + r16, it.hi - 1)) * kHD + 4 * g4;
 #pragma unroll
         for (int u = 0; u < 16; ++u) k[u] = *reinterpret_cast<const float4*>(kr + 16 * u);
-#pragma unroll
-        for (int u = 0; u < 16; ++u) {
-            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].x, q[u].x, s[0], 0, 0, 0);
-            s[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].y, q[u].y, s[1], 0, 0, 0);
-            s[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].z, q[u].z, s[2], 0, 0, 0);
-            s[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].w, q[u].w, s[3], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // V takes K's registers
-        float4 vv[4][4];
+    };
+    const auto load_v = [&](int k0) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const float* vr = V + static_cast<int64_t>(min(k0 + 4 * g4 + v, it.hi - 1)) * kHD + 4 * r16;
 #pragma unroll
             for (int t = 0; t < 4; ++t) vv[v][t] = *reinterpret_cast<const float4*>(vr + 64 * t);
         }
+    };
+    const int first = it.lo + 16 * wave;
+    // query rows 4 wave .. + 3 into LDS, a row's 16-byte chunks c at c ^ row (rows past the last: it again)
+    float4 qrow[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        qrow[i] = *reinterpret_cast<const float4*>(it.Q + static_cast<int64_t>(min(it.row0 + 4 * wave + i, it.rows - 1)) * kHD + 4 * lane);
+    load_k(first);
+    load_v(first);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(buf + (4 * wave + i) * kHD + 4 * (lane ^ (4 * wave + i))) = qrow[i];
+    lds_barrier();
+    float* raw = it.raw && r16 < it.rows ? it.raw + r16 * it.raw_stride : nullptr;
+    float m = -INFINITY, l = 0.0f;
+    floatx4 o[16];
+#pragma unroll
+    for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
+    int qo = r16 * kHD * 4 + ((g4 ^ r16) << 4);  // bytes; ^ (u << 6): chunk 4 u + g4
+    for (int k0 = first; k0 < it.hi; k0 += 64) {
+        const bool more = k0 + 64 < it.hi;  // uniform per wave
+        asm volatile("" : "+v"(qo));
+        floatx4 s[4];
+#pragma unroll
+        for (auto& x : s) x = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const float4 q = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(buf) + (qo ^ (u << 6)));
+            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].x, q.x, s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].y, q.y, s[1], 0, 0, 0);
+            s[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].z, q.z, s[2], 0, 0, 0);
+            s[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u].w, q.w, s[3], 0, 0, 0);
+        }
+        reads_ahead<16, 1, 4>();
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_k(k0 + 64);
         const floatx4 St = (s[0] + s[1]) + (s[2] + s[3]);
-        if (raw) *reinterpret_cast<floatx4*>(raw + k0 + 4 * g4) = St;
+        if (raw) *reinterpret_cast<floatx4*>(raw + k0 + 4 * g4) = St;  // (rows of raw are whole tiles)
         float p[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) p[v] = k0 + 4 * g4 + v < it.hi ? St[v] : -INFINITY;
-        const float f = softmax_step(p, m, l);
-        rescale(f, g4, o);
+        rescale(softmax_step(p, m, l), o);
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                o[4 * t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[v], vv[v][t].x, o[4 * t], 0, 0, 0);
-                o[4 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[v], vv[v][t].y, o[4 * t + 1], 0, 0, 0);
-                o[4 * t + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[v], vv[v][t].z, o[4 * t + 2], 0, 0, 0);
-                o[4 * t + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[v], vv[v][t].w, o[4 * t + 3], 0, 0, 0);
+                o[4 * t] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[v][t].x, p[v], o[4 * t], 0, 0, 0);
+                o[4 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[v][t].y, p[v], o[4 * t + 1], 0, 0, 0);
+                o[4 * t + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[v][t].z, p[v], o[4 * t + 2], 0, 0, 0);
+                o[4 * t + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[v][t].w, p[v], o[4 * t + 3], 0, 0, 0);
             }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_v(k0 + 64);
     }
     // merge of the waves; one without keys has maximum -inf and weight 0
     if (g4 == 0) {
         ms[wave][r16] = m;
         ls[wave][r16] = l;
     }
-    lds_barrier();
+    lds_barrier();  // (and every wave is done with the queries)
     const float top = fmaxf(fmaxf(ms[0][r16], ms[1][r16]), fmaxf(ms[2][r16], ms[3][r16]));
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * kLog2e);
-    rescale(f, g4, o);
+    rescale(f, o);
     const int n = min(16, it.rows - it.row0);
     if (wave == 0 && g4 == 0 && r16 < n) {
         float sum = 0.0f;
@@ -622,34 +743,44 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
             if (ms[w][r16] != -INFINITY) sum += ls[w][r16] * __builtin_amdgcn_exp2f((ms[w][r16] - top) * kLog2e);
         it.ml[it.row0 + r16] = make_float2(top, sum);
     }
+    // (rows' 16-byte chunks c at c ^ row % 16: the 16 lanes of a store lie on all banks)
+    if (r16 < n) {
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-        if (4 * g4 + v < n) {
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-                *reinterpret_cast<float4*>(buf + (wave * 16 + 4 * g4 + v) * kHD + 64 * t + 4 * r16) =
-                    make_float4(o[4 * t][v], o[4 * t + 1][v], o[4 * t + 2][v], o[4 * t + 3][v]);
-        }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(buf + (wave * 16 + r16) * kHD + 4 * ((16 * t + 4 * g4 + i) ^ r16)) =
+                    make_float4(o[4 * t][i], o[4 * t + 1][i], o[4 * t + 2][i], o[4 * t + 3][i]);
+    }
     lds_barrier();
     for (int r = wave; r < n; r += 4) {
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float4 x = *reinterpret_cast<const float4*>(buf + (w * 16 + r) * kHD + 4 * lane);
+            const float4 x = *reinterpret_cast<const float4*>(buf + (w * 16 + r) * kHD + 4 * (lane ^ r));
             y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
         }
         *reinterpret_cast<float4*>(it.part + static_cast<int64_t>(it.row0 + r) * kHD + 4 * lane) = y;
     }
 }
 
-// fp32 caches: four waves, two workgroups per compute unit.
-__global__ __launch_bounds__(256, 2) void attn_batch_f32_kernel(AttnBatchArgs a) {
-    __shared__ __align__(16) uint4 lds[2][2][1024];
-    __shared__ __align__(16) float small[2][4][16];
+// fp32 caches: eight waves, one workgroup per compute unit: a wide item, or two narrow ones (one
+// where there are no more than compute units).
+__global__ __launch_bounds__(512, 1) void attn_batch_f32_kernel(AttnBatchArgs a, int halves) {
+    __shared__ __align__(16) F32Tile tiles[2];
+    __shared__ float small[2][2][4][16];
+    const int wide = a.plan.block == kBatchNarrow ? 0 : prefix_items(a.plan, a.NKV);
     Item it;
-    if (!item_of(a, it)) return;
-    if (it.narrow) f32_narrow(it, reinterpret_cast<float*>(lds), small[0], small[1]);
-    else f32_wide(it, lds[0], lds[1], &small[0][0][0], &small[1][0][0]);
+    if (static_cast<int>(blockIdx.x) < wide) {
+        if (item_of(a, blockIdx.x, it)) f32_wide(it, tiles);
+        return;
+    }
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int i = wide + halves * (blockIdx.x - wide);
+    const bool other = (half ^ 1) < halves && item_of(a, i + (half ^ 1), it);
+    const bool mine = half < halves && item_of(a, i + half, it);
+    if (!mine) it.rows = 0;
+    if (mine || other) f32_narrow(it, reinterpret_cast<float*>(&tiles[half]), small[half][0], small[half][1]);
 }
 
 constexpr int kCombWaves = 8;
@@ -776,9 +907,14 @@ void attn_batch_carve(AttnBatchArgs& a, float* ws) {
 
 hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s) {
     klaunch(attn_batch_prep_kernel, dim3((a.NQ + a.NKV + 3) / 4, a.B), 256, 0, s, a);
-    const uint32_t prefix = (a.plan.pieces * a.NKV + 7) / 8 * 8 * a.plan.nblk, own = a.B * a.NKV * a.plan.own;
-    if (a.kv_bf16) klaunch(attn_batch_bf16_kernel, dim3(prefix + own), 256, 0, s, a);
-    else klaunch(attn_batch_f32_kernel, dim3(prefix + own), 256, 0, s, a);
+    const uint32_t prefix = prefix_items(a.plan, a.NKV), own = a.B * a.NKV * a.plan.own;
+    if (a.kv_bf16) {
+        klaunch(attn_batch_bf16_kernel, dim3(prefix + own), 256, 0, s, a);
+    } else {
+        const uint32_t wide = a.plan.block == kBatchNarrow ? 0 : prefix;
+        const int narrow = prefix - wide + own, halves = narrow > device_cu_count() ? 2 : 1;
+        klaunch(attn_batch_f32_kernel, dim3(wide + (narrow + halves - 1) / halves), 512, 0, s, a, halves);
+    }
     const uint32_t scores = a.own_score ? static_cast<uint32_t>((a.cap + 511) / 512) * a.B * a.NKV : 0;
     klaunch(attn_batch_combine_kernel, dim3(a.B * a.NQ + scores), kCombWaves * 64, (a.plan.pieces + a.plan.own) * 4, s, a);
     return hipGetLastError();

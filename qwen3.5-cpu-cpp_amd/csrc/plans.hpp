@@ -208,16 +208,14 @@ struct AttnBatchPlan {
     int block, nblk, pieces, pkeys;  // of the prefix (0 pieces: none)
     int own, okeys;                  // of an own cache
 };
-constexpr int kBatchNarrow = 16;                                             // query rows of a narrow workgroup
-constexpr int kBatchWide = 64;                                               // of a wide one
-constexpr int batch_unit(bool kv_bf16) { return kv_bf16 ? 32 : 64; }         // keys pieces are multiples of
-constexpr int batch_most_narrow(bool kv_bf16) { return kv_bf16 ? 16 : 32; }  // rows still taken in blocks of 16
+constexpr int kBatchNarrow = 16;                                           // query rows of a narrow workgroup
+constexpr int batch_wide(bool kv_bf16) { return kv_bf16 ? 64 : 128; }      // of a wide one
 inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
-    const int64_t rows = static_cast<int64_t>(B) * GRP, unit = batch_unit(kv_bf16), slots = 2 * n_cu;
+    const int64_t rows = static_cast<int64_t>(B) * GRP, unit = 32, slots = kv_bf16 ? 2 * n_cu : n_cu;
     AttnBatchPlan p{0, 0, 0, 0, 1, 0};
     if (P > 0) {
-        p.block = rows <= batch_most_narrow(kv_bf16) ? kBatchNarrow : kBatchWide;
+        p.block = rows <= kBatchNarrow ? kBatchNarrow : batch_wide(kv_bf16);
         p.nblk = static_cast<int>(up(rows, p.block));
         const int64_t n = std::min<int64_t>(up(P, 2 * unit), std::max<int64_t>(1, slots / (static_cast<int64_t>(NKV) * p.nblk)));
         p.pkeys = static_cast<int>(up(up(P, n), unit) * unit);
