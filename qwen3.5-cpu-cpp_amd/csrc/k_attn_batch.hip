@@ -132,10 +132,9 @@ __device__ __forceinline__ bool item_of(const AttnBatchArgs& a, int i, Item& it)
         return true;
     }
     i -= prefix;
-    // first pieces first: later ones may be empty, and would leave whole XCDs idle side by side
-    const int piece = i / (a.B * a.NKV);
-    if (piece >= a.plan.own) return false;
-    i -= piece * (a.B * a.NKV);
+    // first pieces first, as later ones may be empty, and each piece of a cache another XCD's
+    const int pairs_own = a.B * a.NKV, piece = i / pairs_own;
+    i = (i - piece * pairs_own + piece) % pairs_own;
     const int kh = i % a.NKV, b = i / a.NKV;
     const int slot = new_slot(a, b);
     const int64_t lo = static_cast<int64_t>(piece) * a.plan.okeys;
@@ -641,8 +640,7 @@ __device__ __forceinline__ void f32_wide(const Item& it, F32Tile* tiles) {
 
 // Narrow: 16 query rows on v_mfma_f32_16x16x4_f32, K and V straight from memory as its operands, no
 // staging and no barrier in the loop (splitting a tile costs more vector work than its products
-// here: 2.4 us a tile against 1.4). Four waves take 16 keys in turn and are merged at the end; a
-// workgroup's halves have an item each (one without rows only meets the barriers).
+// here: 2.4 us a tile against 1.4). The eight waves take 16 keys in turn and are merged at the end.
 //   S^T = K Q^T: lane (r16, g4) loads dims 16 u + 4 g4 .. + 3 of key r16; the k slot g4 of product
 //         (u, e) is dim 16 u + 4 g4 + e on both sides
 //   O^T += V^T P^T: product (v, t, e) takes the weights of keys 4 g4 + v as they lie and dims
@@ -651,13 +649,7 @@ __device__ __forceinline__ void f32_wide(const Item& it, F32Tile* tiles) {
 // K and V of the wave's next 16 keys are on their way while this 16's products run; the queries are
 // read from LDS as they are needed, which is what leaves registers for both.
 __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*ms)[16], float (*ls)[16]) {
-    const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4, wave = threadIdx.x >> 6 & 3;
-    if (!it.rows) {
-        lds_barrier();
-        lds_barrier();
-        lds_barrier();
-        return;
-    }
+    const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4, wave = threadIdx.x >> 6;
     const float *K = static_cast<const float*>(it.K), *V = static_cast<const float*>(it.V);
     float4 k[16], vv[4][4];
     const auto load_k = [&](int k0) {  // keys past the last: it again
@@ -674,16 +666,16 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
         }
     };
     const int first = it.lo + 16 * wave;
-    // query rows 4 wave .. + 3 into LDS, a row's 16-byte chunks c at c ^ row (rows past the last: it again)
-    float4 qrow[4];
+    // query rows 2 wave, + 1 into LDS, a row's 16-byte chunks c at c ^ row (rows past the last: it again)
+    float4 qrow[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        qrow[i] = *reinterpret_cast<const float4*>(it.Q + static_cast<int64_t>(min(it.row0 + 4 * wave + i, it.rows - 1)) * kHD + 4 * lane);
+    for (int i = 0; i < 2; ++i)
+        qrow[i] = *reinterpret_cast<const float4*>(it.Q + static_cast<int64_t>(min(it.row0 + 2 * wave + i, it.rows - 1)) * kHD + 4 * lane);
     load_k(first);
     load_v(first);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4*>(buf + (4 * wave + i) * kHD + 4 * (lane ^ (4 * wave + i))) = qrow[i];
+    for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float4*>(buf + (2 * wave + i) * kHD + 4 * (lane ^ (2 * wave + i))) = qrow[i];
     lds_barrier();
     float* raw = it.raw && r16 < it.rows ? it.raw + r16 * it.raw_stride : nullptr;
     float m = -INFINITY, l = 0.0f;
@@ -691,8 +683,8 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
 #pragma unroll
     for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
     int qo = r16 * kHD * 4 + ((g4 ^ r16) << 4);  // bytes; ^ (u << 6): chunk 4 u + g4
-    for (int k0 = first; k0 < it.hi; k0 += 64) {
-        const bool more = k0 + 64 < it.hi;  // uniform per wave
+    for (int k0 = first; k0 < it.hi; k0 += 128) {
+        const bool more = k0 + 128 < it.hi;  // uniform per wave
         asm volatile("" : "+v"(qo));
         floatx4 s[4];
 #pragma unroll
@@ -707,7 +699,7 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
         }
         reads_ahead<16, 1, 4>();
         __builtin_amdgcn_sched_barrier(0);
-        if (more) load_k(k0 + 64);
+        if (more) load_k(k0 + 128);
         const floatx4 St = (s[0] + s[1]) + (s[2] + s[3]);
         if (raw) *reinterpret_cast<floatx4*>(raw + k0 + 4 * g4) = St;  // (rows of raw are whole tiles)
         float p[4];
@@ -724,7 +716,7 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
                 o[4 * t + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[v][t].w, p[v], o[4 * t + 3], 0, 0, 0);
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (more) load_v(k0 + 64);
+        if (more) load_v(k0 + 128);
     }
     // merge of the waves; one without keys has maximum -inf and weight 0
     if (g4 == 0) {
@@ -732,14 +724,16 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
         ls[wave][r16] = l;
     }
     lds_barrier();  // (and every wave is done with the queries)
-    const float top = fmaxf(fmaxf(ms[0][r16], ms[1][r16]), fmaxf(ms[2][r16], ms[3][r16]));
+    float top = ms[0][r16];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) top = fmaxf(top, ms[w][r16]);
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * kLog2e);
     rescale(f, o);
     const int n = min(16, it.rows - it.row0);
     if (wave == 0 && g4 == 0 && r16 < n) {
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 8; ++w)
             if (ms[w][r16] != -INFINITY) sum += ls[w][r16] * __builtin_amdgcn_exp2f((ms[w][r16] - top) * kLog2e);
         it.ml[it.row0 + r16] = make_float2(top, sum);
     }
@@ -753,10 +747,10 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
                     make_float4(o[4 * t][i], o[4 * t + 1][i], o[4 * t + 2][i], o[4 * t + 3][i]);
     }
     lds_barrier();
-    for (int r = wave; r < n; r += 4) {
+    for (int r = wave; r < n; r += 8) {
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 8; ++w) {
             const float4 x = *reinterpret_cast<const float4*>(buf + (w * 16 + r) * kHD + 4 * (lane ^ r));
             y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
         }
@@ -764,23 +758,14 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
     }
 }
 
-// fp32 caches: eight waves, one workgroup per compute unit: a wide item, or two narrow ones (one
-// where there are no more than compute units).
-__global__ __launch_bounds__(512, 1) void attn_batch_f32_kernel(AttnBatchArgs a, int halves) {
+// fp32 caches: eight waves, one workgroup per compute unit.
+__global__ __launch_bounds__(512, 1) void attn_batch_f32_kernel(AttnBatchArgs a) {
     __shared__ __align__(16) F32Tile tiles[2];
-    __shared__ float small[2][2][4][16];
-    const int wide = a.plan.block == kBatchNarrow ? 0 : prefix_items(a.plan, a.NKV);
+    __shared__ float small[2][8][16];
     Item it;
-    if (static_cast<int>(blockIdx.x) < wide) {
-        if (item_of(a, blockIdx.x, it)) f32_wide(it, tiles);
-        return;
-    }
-    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int i = wide + halves * (blockIdx.x - wide);
-    const bool other = (half ^ 1) < halves && item_of(a, i + (half ^ 1), it);
-    const bool mine = half < halves && item_of(a, i + half, it);
-    if (!mine) it.rows = 0;
-    if (mine || other) f32_narrow(it, reinterpret_cast<float*>(&tiles[half]), small[half][0], small[half][1]);
+    if (!item_of(a, blockIdx.x, it)) return;
+    if (it.narrow) f32_narrow(it, reinterpret_cast<float*>(tiles), small[0], small[1]);
+    else f32_wide(it, tiles);
 }
 
 constexpr int kCombWaves = 8;
@@ -908,13 +893,8 @@ void attn_batch_carve(AttnBatchArgs& a, float* ws) {
 hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s) {
     klaunch(attn_batch_prep_kernel, dim3((a.NQ + a.NKV + 3) / 4, a.B), 256, 0, s, a);
     const uint32_t prefix = prefix_items(a.plan, a.NKV), own = a.B * a.NKV * a.plan.own;
-    if (a.kv_bf16) {
-        klaunch(attn_batch_bf16_kernel, dim3(prefix + own), 256, 0, s, a);
-    } else {
-        const uint32_t wide = a.plan.block == kBatchNarrow ? 0 : prefix;
-        const int narrow = prefix - wide + own, halves = narrow > device_cu_count() ? 2 : 1;
-        klaunch(attn_batch_f32_kernel, dim3(wide + (narrow + halves - 1) / halves), 512, 0, s, a, halves);
-    }
+    if (a.kv_bf16) klaunch(attn_batch_bf16_kernel, dim3(prefix + own), 256, 0, s, a);
+    else klaunch(attn_batch_f32_kernel, dim3(prefix + own), 512, 0, s, a);
     const uint32_t scores = a.own_score ? static_cast<uint32_t>((a.cap + 511) / 512) * a.B * a.NKV : 0;
     klaunch(attn_batch_combine_kernel, dim3(a.B * a.NQ + scores), kCombWaves * 64, (a.plan.pieces + a.plan.own) * 4, s, a);
     return hipGetLastError();

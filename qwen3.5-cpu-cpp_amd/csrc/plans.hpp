@@ -210,19 +210,44 @@ struct AttnBatchPlan {
 };
 constexpr int kBatchNarrow = 16;                                           // query rows of a narrow workgroup
 constexpr int batch_wide(bool kv_bf16) { return kv_bf16 ? 64 : 128; }      // of a wide one
+// Workgroups of the prefix are dealt to the 8 XCDs by their piece and kv head (the row blocks of one
+// piece together, for their L2). Times in us on 256 compute units: a tile of 32 keys takes a bf16
+// workgroup 1.65 alone on its compute unit and 2.7 beside another (64 rows; two fit), an fp32 one 4.0
+// (128 rows; one fits); a partial output costs its bytes at 2.2 TB/s, written and merged. Of the
+// piece lengths the fastest by that is taken: 48 sequences of 16 / 2 heads after 30001 bf16 positions,
+// attention and merge with pieces of 256 keys 99 us, 512 83, 768 79, 1504 88; fp32 ones, 512 146, 704
+// 183 (a second round of workgroups), 800 116, 1024 131. With 16 rows or fewer the loads bound
+// the time, and pieces are made for 7/8 of the compute units: 2 after 30001 fp32 ones, 128 keys 46
+// us, 256 35, 512 44.
+// Own caches are taken to be half full: pieces are made for 3/4 of the compute units (bf16: 7/6) to
+// have one that is not empty. 48 caches of 1000 fp32 rows: pieces of 128 39 us, 320 28, 512 36;
+// 48 of 2000 bf16 ones: 64 35, 320 26, 512 32.
 inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
-    const int64_t rows = static_cast<int64_t>(B) * GRP, unit = 32, slots = kv_bf16 ? 2 * n_cu : n_cu;
-    AttnBatchPlan p{0, 0, 0, 0, 1, 0};
+    const int64_t rows = static_cast<int64_t>(B) * GRP, pairs = static_cast<int64_t>(B) * NKV, most = 2 * n_cu;
+    AttnBatchPlan p{};
     if (P > 0) {
+        const int64_t tiles = up(P, 32);
         p.block = rows <= kBatchNarrow ? kBatchNarrow : batch_wide(kv_bf16);
         p.nblk = static_cast<int>(up(rows, p.block));
-        const int64_t n = std::min<int64_t>(up(P, 2 * unit), std::max<int64_t>(1, slots / (static_cast<int64_t>(NKV) * p.nblk)));
-        p.pkeys = static_cast<int>(up(up(P, n), unit) * unit);
+        int64_t c = std::max<int64_t>(2, up(tiles * NKV, std::max(1, n_cu * 7 / 8)));
+        if (p.block != kBatchNarrow) {
+            const int64_t cu = std::max(1, n_cu / 8), slots = kv_bf16 ? 2 * cu : cu;
+            const double alone = kv_bf16 ? 1.65 : 4.0, full = kv_bf16 ? 2.7 : 4.0;
+            double best = 1e300;
+            for (int64_t n = 1; n <= std::min(up(tiles, 2), most); n += 1 + n / 16) {
+                const int64_t len = up(tiles, n), wgs = up(up(tiles, len) * NKV, 8) * p.nblk, rest = wgs % slots;
+                const double t = len * (wgs / slots * full + (rest > cu ? full : rest ? alone : 0.0)) +
+                                 up(tiles, len) * NKV * rows * 1024 / 2.2e6;
+                if (t < best) best = t, c = len;
+            }
+        }
+        p.pkeys = static_cast<int>(32 * std::max(c, up(tiles, most)));
         p.pieces = static_cast<int>(up(P, p.pkeys));
     }
-    const int64_t n = std::min<int64_t>(up(cap, 2 * unit), std::max<int64_t>(1, slots / (static_cast<int64_t>(B) * NKV)));
-    p.okeys = static_cast<int>(up(up(cap, n), unit) * unit);
+    const double share = (kv_bf16 ? n_cu * 7.0 / 6.0 : n_cu * 0.75) / pairs - 0.5;  // pieces of a half full cache
+    const int64_t len = share > 0.5 ? static_cast<int64_t>(cap / (2.0 * share)) : cap;
+    p.okeys = static_cast<int>(32 * up(std::max<int64_t>(std::min(len, cap), std::min<int64_t>(cap, 64)), 32));
     p.own = static_cast<int>(up(cap, p.okeys));
     return p;
 }
