@@ -33,9 +33,21 @@ __device__ __forceinline__ void rows_of(const GdnBatchArgs& a, int b, int& first
     n = a.row0 ? max(min(a.row0[b + 1], a.rows) - first, 0) : 1;
 }
 
+// A channel of the ring after n tokens: slot i receives the last input of a position equal to i mod 4,
+// from this call's rows or, where the batch is forked, from the ring that was read.
+__device__ __forceinline__ void store_ring(const GdnBatchArgs& a, const float* rin, float* rout, uint32_t pos, int row, int n,
+                                           bool fork, int ch, int CONV) {
+#pragma unroll
+    for (int i = 1; i <= 4; ++i) {  // the i-th input from the end
+        const int64_t o = static_cast<int64_t>((pos + n - i) & 3) * CONV + ch;
+        if (i <= n) rout[o] = a.qkv[static_cast<int64_t>(row + n - i) * a.ld_qkv + ch];
+        else if (fork) rout[o] = rin[o];
+    }
+}
+
 // ONE: a token per sequence (row0 null); the ring is written here then, by the workgroup that
 // owns the channel. With more tokens a later token's slot is one that another workgroup may
-// still have to read, so gdn_batch_ring_kernel writes it afterwards.
+// still have to read where v-heads share a k-head: gdn_batch_ring_kernel writes it afterwards.
 template <bool ONE>
 __global__ __launch_bounds__(256) void gdn_batch_kernel(GdnBatchArgs a) {
     constexpr int TC = ONE ? 1 : kTok;
@@ -75,21 +87,43 @@ __global__ __launch_bounds__(256) void gdn_batch_kernel(GdnBatchArgs a) {
     for (int i = 0; i < 16; ++i) s[i] = *reinterpret_cast<const float4*>(Sin + i * kD);
     const float decay = -expf(a.A_log[vh]), dt = a.dt_bias[vh];
 
+    // the rows of a pass are requested together: tokens past the last are the last again
+    constexpr int ZT = (TC + 3) / 4;
     for (int t0 = 0; t0 < n; t0 += TC) {
         const int m = min(TC, n - t0);
+        float x[2][TC], z[ZT][2], ab[2];
+#pragma unroll
+        for (int t = 0; t < TC; ++t) {
+            const float* qkv = a.qkv + static_cast<int64_t>(row + t0 + min(t, m - 1)) * a.ld_qkv;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) x[c][t] = qkv[ch[c]];
+        }
+        {
+            const int64_t r = static_cast<int64_t>(row + t0 + min(tid, m - 1)) * a.ld_ba + vh;
+            ab[0] = a.a[r];
+            ab[1] = a.b[r];
+        }
+        if (a.norm_w) {
+#pragma unroll
+            for (int i = 0; i < ZT; ++i) {
+                const float* zr = a.z + static_cast<int64_t>(row + t0 + min(wave + 4 * i, m - 1)) * a.ld_z + vh * kD;
+                z[i][0] = zr[lane];
+                z[i][1] = zr[lane + 64];
+            }
+        }
         if (t0) __syncthreads();
-        for (int t = 0; t < m; ++t) {
-            const float* qkv = a.qkv + (row + t0 + t) * a.ld_qkv;
+#pragma unroll
+        for (int t = 0; t < TC; ++t) {
+            if (t >= m) break;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float x = qkv[ch[c]];
                 float acc = 0.0f;
                 acc += w[c].x * win[c][0];
                 acc += w[c].y * win[c][1];
                 acc += w[c].z * win[c][2];
-                acc += w[c].w * x;
+                acc += w[c].w * x[c][t];
                 if (ONE && (c ? tid < kD : vh % rep == 0)) {
-                    rout[static_cast<int64_t>(pos & 3) * CONV + ch[c]] = x;
+                    rout[static_cast<int64_t>(pos & 3) * CONV + ch[c]] = x[c][t];
                     if (fork) {
 #pragma unroll
                         for (int i = 0; i < 3; ++i) rout[static_cast<int64_t>((pos + 1 + i) & 3) * CONV + ch[c]] = win[c][i];
@@ -97,14 +131,13 @@ __global__ __launch_bounds__(256) void gdn_batch_kernel(GdnBatchArgs a) {
                 }
                 win[c][0] = win[c][1];
                 win[c][1] = win[c][2];
-                win[c][2] = x;
+                win[c][2] = x[c][t];
                 if (c == 0 || tid < kD) x_s[t][c ? 2 * kD + tid : tid] = silu_f(acc);
             }
         }
         if (tid < m) {
-            const int64_t r = (row + t0 + tid) * a.ld_ba + vh;
-            ab_s[tid][0] = expf(decay * softplus_f(a.a[r] + dt));
-            ab_s[tid][1] = sigmoid_f(a.b[r]);
+            ab_s[tid][0] = expf(decay * softplus_f(ab[0] + dt));
+            ab_s[tid][1] = sigmoid_f(ab[1]);
         }
         __syncthreads();
         // l2 norms (eps 1e-6, sums of squares in double) of q and k; q also scaled by DK^-1/2
@@ -150,16 +183,17 @@ __global__ __launch_bounds__(256) void gdn_batch_kernel(GdnBatchArgs a) {
         }
         __syncthreads();
         // readout, with the gated norm (src/forward_pass.cpp:86-93) where there is one
-        for (int t = wave; t < m; t += 4) {
-            const int64_t r = row + t0 + t;
+#pragma unroll
+        for (int i = 0; i < ZT; ++i) {
+            const int t = wave + 4 * i;
+            if (t >= m) break;
             float o0 = o_s[t][lane], o1 = o_s[t][lane + 64];
-            float* out = a.out + r * (a.VH * kD) + vh * kD;
+            float* out = a.out + static_cast<int64_t>(row + t0 + t) * (a.VH * kD) + vh * kD;
             if (a.norm_w) {
                 const double ss = wave_sum(static_cast<double>(o0) * o0 + static_cast<double>(o1) * o1);
                 const float inv = 1.0f / sqrtf(static_cast<float>(ss / kD) + a.eps);
-                const float* z = a.z + r * a.ld_z + vh * kD;
-                o0 = a.norm_w[lane] * (o0 * inv) * silu_f(z[lane]);
-                o1 = a.norm_w[lane + 64] * (o1 * inv) * silu_f(z[lane + 64]);
+                o0 = a.norm_w[lane] * (o0 * inv) * silu_f(z[i][0]);
+                o1 = a.norm_w[lane + 64] * (o1 * inv) * silu_f(z[i][1]);
             }
             out[lane] = o0;
             out[lane + 64] = o1;
@@ -168,26 +202,20 @@ __global__ __launch_bounds__(256) void gdn_batch_kernel(GdnBatchArgs a) {
     float* Sout = a.state + b * a.s_state + soff;
 #pragma unroll
     for (int i = 0; i < 16; ++i) *reinterpret_cast<float4*>(Sout + i * kD) = s[i];
+    if (!ONE && (fork || rep == 1)) {  // no other workgroup reads what is written here
+        if (vh % rep == 0) store_ring(a, rin, rout, pos, row, n, fork, ch[0], CONV);
+        if (tid < kD) store_ring(a, rin, rout, pos, row, n, fork, ch[1], CONV);
+    }
 }
 
-// grid (CONV / 256, B): slot i of the ring receives the last input of a position equal to i
-// mod 4, from this call's rows or, where the batch is forked, from the ring that was read.
+// grid (CONV / 256, B): the rings, in place, where v-heads share a k-head's channels.
 __global__ __launch_bounds__(256) void gdn_batch_ring_kernel(GdnBatchArgs a) {
     const int b = blockIdx.y, CONV = (2 * a.KH + a.VH) * kD, ch = blockIdx.x * 256 + threadIdx.x;
-    const int pos = a.pos[b];
-    if (pos < 0 || ch >= CONV) return;
+    if (a.pos[b] < 0 || ch >= CONV) return;
     int row, n;
     rows_of(a, b, row, n);
-    const float* rin = a.ring_in + b * a.s_ring_in;
-    float* rout = a.ring + b * a.s_ring;
-    const bool fork = a.ring_in != a.ring;
-#pragma unroll
-    for (int i = 1; i <= 4; ++i) {  // the i-th input from the end
-        const int slot = (pos & 3) + (n & 3) + 4 - i;
-        const int64_t o = static_cast<int64_t>(slot & 3) * CONV + ch;
-        if (i <= n) rout[o] = a.qkv[static_cast<int64_t>(row + n - i) * a.ld_qkv + ch];
-        else if (fork) rout[o] = rin[o];
-    }
+    float* ring = a.ring + b * a.s_ring;
+    store_ring(a, ring, ring, a.pos[b], row, n, false, ch, CONV);
 }
 
 }  // namespace
@@ -198,7 +226,8 @@ hipError_t launch_gdn_batch(const GdnBatchArgs& a, hipStream_t s) {
         klaunch(gdn_batch_kernel<true>, grid, 256, 0, s, a);
     } else {
         klaunch(gdn_batch_kernel<false>, grid, 256, 0, s, a);
-        klaunch(gdn_batch_ring_kernel, dim3(((2 * a.KH + a.VH) * kD + 255) / 256, a.B), 256, 0, s, a);
+        if (a.state_in == a.state && a.VH != a.KH)
+            klaunch(gdn_batch_ring_kernel, dim3(((2 * a.KH + a.VH) * kD + 255) / 256, a.B), 256, 0, s, a);
     }
     return hipGetLastError();
 }
