@@ -2,6 +2,8 @@
 // and each sequence's own cache, in three launches: the queries and the appended rows
 // (prep), partial outputs over pieces of the keys (attend), and their merge with the gate,
 // which also adds the softmax weights to the own rows' scores (combine).
+#include <cmath>
+
 #include "dev_common.hpp"
 #include "launch.hpp"
 
@@ -22,30 +24,34 @@ __device__ __forceinline__ int new_slot(const AttnBatchArgs& a, int b) {
 // stride of the rows of raw scores: whole tiles
 __host__ __device__ inline int64_t raw_stride(int64_t cap) { return (cap + 31) / 32 * 32; }
 
+// theta^(-2i / ROT), formed on the host: 32 double-precision powers cost the kernel 1 us
+struct RopeFreq {
+    double f[kHD / 2];
+};
+
 // grid ((NQ + NKV) / 4, B), a wave per row: rmsnorm (1 + w) + RoPE of a query row -> Qa, or of the
 // new key row -> own cache, with its value row. Angles in double, one lane each.
-__global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a) {
+__global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a, RopeFreq freq) {
     const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 4 + wave;
     __shared__ __align__(16) float buf[4][kHD];
     __shared__ float cs[2][kHD / 2];
-    const int slot = new_slot(a, b);
     const bool is_q = r < a.NQ, there = r < a.NQ + a.NKV;
     const int kh = is_q ? r / a.GRP : min(r - a.NQ, a.NKV - 1);
-    float* q = a.Qa + ((static_cast<int64_t>(kh) * a.B + b) * a.GRP + (r - kh * a.GRP)) * kHD + 4 * lane;
-    if (slot < 0) {
-        if (is_q) *reinterpret_cast<float4*>(q) = make_float4(0.f, 0.f, 0.f, 0.f);
-        return;
-    }
+    // (requested before the lengths are known: rows of empty places are there to be read)
     const int64_t bk = static_cast<int64_t>(b) * a.NKV + kh;
     const float* src = is_q ? a.qg + (static_cast<int64_t>(b) * a.NQ + r) * 2 * kHD : a.k_new + bk * kHD;
     const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
     const float4 w = *reinterpret_cast<const float4*>((is_q ? a.q_norm : a.k_norm) + 4 * lane);
     const float4 v = *reinterpret_cast<const float4*>(a.v_new + bk * kHD + 4 * lane);
-    const int half = a.ROT / 2, pos = a.pos[b];
+    const int half = a.ROT / 2, pos = a.pos[b], slot = new_slot(a, b);
+    float* q = a.Qa + ((static_cast<int64_t>(kh) * a.B + b) * a.GRP + (r - kh * a.GRP)) * kHD + 4 * lane;
+    if (slot < 0) {
+        if (is_q) *reinterpret_cast<float4*>(q) = make_float4(0.f, 0.f, 0.f, 0.f);
+        return;
+    }
     for (int i = threadIdx.x; i < half; i += 256) {
-        const double ang = static_cast<double>(pos) * pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
         double sn, cn;
-        sincos(ang, &sn, &cn);
+        sincos(static_cast<double>(pos) * freq.f[i], &sn, &cn);
         cs[0][i] = static_cast<float>(cn);
         cs[1][i] = static_cast<float>(sn);
     }
@@ -891,7 +897,16 @@ void attn_batch_carve(AttnBatchArgs& a, float* ws) {
 }
 
 hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s) {
-    klaunch(attn_batch_prep_kernel, dim3((a.NQ + a.NKV + 3) / 4, a.B), 256, 0, s, a);
+    // a function of theta and the width alone, kept for the next call of this host thread
+    static thread_local RopeFreq freq;
+    static thread_local double theta = 0.0;
+    static thread_local int rot = -1;
+    if (theta != a.theta || rot != a.ROT) {
+        for (int i = 0; i < a.ROT / 2; ++i) freq.f[i] = std::pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
+        theta = a.theta;
+        rot = a.ROT;
+    }
+    klaunch(attn_batch_prep_kernel, dim3((a.NQ + a.NKV + 3) / 4, a.B), 256, 0, s, a, freq);
     const uint32_t prefix = prefix_items(a.plan, a.NKV), own = a.B * a.NKV * a.plan.own;
     if (a.kv_bf16) klaunch(attn_batch_bf16_kernel, dim3(prefix + own), 256, 0, s, a);
     else klaunch(attn_batch_f32_kernel, dim3(prefix + own), 512, 0, s, a);
