@@ -24,13 +24,49 @@ __device__ __forceinline__ int new_slot(const AttnBatchArgs& a, int b) {
 // stride of the rows of raw scores: whole tiles
 __host__ __device__ inline int64_t raw_stride(int64_t cap) { return (cap + 31) / 32 * 32; }
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+// 2^e
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+// the power of two that brings a largest magnitude (its bits) into [2^14, 2^15), as far as 2^+-100
+__device__ __forceinline__ int row_exp(uint32_t bits) { return min(max(141 - static_cast<int>(bits >> 23), -100), 100); }
+
 // theta^(-2i / ROT), formed on the host: 32 double-precision powers cost the kernel 1 us
 struct RopeFreq {
     double f[kHD / 2];
 };
 
-// grid ((NQ + NKV) / 4, B), a wave per row: rmsnorm (1 + w) + RoPE of a query row -> Qa, or of the
-// new key row -> own cache, with its value row. Angles in double, one lane each.
+// Dims 4 lane .. + 3 of query row `row`.
+__device__ __forceinline__ void store_query(const AttnBatchArgs& a, int64_t row, int lane, float4 y) {
+    if (a.kv_bf16) {  // three exact bf16 parts, [row][3][HD]
+        uint32_t lo[3], hi[3];
+        split3_pair(y.x, y.y, lo[0], lo[1], lo[2]);
+        split3_pair(y.z, y.w, hi[0], hi[1], hi[2]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) static_cast<uint2*>(a.Qs)[(row * 3 + q) * 64 + lane] = make_uint2(lo[q], hi[q]);
+        return;
+    }
+    *reinterpret_cast<float4*>(a.Qa + row * kHD + 4 * lane) = y;
+    if (!a.Qs) return;
+    // two fp16 parts of the row scaled by a power of two, [row][2][HD]
+    const float mx = wave_max(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+    const int e = row_exp(__float_as_uint(mx));
+    uint2 h, l;
+    split2h_pair(y.x * pow2(e), y.y * pow2(e), h.x, l.x);
+    split2h_pair(y.z * pow2(e), y.w * pow2(e), h.y, l.y);
+    static_cast<uint2*>(a.Qs)[(row * 2 + 0) * 64 + lane] = h;
+    static_cast<uint2*>(a.Qs)[(row * 2 + 1) * 64 + lane] = l;
+    if (lane == 0) a.Qscale[row] = pow2(-e);
+}
+
+// grid ((NQ + NKV) / 4, B), a wave per row: rmsnorm (1 + w) + RoPE of a query row, or of the new key
+// row -> own cache, with its value row. Angles in double, one lane each. Query rows, times
+// 1 / sqrt(HD), are stored as the attention reads them: as they are (Qa) where it multiplies in
+// fp32, and split into the parts of its 16-bit products (Qs), which each workgroup would split again.
 __global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a, RopeFreq freq) {
     const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 4 + wave;
     __shared__ __align__(16) float buf[4][kHD];
@@ -44,9 +80,9 @@ __global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a, R
     const float4 w = *reinterpret_cast<const float4*>((is_q ? a.q_norm : a.k_norm) + 4 * lane);
     const float4 v = *reinterpret_cast<const float4*>(a.v_new + bk * kHD + 4 * lane);
     const int half = a.ROT / 2, pos = a.pos[b], slot = new_slot(a, b);
-    float* q = a.Qa + ((static_cast<int64_t>(kh) * a.B + b) * a.GRP + (r - kh * a.GRP)) * kHD + 4 * lane;
+    const int64_t qrow = (static_cast<int64_t>(kh) * a.B + b) * a.GRP + (r - kh * a.GRP);
     if (slot < 0) {
-        if (is_q) *reinterpret_cast<float4*>(q) = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (is_q) store_query(a, qrow, lane, make_float4(0.f, 0.f, 0.f, 0.f));
         return;
     }
     for (int i = threadIdx.x; i < half; i += 256) {
@@ -72,7 +108,7 @@ __global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a, R
         }
     }
     if (is_q) {  // scaled by 1 / sqrt(HD), exact
-        *reinterpret_cast<float4*>(q) = make_float4(y[0] * 0.0625f, y[1] * 0.0625f, y[2] * 0.0625f, y[3] * 0.0625f);
+        store_query(a, qrow, lane, make_float4(y[0] * 0.0625f, y[1] * 0.0625f, y[2] * 0.0625f, y[3] * 0.0625f));
         return;
     }
     const int64_t row = bk * a.cap + slot;
@@ -87,10 +123,6 @@ __global__ __launch_bounds__(256) void attn_batch_prep_kernel(AttnBatchArgs a, R
     if (a.own_pos && lane == 0) a.own_pos[row] = pos;
 }
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef short i16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kKT = 32;         // keys per tile of the 16-bit matrix products
 constexpr int kWaitVm = 0x0f70; // s_waitcnt: vector memory, nothing outstanding
@@ -99,7 +131,7 @@ constexpr int kWaitVm = 0x0f70; // s_waitcnt: vector memory, nothing outstanding
 // cache, and where its partial result goes.
 struct Item {
 
-    const float* Q;         // query rows [rows][HD]
+    int64_t q0;             // first query row, of all
     int rows, row0;
     int lo, hi;
     const void *K, *V;      // row 0 of the cache
@@ -124,7 +156,7 @@ __device__ __forceinline__ bool item_of(const AttnBatchArgs& a, int i, Item& it)
         const int piece = pair / a.NKV, kh = pair - piece * a.NKV;
         it.rows = a.B * a.GRP;
         it.row0 = blk * a.plan.block;
-        it.Q = a.Qa + static_cast<int64_t>(kh) * it.rows * kHD;
+        it.q0 = static_cast<int64_t>(kh) * it.rows;
         it.lo = piece * a.plan.pkeys;
         it.hi = static_cast<int>(min(a.P, static_cast<int64_t>(it.lo) + a.plan.pkeys));
         it.K = static_cast<const char*>(a.k_prefix) + kh * a.prefix_cap * row_bytes;
@@ -148,7 +180,7 @@ __device__ __forceinline__ bool item_of(const AttnBatchArgs& a, int i, Item& it)
     const int64_t bk = static_cast<int64_t>(b) * a.NKV + kh;
     it.rows = a.GRP;
     it.row0 = 0;
-    it.Q = a.Qa + (static_cast<int64_t>(kh) * a.B + b) * a.GRP * kHD;
+    it.q0 = (static_cast<int64_t>(kh) * a.B + b) * a.GRP;
     it.lo = static_cast<int>(lo);
     it.hi = static_cast<int>(min(static_cast<int64_t>(slot) + 1, lo + a.plan.okeys));
     it.K = static_cast<const char*>(a.k_own) + bk * a.cap * row_bytes;
@@ -171,19 +203,14 @@ __device__ __forceinline__ void split3_8(const float (&x)[8], bf16x8 (&part)[3])
     for (int q = 0; q < 3; ++q) part[q] = __builtin_bit_cast(bf16x8, make_uint4(p[q][0], p[q][1], p[q][2], p[q][3]));
 }
 
-// Query row r16 of a wave's 16 (past the last: the last again), dims 32 c + 8 g4 .. + 7, as three
-// bf16 parts.
-__device__ __forceinline__ void load_query(const Item& it, int first, int r16, int g4, bf16x8 (&qp)[3][8]) {
-    const float* src = it.Q + static_cast<int64_t>(min(first + r16, it.rows - 1)) * kHD + 8 * g4;
+// Query row r16 of a wave's 16 (past the last: the last again), dims 32 c + 8 g4 .. + 7, in NP parts.
+template <int NP, class X8>
+__device__ __forceinline__ void load_query(const AttnBatchArgs& a, const Item& it, int first, int r16, int g4, X8 (&q)[NP][8]) {
+    const uint4* src = static_cast<const uint4*>(a.Qs) + (it.q0 + min(first + r16, it.rows - 1)) * NP * 32 + g4;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const float4 u = *reinterpret_cast<const float4*>(src + 32 * c), w = *reinterpret_cast<const float4*>(src + 32 * c + 4);
-        const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-        bf16x8 p[3];
-        split3_8(x, p);
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int q = 0; q < 3; ++q) qp[q][c] = p[q];
-    }
+        for (int c = 0; c < 8; ++c) q[p][c] = __builtin_bit_cast(X8, src[32 * p + 4 * c]);
 }
 
 // max and sum over the four lanes r16 + 16 g of a query (the 16- and 32-lane swaps of gfx950)
@@ -384,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
     copy(it.lo, K0, V0);
     const int first = it.narrow ? it.row0 : it.row0 + 16 * wave;
     bf16x8 qp[3][8];
-    load_query(it, first, r16, g4, qp);
+    load_query(a, it, first, r16, g4, qp);
     float m = -INFINITY, l = 0.0f;
     auto walk = [&](auto& o, int t0, float* raw, bool live) {
 #pragma unroll
@@ -412,11 +439,6 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
     }
 }
 
-typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
-
-// 2^e
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-
 // eight floats times s as two fp16 parts h = fp16(x), l = fp16(x - h): |x - h - l| <= 2^-23 |x|
 __device__ __forceinline__ void split2_8(const float (&x)[8], float s, halfx8 (&part)[2]) {
     uint32_t h[4], l[4];
@@ -440,9 +462,6 @@ __device__ __forceinline__ float max8(const float (&x)[8]) {
     asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[5]), "v"(x[6]));
     return fmaxf(m, fabsf(x[7]));
 }
-// the power of two that brings a largest magnitude (its bits) into [2^14, 2^15), as far as 2^+-100
-__device__ __forceinline__ int row_exp(uint32_t bits) { return min(max(141 - static_cast<int>(bits >> 23), -100), 100); }
-
 // A tile of an fp32 cache in LDS: two fp16 parts of K and of V, and what undoes their rows' scales.
 //
 // fp32 caches run on v_mfma_f32_16x16x32_f16. Every operand row (a query, a key, a value row, a
@@ -460,29 +479,6 @@ struct F32Query {
     halfx8 p[2][8];  // row first + r16, dims 32 c + 8 g4 .. + 7
     float scale;
 };
-
-__device__ __forceinline__ void f32_query(const Item& it, int first, int r16, int g4, F32Query& q) {
-    const float* src = it.Q + static_cast<int64_t>(min(first + r16, it.rows - 1)) * kHD + 8 * g4;
-    float4 u[16];
-    float mx = 0.0f;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        u[2 * c] = *reinterpret_cast<const float4*>(src + 32 * c);
-        u[2 * c + 1] = *reinterpret_cast<const float4*>(src + 32 * c + 4);
-    }
-#pragma unroll
-    for (auto& x : u) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-    const int e = row_exp(__float_as_uint(query_max(mx)));
-    q.scale = pow2(-e);
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const float x[8] = {u[2 * c].x, u[2 * c].y, u[2 * c].z, u[2 * c].w,
-                            u[2 * c + 1].x, u[2 * c + 1].y, u[2 * c + 1].z, u[2 * c + 1].w};
-        halfx8 p[2];
-        split2_8(x, pow2(e), p);
-        q.p[0][c] = p[0], q.p[1][c] = p[1];
-    }
-}
 
 // Dims 8 c .. + 7 (lo, hi) of row `row` of a tile's K or V: the 32 lanes of half a wave hold the row.
 __device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c, floatx4 lo, floatx4 hi) {
@@ -588,7 +584,7 @@ __device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], i
 // into the other of two buffers, one barrier a tile. Of the two waves that share a matrix core one
 // stages before its products with K and the other after, so that one's vector work runs under the
 // other's products.
-__device__ __forceinline__ void f32_wide(const Item& it, F32Tile* tiles) {
+__device__ __forceinline__ void f32_wide(const AttnBatchArgs& a, const Item& it, F32Tile* tiles) {
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = it.row0 + 16 * wave;
@@ -610,7 +606,8 @@ __device__ __forceinline__ void f32_wide(const Item& it, F32Tile* tiles) {
     };
     load(it.lo);
     F32Query q;
-    f32_query(it, first, r16, g4, q);
+    load_query(a, it, first, r16, g4, q.p);
+    q.scale = a.Qscale[it.q0 + min(first + r16, it.rows - 1)];
     stage(tiles[0]);
     load(it.lo + kKT);  // (past the end: the last row again)
     float m = -INFINITY, l = 0.0f;
@@ -654,7 +651,7 @@ __device__ __forceinline__ void f32_wide(const Item& it, F32Tile* tiles) {
 //         query r16 in o[4 t + e][i]
 // K and V of the wave's next 16 keys are on their way while this 16's products run; the queries are
 // read from LDS as they are needed, which is what leaves registers for both.
-__device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*ms)[16], float (*ls)[16]) {
+__device__ __forceinline__ void f32_narrow(const AttnBatchArgs& a, const Item& it, float* buf, float (*ms)[16], float (*ls)[16]) {
     const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4, wave = threadIdx.x >> 6;
     const float *K = static_cast<const float*>(it.K), *V = static_cast<const float*>(it.V);
     float4 k[16], vv[4][4];
@@ -676,7 +673,7 @@ __device__ __forceinline__ void f32_narrow(const Item& it, float* buf, float (*m
     float4 qrow[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        qrow[i] = *reinterpret_cast<const float4*>(it.Q + static_cast<int64_t>(min(it.row0 + 2 * wave + i, it.rows - 1)) * kHD + 4 * lane);
+        qrow[i] = *reinterpret_cast<const float4*>(a.Qa + (it.q0 + min(it.row0 + 2 * wave + i, it.rows - 1)) * kHD + 4 * lane);
     load_k(first);
     load_v(first);
 #pragma unroll
@@ -770,8 +767,8 @@ __global__ __launch_bounds__(512, 1) void attn_batch_f32_kernel(AttnBatchArgs a)
     __shared__ float small[2][8][16];
     Item it;
     if (!item_of(a, blockIdx.x, it)) return;
-    if (it.narrow) f32_narrow(it, reinterpret_cast<float*>(tiles), small[0], small[1]);
-    else f32_wide(it, tiles);
+    if (it.narrow) f32_narrow(a, it, reinterpret_cast<float*>(tiles), small[0], small[1]);
+    else f32_wide(a, it, tiles);
 }
 
 constexpr int kCombWaves = 8;
@@ -864,15 +861,19 @@ __global__ __launch_bounds__(kCombWaves * 64) void attn_batch_combine_kernel(Att
 }
 
 struct Carve {
-    int64_t q, pp, mp, po, mo, raw, total;  // float offsets, multiples of 4
+    int64_t q, qs, sc, pp, mp, po, mo, raw, total;  // float offsets, multiples of 4
+    bool split;
 };
 Carve carve_of(const AttnBatchArgs& a) {
     const auto up4 = [](int64_t x) { return (x + 3) / 4 * 4; };
     const int64_t rows = static_cast<int64_t>(a.B) * a.NQ;
     const AttnBatchPlan p = attn_batch_plan(a.B, a.GRP, a.NKV, a.P, a.cap, a.kv_bf16, device_cu_count());
     Carve c{};
+    c.split = a.kv_bf16 || p.block == batch_wide(false);
     c.q = 0;
-    c.pp = c.q + rows * kHD;
+    c.qs = c.q + (a.kv_bf16 ? 0 : rows * kHD);
+    c.sc = c.qs + (a.kv_bf16 ? rows * (3 * kHD / 2) : c.split ? rows * kHD : 0);
+    c.pp = c.sc + (c.split && !a.kv_bf16 ? up4(rows) : 0);
     c.mp = c.pp + rows * p.pieces * kHD;
     c.po = c.mp + up4(rows * p.pieces * 2);
     c.mo = c.po + rows * p.own * kHD;
@@ -889,6 +890,8 @@ void attn_batch_carve(AttnBatchArgs& a, float* ws) {
     const Carve c = carve_of(a);
     a.plan = attn_batch_plan(a.B, a.GRP, a.NKV, a.P, a.cap, a.kv_bf16, device_cu_count());
     a.Qa = ws + c.q;
+    a.Qs = c.split ? ws + c.qs : nullptr;
+    a.Qscale = ws + c.sc;
     a.part_p = ws + c.pp;
     a.ml_p = reinterpret_cast<float2*>(ws + c.mp);
     a.part_o = ws + c.po;

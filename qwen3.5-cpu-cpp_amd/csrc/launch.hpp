@@ -303,7 +303,11 @@ struct AttnBatchArgs {
     float* out;
     // set by attn_batch_carve
     AttnBatchPlan plan;
-    float* Qa;                          // [NKV][B GRP][HD] normed, rotated queries
+    // normed, rotated, scaled queries, [NKV][B GRP] rows: fp32 (fp32 caches), and (may be null) as
+    // parts for the 16-bit products with what undoes their rows' scales
+    float* Qa;
+    void* Qs;
+    float* Qscale;
     float* part_p;                      // [NKV][prefix pieces][B GRP][HD]
     float2* ml_p;                       // [NKV][prefix pieces][B GRP] (max, sum)
     float* part_o;                      // [B][NKV][own pieces][GRP][HD]
