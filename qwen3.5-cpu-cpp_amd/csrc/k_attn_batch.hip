@@ -228,24 +228,26 @@ __device__ __forceinline__ float query_sum(float v) {
     return over_query(v, [](float x, float y) { return x + y; });
 }
 
-// Online softmax of N scores of the lane's query (four lanes r16 + 16 g share it): s becomes
-// weights, (m, l) the query's running maximum and sum. Returns the factor of the output so
-// far. The reference maximum moves only when a score exceeds it by more than 8; a query without
-// a key yet keeps -inf and weight 0. e^y as the native 2^(y log2 e) of the exactly formed
-// exponent.
+// Online softmax of N scores of the lane's query (four lanes r16 + 16 g share it), each s times the
+// power of two `unit`: s becomes weights, (m, l) the query's running maximum (in the units of s) and
+// sum. Returns the factor of the output so far. The reference maximum moves only when a score
+// exceeds it by more than 8 / unit, so weights reach e^8. e^y as the native 2^(y log2 e) of the
+// exactly formed exponent. Every call holds a key of every query: a maximum is never -inf.
 template <int N>
-__device__ __forceinline__ float softmax_step(float (&s)[N], float& m, float& l) {
-    float tm = s[0];
+__device__ __forceinline__ float softmax_step(float (&s)[N], float unit, float& m, float& l) {
+    float tm;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(tm) : "v"(s[0]), "v"(s[1]), "v"(s[2]));
 #pragma unroll
-    for (int i = 1; i < N; ++i) tm = fmaxf(tm, s[i]);
+    for (int i = 3; i + 1 < N; i += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(tm) : "v"(s[i]), "v"(s[i + 1]));
+    if constexpr (N % 2 == 0) asm("v_max_f32 %0, %0, %1" : "+v"(tm) : "v"(s[N - 1]));
     tm = query_max(tm);
-    const float m_new = tm > m + 8.0f ? tm : m;
-    const bool live = m_new != -INFINITY;
-    const float f = live ? __builtin_amdgcn_exp2f((m - m_new) * kLog2e) : 1.0f;
+    const float k = unit * kLog2e;
+    const float m_new = (tm - m) * unit > 8.0f ? tm : m;
+    const float f = __builtin_amdgcn_exp2f((m - m_new) * k);
     float ps = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        s[i] = live ? __builtin_amdgcn_exp2f((s[i] - m_new) * kLog2e) : 0.0f;
+        s[i] = __builtin_amdgcn_exp2f((s[i] - m_new) * k);
         ps += s[i];
     }
     l = l * f + query_sum(ps);
@@ -288,6 +290,7 @@ __device__ __forceinline__ void reads_ahead() {
 // scores of keys past the last
 __device__ __forceinline__ void mask_tail(float (&s)[8], int k0, int hi, int g4) {
     if (k0 + kKT <= hi) return;  // uniform
+    asm volatile("");            // (a branch: seventeen instructions that only the last tile needs)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (k0 + 16 * (i >> 2) + 4 * g4 + (i & 3) >= hi) s[i] = -INFINITY;
@@ -348,8 +351,7 @@ __device__ __forceinline__ void bf16_tile(const uint4 (&Kc)[1024], const uint4 (
         *reinterpret_cast<floatx4*>(raw + k0 + 16 + 4 * g4) = St[1];
     }
     mask_tail(p, k0, hi, g4);
-    const float f = softmax_step(p, m, l);
-    rescale(f, o);
+    rescale(softmax_step(p, 1.0f, m, l), o);
     bf16x8 pa[3];
     split3_8(p, pa);
     __builtin_amdgcn_sched_barrier(0);
@@ -468,10 +470,11 @@ __device__ __forceinline__ float max8(const float (&x)[8]) {
 // query's weights over the tile) is scaled by a power of two that brings its largest entry into
 // [2^14, 2^15) and split into two fp16 parts; the three part products of lowest order are summed
 // (the fourth is below 2^-22 of the product) and the scales undone exactly: a key's in the scores,
-// a value row's in the weights before their own scaling, and that one as the tile's products,
-// summed from zero, are added to the output. So nothing is lost relative to the largest weight
-// times value row of the tile, whatever rows lie beside it.
-struct F32Tile {
+// a value row's in the weights before their own scaling, and that one, which the output is kept in,
+// at the end. The weights' scale is set by the largest weight times value row of a tile where
+// the softmax's reference moves and where it would be left upwards, so nothing is lost relative to the
+// largest such product so far, whatever rows lie beside it.
+struct alignas(1024) F32Tile {  // (aligned, so that a swizzled offset is one exclusive or on the address)
     uint4 K[2][1024], V[2][1024];
     float kscale[kKT], vscale[kKT];
 };
@@ -498,46 +501,54 @@ __device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c,
     if (c == 0) (v ? tile.vscale : tile.kscale)[row] = pow2(-e);
 }
 
-// Scores of query r16 of the wave: keys 4 g4 + v of the tile's first half, then of its second.
+// Byte address in LDS, to be offset by exclusive or.
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
+}
+template <class X>
+__device__ __forceinline__ X lds_read(uint32_t at) {
+    return *reinterpret_cast<__attribute__((address_space(3))) const X*>(static_cast<uintptr_t>(at));
+}
+
+// Scores of query r16 of the wave, over its scale: keys 4 g4 + v of the tile's first half, then of
+// its second.
 __device__ __forceinline__ void f32_scores(const F32Tile& tile, const F32Query& q, int r16, int g4, float (&p)[8]) {
-    int ko = k_off(r16, g4);
+    uint32_t ko = lds_at(&tile) + k_off(r16, g4);
     asm volatile("" : "+v"(ko));  // addresses formed per tile: kept, they would spill
     floatx4 St[2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-        floatx4 sa[2], sb[2];
+        floatx4 s[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) sa[e] = sb[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 2; ++e) s[e] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
             halfx8 k[2][2];
 #pragma unroll
             for (int h = 1; h >= 0; --h)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    k[h][e] = *reinterpret_cast<const halfx8*>(reinterpret_cast<const char*>(tile.K[h]) + hf * 16 * 512 + (ko ^ ((c + e) << 6)));
+                for (int e = 0; e < 2; ++e) k[h][e] = lds_read<halfx8>((ko ^ ((c + e) << 6)) + h * 16384 + hf * 8192);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) sb[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][e], q.p[0][c + e], sb[e], 0, 0, 0);
+            for (int e = 0; e < 2; ++e) s[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][e], q.p[0][c + e], s[e], 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) sa[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][e], q.p[0][c + e], sa[e], 0, 0, 0);
+            for (int e = 0; e < 2; ++e) s[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][e], q.p[1][c + e], s[e], 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) sb[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][e], q.p[1][c + e], sb[e], 0, 0, 0);
+            for (int e = 0; e < 2; ++e) s[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][e], q.p[0][c + e], s[e], 0, 0, 0);
         }
-        St[hf] = (sb[0] + sb[1]) + (sa[0] + sa[1]);
+        St[hf] = s[0] + s[1];
     }
     reads_ahead<8, 4, 6>();
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
         const floatx4 ks = *reinterpret_cast<const floatx4*>(tile.kscale + 16 * hf + 4 * g4);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) p[4 * hf + v] = (St[hf][v] * q.scale) * ks[v];
+        for (int v = 0; v < 4; ++v) p[4 * hf + v] = St[hf][v] * ks[v];
     }
 }
 
-// O^T += V^T P^T for T tiles of 16 dims from t0 on.
-template <int T>
-__device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], int r16, int g4, int t0, floatx4 (&o)[T]) {
-    int vo = v_off(r16, g4);
+// O^T += V^T P^T, O in units of 2^-exp for the lane's query; f: the softmax's factor of O so far.
+__device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], float f, int r16, int g4, int& exp, floatx4 (&o)[16]) {
+    uint32_t vo = lds_at(&tile) + 32768 + v_off(r16, g4);
     asm volatile("" : "+v"(vo));
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -545,38 +556,49 @@ __device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], i
 #pragma unroll
         for (int v = 0; v < 4; ++v) p[4 * hf + v] *= vs[v];
     }
-    const int e = row_exp(__float_as_uint(query_max(max8(p))));
+    const int e = row_exp(__float_as_uint(query_max(max8(p))));  // the largest weight is brought to [2^14, 2^15)
+    const bool move = f != 1.0f || e < exp;
+    if (__any(move)) {
+        // up no further than keeps what O holds, at most 2^60, within 2^90 (terms that much larger hide these)
+        const int most = exp + (f > 0.0f ? 157 - static_cast<int>(__float_as_uint(f) >> 23) : 400);
+        const int to = move ? min(e, most) : exp, step = to - exp;
+        const int s1 = min(max(step, -126), 126), s2 = min(max(step - s1, -126), 126);
+        const float g = (f * pow2(s1)) * pow2(s2);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) o[t] *= g;
+        exp = to;
+    }
     halfx8 pp[2];
-    split2_8(p, pow2(e), pp);
-    const float undo = pow2(-e);
-    // steps of 32 dims: the next but one's reads and the last one's sums go with this one's products
-    constexpr int kAhead = 2, kSteps = T / 2;
+    split2_8(p, pow2(exp), pp);
+    // steps of 32 dims: the next but one's reads go with this one's products
+    constexpr int kAhead = 2, kSteps = 8;
     halfx8 v[kAhead + 1][2][2];
-    floatx4 x[2][2];
     const auto read = [&](int u) {
+        typedef __attribute__((address_space(3))) i16x4 lds4;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int d = 0; d < 2; ++d) v[u % (kAhead + 1)][h][d] = v_operand<halfx8>(tile.V[h], vo ^ ((t0 + 2 * u + d) << 5));
+            for (int d = 0; d < 2; ++d) {
+                const uint32_t at = (vo ^ ((2 * u + d) << 5)) + h * 16384;
+                const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4*>(static_cast<uintptr_t>(at)));
+                const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4*>(static_cast<uintptr_t>(at + 8192)));
+                const i16x8 z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                v[u % (kAhead + 1)][h][d] = __builtin_bit_cast(halfx8, z);
+            }
     };
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) read(u);
 #pragma unroll
-    for (int u = 0; u <= kSteps; ++u) {
+    for (int u = 0; u < kSteps; ++u) {
         __builtin_amdgcn_sched_barrier(0);
         if (u + kAhead < kSteps) read(u + kAhead);
-        if (u < kSteps) {
-            const halfx8(&w)[2][2] = v[u % (kAhead + 1)];
+        const halfx8(&w)[2][2] = v[u % (kAhead + 1)];
 #pragma unroll
-            for (int d = 0; d < 2; ++d) x[u & 1][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][d], pp[1], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        for (int d = 0; d < 2; ++d) o[2 * u + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][d], pp[1], o[2 * u + d], 0, 0, 0);
 #pragma unroll
-            for (int d = 0; d < 2; ++d) x[u & 1][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[1][d], pp[0], x[u & 1][d], 0, 0, 0);
+        for (int d = 0; d < 2; ++d) o[2 * u + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[1][d], pp[0], o[2 * u + d], 0, 0, 0);
 #pragma unroll
-            for (int d = 0; d < 2; ++d) x[u & 1][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][d], pp[0], x[u & 1][d], 0, 0, 0);
-        }
-#pragma unroll
-        for (int d = 0; d < 2; ++d)
-            if (u) o[2 * u - 2 + d] += x[u & 1 ^ 1][d] * undo;
+        for (int d = 0; d < 2; ++d) o[2 * u + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[0][d], pp[0], o[2 * u + d], 0, 0, 0);
     }
 }
 
@@ -611,6 +633,7 @@ __device__ __forceinline__ void f32_wide(const AttnBatchArgs& a, const Item& it,
     stage(tiles[0]);
     load(it.lo + kKT);  // (past the end: the last row again)
     float m = -INFINITY, l = 0.0f;
+    int exp = 100;
     floatx4 o[16];
 #pragma unroll
     for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -628,17 +651,17 @@ __device__ __forceinline__ void f32_wide(const AttnBatchArgs& a, const Item& it,
         if (live) {
             f32_scores(tiles[cur], q, r16, g4, p);
             mask_tail(p, k0, it.hi, g4);
-            f = softmax_step(p, m, l);
+            f = softmax_step(p, q.scale, m, l);
         }
         if (wave >= 4) next();
-        if (live) {
-            rescale(f, o);
-            f32_output(tiles[cur], p, r16, g4, 0, o);
-        }
+        if (live) f32_output(tiles[cur], p, f, r16, g4, exp, o);
         cur ^= 1;
         lds_barrier();  // every wave is done with this tile, every share of the next one is in
     }
-    if (live) store_part(it, first, r16, g4, 0, o, m, l, true);
+    if (!live) return;
+#pragma unroll
+    for (auto& x : o) x *= pow2(-exp);
+    store_part(it, first, r16, g4, 0, o, m * q.scale, l, true);
 }
 
 // Narrow: 16 query rows on v_mfma_f32_16x16x4_f32, K and V straight from memory as its operands, no
@@ -708,7 +731,7 @@ __device__ __forceinline__ void f32_narrow(const AttnBatchArgs& a, const Item& i
         float p[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) p[v] = k0 + 4 * g4 + v < it.hi ? St[v] : -INFINITY;
-        rescale(softmax_step(p, m, l), o);
+        rescale(softmax_step(p, 1.0f, m, l), o);
 #pragma unroll
         for (int v = 0; v < 4; ++v)
 #pragma unroll

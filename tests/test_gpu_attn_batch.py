@@ -240,3 +240,33 @@ def test_two_calls_at_once(hip):
     for s, b in zip(streams, bufs):
         hip._ck(hip.rt.hipStreamDestroy(s), "hipStreamDestroy")
         b.__exit__()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("order", [1, -1])
+def test_value_rows_of_every_size(hip, order, bf16):
+    """Value rows of one sequence over 2^-60 .. 2^60, rising or falling, with scores that make the small
+    ones count: each row's size is undone by its score, 0.69 a power of two, so that the weights
+    move by e^83. The keys' errors (a score of 40 carries 40 * 2^-24 and 3e-6 a unit of its norm)
+    set the bar: 40 times the usual one. Next to them a sequence of ordinary rows."""
+    x = make(16, 2, 640, [0, 100, 70, 3, 33, 20, 64], 101, seed=12, bf16=bf16)
+    p = np.linspace(-60, 60, 640)[::order]
+    q = rope64(rms64(x["qg"][2, :, :HD], x["q_norm"]), x["pos"][2], x["rot"])
+    for kv in range(2):
+        u = q[8 * kv] / np.linalg.norm(q[8 * kv])
+        k = x["k_prefix"][kv] - np.outer(x["k_prefix"][kv] @ u, u)
+        k = k + np.outer(-np.round(p) * np.log(2.0) * 16.0 / np.linalg.norm(q[8 * kv]), u)
+        x["k_prefix"][kv] = bf16_to_f32(bf16_bits(k.astype(np.float32))) if bf16 else k.astype(np.float32)
+        x["v_prefix"][kv] *= np.exp2(np.round(p))[:, None].astype(np.float32)
+    run(hip, x, 640, bf16, bar=40 * REL_L2)
+
+
+@pytest.mark.parametrize("big", [2.0 ** 40, 2.0 ** -40, 2.0 ** 100, 2.0 ** -90])
+def test_scales_of_values(hip, big):
+    """All value rows times a power of two, and every other row: results scale with them."""
+    x = make(16, 2, 300, [5, 40, 0, 12, 9, 22, 7, 1], 64, seed=13)
+    for c in ("v_prefix", "v_own", "v_new"):
+        x[c] *= np.float32(big)
+    run(hip, x, 300, False)
+    x["v_prefix"][:, ::2] *= np.float32(1.0 / big)
+    run(hip, x, 300, False)
