@@ -242,7 +242,7 @@ inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t
                 if (t < best) best = t, c = len;
             }
         }
-        p.pkeys = static_cast<int>(32 * std::max(c, up(tiles, most)));
+        p.pkeys = static_cast<int>(32 * std::min(tiles, std::max(c, up(tiles, most))));
         p.pieces = static_cast<int>(up(P, p.pkeys));
     }
     const double share = (kv_bf16 ? n_cu * 7.0 / 6.0 : n_cu * 0.75) / pairs - 0.5;  // pieces of a half full cache
