@@ -445,8 +445,9 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  *   k_own, v_own [batch][NKV][own_capacity][HD]; rows from own_len[b] on are not read
  *   own_len (device) [batch]: rows in the own cache before this call; the new row goes to slot
  *     own_len[b] (the array itself is left as it is: it serves every layer). A negative entry
- *     marks an empty place: nothing of it is read or written. An entry at or above
- *     own_capacity is a caller's mistake: nothing is appended and its out rows are NaN.
+ *     marks an empty place: nothing of it is written, and what its rows hold does not matter.
+ *     An entry at or above own_capacity is a caller's mistake: nothing is appended and its out
+ *     rows are NaN.
  *   pos (device) [batch]: RoPE position of the new token
  *   own_score [batch][NKV][own_capacity], may be NULL: the softmax weight that each own row
  *     received, summed over the query heads of its kv head, is added to the row's entry; the
@@ -454,7 +455,8 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  *   own_pos [batch][NKV][own_capacity], may be NULL: receives pos[b] at the new slot
  *   out [batch][NQ][HD]
  * workspace (16-byte aligned): q35_attn_batch_workspace_bytes() bytes; its size depends on
- * sizes alone, never on the lengths. Requires HD == 256, NQ / NKV at most 16, an even
+ * sizes alone, never on the lengths. A captured graph holds the sizes of its capture, prefix_len
+ * among them. Results do not depend on the order in which workgroups run. Requires HD == 256, NQ / NKV at most 16, an even
  * rotary_dim, and 16-byte aligned fp32 rows and caches. */
 typedef struct q35_attn_batch_args {
     int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;
@@ -517,10 +519,11 @@ q35_status q35_kv_evict(const q35_kv_evict_args *args, q35_stream s);
  * and brings one token or a few (drafted tokens to verify); q35_gdn_prefill is the faster
  * form for many. The arithmetic of q35_gdn_decode.
  *   row0 (device) [batch + 1], may be NULL: sequence b's tokens are rows row0[b] ..
- *     row0[b+1] - 1 of the token-major inputs; NULL: row b. Rows beyond `rows` are not read or
- *     written, nor are rows of no sequence. A sequence may have no token.
+ *     row0[b+1] - 1 of the token-major inputs (the offsets do not decrease); NULL: row b. Rows
+ *     beyond `rows` are not read or written, nor are rows of no sequence. A sequence may have no
+ *     token.
  *   pos (device) [batch]: position of each sequence's first token (selects the ring slots). A
- *     negative entry marks an empty place: nothing of it is read or written.
+ *     negative entry marks an empty place: nothing of it is written.
  *   qkv [rows][ld_qkv] (CONV pre-conv channels), z [rows][ld_z] (VD), b, a [rows][ld_ba] (VH each)
  *   conv_w, A_log, dt_bias, norm_w as for q35_gdn_decode
  *   conv_ring [KER][CONV] and state [VH][DK][DV] of sequence b at b * stride_ring, b *

@@ -52,6 +52,9 @@ q35_status attn_batch_sizes(const q35_attn_batch_args* args, const char* who, q3
         return q35::fail(Q35_ERR_RANGE, "%s: prefix of %lld rows in %lld, own caches of %lld", who,
                          static_cast<long long>(g.prefix_len), static_cast<long long>(g.prefix_capacity),
                          static_cast<long long>(g.own_capacity));
+    if (g.own_score && (g.own_capacity + 511) / 512 * g.batch * g.kv_heads + static_cast<int64_t>(g.batch) * g.q_heads > INT32_MAX)
+        return q35::fail(Q35_ERR_UNSUPPORTED, "%s: scores of %d caches of %lld rows", who, g.batch * g.kv_heads,
+                         static_cast<long long>(g.own_capacity));
     q35k::AttnBatchArgs a{};
     a.B = g.batch;
     a.NQ = g.q_heads;

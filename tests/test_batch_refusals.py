@@ -51,6 +51,7 @@ def status(fn, a):
     (dict(rotary_dim=-2), ARG), (dict(rotary_dim=258), ARG), (dict(rotary_dim=63), ARG), (dict(kv_dtype=2), ARG),
     (dict(prefix_len=-1), RANGE), (dict(prefix_len=129), RANGE), (dict(own_capacity=0), RANGE),
     (dict(own_capacity=1 << 31), RANGE), (dict(prefix_capacity=1 << 31), RANGE),
+    (dict(batch=65535, own_capacity=1 << 24, own_score=BASE), UNSUPPORTED),
     (dict(own_len=None), ARG), (dict(pos=None), ARG), (dict(qg=None), ARG), (dict(k_new=None), ARG), (dict(v_new=None), ARG),
     (dict(q_norm=None), ARG), (dict(k_norm=None), ARG), (dict(k_prefix=None), ARG), (dict(v_prefix=None), ARG),
     (dict(k_own=None), ARG), (dict(v_own=None), ARG), (dict(out=None), ARG), (dict(workspace=None), ARG),
