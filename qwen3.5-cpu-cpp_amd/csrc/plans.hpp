@@ -219,9 +219,9 @@ constexpr int batch_wide(bool kv_bf16) { return kv_bf16 ? 64 : 128; }      // of
 // 183 (a second round of workgroups), 800 116, 1024 131. With 16 rows or fewer the loads bound
 // the time, and pieces are made for 7/8 of the compute units: 2 after 30001 fp32 ones, 128 keys 46
 // us, 256 35, 512 44.
-// Own caches are taken to be half full: pieces are made for 3/4 of the compute units (bf16: 7/6) to
-// have one that is not empty. 48 caches of 1000 fp32 rows: pieces of 128 39 us, 320 28, 512 36;
-// 48 of 2000 bf16 ones: 64 35, 320 26, 512 32.
+// Own caches are taken to be half full: pieces are made for 3/4 of the compute units (bf16, of which
+// two fit: 3/2) to have one that is not empty. 48 caches of 1000 fp32 rows: pieces of 128 39 us, 320
+// 28, 512 36; 32 of 2304 bf16 ones: 96 30, 224 25, 320 28; 24 of 2304 with 8 heads: 96 23, 160 20, 320 26.
 inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
     const int64_t rows = static_cast<int64_t>(B) * GRP, pairs = static_cast<int64_t>(B) * NKV, most = 2 * n_cu;
@@ -245,7 +245,7 @@ inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t
         p.pkeys = static_cast<int>(32 * std::min(tiles, std::max(c, up(tiles, most))));
         p.pieces = static_cast<int>(up(P, p.pkeys));
     }
-    const double share = (kv_bf16 ? n_cu * 7.0 / 6.0 : n_cu * 0.75) / pairs - 0.5;  // pieces of a half full cache
+    const double share = (kv_bf16 ? n_cu * 1.5 : n_cu * 0.75) / pairs - 0.5;  // pieces of a half full cache
     const int64_t len = share > 0.5 ? static_cast<int64_t>(cap / (2.0 * share)) : cap;
     p.okeys = static_cast<int>(32 * up(std::max<int64_t>(std::min(len, cap), std::min<int64_t>(cap, 64)), 32));
     p.own = static_cast<int>(up(cap, p.okeys));
