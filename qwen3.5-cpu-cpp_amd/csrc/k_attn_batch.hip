@@ -442,16 +442,16 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
 }
 
 // eight floats times s as two fp16 parts h = fp16(x), l = fp16(x - h): |x - h - l| <= 2^-23 |x|
+// (the mixed-precision fused multiply-adds round straight to fp16; in instructions: the compiler
+// forms the upper h twice, five for a pair instead of four)
 __device__ __forceinline__ void split2_8(const float (&x)[8], float s, halfx8 (&part)[2]) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {  // (the mixed-precision fused multiply-adds round straight to fp16)
-        const float a = x[2 * e], b = x[2 * e + 1];
-        const _Float16 ha = static_cast<_Float16>(__builtin_fmaf(a, s, 0.0f)), hb = static_cast<_Float16>(__builtin_fmaf(b, s, 0.0f));
-        const _Float16 la = static_cast<_Float16>(__builtin_fmaf(a, s, -static_cast<float>(ha)));
-        const _Float16 lb = static_cast<_Float16>(__builtin_fmaf(b, s, -static_cast<float>(hb)));
-        h[e] = __builtin_bit_cast(uint32_t, split_h2_t{ha, hb});
-        l[e] = __builtin_bit_cast(uint32_t, split_h2_t{la, lb});
+    for (int e = 0; e < 4; ++e) {
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h[e]) : "v"(x[2 * e]), "v"(s));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h[e]) : "v"(x[2 * e + 1]), "v"(s));
+        asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l[e]) : "v"(x[2 * e]), "v"(s), "v"(h[e]));
+        asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l[e]) : "v"(x[2 * e + 1]), "v"(s), "v"(h[e]));
     }
     part[0] = __builtin_bit_cast(halfx8, make_uint4(h[0], h[1], h[2], h[3]));
     part[1] = __builtin_bit_cast(halfx8, make_uint4(l[0], l[1], l[2], l[3]));
@@ -483,21 +483,25 @@ struct F32Query {
     float scale;
 };
 
-// Dims 8 c .. + 7 (lo, hi) of row `row` of a tile's K or V: the 32 lanes of half a wave hold the row.
-__device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c, floatx4 lo, floatx4 hi) {
-    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    uint32_t mx = __float_as_uint(max8(x));
+// Dims 8 c .. + 7 and 128 + 8 c .. + 7 of row `row` of a tile's K or V: 16 lanes hold the row.
+__device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c, const floatx4 (&y)[4]) {
+    float x[2][8];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i >> 3][i & 7] = y[i >> 2][i & 3];
+    uint32_t mx = __float_as_uint(fmaxf(max8(x[0]), max8(x[1])));
     mx = max(mx, static_cast<uint32_t>(dpp_i<0xB1>(mx)));
     mx = max(mx, static_cast<uint32_t>(dpp_i<0x4E>(mx)));
     mx = max(mx, static_cast<uint32_t>(dpp_i<0x141>(mx)));
     mx = max(mx, static_cast<uint32_t>(dpp_i<0x140>(mx)));
-    const auto r = __builtin_amdgcn_permlane16_swap(mx, mx, false, false);
-    const int e = row_exp(max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1])));
-    halfx8 p[2];
-    split2_8(x, pow2(e), p);
+    const int e = row_exp(mx);
     const int at = 32 * row + (c ^ ((v ? 2 * row : row) & 15));
 #pragma unroll
-    for (int q = 0; q < 2; ++q) (v ? tile.V : tile.K)[q][at] = __builtin_bit_cast(uint4, p[q]);
+    for (int i = 0; i < 2; ++i) {
+        halfx8 p[2];
+        split2_8(x[i], pow2(e), p);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) (v ? tile.V : tile.K)[q][at + 16 * i] = __builtin_bit_cast(uint4, p[q]);
+    }
     if (c == 0) (v ? tile.vscale : tile.kscale)[row] = pow2(-e);
 }
 
@@ -570,6 +574,7 @@ __device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], f
     }
     halfx8 pp[2];
     split2_8(p, pow2(exp), pp);
+    asm("s_nop 1" : "+v"(pp[0]), "+v"(pp[1]));  // two states between a vector write and a product's read (the compiler sees no such write)
     // steps of 32 dims: the next but one's reads go with this one's products
     constexpr int kAhead = 2, kSteps = 8;
     halfx8 v[kAhead + 1][2][2];
@@ -604,27 +609,31 @@ __device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], f
 
 // Wide: 128 query rows, 16 a wave. Tiles come through registers and are split once for all waves
 // into the other of two buffers, one barrier a tile. Of the two waves that share a matrix core one
-// stages before its products with K and the other after, so that one's vector work runs under the
-// other's products.
+// stages before its products with K and the other after, so that one's vector work runs beside the
+// other's products. A product takes its matrix core 17.5 cycles and an issue slot 9, a vector
+// instruction 4: a tile's 192 products and 650 vector instructions per core are bound by issue. 3.1 us
+// a tile of 128 rows and 32 keys, 1040 TFLOP/s in fp16 products over the compute units, where a large
+// fp16 matrix product reaches 1221. (Four waves of 32 rows, which read half as much of LDS, softmax and
+// staging interleaved with the products one by one: 4.0 us.)
 __device__ __forceinline__ void f32_wide(const AttnBatchArgs& a, const Item& it, F32Tile* tiles) {
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = it.row0 + 16 * wave;
     const bool live = first < it.rows;  // uniform per wave
-    floatx4 st[8];
+    floatx4 st[2][4];  // dims 8 c .. + 7 and 128 + 8 c .. + 7 of a row of K, of V
+    const int row = tid >> 4, c = tid & 15;
     const auto load = [&](int k0) {
+        const int64_t at = static_cast<int64_t>(min(k0 + row, it.hi - 1)) * kHD + 8 * c;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t at = static_cast<int64_t>(min(k0 + (tid >> 5) + 16 * i, it.hi - 1)) * kHD + 8 * (tid & 31);
-            const floatx4 *k = reinterpret_cast<const floatx4*>(static_cast<const float*>(it.K) + at),
-                          *v = reinterpret_cast<const floatx4*>(static_cast<const float*>(it.V) + at);
-            st[2 * i] = k[0], st[2 * i + 1] = k[1];
-            st[4 + 2 * i] = v[0], st[5 + 2 * i] = v[1];
+        for (int v = 0; v < 2; ++v) {
+            const floatx4* src = reinterpret_cast<const floatx4*>(static_cast<const float*>(v ? it.V : it.K) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[v][i] = src[(i >> 1) * 32 + (i & 1)];
         }
     };
     const auto stage = [&](F32Tile& dst) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f32_stage(dst, i >= 2, (tid >> 5) + 16 * (i & 1), tid & 31, st[2 * i], st[2 * i + 1]);
+        for (int v = 0; v < 2; ++v) f32_stage(dst, v, row, c, st[v]);
     };
     load(it.lo);
     F32Query q;

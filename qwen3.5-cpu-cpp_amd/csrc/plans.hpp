@@ -211,14 +211,16 @@ struct AttnBatchPlan {
 constexpr int kBatchNarrow = 16;                                           // query rows of a narrow workgroup
 constexpr int batch_wide(bool kv_bf16) { return kv_bf16 ? 64 : 128; }      // of a wide one
 // Workgroups of the prefix are dealt to the 8 XCDs by their piece and kv head (the row blocks of one
-// piece together, for their L2). Times in us on 256 compute units: a tile of 32 keys takes a bf16
-// workgroup 1.65 alone on its compute unit and 2.7 beside another (64 rows; two fit), an fp32 one 4.0
-// (128 rows; one fits); a partial output costs its bytes at 2.2 TB/s, written and merged. Of the
-// piece lengths the fastest by that is taken: 48 sequences of 16 / 2 heads after 30001 bf16 positions,
-// attention and merge with pieces of 256 keys 99 us, 512 83, 768 79, 1504 88; fp32 ones, 512 146, 704
-// 183 (a second round of workgroups), 800 116, 1024 131. With 16 rows or fewer the loads bound
-// the time, and pieces are made for 7/8 of the compute units: 2 after 30001 fp32 ones, 128 keys 46
-// us, 256 35, 512 44.
+// piece together, for their L2), those of the own caches come after them. Times in us on 256 compute
+// units: a tile of 32 keys takes a bf16 workgroup 1.65 alone on its compute unit and 2.7 beside another
+// (64 rows; two fit), an fp32 one 3.1 (128 rows; one fits), a start and an end 8; an own cache's tile
+// 1.8 and 2.0; a partial output costs its bytes at 2.2 TB/s, written and merged. Of the piece lengths
+// the fastest by that is taken, the own caches running where the prefix leaves room: 48 sequences of
+// 16 / 2 heads after 30001 fp32 positions with own caches of 1000, attention and merge with pieces of
+// 640 keys 160 us (a second round of workgroups), 768 128, 896 128, 960 113, 1024 119, 1280 136; without
+// own rows 768 105, 1024 114; bf16 512 94, 640 100, 768 87, 896 86, 1280 103, 1504 88. With 16 rows or
+// fewer the loads bound the time, and pieces are made for 7/8 of the compute units: 2 after 30001 fp32
+// ones, 128 keys 46 us, 256 35, 512 44.
 // Own caches are taken to be half full: pieces are made for 3/4 of the compute units (bf16, of which
 // two fit: 3/2) to have one that is not empty. 48 caches of 1000 fp32 rows: pieces of 128 39 us, 320
 // 28, 512 36; 32 of 2304 bf16 ones: 96 30, 224 25, 320 28; 24 of 2304 with 8 heads: 96 23, 160 20, 320 26.
@@ -226,29 +228,30 @@ inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
     const int64_t rows = static_cast<int64_t>(B) * GRP, pairs = static_cast<int64_t>(B) * NKV, most = 2 * n_cu;
     AttnBatchPlan p{};
-    if (P > 0) {
-        const int64_t tiles = up(P, 32);
-        p.block = rows <= kBatchNarrow ? kBatchNarrow : batch_wide(kv_bf16);
-        p.nblk = static_cast<int>(up(rows, p.block));
-        int64_t c = std::max<int64_t>(2, up(tiles * NKV, std::max(1, n_cu * 7 / 8)));
-        if (p.block != kBatchNarrow) {
-            const int64_t cu = std::max(1, n_cu / 8), slots = kv_bf16 ? 2 * cu : cu;
-            const double alone = kv_bf16 ? 1.65 : 4.0, full = kv_bf16 ? 2.7 : 4.0;
-            double best = 1e300;
-            for (int64_t n = 1; n <= std::min(up(tiles, 2), most); n += 1 + n / 16) {
-                const int64_t len = up(tiles, n), wgs = up(up(tiles, len) * NKV, 8) * p.nblk, rest = wgs % slots;
-                const double t = len * (wgs / slots * full + (rest > cu ? full : rest ? alone : 0.0)) +
-                                 up(tiles, len) * NKV * rows * 1024 / 2.2e6;
-                if (t < best) best = t, c = len;
-            }
-        }
-        p.pkeys = static_cast<int>(32 * std::min(tiles, std::max(c, up(tiles, most))));
-        p.pieces = static_cast<int>(up(P, p.pkeys));
-    }
     const double share = (kv_bf16 ? n_cu * 1.5 : n_cu * 0.75) / pairs - 0.5;  // pieces of a half full cache
-    const int64_t len = share > 0.5 ? static_cast<int64_t>(cap / (2.0 * share)) : cap;
-    p.okeys = static_cast<int>(32 * up(std::max<int64_t>(std::min(len, cap), std::min<int64_t>(cap, 64)), 32));
+    const int64_t own = share > 0.5 ? static_cast<int64_t>(cap / (2.0 * share)) : cap;
+    p.okeys = static_cast<int>(32 * up(std::max<int64_t>(std::min(own, cap), std::min<int64_t>(cap, 64)), 32));
     p.own = static_cast<int>(up(cap, p.okeys));
+    if (P <= 0) return p;
+    const int64_t tiles = up(P, 32);
+    p.block = rows <= kBatchNarrow ? kBatchNarrow : batch_wide(kv_bf16);
+    p.nblk = static_cast<int>(up(rows, p.block));
+    int64_t c = std::max<int64_t>(2, up(tiles * NKV, std::max(1, n_cu * 7 / 8)));
+    if (p.block != kBatchNarrow) {
+        const int64_t cu = std::max(1, n_cu / 8), slots = kv_bf16 ? 2 * cu : cu;
+        const double alone = kv_bf16 ? 1.65 : 3.1, full = kv_bf16 ? 2.7 : 3.1, start = 8.0;
+        const double t_own = start + p.okeys / 32.0 * (kv_bf16 ? 1.8 : 2.0), n_own = pairs / 8.0 * (cap / 2.0 / p.okeys + 0.5);
+        double best = 1e300;
+        for (int64_t n = 1; n <= std::min(up(tiles, 2), most); n += 1 + n / 16) {
+            const int64_t len = up(tiles, n), wgs = up(up(tiles, len) * NKV, 8) * p.nblk, rest = wgs % slots;
+            const double alone_t = wgs / slots * (start + len * full) + (rest ? start + len * (rest > cu ? full : alone) : 0.0);
+            const double with_own = (wgs * (start + len * full) + n_own * t_own) / slots + t_own / 3;
+            const double t = std::max(alone_t, with_own) + up(tiles, len) * NKV * rows * 1024 / 2.2e6;
+            if (t < best) best = t, c = len;
+        }
+    }
+    p.pkeys = static_cast<int>(32 * std::min(tiles, std::max(c, up(tiles, most))));
+    p.pieces = static_cast<int>(up(P, p.pkeys));
     return p;
 }
 
