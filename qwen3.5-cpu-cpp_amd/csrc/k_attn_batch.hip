@@ -34,6 +34,9 @@ typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 // the power of two that brings a largest magnitude (its bits) into [2^14, 2^15), as far as 2^+-100
 __device__ __forceinline__ int row_exp(uint32_t bits) { return min(max(141 - static_cast<int>(bits >> 23), -100), 100); }
+// what undoes it; NaN for a row of 2^115 or more, an infinity or a NaN (whose other entries the parts
+// would lose, and the row's outputs be finite and wrong)
+__device__ __forceinline__ float row_scale(uint32_t bits, int e) { return bits < 0x79000000u ? pow2(-e) : NAN; }
 
 // theta^(-2i / ROT), formed on the host: 32 double-precision powers cost the kernel 1 us
 struct RopeFreq {
@@ -60,7 +63,7 @@ __device__ __forceinline__ void store_query(const AttnBatchArgs& a, int64_t row,
     split2h_pair(y.z * pow2(e), y.w * pow2(e), h.y, l.y);
     static_cast<uint2*>(a.Qs)[(row * 2 + 0) * 64 + lane] = h;
     static_cast<uint2*>(a.Qs)[(row * 2 + 1) * 64 + lane] = l;
-    if (lane == 0) a.Qscale[row] = pow2(-e);
+    if (lane == 0) a.Qscale[row] = row_scale(__float_as_uint(mx), e);
 }
 
 // grid ((NQ + NKV) / 4, B), a wave per row: rmsnorm (1 + w) + RoPE of a query row, or of the new key
@@ -502,7 +505,7 @@ __device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c,
 #pragma unroll
         for (int q = 0; q < 2; ++q) (v ? tile.V : tile.K)[q][at + 16 * i] = __builtin_bit_cast(uint4, p[q]);
     }
-    if (c == 0) (v ? tile.vscale : tile.kscale)[row] = pow2(-e);
+    if (c == 0) (v ? tile.vscale : tile.kscale)[row] = row_scale(mx, e);
 }
 
 // Byte address in LDS, to be offset by exclusive or.

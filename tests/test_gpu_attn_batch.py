@@ -270,3 +270,39 @@ def test_scales_of_values(hip, big):
     run(hip, x, 300, False)
     x["v_prefix"][:, ::2] *= np.float32(1.0 / big)
     run(hip, x, 300, False)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan, 3e38])
+@pytest.mark.parametrize("where", ["v_prefix", "k_prefix", "v_own", "k_own", "qg"])
+@pytest.mark.parametrize("nq", [16, 2])
+def test_no_wrong_finite_outputs(hip, nq, where, what, bf16):
+    """One infinity, NaN or value near the type's largest: an output that depends on it is the
+    definition's or not finite (a square of 3e38 is no float, so not that in a query), all others are
+    as without it. The bar: ten times that of a run, of the value or of the outputs' mean size."""
+    if where == "qg" and what == 3e38:
+        what = -np.nan
+    x = make(nq, 2, 500, [20, 40, 0, 30, 12, 9, 5, 3], 64, seed=14, bf16=bf16)
+    clean = run(hip, x, 500, bf16)["out"]
+    at = {"v_prefix": (1, 77, 5), "k_prefix": (1, 77, 5), "v_own": (3, 1, 11, 5), "k_own": (3, 1, 11, 5), "qg": (3, nq - 1, 5)}[where]
+    val = np.array([what], np.float32)
+    x[where][at] = bf16_to_f32(bf16_bits(val))[0] if bf16 and where != "qg" else val[0]
+    with upload(hip, x, bf16) as bufs:
+        pyq35.check(pyq35.lib.q35_attn_batch(attn_args(bufs, x, bf16, 64, 500, 500), None))
+        hip.sync()
+        got, ko, vo = bufs.get("out"), cache_out(bufs.get("k_own")), cache_out(bufs.get("v_own"))
+    seen = np.zeros(got.shape[:2], bool)
+    if where == "qg":
+        seen[3, nq - 1] = True
+    elif where.endswith("own"):
+        seen[3, nq // 2:] = True
+    else:
+        seen[:, nq // 2:] = True
+    assert np.array_equal(got[~seen], clean[~seen])
+    size = np.sqrt(np.mean(clean.astype(np.float64) ** 2))
+    for b in range(8):
+        n = x["own_len"][b] + 1
+        with np.errstate(all="ignore"):
+            want = attn64(x, b, np.concatenate([x["k_prefix"], ko[b, :, :n]], 1), np.concatenate([x["v_prefix"], vo[b, :, :n]], 1))[0]
+        fine = np.isfinite(got[b]) & seen[b][:, None]
+        assert (np.abs(got[b] - want) <= 10 * REL_L2 * np.maximum(np.abs(want), size))[fine].all(), f"sequence {b}"
