@@ -5,14 +5,14 @@
 //
 // Choosing is a radix selection of the keep-th largest 32-bit key over 11 + 11 + 10 bits with
 // histograms in LDS (after the first 11 mostly few keys are left, which are then compared with one
-// another: 1152 rows 8.0 -> 6.2 us), then a pass that ranks the rows in slot order: of the rows equal to that
+// another: 1152 rows 8.0 -> 6.3 us), then a pass that ranks the rows in slot order: of the rows equal to that
 // key the lowest slots stay, and the number of rows kept before a row gives its place in the move
 // lists. Up to kRegRows rows one workgroup holds all keys in registers and does it in one
 // launch. Longer caches are cut into slices of kSlice rows, a workgroup each, in three launches:
 // the keys and their histogram; from all slices' histograms the bin of the wanted key, and the
 // slice's keys that lie in it (candidates); from all candidates the key itself, and the slice's
 // ranks. What every slice needs of the others it forms for itself, so no launch has a single
-// workgroup: 131072 rows of two heads 25 us against 56 with one workgroup that
+// workgroup: 131072 rows of two heads 22 us against 56 with one workgroup that
 // finds the key and slices that count the rows before them.
 #include "dev_common.hpp"
 #include "launch.hpp"
@@ -25,7 +25,7 @@ constexpr int kBins = 2048;
 constexpr int kRegRows = 16384;      // most rows of the one-launch selection (16 keys a thread)
 constexpr int kSlice = 4096;         // rows of a slice of a longer cache
 constexpr int kCandidates = 16384;   // keys of one bin held in LDS
-constexpr int kFew = 256;            // keys of one bin that are compared with one another
+constexpr int kFew = kSelThreads / 4; // keys of one bin that are compared with one another
 
 // Order of the rows: larger keys stay. Rows kept whatever their weight come first, a NaN
 // last; -0 equals 0.
@@ -39,6 +39,18 @@ __device__ __forceinline__ uint32_t row_key(float score, int pos, int n_sink, in
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
+// Sums over the lanes up to each one's, by shifts within rows of 16 lanes and broadcasts of a row's
+// and of half a wave's last lane (no LDS: six exchanges through it take 0.35 us).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);
+    return v;
 }
 
 // One (sequence, kv head): its arrays, its rows n, and whether there is anything to choose.
@@ -79,12 +91,7 @@ __device__ __forceinline__ void keep_all(const KvEvictArgs& a, const Cache& c, i
 // lower.
 __device__ __forceinline__ uint3 find_bin(uint32_t c0, uint32_t c1, uint32_t want, uint32_t* wsum, uint32_t* found) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi_bin = kBins - 1 - 2 * tid;
-    uint32_t inc = c0 + c1;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t up = __shfl_up(inc, o);
-        if (lane >= o) inc += up;
-    }
+    const uint32_t inc = wave_scan(c0 + c1);
     if (lane == 63) wsum[wave] = inc;
     __syncthreads();
     uint32_t before = inc - c0 - c1;
@@ -129,17 +136,19 @@ __device__ __forceinline__ uint2 radix_limit(uint32_t* hist, uint32_t* wsum, uin
         if (key >> (pass == 1 ? 21 : 10) == prefix) few[atomicAdd(&listed, 1u)] = key;
     });
     __syncthreads();
-    if (tid < static_cast<int>(left)) {
-        const uint32_t key = few[tid];
-        uint32_t above = 0, equal = 0;
-        for (uint32_t i = 0; i < left; ++i) {
-            above += few[i] > key;
-            equal += few[i] == key;
-        }
-        if (above < want && want <= above + equal) {  // the wanted key: every thread that has it writes the same
-            found[0] = key;
-            found[1] = want - above;
-        }
+    // (four threads a key, a quarter of the comparisons each)
+    const uint32_t key = few[min(static_cast<uint32_t>(tid >> 2), left - 1)];
+    uint32_t above = 0, equal = 0;
+#pragma unroll 4
+    for (uint32_t i = tid & 3; i < left; i += 4) {
+        above += few[i] > key;
+        equal += few[i] == key;
+    }
+    above += dpp_i<0xB1>(above), equal += dpp_i<0xB1>(equal);
+    above += dpp_i<0x4E>(above), equal += dpp_i<0x4E>(equal);
+    if (above < want && want <= above + equal) {  // the wanted key: every thread that has it writes the same
+        found[0] = key;
+        found[1] = want - above;
     }
     __syncthreads();
     return make_uint2(found[0], found[1]);
@@ -267,9 +276,8 @@ __device__ __forceinline__ void block_sums(uint32_t (&s)[N], uint32_t (*red)[kSe
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o);
-        if (lane == 0) red[i][wave] = s[i];
+        s[i] = wave_scan(s[i]);
+        if (lane == 63) red[i][wave] = s[i];
     }
     __syncthreads();
 #pragma unroll
@@ -366,13 +374,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_rank_kernel(KvEvictArgs a) {
     const auto listed = [&](auto&& f) {
         uint32_t off = 0;
         for (int i0 = 0; i0 < used; i0 += 16) {  // counts of sixteen slices at a time, one a lane
-            const uint32_t mine = lane < 16 && i0 + lane < used ? sl[i0 + lane].y : 0;
-            uint32_t inc = mine;
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) {
-                const uint32_t up = __shfl_up(inc, o);
-                if (lane >= o) inc += up;
-            }
+            const uint32_t mine = lane < 16 && i0 + lane < used ? sl[i0 + lane].y : 0, inc = wave_scan(mine);
             const uint32_t n = __shfl(mine, wave), first = off + __shfl(inc, wave) - n;
             for (uint32_t k = lane; k < n; k += 64) f(a.cand[c.bk * a.cap + (i0 + wave) * static_cast<int64_t>(kSlice) + k], first + k);
             off += __shfl(inc, 15);
@@ -383,7 +385,14 @@ __global__ __launch_bounds__(kSelThreads) void kv_rank_kernel(KvEvictArgs a) {
     __syncthreads();
     const auto each = [&](auto&& f) {
         if (!fits) return listed(f);
-        for (uint32_t i = tid; i < total; i += kSelThreads) f(cand[i], i);
+        for (uint32_t i = tid; i < total; i += 4 * kSelThreads) {  // (four reads on their way at once)
+            uint32_t k[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = cand[min(i + j * kSelThreads, total - 1)];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j * kSelThreads < total) f(k[j], i + j * kSelThreads);
+        }
     };
     const uint2 limit = radix_limit(hist, wsum, found, 1, top.x, top.y, [&](auto&& f) { each([&](uint32_t k, uint32_t) { f(k); }); });
     uint32_t q[4] = {0, 0, 0, 0};  // before this slice: above, equal; below `keep`: above, equal
