@@ -806,7 +806,7 @@ __global__ __launch_bounds__(512, 1) void attn_batch_f32_kernel(AttnBatchArgs a)
     else f32_wide(a, it, tiles);
 }
 
-constexpr int kCombWaves = 8;
+constexpr int kCombWaves = 8, kCombAhead = 8;
 
 // The (max, sum) of piece i of row g of (b, kh): the prefix's pieces, then the own cache's.
 __device__ __forceinline__ int64_t piece_row(const AttnBatchArgs& a, int b, int kh, int g, int i) {
@@ -817,28 +817,30 @@ __device__ __forceinline__ int64_t piece_row(const AttnBatchArgs& a, int b, int 
 __device__ __forceinline__ float2 piece_ml(const AttnBatchArgs& a, int b, int kh, int g, int i) {
     return (i < a.plan.pieces ? a.ml_p : a.ml_o)[piece_row(a, b, kh, g, i)];
 }
-// (max, sum) over n pieces, by the lanes of a wave
-__device__ __forceinline__ float2 merge_ml(const AttnBatchArgs& a, int b, int kh, int g, int n, int lane) {
-    float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, piece_ml(a, b, kh, g, i).x);
+// (max, sum) over n pieces, by the lanes of a wave; first: the lane's first piece's
+__device__ __forceinline__ float2 merge_ml(const AttnBatchArgs& a, int b, int kh, int g, int n, int lane, float2& first) {
+    first = lane < n ? piece_ml(a, b, kh, g, lane) : make_float2(-INFINITY, 0.0f);
+    float m = first.x;
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, piece_ml(a, b, kh, g, i).x);
     m = wave_max(m);
-    for (int i = lane; i < n; i += 64) {
+    float l = first.y * __builtin_amdgcn_exp2f((first.x - m) * kLog2e);
+    for (int i = lane + 64; i < n; i += 64) {
         const float2 x = piece_ml(a, b, kh, g, i);
         l += x.y * __builtin_amdgcn_exp2f((x.x - m) * kLog2e);
     }
     return make_float2(m, wave_sum(l));
 }
 
-// Workgroups [0, B NQ): one output row each. The pieces' factors e^(their maximum - the row's) / sum
-// first, into LDS, so that the partial outputs stream with nothing between their loads: a wave
-// takes every eighth piece, a lane four dims. Then the gate.
+// Workgroups [0, B NQ): one output row each. A wave takes every eighth piece, a lane four dims; the
+// partial outputs of a wave's first pieces are on their way while the pieces' factors e^(their
+// maximum - the row's) are formed, into LDS. Then the gate.
 // The others (with own_score): 512 own rows of a (sequence, kv head) each: their weights, summed
 // over the heads of the group in order, into the scores.
 __global__ __launch_bounds__(kCombWaves * 64) void attn_batch_combine_kernel(AttnBatchArgs a) {
     extern __shared__ __align__(16) float fac[];  // a factor per piece
     __shared__ __align__(16) float part[kCombWaves][kHD];
     __shared__ float ms[16], ls[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rows = a.B * a.NQ;
     if (static_cast<int>(blockIdx.x) >= rows) {
         const int chunks = static_cast<int>((a.cap + 511) / 512);
@@ -849,7 +851,8 @@ __global__ __launch_bounds__(kCombWaves * 64) void attn_batch_combine_kernel(Att
         if (slot < 0 || chunk * 512LL > slot) return;
         const int n = a.plan.pieces + slot / a.plan.okeys + 1;
         for (int g = wave; g < a.GRP; g += kCombWaves) {
-            const float2 x = merge_ml(a, b, kh, g, n, lane);
+            float2 first;
+            const float2 x = merge_ml(a, b, kh, g, n, lane, first);
             if (lane == 0) ms[g] = x.x, ls[g] = 1.0f / x.y;
         }
         __syncthreads();
@@ -872,17 +875,25 @@ __global__ __launch_bounds__(kCombWaves * 64) void attn_batch_combine_kernel(Att
     }
     const int kh = h / a.GRP, g = h - kh * a.GRP, n = a.plan.pieces + len / a.plan.okeys + 1;
     const float4 gate = *reinterpret_cast<const float4*>(a.qg + (static_cast<int64_t>(b) * a.NQ + h) * 2 * kHD + kHD + 4 * lane);
-    const float2 all = merge_ml(a, b, kh, g, n, lane);  // every wave the same
-    for (int i = tid; i < n; i += kCombWaves * 64)
-        fac[i] = __builtin_amdgcn_exp2f((piece_ml(a, b, kh, g, i).x - all.x) * kLog2e);
-    __syncthreads();
+    const auto partial = [&](int i) {
+        return *reinterpret_cast<const float4*>((i < a.plan.pieces ? a.part_p : a.part_o) + piece_row(a, b, kh, g, i) * kHD + 4 * lane);
+    };
+    float4 x[kCombAhead];
+#pragma unroll
+    for (int j = 0; j < kCombAhead; ++j)
+        if (wave + j * kCombWaves < n) x[j] = partial(wave + j * kCombWaves);  // uniform
+    float2 first;
+    const float2 all = merge_ml(a, b, kh, g, n, lane, first);  // every wave the same
+    if (tid < min(n, 64)) fac[tid] = __builtin_amdgcn_exp2f((first.x - all.x) * kLog2e);
+    for (int i = tid + 64; i < n; i += kCombWaves * 64) fac[i] = __builtin_amdgcn_exp2f((piece_ml(a, b, kh, g, i).x - all.x) * kLog2e);
+    lds_barrier();
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](float4 v, float f) { y.x += v.x * f, y.y += v.y * f, y.z += v.z * f, y.w += v.w * f; };
+#pragma unroll
+    for (int j = 0; j < kCombAhead; ++j)
+        if (wave + j * kCombWaves < n) add(x[j], fac[wave + j * kCombWaves]);
 #pragma unroll 4
-    for (int i = wave; i < n; i += kCombWaves) {
-        const float4 x = *reinterpret_cast<const float4*>((i < a.plan.pieces ? a.part_p : a.part_o) + piece_row(a, b, kh, g, i) * kHD + 4 * lane);
-        const float f = fac[i];
-        y.x += x.x * f, y.y += x.y * f, y.z += x.z * f, y.w += x.w * f;
-    }
+    for (int i = wave + kCombAhead * kCombWaves; i < n; i += kCombWaves) add(partial(i), fac[i]);
     *reinterpret_cast<float4*>(&part[wave][4 * lane]) = y;
     __syncthreads();
     if (wave) return;
