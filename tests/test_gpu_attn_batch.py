@@ -306,3 +306,11 @@ def test_no_wrong_finite_outputs(hip, nq, where, what, bf16):
             want = attn64(x, b, np.concatenate([x["k_prefix"], ko[b, :, :n]], 1), np.concatenate([x["v_prefix"], vo[b, :, :n]], 1))[0]
         fine = np.isfinite(got[b]) & seen[b][:, None]
         assert (np.abs(got[b] - want) <= 10 * REL_L2 * np.maximum(np.abs(want), size))[fine].all(), f"sequence {b}"
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("nq,nkv,P,lens,cap", [(8, 1, 20000, [63], 64), (16, 1, 20000, [10, 63, -1, 5], 64), (2, 2, 1, [4999, 70], 5000),
+                                               (1, 1, 0, [59999], 60000), (4, 1, 9000, [8000, 3], 9000)])
+def test_many_pieces(hip, nq, nkv, P, lens, cap, bf16):
+    """More pieces of a row than a wave has lanes (its merge then takes several a lane)."""
+    run(hip, make(nq, nkv, P, lens, cap, seed=P + cap, bf16=bf16), P, bf16)
