@@ -18,20 +18,29 @@ namespace {
 constexpr int kD = 128;
 constexpr int kTok = 8;  // tokens per pass through LDS
 
-// sum over the row groups: lanes C apart, by DPP rotations within each 16-lane row and the 16- and
-// 32-lane swaps of gfx950
+// Four sums over the row groups (lanes C apart), one a lane: those of the r-th 16 lanes end with component
+// 0, 2, 1, 3 for r = 0 .. 3. The 32- and 16-lane swaps of gfx950 add two values at once, rotations within
+// the 16 lanes the rest: 7 instructions, where four sums in every lane take 28.
 template <int C>
-__device__ __forceinline__ float group_sum(float v) {
-    if constexpr (C == 4) v += dpp_f<0x124>(v);  // rotation by 4
-    v += dpp_f<0x128>(v);                        // by 8
-    auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
-    v = __builtin_bit_cast(float, static_cast<int>(r[0])) + __builtin_bit_cast(float, static_cast<int>(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
-    return __builtin_bit_cast(float, static_cast<int>(r[0])) + __builtin_bit_cast(float, static_cast<int>(r[1]));
+__device__ __forceinline__ float group_sums(float4 v) {
+    const auto add = [](auto r) {
+        return __builtin_bit_cast(float, static_cast<int>(r[0])) + __builtin_bit_cast(float, static_cast<int>(r[1]));
+    };
+    const auto bits = [](float x) { return __builtin_bit_cast(int, x); };
+    const float a = add(__builtin_amdgcn_permlane32_swap(bits(v.x), bits(v.y), false, false));
+    const float b = add(__builtin_amdgcn_permlane32_swap(bits(v.z), bits(v.w), false, false));
+    float s = add(__builtin_amdgcn_permlane16_swap(bits(a), bits(b), false, false));
+    if constexpr (C == 4) s += dpp_f<0x124>(s);  // rotation by 4
+    return s + dpp_f<0x128>(s);                  // by 8
 }
-template <int C>
-__device__ __forceinline__ float4 group_sum4(float4 v) {
-    return make_float4(group_sum<C>(v.x), group_sum<C>(v.y), group_sum<C>(v.z), group_sum<C>(v.w));
+__device__ __forceinline__ int component(int lane) { return (lane >> 5) + (lane >> 3 & 2); }
+// the way back: all four components in every lane
+__device__ __forceinline__ float4 all_components(float s) {
+    const int i = __builtin_bit_cast(int, s);
+    const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+    const auto p = __builtin_amdgcn_permlane32_swap(r[0], r[0], false, false), q = __builtin_amdgcn_permlane32_swap(r[1], r[1], false, false);
+    const auto f = [](auto x) { return __builtin_bit_cast(float, static_cast<int>(x)); };
+    return make_float4(f(p[0]), f(p[1]), f(q[0]), f(q[1]));
 }
 
 // rows [first, first + n) of sequence b, within the rows there are
@@ -92,7 +101,7 @@ __global__ __launch_bounds__(64 * W) void gdn_batch_kernel(GdnBatchArgs a) {
         for (int k = 0; k < 3; ++k) win[c][k] = rin[static_cast<int64_t>((pos + 1 + k) & 3) * CONV + ch[c]];
     }
     // the state slice
-    const int rg = lane / C, col = 4 * C * wave + 4 * (lane % C);
+    const int rg = lane / C, col = 4 * C * wave + 4 * (lane % C), one = col + component(lane);
     const int64_t soff = static_cast<int64_t>(vh) * kD * kD + (R * rg) * kD + col;
     const float* Sin = a.state_in + b * a.s_state_in + soff;
     float4 s[R];
@@ -173,7 +182,7 @@ __global__ __launch_bounds__(64 * W) void gdn_batch_kernel(GdnBatchArgs a) {
         lds_barrier();
         for (int t = 0; t < m; ++t) {
             const float alpha = ab_s[t][0], beta = ab_s[t][1], kq = ab_s[t][2];
-            const float4 v = *reinterpret_cast<const float4*>(&x_s[t][2 * kD + col]);
+            const float v = x_s[t][2 * kD + one];
             float kn[R], qn[R];
 #pragma unroll
             for (int j = 0; j < R; j += 4) {
@@ -189,13 +198,14 @@ __global__ __launch_bounds__(64 * W) void gdn_batch_kernel(GdnBatchArgs a) {
                 km.x += s[i].x * kn[i], km.y += s[i].y * kn[i], km.z += s[i].z * kn[i], km.w += s[i].w * kn[i];
                 o.x += s[i].x * qn[i], o.y += s[i].y * qn[i], o.z += s[i].z * qn[i], o.w += s[i].w * qn[i];
             }
-            km = group_sum4<C>(km);
-            o = group_sum4<C>(o);
-            const float4 d = make_float4((v.x - km.x) * beta, (v.y - km.y) * beta, (v.z - km.z) * beta, (v.w - km.w) * beta);
+            // (a lane forms one component of d and of the readout)
+            const float d1 = (v - group_sums<C>(km)) * beta;
+            const float4 d = all_components(d1);
 #pragma unroll
             for (int i = 0; i < R; ++i)
                 s[i].x += kn[i] * d.x, s[i].y += kn[i] * d.y, s[i].z += kn[i] * d.z, s[i].w += kn[i] * d.w;
-            if (rg == 0) *reinterpret_cast<float4*>(&o_s[t][col]) = make_float4(o.x + kq * d.x, o.y + kq * d.y, o.z + kq * d.z, o.w + kq * d.w);
+            const float o1 = group_sums<C>(o) + kq * d1;
+            if ((lane & 15) < C) o_s[t][one] = o1;
         }
         lds_barrier();
         // readout, with the gated norm (src/forward_pass.cpp:86-93) where there is one
