@@ -249,9 +249,10 @@ __global__ __launch_bounds__(256) void gdn_batch_ring_kernel(GdnBatchArgs a) {
 
 hipError_t launch_gdn_batch(const GdnBatchArgs& a, hipStream_t s) {
     const dim3 grid(a.VH, a.B);
-    // eight waves a head where every workgroup has a compute unit to itself (3 sequences of 16 heads, 8
-    // tokens: 14.6 us with four, 13.2 with eight), else four (64 sequences, 1 token: 24.6 against 27.3)
-    const bool few = static_cast<int64_t>(a.VH) * a.B <= device_cu_count();
+    // eight waves a head while the token loop bounds the time, else four. Eight and four waves: 3 sequences
+    // of 16 heads, 8 tokens, 13.2 us and 14.6; 20 of 0..8 19.0 and 20.3, 40 26.5 and 29.3, 64 34.4 and
+    // 34.0; of one token 18 10.9 and 10.6, 64 26.9 and 24.2
+    const bool few = static_cast<int64_t>(a.VH) * a.B <= device_cu_count() * (a.row0 ? 3 : 1);
     if (!a.row0) {
         if (few) klaunch(gdn_batch_kernel<true, 8>, grid, 512, 0, s, a);
         else klaunch(gdn_batch_kernel<true, 4>, grid, 256, 0, s, a);
