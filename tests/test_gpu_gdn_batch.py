@@ -210,3 +210,15 @@ def test_captured(hip):
             res.append(outs)
     for i, (u, v) in enumerate(zip(*res)):
         assert all(np.array_equal(u[c], v[c]) for c in u), i
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("fork", [False, True])
+@pytest.mark.parametrize("KH,VH", [(8, 16), (16, 16)])
+def test_many_sequences(hip, KH, VH, fork, norm):
+    """More workgroups than the chip holds at three a compute unit: four waves a head."""
+    counts = np.random.default_rng(VH + KH).integers(0, 12, 60).tolist()
+    x = make(KH, VH, counts, seed=KH, norm=norm, fork=fork)
+    x["pos"][[3, 59]] = -1
+    with device(hip, x) as bufs:
+        check(x, call(hip, bufs, x, len(x["out"]), fork), fork)
