@@ -661,12 +661,16 @@ __device__ __forceinline__ void f32_wide(const AttnBatchArgs& a, const Item& it,
         if (wave < 4) next();
         float p[8], f = 1.0f;
         if (live) {
+            __builtin_amdgcn_s_setprio(1);  // products before the other wave's vector work: 2% of the whole
             f32_scores(tiles[cur], q, r16, g4, p);
+            __builtin_amdgcn_s_setprio(0);
             mask_tail(p, k0, it.hi, g4);
             f = softmax_step(p, q.scale, m, l);
         }
         if (wave >= 4) next();
+        __builtin_amdgcn_s_setprio(1);
         if (live) f32_output(tiles[cur], p, f, r16, g4, exp, o);
+        __builtin_amdgcn_s_setprio(0);
         cur ^= 1;
         lds_barrier();  // every wave is done with this tile, every share of the next one is in
     }
