@@ -566,9 +566,18 @@ __device__ __forceinline__ void f32_output(const F32Tile& tile, float (&p)[8], f
     const int e = row_exp(__float_as_uint(query_max(max8(p))));  // the largest weight is brought to [2^14, 2^15)
     const bool move = f != 1.0f || e < exp;
     if (__any(move)) {
-        // up no further than keeps what O holds, at most 2^60, within 2^90 (terms that much larger hide these)
-        const int most = exp + (f > 0.0f ? 157 - static_cast<int>(__float_as_uint(f) >> 23) : 400);
-        const int to = move ? min(e, most) : exp, step = to - exp;
+        int to = move ? e : exp;
+        if (__any(to > exp && f > 0.0f)) {
+            // up no further than keeps O, by its present largest, below 2^90 (a tile adds less than 2^36, and
+            // terms that it would take further are below 2^-59 of that largest)
+            float mx = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                mx = fmaxf(fmaxf(fmaxf(mx, fabsf(o[t][0])), fmaxf(fabsf(o[t][1]), fabsf(o[t][2]))), fabsf(o[t][3]));
+            mx = query_max(mx) * f;
+            if (mx > 0.0f) to = min(to, exp + max(216 - static_cast<int>(__float_as_uint(mx) >> 23), 0));
+        }
+        const int step = to - exp;
         const int s1 = min(max(step, -126), 126), s2 = min(max(step - s1, -126), 126);
         const float g = (f * pow2(s1)) * pow2(s2);
 #pragma unroll
