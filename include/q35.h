@@ -459,8 +459,9 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  * among them. Results do not depend on the order in which workgroups run. Sums are fp32. bf16
  * caches and fp32 own caches enter exactly; an fp32 prefix that more than 16 query rows share
  * enters as two fp16 parts a row, each product off by at most 2^-21 of itself and 2^-38 of the
- * product of both rows' largest entries, and a row of it with an infinity, a NaN or an entry of
- * 2^115 or more makes the outputs over it NaN. Requires HD == 256, NQ / NKV at most 16, an even
+ * product of both rows' largest entries (taken as 2^-86, of value rows 2^-71, where they are
+ * smaller), and a row of it with an infinity, a NaN or an entry of 2^115 or more makes the
+ * outputs over it NaN. Requires HD == 256, NQ / NKV at most 16, an even
  * rotary_dim, and 16-byte aligned fp32 rows and caches. */
 typedef struct q35_attn_batch_args {
     int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;

@@ -37,6 +37,9 @@ __device__ __forceinline__ int row_exp(uint32_t bits) { return min(max(141 - sta
 // what undoes it; NaN for a row of 2^115 or more, an infinity or a NaN (whose other entries the parts
 // would lose, and the row's outputs be finite and wrong)
 __device__ __forceinline__ float row_scale(uint32_t bits, int e) { return bits < 0x79000000u ? pow2(-e) : NAN; }
+// Scores are formed over 2^kScoreExp times their query's scale: a sum of scaled products (below 2^39) times
+// its key's 2^100 at most then stays below 2^123.
+constexpr int kScoreExp = 16;
 
 // theta^(-2i / ROT), formed on the host: 32 double-precision powers cost the kernel 1 us
 struct RopeFreq {
@@ -63,7 +66,7 @@ __device__ __forceinline__ void store_query(const AttnBatchArgs& a, int64_t row,
     split2h_pair(y.z * pow2(e), y.w * pow2(e), h.y, l.y);
     static_cast<uint2*>(a.Qs)[(row * 2 + 0) * 64 + lane] = h;
     static_cast<uint2*>(a.Qs)[(row * 2 + 1) * 64 + lane] = l;
-    if (lane == 0) a.Qscale[row] = row_scale(__float_as_uint(mx), e);
+    if (lane == 0) a.Qscale[row] = row_scale(__float_as_uint(mx), e - kScoreExp);
 }
 
 // grid ((NQ + NKV) / 4, B), a wave per row: rmsnorm (1 + w) + RoPE of a query row, or of the new key
@@ -505,7 +508,7 @@ __device__ __forceinline__ void f32_stage(F32Tile& tile, bool v, int row, int c,
 #pragma unroll
         for (int q = 0; q < 2; ++q) (v ? tile.V : tile.K)[q][at + 16 * i] = __builtin_bit_cast(uint4, p[q]);
     }
-    if (c == 0) (v ? tile.vscale : tile.kscale)[row] = row_scale(mx, e);
+    if (c == 0) (v ? tile.vscale : tile.kscale)[row] = row_scale(mx, v ? e : e + kScoreExp);
 }
 
 // Byte address in LDS, to be offset by exclusive or.
@@ -517,7 +520,7 @@ __device__ __forceinline__ X lds_read(uint32_t at) {
     return *reinterpret_cast<__attribute__((address_space(3))) const X*>(static_cast<uintptr_t>(at));
 }
 
-// Scores of query r16 of the wave, over its scale: keys 4 g4 + v of the tile's first half, then of
+// Scores of query r16 of the wave, over its scale (the stored one, with 2^kScoreExp): keys 4 g4 + v of the tile's first half, then of
 // its second.
 __device__ __forceinline__ void f32_scores(const F32Tile& tile, const F32Query& q, int r16, int g4, float (&p)[8]) {
     uint32_t ko = lds_at(&tile) + k_off(r16, g4);

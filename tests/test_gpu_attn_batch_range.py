@@ -38,3 +38,27 @@ def test_large_values_before_small_ones(hip, small, large):
         x["k_prefix"][kv] = k + np.outer(8.5 * (tile - 7.5) * 16.0 / np.linalg.norm(q), u)
     x["v_prefix"] *= np.where(tile % 8 == 0, large, small).astype(np.float32)[None, :, None]
     run(hip, x, P, False, bar=15 * REL_L2)
+
+
+@pytest.mark.parametrize("nq", [16, 2])
+@pytest.mark.parametrize("power", [60, 100, 110, 112])
+def test_large_keys(hip, power, nq):
+    """One key row, or every one, times 2^power: entries up to 2^114, scores up to 2^113. The softmax is
+    then 1 at one key and 0 at all others (for scores of that size to be within 2^7 of one another
+    they would have to agree in 50 bits), so that no rounding reaches the outputs."""
+    x = make(nq, 2, 500, [20, 40, 0, 30, 12, 9, 5, 3], 64, seed=22)
+    rows = x["k_prefix"].copy()
+    x["k_prefix"][:, 77] *= np.float32(2.0 ** power)
+    run(hip, x, 500, False)
+    x["k_prefix"] = rows * np.float32(2.0 ** power)
+    run(hip, x, 500, False)
+
+
+@pytest.mark.parametrize("nq", [16, 2])
+@pytest.mark.parametrize("size", [2.0 ** 114, -2.0 ** 114])
+def test_key_entry_along_the_query(hip, size, nq):
+    """A key entry of 2^114 where the queries have their largest entry."""
+    x = make(nq, 2, 300, [20, 40, 0, 30, 12, 9, 5, 3], 64, seed=23)
+    x["qg"][..., 200] = 12.0
+    x["k_prefix"][1, 40, 200] = size
+    run(hip, x, 300, False)
