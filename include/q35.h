@@ -461,7 +461,10 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  * enters as two fp16 parts a row, each product off by at most 2^-21 of itself and 2^-38 of the
  * product of both rows' largest entries (taken as 2^-86, of value rows 2^-71, where they are
  * smaller), and a row of it with an infinity, a NaN or an entry of 2^115 or more makes the
- * outputs over it NaN. Requires HD == 256, NQ / NKV at most 16, an even
+ * outputs over it NaN. Elsewhere a key whose score is -inf has weight 0; an infinity in a bf16
+ * cache, or in any value row, may make NaN what is a number or an infinity by the definition.
+ * Weights are summed before they are divided, and reach e^8: value entries of 2^116 and more
+ * may overflow, over n rows of like weight those of 2^116 / n. Requires HD == 256, NQ / NKV at most 16, an even
  * rotary_dim, and 16-byte aligned fp32 rows and caches. */
 typedef struct q35_attn_batch_args {
     int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;

@@ -238,7 +238,9 @@ __device__ __forceinline__ float query_sum(float v) {
 // power of two `unit`: s becomes weights, (m, l) the query's running maximum (in the units of s) and
 // sum. Returns the factor of the output so far. The reference maximum moves only when a score
 // exceeds it by more than 8 / unit, so weights reach e^8. e^y as the native 2^(y log2 e) of the
-// exactly formed exponent. Every call holds a key of every query: a maximum is never -inf.
+// exactly formed exponent. The maximum starts at kNoMax: with a score of -inf alone it stays there, and the
+// weight is 0.
+constexpr float kNoMax = -3.402823466e38f;  // the lowest float
 template <int N>
 __device__ __forceinline__ float softmax_step(float (&s)[N], float unit, float& m, float& l) {
     float tm;
@@ -420,7 +422,7 @@ __global__ __launch_bounds__(256, 2) void attn_batch_bf16_kernel(AttnBatchArgs a
     const int first = it.narrow ? it.row0 : it.row0 + 16 * wave;
     bf16x8 qp[3][8];
     load_query(a, it, first, r16, g4, qp);
-    float m = -INFINITY, l = 0.0f;
+    float m = kNoMax, l = 0.0f;
     auto walk = [&](auto& o, int t0, float* raw, bool live) {
 #pragma unroll
         for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -656,7 +658,7 @@ __device__ __forceinline__ void f32_wide(const AttnBatchArgs& a, const Item& it,
     q.scale = a.Qscale[it.q0 + min(first + r16, it.rows - 1)];
     stage(tiles[0]);
     load(it.lo + kKT);  // (past the end: the last row again)
-    float m = -INFINITY, l = 0.0f;
+    float m = kNoMax, l = 0.0f;
     int exp = 100;
     floatx4 o[16];
 #pragma unroll
@@ -732,7 +734,7 @@ __device__ __forceinline__ void f32_narrow(const AttnBatchArgs& a, const Item& i
         *reinterpret_cast<float4*>(buf + (2 * wave + i) * kHD + 4 * (lane ^ (2 * wave + i))) = qrow[i];
     lds_barrier();
     float* raw = it.raw && r16 < it.rows ? it.raw + r16 * it.raw_stride : nullptr;
-    float m = -INFINITY, l = 0.0f;
+    float m = kNoMax, l = 0.0f;
     floatx4 o[16];
 #pragma unroll
     for (auto& x : o) x = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -772,7 +774,7 @@ __device__ __forceinline__ void f32_narrow(const AttnBatchArgs& a, const Item& i
         __builtin_amdgcn_sched_barrier(0);
         if (more) load_v(k0 + 128);
     }
-    // merge of the waves; one without keys has maximum -inf and weight 0
+    // merge of the waves; one without keys has maximum kNoMax, and output and sum 0
     if (g4 == 0) {
         ms[wave][r16] = m;
         ls[wave][r16] = l;
@@ -781,14 +783,12 @@ __device__ __forceinline__ void f32_narrow(const AttnBatchArgs& a, const Item& i
     float top = ms[0][r16];
 #pragma unroll
     for (int w = 1; w < 8; ++w) top = fmaxf(top, ms[w][r16]);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * kLog2e);
-    rescale(f, o);
+    rescale(__builtin_amdgcn_exp2f((m - top) * kLog2e), o);
     const int n = min(16, it.rows - it.row0);
     if (wave == 0 && g4 == 0 && r16 < n) {
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
-            if (ms[w][r16] != -INFINITY) sum += ls[w][r16] * __builtin_amdgcn_exp2f((ms[w][r16] - top) * kLog2e);
+        for (int w = 0; w < 8; ++w) sum += ls[w][r16] * __builtin_amdgcn_exp2f((ms[w][r16] - top) * kLog2e);
         it.ml[it.row0 + r16] = make_float2(top, sum);
     }
     // (rows' 16-byte chunks c at c ^ row % 16: the 16 lanes of a store lie on all banks)
