@@ -464,8 +464,10 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  * outputs over it NaN. Elsewhere a key whose score is -inf has weight 0; an infinity in a bf16
  * cache, or in any value row, may make NaN what is a number or an infinity by the definition.
  * Weights are summed before they are divided, and reach e^8: value entries of 2^116 and more
- * may overflow, over n rows of like weight those of 2^116 / n. Requires HD == 256, NQ / NKV at most 16, an even
- * rotary_dim, and 16-byte aligned fp32 rows and caches. */
+ * may overflow, over n rows of like weight those of 2^116 / n.
+ * Requires HD == 256, NQ / NKV at most 16, an even rotary_dim, and 16-byte aligned fp32 rows and
+ * caches. A launch holds 2^23 - 1 workgroups: batch * NQ (with own_score, and a workgroup for
+ * every 512 rows of capacity of every own cache) beyond that is refused. */
 typedef struct q35_attn_batch_args {
     int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;
     int32_t kv_dtype;      /* elements of both caches: 0 = fp32, 1 = bf16 (appended rows rounded to nearest even) */

@@ -101,6 +101,9 @@ q35_status q35_attn_batch(const q35_attn_batch_args* args, q35_stream s) {
     q35_status st = attn_batch_sizes(args, who, &a);
     if (st != Q35_OK) return st;
     const q35_attn_batch_args& g = *args;
+    if (!q35k::attn_batch_launches(a))
+        return q35::fail(Q35_ERR_UNSUPPORTED, "%s: batch %d of %d / %d heads is more than one launch holds", who, g.batch,
+                         g.q_heads, g.kv_heads);
     if (!g.own_len || !g.pos || !g.qg || !g.k_new || !g.v_new || !g.q_norm || !g.k_norm || !g.k_own || !g.v_own ||
         !g.out || !g.workspace || (g.prefix_len > 0 && (!g.k_prefix || !g.v_prefix)))
         return q35::fail(Q35_ERR_ARG, "%s: null pointer", who);

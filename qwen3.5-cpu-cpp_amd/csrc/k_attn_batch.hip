@@ -961,6 +961,14 @@ void attn_batch_carve(AttnBatchArgs& a, float* ws) {
     a.raw = ws + c.raw;
 }
 
+bool attn_batch_launches(const AttnBatchArgs& a) {
+    const AttnBatchPlan p = attn_batch_plan(a.B, a.GRP, a.NKV, a.P, a.cap, a.kv_bf16, device_cu_count());
+    const int64_t pairs = static_cast<int64_t>(a.B) * a.NKV, most = UINT32_MAX;  // threads of a launch
+    const int64_t attend = (static_cast<int64_t>(p.pieces) * a.NKV + 7) / 8 * 8 * p.nblk + pairs * p.own;
+    const int64_t combine = static_cast<int64_t>(a.B) * a.NQ + (a.own_score ? (a.cap + 511) / 512 * pairs : 0);
+    return attend <= most / (a.kv_bf16 ? 256 : 512) && combine <= most / (kCombWaves * 64);
+}
+
 hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s) {
     // a function of theta and the width alone, kept for the next call of this host thread
     static thread_local RopeFreq freq;

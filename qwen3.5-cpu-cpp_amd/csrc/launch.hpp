@@ -316,6 +316,8 @@ struct AttnBatchArgs {
 };
 int64_t attn_batch_workspace_floats(const AttnBatchArgs& a);
 void attn_batch_carve(AttnBatchArgs& a, float* ws);
+// whether every launch of the call stays below the 2^32 threads that a grid's dimension holds
+bool attn_batch_launches(const AttnBatchArgs& a);
 hipError_t launch_attn_batch(const AttnBatchArgs& a, hipStream_t s);
 
 // Eviction by score: the select kernel chooses, the move kernel copies.
