@@ -454,8 +454,8 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  *     new row's entry is set to its weight (q35_kv_evict's order)
  *   own_pos [batch][NKV][own_capacity], may be NULL: receives pos[b] at the new slot
  *   out [batch][NQ][HD]
- * workspace (16-byte aligned): q35_attn_batch_workspace_bytes() bytes; its size depends on
- * sizes alone, never on the lengths. A captured graph holds the sizes of its capture, prefix_len
+ * workspace (16-byte aligned): q35_attn_batch_workspace_bytes() bytes; that depends on the sizes
+ * and on whether own_score is given, never on the lengths. A captured graph holds the sizes of its capture, prefix_len
  * among them. Results do not depend on the order in which workgroups run. Sums are fp32. bf16
  * caches and fp32 own caches enter exactly; an fp32 prefix that more than 16 query rows share
  * enters as two fp16 parts a row, each product off by at most 2^-21 of itself and 2^-38 of the
