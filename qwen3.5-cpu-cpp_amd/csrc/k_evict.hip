@@ -5,7 +5,8 @@
 //
 // Choosing is a radix selection of the keep-th largest 32-bit key over 11 + 11 + 10 bits with
 // histograms in LDS (after the first 11 mostly few keys are left, which are then compared with one
-// another: 1152 rows 8.0 -> 6.3 us), then a pass that ranks the rows in slot order: of the rows equal to that
+// another: 1152 rows 10.0 us a call, 11.3 by three passes; with up to 64 keys for few instead of 256
+// the same), then a pass that ranks the rows in slot order: of the rows equal to that
 // key the lowest slots stay, and the number of rows kept before a row gives its place in the move
 // lists. Up to kRegRows rows one workgroup holds all keys in registers and does it in one
 // launch. Longer caches are cut into slices of kSlice rows, a workgroup each, in three launches:
@@ -13,7 +14,12 @@
 // slice's keys that lie in it (candidates); from all candidates the key itself, and the slice's
 // ranks. What every slice needs of the others it forms for itself, so no launch has a single
 // workgroup: 131072 rows of two heads 22 us against 56 with one workgroup that
-// finds the key and slices that count the rows before them.
+// finds the key and slices that count the rows before them. One workgroup and slices, whole calls in us, bf16
+// caches of two heads cut to 7/8, 1 / 4 / 24 sequences: 4096 rows 12.1 / 13.0 / 19.4 and 19.5 / 20.4 / 27.4; 4097
+// (16 keys a thread instead of 4) 19.3 / 20.4 / 27.2 and 19.6 / 21.3 / 29.8; 8192 21.9 / 23.6 / 37.1 and 20.8 /
+// 22.0 / 37.9; 16384 26.7 / 28.9 / 57.5 and 21.6 / 25.0 / 55.4; beyond, 16385 and 32768 rows of one sequence
+// 22.3 and 24.5. So the border is where the registers end, and slices would do for a few sequences from 6000
+// rows on.
 #include "dev_common.hpp"
 #include "launch.hpp"
 

@@ -215,15 +215,23 @@ constexpr int batch_wide(bool kv_bf16) { return kv_bf16 ? 64 : 128; }      // of
 // units: a tile of 32 keys takes a bf16 workgroup 1.65 alone on its compute unit and 2.7 beside another
 // (64 rows; two fit), an fp32 one 3.1 (128 rows; one fits), a start and an end 8; an own cache's tile
 // 1.8 and 2.0; a partial output costs its bytes at 2.2 TB/s, written and merged. Of the piece lengths
-// the fastest by that is taken, the own caches running where the prefix leaves room: 48 sequences of
-// 16 / 2 heads after 30001 fp32 positions with own caches of 1000, attention and merge with pieces of
-// 640 keys 160 us (a second round of workgroups), 768 128, 896 128, 960 113, 1024 119, 1280 136; without
-// own rows 768 105, 1024 114; bf16 512 94, 640 100, 768 87, 896 86, 1280 103, 1504 88. With 16 rows or
-// fewer the loads bound the time, and pieces are made for 7/8 of the compute units: 2 after 30001 fp32
-// ones, 128 keys 46 us, 256 35, 512 44.
+// the fastest by that is taken, the own caches running where the prefix leaves room. Whole calls in us: 48
+// sequences of 16 / 2 heads after 30001 fp32 positions with own caches of 1000, pieces of 640 keys 160 (a
+// second round of workgroups), 768 129, 896 134, 960 (taken) 118, 1024 120, 1280 139; without own rows 640
+// 155, 768 107, 800 (taken) 107, 896 107, 960 112, 1024 117, 1280 137; bf16 512 89, 640 99, 768 81, 800
+// (taken) 82, 896 85, 1280 104, 1504 90. With 16 rows or fewer the loads bound the time, and pieces are made for 7/8 of the
+// compute units: 2 after 30001 fp32 ones, 128 keys 49 us, 256 38, 288 (taken) 39, 512 46.
+// Up to 16 query rows (kBatchNarrow) blocks are narrow, where fp32 rows are multiplied as they are; more rows go
+// into wide blocks, whatever the prefix's length. Narrow blocks (of 16 rows, in the fastest pieces for them)
+// and wide ones, 8 / 2 heads, whole calls after 700, 5003 and 30001 positions: fp32, 8 rows 16.1 and 15.9, 20.2
+// and 20.0, 39.3 and 37.6; 16 rows 16.4 and 16.2, 20.6 and 20.6, 40.0 and 39.0; 20 rows 16.5 and 16.6, 21.6
+// and 21.2, 49 and 39.7; 64 rows 17.2 and 19.4, 24.3 and 24.5, 82 and 46. bf16, 8 rows 13.6 and 13.6, 17.2 and
+// 16.8, 26.4 and 27.3; 16 rows 14.9 and 14.1, 18.8 and 17.6, 27.7 and 27.9; 20 rows 14.9 and 14.5, 18.3 and
+// 18.1, 33 and 29; 64 rows 15.5 and 17.5, 21.4 and 21.5, 45 and 34.
 // Own caches are taken to be half full: pieces are made for 3/4 of the compute units (bf16, of which
-// two fit: 3/2) to have one that is not empty. 48 caches of 1000 fp32 rows: pieces of 128 39 us, 320
-// 28, 512 36; 32 of 2304 bf16 ones: 96 30, 224 25, 320 28; 24 of 2304 with 8 heads: 96 23, 160 20, 320 26.
+// two fit: 3/2) to have one that is not empty. 48 caches of 1000 fp32 rows: pieces of 128 49 us, 320
+// 38, 352 (taken) 40, 512 45; 32 of 2304 bf16 ones: 96 33, 224 (taken) 28, 320 32; 24 of 2304 with 8 heads:
+// 96 26, 160 (taken) 23, 320 29.
 inline AttnBatchPlan attn_batch_plan(int B, int GRP, int NKV, int64_t P, int64_t cap, bool kv_bf16, int n_cu) {
     const auto up = [](int64_t x, int64_t m) { return (x + m - 1) / m; };
     const int64_t rows = static_cast<int64_t>(B) * GRP, pairs = static_cast<int64_t>(B) * NKV, most = 2 * n_cu;
