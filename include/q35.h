@@ -455,16 +455,16 @@ q35_status q35_attn_prefill(const q35_attn_prefill_args *args, q35_stream s);
  *   own_pos [batch][NKV][own_capacity], may be NULL: receives pos[b] at the new slot
  *   out [batch][NQ][HD]
  * workspace (16-byte aligned): q35_attn_batch_workspace_bytes() bytes; that depends on the sizes
- * and on whether own_score is given, never on the lengths. A captured graph holds the sizes of its capture, prefix_len
- * among them. Results do not depend on the order in which workgroups run. Sums are fp32. bf16
- * caches and fp32 own caches enter exactly; an fp32 prefix that more than 16 query rows share
- * enters as two fp16 parts a row, each product off by at most 2^-21 of itself and 2^-38 of the
- * product of both rows' largest entries (taken as 2^-86, of value rows 2^-71, where they are
- * smaller), and a row of it with an infinity, a NaN or an entry of 2^115 or more makes the
- * outputs over it NaN. Elsewhere a key whose score is -inf has weight 0; an infinity in a bf16
- * cache, or in any value row, may make NaN what is a number or an infinity by the definition.
- * Weights are summed before they are divided, and reach e^8: value entries of 2^116 and more
- * may overflow, over n rows of like weight those of 2^116 / n.
+ * and on whether own_score is given, never on the lengths. A captured graph holds the sizes of
+ * its capture, prefix_len among them. Results do not depend on the order in which workgroups
+ * run. Sums are fp32. bf16 caches and fp32 own caches enter exactly; an fp32 prefix that more
+ * than 16 query rows share enters as two fp16 parts a row, each product off by at most 2^-21 of
+ * itself and 2^-38 of the product of both rows' largest entries (taken as 2^-86, of value rows
+ * 2^-71, where they are smaller), and a row of it with an infinity, a NaN or an entry of 2^115
+ * or more makes the outputs over it NaN. Elsewhere a key whose score is -inf has weight 0; an
+ * infinity in a bf16 cache, or in any value row, may make NaN what is a number or an infinity by
+ * the definition. Weights are summed before they are divided, and reach e^8: value entries of
+ * 2^116 and more may overflow, over n rows of like weight those of 2^116 / n.
  * Requires HD == 256, NQ / NKV at most 16, an even rotary_dim, and 16-byte aligned fp32 rows and
  * caches. A launch holds 2^23 - 1 workgroups: batch * NQ (with own_score, and a workgroup for
  * every 512 rows of capacity of every own cache) beyond that is refused. */
