@@ -560,6 +560,129 @@ typedef struct q35_gdn_batch_args {
 } q35_gdn_batch_args;
 q35_status q35_gdn_batch(const q35_gdn_batch_args *args, q35_stream s);
 
+/* ------------------------------------------------------------------------------------ */
+/* a decode step held in 4 bits                                                          */
+/* ------------------------------------------------------------------------------------ */
+/* Products with 4-bit weights, attention over a cache of 4-bit rows and the draw of a token (the
+ * reference has none of them). Device arrays, one captured graph for every step, calls that overlap in
+ * time with a workspace each: as in the section above. */
+
+/* 4-bit weights: w[n][k] = scale[n][g] * (code[n][k] - zero[n][g]), g = k / group, groups of 32, 64 or 128
+ * (the last of a row may be cut short), codes and zeros 0 .. 15.
+ *   codes [N][(K + 1) / 2]: k even in the low four bits of byte k / 2, k odd in the high four
+ *   scales [N][ceil(K / group)] fp16; zeros the same shape, NULL: 8 everywhere (of a value above 15 the
+ *     low four bits count)
+ * q35_q4_quantize makes them from bf16 (w_dtype 1) or fp32 (0) weights W [N][K]. With zeros NULL the entry
+ * of a group that is largest in magnitude becomes code 0: scale = fp16(-entry / 8) (it may be negative). With
+ * zeros a group's codes span [min(least, 0), max(largest, 0)]: scale = fp16(span / 15), zero =
+ * round(-least / scale). code = round(w / scale) + zero, kept within 0 .. 15; fp32 arithmetic, halves to
+ * even. A group with an infinity or a NaN gets scale NaN, one whose scale rounds to 0 the value 0.
+ * q35_q4_pack lays such weights out for q35_matmul_q4, once: q35_q4_packed_bytes() bytes, 16-byte aligned,
+ * of tiles of 16 rows by 256 k with their scales (0 for refused sizes). N * K, padded to such tiles, is at
+ * most 2^32. */
+uint64_t q35_q4_packed_bytes(int32_t N, int32_t K, int32_t group, int32_t has_zeros);
+q35_status q35_q4_quantize(const void *W, int32_t w_dtype, int32_t N, int32_t K, int32_t group, uint8_t *codes,
+                           uint16_t *scales, uint8_t *zeros, q35_stream s);
+q35_status q35_q4_pack(const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, int32_t N, int32_t K,
+                       int32_t group, void *packed, q35_stream s);
+/* Y[M][N] = (R ? R : 0) + X[M][K] . w[N][K]^T for packed weights w: q35_matmul_bf16 (M = 1) and q35_gemm_bf16
+ * for 4-bit weights, fp32 X / R / Y with leading dimensions (elements). has_zeros (0 or 1) and group as they
+ * were packed. R may be Y itself. workspace (16-byte aligned): q35_matmul_q4_workspace_bytes() bytes.
+ * Meant for the rows of a decode step (one to some dozens); M is at most Q35_MATMUL_Q4_MOST_ROWS. */
+#define Q35_MATMUL_Q4_MOST_ROWS 4096
+uint64_t q35_matmul_q4_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t group);
+q35_status q35_matmul_q4(const float *X, int64_t ldx, const void *packed, int32_t has_zeros, int32_t M, int32_t N,
+                         int32_t K, int32_t group, const float *R, int64_t ldr, float *Y, int64_t ldy,
+                         void *workspace, uint64_t workspace_bytes, q35_stream s);
+
+/* 4-bit cache rows: a row of 256 values is 128 bytes of codes (value 2 i in the low four bits of byte i)
+ * and, for each 64 values, (step, least) as two fp16: x = least + step * code. Caches are
+ *   k, v [batch][NKV][capacity][128] bytes, k_scale, v_scale [batch][NKV][capacity][4][2] fp16
+ * Quantizing: least = fp16(min), step = fp16((max - least) / 15) (both through fp32), code = round((x -
+ * least) / step), kept within 0 .. 15, halves to even, in 64 bits. A group with an infinity or a NaN, or whose
+ * least or step exceeds fp16, gets NaN for both.
+ *
+ * Gated GQA attention for one token per sequence, each over its own cache: q35_attn_decode for a batch,
+ * on such caches. The new row is quantized and appended, and attended as it then is.
+ *   qg [batch][NQ][2*HD] (per head: q then gate), k_new, v_new [batch][NKV][HD]; rows from len[b] on are not read
+ *   len (device) [batch]: rows in the cache before this call; the new row goes to slot len[b] (the array is
+ *     left as it is). A negative entry marks an empty place: nothing of it is written, and what its
+ *     rows hold does not matter. An entry at or above capacity is a caller's mistake: nothing is
+ *     appended and its out rows are NaN.
+ *   pos (device) [batch]: RoPE position of the new token
+ *   out [batch][NQ][HD]
+ * workspace (16-byte aligned): q35_attn_q4_workspace_bytes() bytes; that depends on the sizes, never on the
+ * lengths. Results do not depend on the order in which workgroups run.
+ * Requires HD == 256, NQ / NKV at most 16, an even rotary_dim, 16-byte aligned arrays. */
+typedef struct q35_attn_q4_args {
+    int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;
+    int32_t reserved;
+    int64_t capacity;
+    double rope_theta;
+    float eps;
+    const int32_t *len, *pos;
+    const float *qg, *k_new, *v_new, *q_norm, *k_norm;
+    uint8_t *k, *v;
+    void *k_scale, *v_scale;
+    float *out;
+    void *workspace;
+    uint64_t workspace_bytes;
+} q35_attn_q4_args;
+uint64_t q35_attn_q4_workspace_bytes(const q35_attn_q4_args *args);
+q35_status q35_attn_q4(const q35_attn_q4_args *args, q35_stream s);
+
+/* Rows begin[b] .. end[b] - 1 of every sequence's cache, all heads, K and V, from an fp32 or bf16 cache
+ * (q35_attn_prefill's, q35_attn_batch's) into the same slots of its 4-bit cache (store), or from there back
+ * (load: so that a prefill can go on from it; bf16 rounded to nearest even).
+ *   begin, end (device) [batch]; begin NULL: 0. Nothing of a sequence is touched where end <= begin, begin < 0
+ *     or end exceeds either capacity.
+ *   k_rows, v_rows [batch][NKV][rows_capacity][HD]; with shared_rows = 1 (store alone) [NKV][rows_capacity][HD],
+ *     one prompt's for all sequences
+ * What is written may overlap no other array. Requires HD == 256 and 16-byte aligned caches. */
+typedef struct q35_kv_q4_args {
+    int32_t batch, kv_heads, head_dim;
+    int32_t kv_dtype;      /* elements of k_rows, v_rows: 0 = fp32, 1 = bf16 */
+    int32_t shared_rows, reserved;
+    int64_t rows_capacity, capacity;
+    const int32_t *begin, *end;
+    void *k_rows, *v_rows;
+    uint8_t *k, *v;
+    void *k_scale, *v_scale;
+} q35_kv_q4_args;
+q35_status q35_kv_q4_store(const q35_kv_q4_args *args, q35_stream s);
+q35_status q35_kv_q4_load(const q35_kv_q4_args *args, q35_stream s);
+
+/* One token a row of logits. The candidates are ranked by logit, equal ones by id, and weighted by
+ * exp((l - largest) / temperature); then each filter keeps a prefix of the ranking, never less than the
+ * first candidate:
+ *   top_k: the first top_k candidates (0 or less: all)
+ *   top_p: of these, every candidate before which less than top_p of their weight lies (1 or more: all)
+ *   min_p: of these, those with at least min_p times the first one's weight (0 or less: all)
+ * The token is the first of the ranking at which the running weight exceeds u times the weight that is
+ * left. Weights are whole multiples of 2^-50 of the largest or, of 2^n > 4096 candidates, of 2^(n - 62), and
+ * their sums are exact.
+ *   logits [batch][ld_logits]; -inf rules a candidate out, a NaN counts as -inf, +inf takes all the weight
+ *   temperature (device) [batch]: 0 takes the first candidate (u and the filters do not matter); a negative entry
+ *     or a NaN marks an empty place: nothing of it is written
+ *   top_k, top_p, min_p (device) [batch], each may be NULL: off; a NaN is off
+ *   u (device) [batch]: in [0, 1) (values outside count as the nearest of it, a NaN as 0)
+ *   token [batch]: the id, -1 where every candidate is ruled out
+ *   prob [batch], may be NULL: the share of the token in the weight that is left (0 with token -1)
+ * workspace (16-byte aligned): q35_sample_workspace_bytes() bytes. vocab is at most 2^22. */
+typedef struct q35_sample_args {
+    int32_t batch, vocab;
+    int64_t ld_logits;
+    const float *logits, *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p, *u;
+    int32_t *token;
+    float *prob;
+    void *workspace;
+    uint64_t workspace_bytes;
+} q35_sample_args;
+uint64_t q35_sample_workspace_bytes(const q35_sample_args *args);
+q35_status q35_sample(const q35_sample_args *args, q35_stream s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -124,6 +124,27 @@ class GdnBatchArgs(C.Structure):
         (n, C.c_int64) for n in ("stride_ring", "stride_state")] + [("out", C.c_void_p)]
 
 
+class AttnQ4Args(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in (
+        "batch", "q_heads", "kv_heads", "head_dim", "rotary_dim", "reserved")] + [
+        ("capacity", C.c_int64), ("rope_theta", C.c_double), ("eps", C.c_float)] + [
+        (n, C.c_void_p) for n in ("len", "pos", "qg", "k_new", "v_new", "q_norm", "k_norm", "k", "v", "k_scale",
+                                  "v_scale", "out", "workspace")] + [("workspace_bytes", C.c_uint64)]
+
+
+class KvQ4Args(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in (
+        "batch", "kv_heads", "head_dim", "kv_dtype", "shared_rows", "reserved")] + [
+        (n, C.c_int64) for n in ("rows_capacity", "capacity")] + [
+        (n, C.c_void_p) for n in ("begin", "end", "k_rows", "v_rows", "k", "v", "k_scale", "v_scale")]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("vocab", C.c_int32), ("ld_logits", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("logits", "temperature", "top_k", "top_p", "min_p", "u", "token", "prob",
+                                  "workspace")] + [("workspace_bytes", C.c_uint64)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built: run __graft_entry__.build() "
@@ -203,6 +224,17 @@ def _load():
         "q35_kv_evict_workspace_bytes": (U64, [C.POINTER(KvEvictArgs)]),
         "q35_kv_evict": (S, [C.POINTER(KvEvictArgs), P]),
         "q35_gdn_batch": (S, [C.POINTER(GdnBatchArgs), P]),
+        "q35_q4_packed_bytes": (U64, [I32, I32, I32, I32]),
+        "q35_q4_quantize": (S, [P, I32, I32, I32, I32, P, P, P, P]),
+        "q35_q4_pack": (S, [P, P, P, I32, I32, I32, P, P]),
+        "q35_matmul_q4_workspace_bytes": (U64, [I32, I32, I32, I32]),
+        "q35_matmul_q4": (S, [P, I64, P, I32, I32, I32, I32, I32, P, I64, P, I64, P, U64, P]),
+        "q35_attn_q4_workspace_bytes": (U64, [C.POINTER(AttnQ4Args)]),
+        "q35_attn_q4": (S, [C.POINTER(AttnQ4Args), P]),
+        "q35_kv_q4_store": (S, [C.POINTER(KvQ4Args), P]),
+        "q35_kv_q4_load": (S, [C.POINTER(KvQ4Args), P]),
+        "q35_sample_workspace_bytes": (U64, [C.POINTER(SampleArgs)]),
+        "q35_sample": (S, [C.POINTER(SampleArgs), P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
