@@ -1,6 +1,9 @@
 // Products with 4-bit weights and group scales: Y[m][n] = R[m][n] + sum_g s[n][g] sum_{k in g}
 // X[m][k] (c[n][k] - z[n][g]), and the kernels that make such weights. The layout of packed weights
 // is in launch_q4.hpp.
+#include <mutex>
+#include <type_traits>
+
 #include "dev_common.hpp"
 #include "launch_q4.hpp"
 
@@ -12,39 +15,276 @@ __device__ __forceinline__ float half_bits(uint32_t h) {
 }
 __device__ __forceinline__ uint16_t bits_half(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
 
-// One wave an output, k spread over its lanes.
-__global__ __launch_bounds__(256) void q4_mul_kernel(Q4MulArgs a) {
-    const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + threadIdx.x / 64, m = blockIdx.y;
-    if (n >= a.N) return;
-    const int unit = 2048 + 16 * (256 / a.G) * (a.zeros ? 4 : 2), blocks = (a.K + 255) / 256, r = n & 15;
-    float acc = 0.0f;
-    for (int k = lane; k < a.K; k += 64) {
-        const uint8_t* u = a.W + (static_cast<int64_t>(n / 16) * blocks + k / 256) * unit;
-        const int h = k / 128 % 2, kk = k & 127;
-        int i, c;
-        if (a.G == 32) {
-            i = kk / 32;
-            c = kk / 8 % 4;
-        } else {
-            c = kk / 16 % 4;
-            i = 2 * (kk / 64) + kk / 8 % 2;
-        }
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(u + 1024 * h + 16 * (16 * c + r) + 4 * i);
-        const int j = k & 7, q = static_cast<int>(w << (28 - 8 * (j & 3) - (j & 4))) >> 28;
-        const int g = (k & 255) / a.G;
-        float scale;
-        int zero = 0;
-        if (a.zeros) {
-            const uint32_t s = reinterpret_cast<const uint32_t*>(u + 2048)[r * (256 / a.G) + g];
-            scale = half_bits(s);
-            zero = static_cast<int>(s) >> 16;
-        } else {
-            scale = half_bits(reinterpret_cast<const uint16_t*>(u + 2048)[r * (256 / a.G) + g]);
-        }
-        acc = fmaf(a.X[m * a.ldx + k], scale * static_cast<float>(q - zero), acc);
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 512, kWaves = 8;
+
+// ---- rows of X as whole numbers
+// A group of a row's entries becomes multiples of 2^-e: x = i 2^-e, |i| <= 8355711 = 127 2^16 + 127 2^8 + 127, with
+// the largest entry above 2^21.99, so an entry is off by at most 2^-23 of the largest. Such an i is three
+// signed bytes, i = d2 2^16 + d1 2^8 + d0: integer products with 4-bit codes are exact.
+struct Digits {
+    uint32_t d[3][2];                   // eight entries: plane, four bytes each
+};
+// the multiples of eight entries whose group's largest magnitude has the bits `top`, and 2^-e / 16 (codes are
+// multiplied as 16 times themselves); NaN for a group with an infinity or a NaN
+__device__ __forceinline__ Digits digits8(const float* x, uint32_t top, float& scale) {
+    const float m = __uint_as_float(top);
+    int e = 23 - __builtin_amdgcn_frexp_expf(m);
+    if (ldexpf(m, e) > 8355711.0f) --e;
+    e = min(e, 100);                    // below 2^-100: multiples of that
+    const bool ok = top < 0x7f800000u && top != 0;
+    scale = top >= 0x7f800000u ? NAN : ldexpf(0.0625f, ok ? -e : 0);
+    uint32_t y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int v = ok ? static_cast<int>(rintf(ldexpf(x[i], e))) : 0;
+        y[i] = (static_cast<uint32_t>(v) + 0x8080u) ^ 0x8080u;  // the three signed digits in bytes 0, 1, 2
     }
-    acc = wave_sum(acc);
-    if (lane == 0) a.Y[m * a.ldy + n] = acc + (a.R ? a.R[m * a.ldr + n] : 0.0f);
+    Digits r;
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = 0x0c0c0400u + p * 0x0101u, hi = 0x04000c0cu + p * 0x01010000u;
+            r.d[p][h] = __builtin_amdgcn_perm(y[4 * h + 1], y[4 * h], lo) | __builtin_amdgcn_perm(y[4 * h + 3], y[4 * h + 2], hi);
+        }
+    return r;
+}
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {  // over the G / 8 lanes that hold a group
+    v = max(v, static_cast<uint32_t>(dpp_i<0xB1>(static_cast<int>(v))));
+    v = max(v, static_cast<uint32_t>(dpp_i<0x4E>(static_cast<int>(v))));
+    if constexpr (G >= 64) v = max(v, static_cast<uint32_t>(dpp_i<0x141>(static_cast<int>(v))));
+    if constexpr (G >= 128) v = max(v, static_cast<uint32_t>(dpp_i<0x140>(static_cast<int>(v))));
+    return v;
+}
+template <int G>
+__device__ __forceinline__ int group_sum(int v) {
+    v += dpp_i<0xB1>(v);
+    v += dpp_i<0x4E>(v);
+    if constexpr (G >= 64) v += dpp_i<0x141>(v);
+    if constexpr (G >= 128) v += dpp_i<0x140>(v);
+    return v;
+}
+
+// An image of `rows` rows of X over some blocks of 64 k, the operand of the products as it is read: digit d of
+// row r at k 64 b + 16 c + j in byte ((4 b + c) rows + r) 48 + 16 d + j; then the groups' factors [group][rows],
+// floats, or with zero points four words: the sums of the three digits and the factor's bits.
+template <int G, bool ZP>
+__host__ __device__ constexpr int meta_bytes(int rows, int k) { return rows * (k / G) * (ZP ? 16 : 4); }
+
+// Makes the image of k [k0, k0 + kn) (kn a multiple of 256) with the threads first, first + step, ..
+template <int G, bool ZP>
+__device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, int rows, int k0, int kn, uint8_t* img, uint8_t* meta,
+                                           int first, int step) {
+    const int per = kn / 8;
+    const bool wide = (ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(X) & 15) == 0;
+    for (int id = first; id < rows * per; id += step) {  // 32 lanes are in or out together
+        const int r = id / per, kk = (id % per) * 8, k = k0 + kk;
+        const float* src = X + r * ldx + k;
+        float x[8];
+        if (wide && k + 8 <= K) {
+            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = k + i < K ? src[i] : 0.0f;
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        float scale;
+        const Digits d = digits8(x, group_max<G>(top), scale);
+        uint8_t* at = img + (((kk >> 6) * 4 + (kk >> 4 & 3)) * rows + r) * 48 + (kk & 8);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(at + 16 * p) = make_uint2(d.d[p][0], d.d[p][1]);
+        const int g = kk / G * rows + r;
+        if constexpr (ZP) {
+            int s[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                s[p] = group_sum<G>(__builtin_amdgcn_sdot4(static_cast<int>(d.d[p][1]), 0x01010101,
+                                                           __builtin_amdgcn_sdot4(static_cast<int>(d.d[p][0]), 0x01010101, 0, false), false));
+            if (kk % G == 0) reinterpret_cast<int4*>(meta)[g] = make_int4(s[0], s[1], s[2], __float_as_int(scale));
+        } else {
+            if (kk % G == 0) reinterpret_cast<float*>(meta)[g] = scale;
+        }
+    }
+}
+
+// The images of all blocks of rows, in the workspace: block r0 at r0 x (bytes of a row).
+template <int G, bool ZP>
+__global__ __launch_bounds__(256) void q4_image_kernel(const float* X, int64_t ldx, int M, int K, int most, uint8_t* img, uint8_t* meta) {
+    const int r0 = blockIdx.y * most, rows = min(most, M - r0), kp = (K + 255) / 256 * 256;
+    make_image<G, ZP>(X + r0 * ldx, ldx, K, rows, 0, kp, img + static_cast<int64_t>(r0) * 3 * kp,
+                      meta + static_cast<int64_t>(r0) * (kp / G) * (ZP ? 16 : 4), blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+// ---- the products
+// A 16 x 16 x 64 integer product takes 16 rows of weights and, on its other side, four rows of X as four times
+// three digits (the fourth row of each four is never looked at): lane 16 c + n holds the three digits' sums of
+// row c of the four and weight row n side by side, and only there are they put together, scaled and added
+// in fp32. A group is one such product (two for 128, one of depth 32 for 32), so sums are exact until they
+// are scaled. Zero points start the sums at -16 zero x (sum of the digits).
+//
+// A workgroup's waves take tiles of 16 weight rows, `ks` waves a tile, which share its k by blocks of 256 and
+// add up in LDS. Weights go from memory to registers kDepth blocks ahead.
+constexpr int kDepth = 4;
+
+template <int G, bool ZP>
+struct Unit {
+    static constexpr int kScales = 256 / G, kWords = ZP ? kScales : kScales / 2, kBytes = 2048 + 64 * kWords;
+    uint4 c[2];
+    uint32_t s[kWords];
+    __device__ void load(const uint8_t* u, int lane) {
+        c[0] = *reinterpret_cast<const uint4*>(u + 16 * lane);
+        c[1] = *reinterpret_cast<const uint4*>(u + 1024 + 16 * lane);
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(u + 2048) + (lane & 15) * kWords;
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(p + i);
+                s[i] = v.x, s[i + 1] = v.y, s[i + 2] = v.z, s[i + 3] = v.w;
+            }
+        } else if constexpr (kWords == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            s[0] = v.x, s[1] = v.y;
+        } else {
+            s[0] = *p;
+        }
+    }
+    __device__ float scale(int g) const { return half_bits(ZP ? s[g] : g & 1 ? s[g / 2] >> 16 : s[g / 2]); }
+    __device__ int zero(int g) const { return static_cast<int>(s[g]) >> 16; }
+    __device__ uint32_t word(int i) const {
+        const uint4& v = c[i / 4];
+        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+    }
+};
+
+template <int G, bool ZP, int QN>
+__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, int rows, int lane, float* acc) {
+    const int c = lane >> 4, m = lane & 15;
+#pragma unroll
+    for (int g = 0; g < 256 / G; ++g) {
+        const float sw = u.scale(g);
+        // eight codes a word: bytes of 16 times the low and the high ones
+        v4i b[G == 128 ? 2 : 1];
+        if constexpr (G == 32) {
+            const uint32_t w = u.word(g);
+            b[0] = v4i{static_cast<int>(w << 4 & 0xf0f0f0f0u), static_cast<int>(w & 0xf0f0f0f0u), 0, 0};
+        } else {
+#pragma unroll
+            for (int h = 0; h < G / 64; ++h) {
+                const uint32_t w0 = u.word(2 * (g * (G / 64) + h)), w1 = u.word(2 * (g * (G / 64) + h) + 1);
+                b[h] = v4i{static_cast<int>(w0 << 4 & 0xf0f0f0f0u), static_cast<int>(w0 & 0xf0f0f0f0u),
+                           static_cast<int>(w1 << 4 & 0xf0f0f0f0u), static_cast<int>(w1 & 0xf0f0f0f0u)};
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < QN; ++q) {
+            const int r = min(4 * q + (m >> 2), rows - 1), mine = min(4 * q + c, rows - 1);  // rows beyond the last: whatever
+            const uint8_t* at = img + r * 48 + min(m & 3, 2) * 16;
+            float sx;
+            v4i d = {0, 0, 0, 0};
+            if constexpr (ZP) {
+                const int4 t = reinterpret_cast<const int4*>(meta)[g * rows + mine];
+                const int z = -16 * u.zero(g);
+                d = v4i{z * t.x, z * t.y, z * t.z, 0};
+                sx = __int_as_float(t.w);
+            } else {
+                sx = reinterpret_cast<const float*>(meta)[g * rows + mine];
+            }
+            if constexpr (G == 32) {
+                const long a = *reinterpret_cast<const long*>(at + ((g >> 1) * 4 + (g & 1) * 2 + (c >> 1)) * rows * 48 + (c & 1) * 8);
+                d = __builtin_amdgcn_mfma_i32_16x16x32_i8(a, __builtin_bit_cast(long, make_int2(b[0][0], b[0][1])), d, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int h = 0; h < G / 64; ++h) {
+                    const v4i a = *reinterpret_cast<const v4i*>(at + ((g * (G / 64) + h) * 4 + c) * rows * 48);
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[h], d, 0, 0, 0);
+                }
+            }
+            const float f = fmaf(static_cast<float>(d[2] * 256 + d[1]), 256.0f, static_cast<float>(d[0]));
+            acc[q] = fmaf(f, sw * sx, acc[q]);
+        }
+    }
+}
+
+template <int G, bool ZP, int QN, bool PRE>
+__global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most, int ks, int chunk) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane >> 4, n = lane & 15;
+    const int r0 = blockIdx.y * most, rows = min(most, a.M - r0);
+    const int tiles = (a.N + 15) / 16, blocks = (a.K + 255) / 256, rt = kWaves / ks, part = wave % ks;
+    const int sets = (tiles + rt - 1) / rt;
+    uint8_t* meta = lds + most * 3 * chunk * 256;
+    float* red = reinterpret_cast<float*>(meta + meta_bytes<G, ZP>(most, chunk * 256));
+    typedef Unit<G, ZP> U;
+    const bool one = chunk >= blocks;   // one image serves all tiles
+    bool made = false;
+    for (int set = blockIdx.x; set < sets; set += gridDim.x) {
+        const int tile = set * rt + wave / ks;
+        const uint8_t* W = a.W + static_cast<int64_t>(min(tile, tiles - 1)) * blocks * U::kBytes;
+        float acc[QN];
+#pragma unroll
+        for (int q = 0; q < QN; ++q) acc[q] = 0.0f;
+        for (int b0 = 0; b0 < blocks; b0 += chunk) {
+            const int bn = min(chunk, blocks - b0), its = (bn - part + ks - 1) / ks;  // blocks b0 + part + i ks
+            U u[kDepth];
+#pragma unroll
+            for (int i = 0; i < kDepth; ++i)
+                if (i < its) u[i].load(W + static_cast<int64_t>(b0 + part + i * ks) * U::kBytes, lane);
+            if (!one || !made) {
+                if (made) lds_barrier();
+                if constexpr (PRE) {
+                    const int kp = blocks * 256;
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(r0) * 3 * kp +
+                                                                      static_cast<int64_t>(rows) * 3 * b0 * 256);
+                    for (int i = threadIdx.x; i < rows * 3 * bn * 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = src[i];
+                    const uint32_t* ms = reinterpret_cast<const uint32_t*>(
+                        static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(a.M) * 3 * kp + meta_bytes<G, ZP>(r0, kp) + meta_bytes<G, ZP>(rows, b0 * 256));
+                    for (int i = threadIdx.x; i < meta_bytes<G, ZP>(rows, bn * 256) / 4; i += kThreads) reinterpret_cast<uint32_t*>(meta)[i] = ms[i];
+                } else {
+                    make_image<G, ZP>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, threadIdx.x, kThreads);
+                }
+                made = true;
+                lds_barrier();
+            }
+            for (int i = 0; i < its; i += kDepth) {
+#pragma unroll
+                for (int j = 0; j < kDepth; ++j)
+                    if (i + j < its) {
+                        const int b = part + (i + j) * ks;
+                        multiply<G, ZP, QN>(u[j], lds + b * rows * 768, meta + meta_bytes<G, ZP>(rows, b * 256), rows, lane, acc);
+                        if (i + j + kDepth < its) u[j].load(W + static_cast<int64_t>(b0 + b + kDepth * ks) * U::kBytes, lane);
+                    }
+            }
+        }
+        const auto store = [&](int q, float y) {
+            const int r = 4 * q + c, col = tile * 16 + n;
+            if (r < rows && tile < tiles && col < a.N) {
+                const int64_t row = r0 + r;
+                a.Y[row * a.ldy + col] = y + (a.R ? a.R[row * a.ldr + col] : 0.0f);
+            }
+        };
+        if (ks == 1) {
+#pragma unroll
+            for (int q = 0; q < QN; ++q) store(q, acc[q]);
+            continue;
+        }
+#pragma unroll
+        for (int q = 0; q < QN; ++q) red[(wave * QN + q) * 64 + lane] = acc[q];
+        lds_barrier();
+#pragma unroll
+        for (int q = 0; q < QN; ++q)
+            if (q % ks == part) {
+                float y = 0.0f;
+                for (int i = 0; i < ks; ++i) y += red[((wave - part + i) * QN + q) * 64 + lane];
+                store(q, y);
+            }
+        lds_barrier();
+    }
 }
 
 // 16 lanes a group. Without zero points the entry of the largest magnitude becomes code 0, -8 steps:
@@ -125,13 +365,78 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* codes, cons
     reinterpret_cast<uint32_t*>(packed)[id] = out;
 }
 
+// Rows a block, waves a tile, workgroups, blocks of 256 k an image holds, and whether the image is made by
+// a launch of its own.
+struct Q4Plan {
+    int quads, most, row_blocks, ks, wgs, chunk;
+    bool pre;
+    uint32_t lds;
+};
+template <int G, bool ZP>
+Q4Plan q4_plan(int M, int N, int K) {
+    Q4Plan p{};
+    const int blocks = q4_blocks(K), tiles = q4_tiles(N);
+    p.row_blocks = (M + 15) / 16;
+    p.most = (M + p.row_blocks - 1) / p.row_blocks;
+    p.quads = p.most <= 4 ? 1 : p.most <= 8 ? 2 : 4;
+    p.pre = p.most > 4;
+    p.ks = 8;
+    while (p.ks > 1 && tiles * p.ks * p.row_blocks >= 2 * kWaves * 512) p.ks /= 2;
+    while (p.ks > 1 && p.ks / 2 >= blocks) p.ks /= 2;
+    const int budget = 120 * 1024, each = p.most * 3 * 256 + meta_bytes<G, ZP>(p.most, 256);
+    p.chunk = std::min(blocks, std::max(1, budget / each));
+    const int rt = kWaves / p.ks, sets = (tiles + rt - 1) / rt;
+    p.wgs = std::min(sets, std::max(1, 512 / p.row_blocks));
+    p.lds = p.most * 3 * p.chunk * 256 + meta_bytes<G, ZP>(p.most, p.chunk * 256) + (p.ks > 1 ? kWaves * p.quads * 64 * 4 : 0);
+    return p;
+}
+
+template <int G, bool ZP, int QN, bool PRE>
+hipError_t launch_q4_form(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
+    static std::once_flag once;         // LDS beyond the default limit
+    static hipError_t limit;
+    std::call_once(once, [] {
+        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, QN, PRE>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    160 * 1024);
+    });
+    if (limit != hipSuccess) return limit;
+    klaunch(q4_mul_kernel<G, ZP, QN, PRE>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
+    return hipGetLastError();
+}
+
+template <int G, bool ZP>
+hipError_t launch_q4_plan(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
+    if (p.pre) {
+        const int kp = q4_blocks(a.K) * 256;
+        uint8_t* ws = static_cast<uint8_t*>(a.ws);
+        klaunch(q4_image_kernel<G, ZP>, dim3((p.most * kp / 8 + 255) / 256, p.row_blocks), dim3(256), 0, s, a.X, a.ldx, a.M, a.K, p.most, ws,
+                ws + static_cast<int64_t>(a.M) * 3 * kp);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (!p.pre) return launch_q4_form<G, ZP, 1, false>(a, p, s);
+    if (p.quads == 1) return launch_q4_form<G, ZP, 1, true>(a, p, s);
+    if (p.quads == 2) return launch_q4_form<G, ZP, 2, true>(a, p, s);
+    return launch_q4_form<G, ZP, 4, true>(a, p, s);
+}
+
 }  // namespace
 
-uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) { return 16; }
+uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) {
+    const uint64_t kp = static_cast<uint64_t>(q4_blocks(K)) * 256;
+    return M * (3 * kp + kp / G * 16);
+}
 
 hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s) {
-    klaunch(q4_mul_kernel, dim3((a.N + 3) / 4, a.M), dim3(256), 0, s, a);
-    return hipGetLastError();
+    const auto go = [&](auto g, auto z) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool Z = decltype(z)::value;
+        return launch_q4_plan<G, Z>(a, q4_plan<G, Z>(a.M, a.N, a.K), s);
+    };
+    const auto by_zeros = [&](auto g) { return a.zeros ? go(g, std::true_type()) : go(g, std::false_type()); };
+    return a.G == 32   ? by_zeros(std::integral_constant<int, 32>())
+           : a.G == 64 ? by_zeros(std::integral_constant<int, 64>())
+                       : by_zeros(std::integral_constant<int, 128>());
 }
 
 hipError_t launch_q4_quantize(const void* W, bool bf16, int N, int K, int G, uint8_t* codes, uint16_t* scales, uint8_t* zeros,
