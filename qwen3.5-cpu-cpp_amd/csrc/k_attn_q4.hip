@@ -4,7 +4,10 @@
 // A row is quantized by 64 dims: least = fp16(min), step = fp16((max - least) / 15), code =
 // round((x - least) / step), all from 64-bit values rounded to fp32 and then fp16: a value next to the
 // border of two codes is on the same side for whoever computes it from the same inputs.
-#include "dev_common.hpp"
+#include <cmath>
+#include <mutex>
+
+#include "dev_q4.hpp"
 #include "launch_q4.hpp"
 
 namespace q35k {
@@ -12,17 +15,11 @@ namespace {
 
 constexpr int kHD = 256;
 
-__device__ __forceinline__ float half_bits(uint32_t h) {
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
-}
-__device__ __forceinline__ uint32_t bits_half(float x) {
-    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
-}
 // fp16 through fp32: without the barrier the two roundings are compiled as one
 __device__ __forceinline__ uint32_t bits_half(double x) {
     float f = static_cast<float>(x);
     asm("" : "+v"(f));
-    return bits_half(f);
+    return q35k::bits_half(f);
 }
 // least and step of a (step, least) dword
 __device__ __forceinline__ float step_of(uint32_t s) { return half_bits(s & 0xffffu); }
@@ -34,6 +31,32 @@ __device__ __forceinline__ double min16(double v) {
     v = fmin(v, dpp_d<0x141>(v));
     return fmin(v, dpp_d<0x140>(v));
 }
+// over the 16 lanes of a row
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(dpp_i<0xB1>(static_cast<int>(v))));
+    v = max(v, static_cast<uint32_t>(dpp_i<0x4E>(static_cast<int>(v))));
+    v = max(v, static_cast<uint32_t>(dpp_i<0x141>(static_cast<int>(v))));
+    return max(v, static_cast<uint32_t>(dpp_i<0x140>(static_cast<int>(v))));
+}
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    return fmaxf(v, dpp_f<0x140>(v));
+}
+__device__ __forceinline__ int sum16(int v) {
+    v += dpp_i<0xB1>(v);
+    v += dpp_i<0x4E>(v);
+    v += dpp_i<0x141>(v);
+    return v + dpp_i<0x140>(v);
+}
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp_f<0xB1>(v);
+    v += dpp_f<0x4E>(v);
+    v += dpp_f<0x141>(v);
+    return v + dpp_f<0x140>(v);
+}
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int or16(int v) {
     v |= dpp_i<0xB1>(v);
     v |= dpp_i<0x4E>(v);
@@ -74,9 +97,24 @@ __device__ __forceinline__ uint32_t quantize4(const double* x, uint32_t& scale) 
     return c;
 }
 
-// A wave a row: the batch's query rows (normed, rotated, scaled, to the workspace), then the new
+// theta^(-2i / ROT), formed on the host
+struct RopeFreq {
+    double f[kHD / 2];
+};
+
+// What the products read of a query head: the three digits of its rows, by quads of heads: [quad][group of
+// 64 dims][c][head of the quad][digit] 16 bytes, the dims 16 c .. + 15 of the group in the order
+// in which a cache row's nibbles come apart (0 2 4 6 1 3 5 7 8 10 ..); and per head and group (2^-e, 2^-e times the
+// sum of the multiples), which the rows' least values are multiplied by.
+struct QueryImage {
+    uint8_t* digits;                    // [B][NKV][quads][4][4][4][3][16]
+    float2* factors;                    // [B][NKV][4 quads][4]
+};
+constexpr int kQuadBytes = 4 * 4 * 4 * 3 * 16;
+
+// A wave a row: the batch's query rows (normed, rotated, times log2(e) / sqrt(HD), split into digits), then the new
 // key rows (normed, rotated) and value rows, quantized and appended at slot len[b].
-__global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, float* q) {
+__global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, RopeFreq freq, QueryImage img, int quads) {
     __shared__ double row[4][kHD], cs[4][kHD];
     const int lane = threadIdx.x & 63, w = threadIdx.x / 64;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + w;
@@ -85,6 +123,7 @@ __global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, float* 
     const int len = b < a.B ? a.len[b] : -1;
     const bool on = len >= 0 && len < a.cap, is_q = r < a.NQ, is_k = !is_q && r < a.NQ + a.NKV;
     const int h = is_q ? r : is_k ? r - a.NQ : r - a.NQ - a.NKV;
+    const int half = a.ROT / 2;
     double x[4] = {0, 0, 0, 0};
     if (on) {
         const float* src = is_q ? a.qg + (static_cast<int64_t>(b) * a.NQ + h) * 2 * kHD
@@ -92,23 +131,17 @@ __global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, float* 
         const float4 f = reinterpret_cast<const float4*>(src)[lane];
         x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
         if (is_q || is_k) {
+            const float4 nw = reinterpret_cast<const float4*>(is_q ? a.q_norm : a.k_norm)[lane];
+            for (int i = lane; i < half; i += 64) sincos(static_cast<double>(a.pos[b]) * freq.f[i], &cs[w][128 + i], &cs[w][i]);
             const double ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
             const double inv = 1.0 / sqrt(ss / kHD + static_cast<double>(a.eps));
-            const float4 nw = reinterpret_cast<const float4*>(is_q ? a.q_norm : a.k_norm)[lane];
             x[0] *= inv * (1.0 + nw.x), x[1] *= inv * (1.0 + nw.y), x[2] *= inv * (1.0 + nw.z), x[3] *= inv * (1.0 + nw.w);
-            const int half = a.ROT / 2;
-            for (int i = lane; i < half; i += 64) {
-                const double ang = static_cast<double>(a.pos[b]) * pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
-                cs[w][i] = cos(ang);
-                cs[w][128 + i] = sin(ang);
-            }
             for (int i = 0; i < 4; ++i) row[w][4 * lane + i] = x[i];
         }
     }
     __syncthreads();
     if (!on) return;
     if (is_q || is_k) {
-        const int half = a.ROT / 2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = 4 * lane + i;
@@ -117,9 +150,38 @@ __global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, float* 
         }
     }
     if (is_q) {
-        reinterpret_cast<float4*>(q + (static_cast<int64_t>(b) * a.NQ + h) * kHD)[lane] =
-            make_float4(static_cast<float>(x[0] * 0.0625), static_cast<float>(x[1] * 0.0625), static_cast<float>(x[2] * 0.0625),
-                        static_cast<float>(x[3] * 0.0625));
+        constexpr double kScale = 0.0625 * 1.4426950408889634;
+        float f[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[i] = static_cast<float>(x[i] * kScale);
+            top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+        }
+        top = max16(top);
+        const bool ok = top < 0x7f800000u && top != 0;
+        const int e = ok ? multiple_exp(__uint_as_float(top)) : 0;
+        int sum = 0;
+        uint32_t y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = ok ? static_cast<int>(rintf(ldexpf(f[i], e))) : 0;
+            sum += v;
+            y[i] = signed_digits(v);
+        }
+        sum = sum16(sum);
+        const int g = lane >> 4, c = lane >> 2 & 3, o = lane & 3, hk = h / a.GRP, hq = h % a.GRP;
+        const int64_t bk = static_cast<int64_t>(b) * a.NKV + hk;
+        uint8_t* at = img.digits + (bk * quads + hq / 4) * kQuadBytes + ((g * 4 + c) * 4 + hq % 4) * 48 + (o >> 1) * 8 + (o & 1) * 2;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {  // dims 4 o, 4 o + 2 and 4 o + 1, 4 o + 3 of the sixteen
+            *reinterpret_cast<uint16_t*>(at + 16 * p) = static_cast<uint16_t>((y[0] >> (8 * p) & 0xffu) | (y[2] >> (8 * p) & 0xffu) << 8);
+            *reinterpret_cast<uint16_t*>(at + 16 * p + 4) = static_cast<uint16_t>((y[1] >> (8 * p) & 0xffu) | (y[3] >> (8 * p) & 0xffu) << 8);
+        }
+        if ((lane & 15) == 0) {
+            const float s = top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
+            img.factors[(bk * quads * 4 + hq) * 4 + g] = make_float2(s, s * static_cast<float>(sum));
+        }
         return;
     }
     uint32_t scale;
@@ -129,33 +191,328 @@ __global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, float* 
     if ((lane & 15) == 0) (is_k ? a.k_scale : a.v_scale)[at * 4 + lane / 16] = scale;
 }
 
-// a wave per query head: the keys one after another
-__global__ __launch_bounds__(64) void attn_q4_kernel(AttnQ4Args a, const float* q) {
-    const int lane = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// What lanes of a wave have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// Here the value exists: without it the compiler puts off what follows the products, whose sums (four
+// registers for one value) then outnumber the registers.
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
+
+constexpr int kTile = 64;       // keys a wave takes at a time
+constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16;
+
+struct Partials {
+    float* o;                           // [B][NKV][pieces][GRP][HD]
+    float2* ml;                         // [B][NKV][pieces][GRP] (max, sum)
+};
+
+// Eight waves (four with more than 8 heads) a piece of one cache's keys, tiles of 64 keys a wave, for all query heads of the kv head.
+//
+// Scores: a 16 x 16 x 64 integer product takes four heads as four times three digits (the fourth row is never
+// looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
+//   s = sum_g 2^-e (step_g sum_d i_d code_d + least_g sum_d i_d).
+// Weights: p = 2^(s - tile's largest) <= 1 is multiplied by its value row's step, which differs by group, and becomes
+// multiples of a 4190000th of the tile's largest such product: p step code summed over 64 keys is again one
+// integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
+// operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time)
+// in that order. The part of the least values, sum_t p_t least_t, is a sum a head and group.
+template <int HQ>
+constexpr int attn_q4_waves = HQ > 2 ? 4 : 8;  // with 16 heads a wave holds more than 256 registers
+template <int HQ>
+__global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4Args a, QueryImage img, int pieces, int piece_len, Partials part) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr int kWaves = attn_q4_waves<HQ>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane >> 4, n = lane & 15;
+    const int piece = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
     const int len = a.len[b];
     if (len < 0) return;
-    const int64_t o = static_cast<int64_t>(b) * a.NQ + h;
-    float4* out = reinterpret_cast<float4*>(a.out + o * kHD) + lane;
     if (len >= a.cap) {  // nothing was appended
-        *out = make_float4(NAN, NAN, NAN, NAN);
+        if (piece == 0)
+            for (int i = threadIdx.x; i < a.GRP * kHD; i += kWaves * 64)
+                a.out[(static_cast<int64_t>(b) * a.NQ + hk * a.GRP) * kHD + i] = NAN;
         return;
     }
-    const float4 x = reinterpret_cast<const float4*>(q + o * kHD)[lane];
-    float m = -INFINITY, l = 0.0f;
-    float acc[4] = {0, 0, 0, 0};
-    for (int t = 0; t <= len; ++t) {
-        const int64_t at = (static_cast<int64_t>(b) * a.NKV + h / a.GRP) * a.cap + t;
-        const uint32_t kc = reinterpret_cast<const uint16_t*>(a.k)[at * 64 + lane], ks = a.k_scale[at * 4 + lane / 16];
-        const uint32_t vc = reinterpret_cast<const uint16_t*>(a.v)[at * 64 + lane], vs = a.v_scale[at * 4 + lane / 16];
-        const auto val = [](uint32_t c, int i, uint32_t s) { return fmaf(step_of(s), static_cast<float>(c >> (4 * i) & 15u), least_of(s)); };
-        const float s = wave_sum(x.x * val(kc, 0, ks) + x.y * val(kc, 1, ks) + x.z * val(kc, 2, ks) + x.w * val(kc, 3, ks));
-        const float mn = fmaxf(m, s), al = expf(m - mn), p = expf(s - mn);
-        m = mn;
-        l = l * al + p;
-        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * al + p * val(vc, i, vs);
+    const int rows = len + 1, first = piece * piece_len, end = min(rows, first + piece_len);
+    if (first >= rows) return;
+    const int64_t bk = static_cast<int64_t>(b) * a.NKV + hk;
+    // the piece's rows; offsets within it stay within 32 bits
+    const int count = end - first;
+    const int64_t row0 = bk * a.cap + first;
+    const uint8_t *K = a.k + row0 * kQ4RowBytes, *V = a.v + row0 * kQ4RowBytes;
+    const uint8_t *KS = reinterpret_cast<const uint8_t*>(a.k_scale) + row0 * 16, *VS = reinterpret_cast<const uint8_t*>(a.v_scale) + row0 * 16;
+
+    // the queries, for all waves; each wave's value rows and weights
+    constexpr int JB = HQ < 2 ? HQ : 2;  // quads whose weights lie in LDS at a time
+    uint8_t* qbuf = lds;
+    float2* fbuf = reinterpret_cast<float2*>(lds + HQ * kQuadBytes);
+    uint8_t* vbuf = lds + HQ * (kQuadBytes + 128) + wave * (kVBytes + JB * kPBytes);
+    uint8_t* pbuf = vbuf + kVBytes;
+    for (int i = threadIdx.x; i < HQ * kQuadBytes / 16; i += kWaves * 64)
+        reinterpret_cast<uint4*>(qbuf)[i] = reinterpret_cast<const uint4*>(img.digits + bk * HQ * kQuadBytes)[i];
+    if (threadIdx.x < HQ * 16) fbuf[threadIdx.x] = img.factors[bk * HQ * 16 + threadIdx.x];
+
+    uint2 k[4][4];
+    uint4 ks[4], vs[4];
+    const auto load_k = [&](int t0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint32_t r = min(t0 + 16 * t + n, count - 1);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) k[t][g] = *reinterpret_cast<const uint2*>(K + (r * kQ4RowBytes + 8 * c) + 32 * g);
+            ks[t] = *reinterpret_cast<const uint4*>(KS + r * 16);
+        }
+    };
+    // a row's eight 16-byte pieces lie in LDS in an order that spreads the rows over the banks
+    v4i v[8];
+    const auto load_v = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t r = min(t0 + 8 * i + (lane >> 3), count - 1);
+            v[i] = *reinterpret_cast<const v4i*>(V + (r * kQ4RowBytes + 16 * (lane & 7)));
+        }
+    };
+    const auto place_v = [&] {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<v4i*>(vbuf + (8 * i + (lane >> 3)) * kQ4RowBytes + 16 * ((lane & 7) ^ (lane >> 3))) = v[i];
+    };
+    const auto load_vs = [&](int t0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vs[t] = *reinterpret_cast<const uint4*>(VS + static_cast<uint32_t>(min(t0 + 16 * t + n, count - 1)) * 16);
+    };
+
+    float m[HQ], l[HQ], lo[HQ][4], o[HQ][16];
+#pragma unroll
+    for (int j = 0; j < HQ; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) lo[j][g] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[j][d] = 0.0f;
     }
+
+    // nibble n of the transposed 16 keys: which key its place in the operand is
+    const int spot = (n & 8) + (n & 1) * 4 + ((n & 7) >> 1), key = 16 * (spot & 3) + 4 * c + (spot >> 2);
+    int t0 = wave * kTile;
+    if (t0 < count) {
+        load_k(t0);
+        load_v(t0);
+        load_vs(t0);
+    }
+    lds_barrier();
+    for (; t0 < count; t0 += kWaves * kTile) {
+        float s[HQ][4];
+#pragma unroll
+        for (int j = 0; j < HQ; ++j)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[j][t] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            v4i q[HQ];
+            float2 f[HQ];
+#pragma unroll
+            for (int j = 0; j < HQ; ++j) {
+                q[j] = *reinterpret_cast<const v4i*>(qbuf + j * kQuadBytes + ((g * 4 + c) * 4 + (n >> 2)) * 48 + min(n & 3, 2) * 16);
+                f[j] = fbuf[(j * 4 + c) * 4 + g];
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint2 w = k[t][g];
+                const v4i kb = {static_cast<int>(w.x & 0x0f0f0f0fu), static_cast<int>(w.x >> 4 & 0x0f0f0f0fu),
+                                static_cast<int>(w.y & 0x0f0f0f0fu), static_cast<int>(w.y >> 4 & 0x0f0f0f0fu)};
+                const uint32_t sc = word(ks[t], g);
+                const float step = step_of(sc), least = least_of(sc);
+#pragma unroll
+                for (int j = 0; j < HQ; ++j) {
+                    const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[j], kb, v4i{0, 0, 0, 0}, 0, 0, 0);
+                    s[j][t] = fmaf(from_digits(d), step * f[j].x, fmaf(least, f[j].y, s[j][t]));
+                    if constexpr (HQ > 2) pin(s[j][t]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int j = 0; j < HQ; ++j) pin(s[j][t]);
+        }
+        const int next = t0 + kWaves * kTile;
+        place_v();
+        if (next < count) {
+            load_k(next);
+            load_v(next);
+        }
+        float alpha[HQ], beta[HQ];
+#pragma unroll
+        for (int j = 0; j < HQ; ++j) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[j][t] = t0 + 16 * t + n < count ? s[j][t] : -INFINITY;
+            const float top = max16(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
+            const float ref = top == -INFINITY ? 0.0f : top, mn = fmaxf(m[j], top), mref = mn == -INFINITY ? 0.0f : mn;
+            alpha[j] = exp2_f(m[j] - mref);
+            beta[j] = exp2_f(top - mref);
+            m[j] = mn;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[j][t] = exp2_f(s[j][t] - ref);
+            l[j] = fmaf(l[j], alpha[j], beta[j] * ((s[j][0] + s[j][1]) + (s[j][2] + s[j][3])));
+        }
+#pragma unroll
+        for (int j0 = 0; j0 < HQ; j0 += JB) {
+            // weights times steps, in units of the tile's largest such product: digits through LDS into the
+            // operand's order
+            float unit[JB][4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float st[4], le[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    st[t] = step_of(word(vs[t], g));
+                    le[t] = fmaf(st[t], 0.0f, least_of(word(vs[t], g)));  // NaN where the step is
+                }
+#pragma unroll
+                for (int j = j0; j < j0 + JB; ++j) {
+                    float x[4], part_lo = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        x[t] = s[j][t] * st[t];
+                        part_lo = fmaf(s[j][t], le[t], part_lo);
+                    }
+                    lo[j][g] = fmaf(lo[j][g], alpha[j], beta[j] * part_lo);
+                    const float big = max16(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+                    const float inv = big > 1e-30f ? 4190000.0f * __builtin_amdgcn_rcpf(big) : 0.0f;
+                    unit[j - j0][g] = beta[j] * big * (1.0f / 4190000.0f);
+                    uint32_t y[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)  // 1.5 2^23 + i: i in the low bits
+                        y[t] = (__float_as_uint(fmaf(x[t], inv, 12582912.0f)) + (0x8080u - 0x4b400000u)) ^ 0x8080u;
+                    uint8_t* at = pbuf + (j - j0) * kPBytes + (g * 4 + (n >> 2)) * 192 + c * 48 + 4 * (n & 3);
+                    *reinterpret_cast<uint32_t*>(at) = plane<0>(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint32_t*>(at + 16) = plane<1>(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint32_t*>(at + 32) = plane<2>(y[0], y[1], y[2], y[3]);
+                    pin(lo[j][g]);
+                    pin(unit[j - j0][g]);
+                }
+            }
+            if (j0 + JB >= HQ && next < count) load_vs(next);
+#pragma unroll
+            for (int j = j0; j < j0 + JB; ++j)
+                if (__any(alpha[j] != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) o[j][d] *= alpha[j];
+                }
+            wave_sync();
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                v4i p[JB];
+#pragma unroll
+                for (int j = 0; j < JB; ++j)
+                    p[j] = *reinterpret_cast<const v4i*>(pbuf + j * kPBytes + (g * 4 + c) * 192 + (n >> 2) * 48 + min(n & 3, 2) * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 4 * g + i;  // dims 16 d .. + 15
+                    const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) v2i*>(
+                        reinterpret_cast<uintptr_t>(vbuf + key * kQ4RowBytes + 16 * ((d >> 1) ^ (key & 7)) + 8 * (d & 1))));
+                    const v4i vb = {w[0] & 0x0f0f0f0f, static_cast<int>(static_cast<uint32_t>(w[0]) >> 4 & 0x0f0f0f0fu), w[1] & 0x0f0f0f0f,
+                                    static_cast<int>(static_cast<uint32_t>(w[1]) >> 4 & 0x0f0f0f0fu)};
+#pragma unroll
+                    for (int j = 0; j < JB; ++j) {
+                        o[j0 + j][d] = fmaf(from_digits(__builtin_amdgcn_mfma_i32_16x16x64_i8(p[j], vb, v4i{0, 0, 0, 0}, 0, 0, 0)),
+                                            unit[j][g], o[j0 + j][d]);
+                        if constexpr (HQ > 2) pin(o[j0 + j][d]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < JB; ++j) pin(o[j0 + j][4 * g + i]);
+            }
+            wave_sync();
+        }
+    }
+    __syncthreads();
+    // the waves' parts
+    float* wo = reinterpret_cast<float*>(lds);
+    float2* wml = reinterpret_cast<float2*>(lds + kWaves * HQ * 4 * kHD * 4);
+#pragma unroll
+    for (int j = 0; j < HQ; ++j) {
+        l[j] = sum16(l[j]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            lo[j][g] = sum16(lo[j][g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wo[((wave * HQ + j) * 4 + c) * kHD + 16 * (4 * g + i) + n] = o[j][4 * g + i] + lo[j][g];
+        }
+        if (n == 0) wml[wave * HQ * 4 + 4 * j + c] = make_float2(m[j], l[j]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.GRP * kHD; i += kWaves * 64) {
+        const int h = i / kHD, d = i % kHD;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wml[w * HQ * 4 + h].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 ml = wml[w * HQ * 4 + h];
+            const float f = exp2_f(ml.x - ref);
+            sum = fmaf(f, ml.y, sum);
+            x = fmaf(f, wo[(w * HQ * 4 + h) * kHD + d], x);
+        }
+        if (pieces == 1) {
+            const int64_t at = static_cast<int64_t>(b) * a.NQ + hk * a.GRP + h;
+            a.out[at * kHD + d] = x / sum * sigmoid_f(a.qg[at * 2 * kHD + kHD + d]);
+        } else {
+            const int64_t at = (bk * pieces + piece) * a.GRP + h;
+            part.o[at * kHD + d] = x;
+            if (d == 0) part.ml[at] = make_float2(top, sum);
+        }
+    }
+}
+
+// A workgroup a query head: the pieces' parts, four waves taking them in turn, and the gate.
+__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, int pieces, int piece_len, Partials part) {
+    __shared__ float4 ws[4][64];
+    __shared__ float2 wml[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.x, b = blockIdx.y, hk = h / a.GRP;
+    const int len = a.len[b];
+    if (len < 0 || len >= a.cap) return;
+    const int np = len / piece_len + 1;
+    const int64_t first = (static_cast<int64_t>(b) * a.NKV + hk) * pieces * a.GRP + h % a.GRP;
+    float m = -INFINITY, l = 0.0f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = wave; i < np; i += 4) {
+        const int64_t at = first + static_cast<int64_t>(i) * a.GRP;
+        const float2 ml = part.ml[at];
+        const float4 v = reinterpret_cast<const float4*>(part.o + at * kHD)[lane];
+        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn, f = exp2_f(m - ref), g = exp2_f(ml.x - ref);
+        m = mn;
+        l = l * f + ml.y * g;
+        x = make_float4(x.x * f + v.x * g, x.y * f + v.y * g, x.z * f + v.z * g, x.w * f + v.w * g);
+    }
+    ws[wave][lane] = x;
+    if (lane == 0) wml[wave] = make_float2(m, l);
+    __syncthreads();
+    if (wave) return;
+    float top = fmaxf(fmaxf(wml[0].x, wml[1].x), fmaxf(wml[2].x, wml[3].x));
+    top = top == -INFINITY ? 0.0f : top;
+    l = 0.0f;
+    x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = exp2_f(wml[i].x - top);
+        const float4 v = ws[i][lane];
+        l = fmaf(wml[i].y, f, l);
+        x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
+    }
+    const int64_t o = static_cast<int64_t>(b) * a.NQ + h;
     const float4 g = reinterpret_cast<const float4*>(a.qg + o * 2 * kHD + kHD)[lane];
-    *out = make_float4(acc[0] / l * sigmoid_f(g.x), acc[1] / l * sigmoid_f(g.y), acc[2] / l * sigmoid_f(g.z), acc[3] / l * sigmoid_f(g.w));
+    reinterpret_cast<float4*>(a.out + o * kHD)[lane] =
+        make_float4(x.x / l * sigmoid_f(g.x), x.y / l * sigmoid_f(g.y), x.z / l * sigmoid_f(g.z), x.w / l * sigmoid_f(g.w));
 }
 
 // whether rows [i, e) of sequence b are there
@@ -209,14 +566,63 @@ __global__ __launch_bounds__(256) void kv_q4_kernel(KvQ4Args a) {
 
 }  // namespace
 
-int64_t attn_q4_workspace_floats(const AttnQ4Args& a) { return static_cast<int64_t>(a.B) * a.NQ * kHD; }
+namespace {
+
+struct AttnQ4Plan {
+    int quads, pieces, piece_len;
+};
+AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
+    AttnQ4Plan p{};
+    p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
+    const int64_t round = (p.quads > 2 ? attn_q4_waves<4> : attn_q4_waves<2>) * kTile, heads = static_cast<int64_t>(a.B) * a.NKV;
+    int64_t rounds = 1;
+    while ((a.cap + rounds * round - 1) / (rounds * round) * heads > 1024 && rounds * round < a.cap) ++rounds;
+    p.piece_len = static_cast<int>(rounds * round);
+    p.pieces = static_cast<int>((a.cap + p.piece_len - 1) / p.piece_len);
+    return p;
+}
+
+template <int HQ>
+hipError_t launch_attend(const AttnQ4Args& a, const AttnQ4Plan& p, const QueryImage& img, const Partials& part, hipStream_t s) {
+    constexpr int kWaves = attn_q4_waves<HQ>;
+    const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
+    static std::once_flag once;         // LDS beyond the default limit
+    static hipError_t limit;
+    std::call_once(once, [&] {
+        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_q4_kernel<HQ>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    });
+    if (limit != hipSuccess) return limit;
+    klaunch(attn_q4_kernel<HQ>, dim3(p.pieces, a.NKV, a.B), dim3(kWaves * 64), lds, s, a, img, p.pieces, p.piece_len, part);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t attn_q4_workspace_floats(const AttnQ4Args& a) {
+    const AttnQ4Plan p = attn_q4_plan(a);
+    const int64_t heads = static_cast<int64_t>(a.B) * a.NKV;
+    return heads * p.quads * (kQuadBytes / 4 + 4 * 4 * 2) + (p.pieces > 1 ? heads * p.pieces * a.GRP * (kHD + 2) : 0);
+}
 
 hipError_t launch_attn_q4(const AttnQ4Args& a, hipStream_t s) {
-    const int64_t rows = static_cast<int64_t>(a.B) * (a.NQ + 2 * a.NKV);
-    klaunch(attn_q4_prep_kernel, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, s, a, a.ws);
+    const AttnQ4Plan p = attn_q4_plan(a);
+    const int64_t heads = static_cast<int64_t>(a.B) * a.NKV, rows = static_cast<int64_t>(a.B) * (a.NQ + 2 * a.NKV);
+    RopeFreq freq{};
+    for (int i = 0; i < a.ROT / 2; ++i) freq.f[i] = std::pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
+    QueryImage img;
+    img.digits = reinterpret_cast<uint8_t*>(a.ws);
+    img.factors = reinterpret_cast<float2*>(img.digits + heads * p.quads * kQuadBytes);
+    Partials part;
+    part.o = reinterpret_cast<float*>(img.factors + heads * p.quads * 16);
+    part.ml = reinterpret_cast<float2*>(part.o + heads * p.pieces * a.GRP * kHD);
+    klaunch(attn_q4_prep_kernel, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, s, a, freq, img, p.quads);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    klaunch(attn_q4_kernel, dim3(a.NQ, a.B), dim3(64), 0, s, a, static_cast<const float*>(a.ws));
+    e = p.quads == 1   ? launch_attend<1>(a, p, img, part, s)
+        : p.quads == 2 ? launch_attend<2>(a, p, img, part, s)
+                       : launch_attend<4>(a, p, img, part, s);
+    if (e != hipSuccess || p.pieces == 1) return e;
+    klaunch(attn_q4_combine_kernel, dim3(a.NQ, a.B), dim3(256), 0, s, a, p.pieces, p.piece_len, part);
     return hipGetLastError();
 }
 

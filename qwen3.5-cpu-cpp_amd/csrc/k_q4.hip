@@ -4,25 +4,17 @@
 #include <mutex>
 #include <type_traits>
 
-#include "dev_common.hpp"
+#include "dev_q4.hpp"
 #include "launch_q4.hpp"
 
 namespace q35k {
 namespace {
 
-__device__ __forceinline__ float half_bits(uint32_t h) {
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
-}
-__device__ __forceinline__ uint16_t bits_half(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-
 constexpr int kThreads = 512, kWaves = 8;
 
 // ---- rows of X as whole numbers
-// A group of a row's entries becomes multiples of 2^-e: x = i 2^-e, |i| <= 8355711 = 127 2^16 + 127 2^8 + 127, with
-// the largest entry above 2^21.99, so an entry is off by at most 2^-23 of the largest. Such an i is three
-// signed bytes, i = d2 2^16 + d1 2^8 + d0: integer products with 4-bit codes are exact.
+// A group of a row's entries becomes multiples of a power of two, each three signed bytes: integer products
+// with 4-bit codes are exact.
 struct Digits {
     uint32_t d[3][2];                   // eight entries: plane, four bytes each
 };
@@ -30,25 +22,19 @@ struct Digits {
 // multiplied as 16 times themselves); NaN for a group with an infinity or a NaN
 __device__ __forceinline__ Digits digits8(const float* x, uint32_t top, float& scale) {
     const float m = __uint_as_float(top);
-    int e = 23 - __builtin_amdgcn_frexp_expf(m);
-    if (ldexpf(m, e) > 8355711.0f) --e;
-    e = min(e, 100);                    // below 2^-100: multiples of that
+    const int e = multiple_exp(m);
     const bool ok = top < 0x7f800000u && top != 0;
     scale = top >= 0x7f800000u ? NAN : ldexpf(0.0625f, ok ? -e : 0);
     uint32_t y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int v = ok ? static_cast<int>(rintf(ldexpf(x[i], e))) : 0;
-        y[i] = (static_cast<uint32_t>(v) + 0x8080u) ^ 0x8080u;  // the three signed digits in bytes 0, 1, 2
-    }
+    for (int i = 0; i < 8; ++i) y[i] = signed_digits(ok ? static_cast<int>(rintf(ldexpf(x[i], e))) : 0);
     Digits r;
 #pragma unroll
-    for (int p = 0; p < 3; ++p)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t lo = 0x0c0c0400u + p * 0x0101u, hi = 0x04000c0cu + p * 0x01010000u;
-            r.d[p][h] = __builtin_amdgcn_perm(y[4 * h + 1], y[4 * h], lo) | __builtin_amdgcn_perm(y[4 * h + 3], y[4 * h + 2], hi);
-        }
+    for (int h = 0; h < 2; ++h) {
+        r.d[0][h] = plane<0>(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
+        r.d[1][h] = plane<1>(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
+        r.d[2][h] = plane<2>(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
+    }
     return r;
 }
 template <int G>
@@ -205,8 +191,7 @@ __device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* im
                     d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[h], d, 0, 0, 0);
                 }
             }
-            const float f = fmaf(static_cast<float>(d[2] * 256 + d[1]), 256.0f, static_cast<float>(d[0]));
-            acc[q] = fmaf(f, sw * sx, acc[q]);
+            acc[q] = fmaf(from_digits(d), sw * sx, acc[q]);
         }
     }
 }
