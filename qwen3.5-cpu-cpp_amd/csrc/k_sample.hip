@@ -8,11 +8,11 @@
 //
 // A row is cut into slices, a workgroup each. The first launch finds the largest logit; the second counts
 // candidates and mass by bins of 1/128 of (max - l) / T, down to 36, below which weights are 0; the third
-// reads off which bins the borders and the draw may lie in (a border that is known to a bin leaves the next one
-// open to as much mass, so mostly to a bin as well), gathers their candidates, and the workgroup that is done
-// last sorts those and finds the exact places. Rows of one slice take one launch. Where the open bins
-// hold more than kList candidates (thousands of equal logits), it finds the places by radix descent over
-// the row instead.
+// gathers the candidates of the bins that the borders and the draw may lie in (a border that is known to a bin
+// leaves the next one open to as much mass, so mostly to a bin as well). The workgroup that is done last
+// with a row plans that, or sorts the candidates and finds the exact places. Rows of one slice take one
+// launch. Where the open bins hold more than kList candidates (thousands of equal logits), the places are
+// found by radix descent over the row.
 #include "dev_common.hpp"
 #include "launch_q4.hpp"
 
@@ -33,10 +33,36 @@ constexpr uint32_t kKeyInf = 0xff800000u;   // +inf
 
 constexpr int kBins = 36 * 128;  // and one for what has no weight
 
+// e^-z for 0 <= z < 36, to a unit in the last place or two: z = n ln 2 / 64 + r, |r| <= ln 2 / 128, so e^-z =
+// 2^-(n div 64) 2^-(n mod 64 / 64) e^-r, the second factor from a table and the last by five terms of its
+// series (the sixth is below 2^-54).
+struct ExpTable {
+    double t[64];
+    __device__ void fill() {
+        if (threadIdx.x < 64) t[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+    }
+};
+__device__ __forceinline__ double exp_minus(double z, const ExpTable& e) {
+    constexpr double kLn2 = 0.69314718055994530942, kStep = 64.0 / kLn2;
+    // ln 2 / 64 to 32 bits, so that n times it is exact, and the rest of it
+    constexpr double kHigh = 0x1.62e42fefp-7, kLow = 0x1.473de6af278edp-40;
+    const double n = rint(z * kStep);
+    const int i = static_cast<int>(n);
+    const double r = fma(-n, kLow, fma(-n, kHigh, z));
+    double p = fma(r, -1.0 / 120.0, 1.0 / 24.0);
+    p = fma(-r, p, 1.0 / 6.0);
+    p = fma(-r, p, 0.5);
+    p = fma(-r, p, 1.0);
+    p = fma(-r, p, 1.0);
+    return ldexp(e.t[i & 63] * p, -(i >> 6));
+}
+
 struct Weigher {
     double top, rt, unit;
+    const ExpTable& table;
     bool inf;
-    __device__ Weigher(uint32_t key, float T, double unit_) : top(of_key(key)), rt(1.0 / static_cast<double>(T)), unit(unit_), inf(key == kKeyInf) {}
+    __device__ Weigher(uint32_t key, float T, double unit_, const ExpTable& e)
+        : top(of_key(key)), rt(1.0 / static_cast<double>(T)), unit(unit_), table(e), inf(key == kKeyInf) {}
     // (max - l) / T
     __device__ double depth(uint32_t key) const {
         if (inf) return key == kKeyInf ? 0.0 : INFINITY;
@@ -48,9 +74,12 @@ struct Weigher {
     // the weight in 64 bits, of the largest
     __device__ double share(uint32_t key) const {
         const double z = depth(key);
-        return z < 36.0 ? exp(-z) : 0.0;
+        return z < 36.0 ? exp_minus(z, table) : 0.0;
     }
-    __device__ uint64_t units(double depth) const { return depth < 36.0 ? static_cast<uint64_t>(rint(exp(-depth) * unit)) : 0; }
+    __device__ uint64_t units(double depth) const {
+        // rounded to a whole number by what 2^52 more leaves of it
+        return depth < 36.0 ? __builtin_bit_cast(uint64_t, fma(exp_minus(depth, table), unit, 0x1p52)) & 0xfffffffffffffull : 0;
+    }
     __device__ uint64_t operator()(uint32_t key) const { return units(depth(key)); }
 };
 
@@ -186,45 +215,74 @@ __device__ void sample_by_descent(const SampleArgs& a, int b, uint32_t top, cons
 }
 
 // ---- by bins
-constexpr int kList = 4096;             // candidates of the open bins
-constexpr int kPer = (kBins + 1 + kThreads - 1) / kThreads;
+constexpr int kList = 2048;             // candidates of the open bins
+constexpr int kOpen = 512;              // open bins
+constexpr int kPer = (kBins + kThreads) / kThreads;
 
 // a candidate in the ranking's order: larger ones first
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) { return static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~id); }
+
+// What is asked of a row, and the bins its answers lie in: up to four ranges of bins, apart and in order.
+struct Plan {
+    int lo[4], hi[4], ranges;
+    uint32_t listed;                    // candidates of all open bins; more than kList: by descent
+    int k_bin;                          // the open bin of the last candidate of top_k, and its place in the list
+    uint32_t k_at;                      // ~0: top_k leaves out nothing that has weight
+    int m_bin;                          // the first open bin that min_p may part, -1: none
+    uint32_t m_end;                     // the candidates of those bins end here in the list
+    uint64_t all;                       // mass of the row
+    struct {
+        uint64_t mass, end;             // mass before the bin, and with it
+        uint32_t first;                 // candidates of open bins before it
+    } bin[kOpen];
+};
 
 // What a row's workgroups share, in the workspace. Cleared by the first launch.
 struct Row {
     uint64_t mass[kBins];
     uint32_t count[kBins];
-    uint32_t listed, done;
+    uint32_t listed, counted, gathered, reserved;
+    Plan plan;
     uint64_t list[kList];
 };
 
 struct Work {
     union {
         struct {
-            uint64_t mass[kBins + 2];   // by bin, then of the bins before
-            uint32_t count[kBins + 2];
-            uint64_t list[kList], run[kList];
-            uint64_t wave_mass[kThreads / 64];
-            uint32_t wave_count[kThreads / 64];
-            uint64_t found;
-            uint32_t listed, last;
-        } s;
+            uint64_t mass[kBins + 1];   // by bin, then of the bins before
+            uint32_t count[kBins + 1];
+        } bins;
+        struct {
+            uint64_t list[kList], run[kList], sorted[kThreads];
+        } pick;
         Shared descent;
     };
+    Plan plan;
+    ExpTable exp;
+    uint64_t wave_mass[kThreads / 64];
+    uint32_t wave_count[kThreads / 64];
+    uint64_t found;
+    uint32_t listed, last;
 };
 
+__device__ __forceinline__ uint64_t wave_top(uint64_t v) {
+    for (int d = 1; d < 64; d <<= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), d)));
+    return v;
+}
 // largest entry of ids [i, e)
-__device__ uint64_t slice_top(const float* x, int i, int e, Work& sh) {
+__device__ uint64_t slice_top(const float* x, int i, int e, uint64_t* waves) {
     uint64_t top = 0;
+#pragma unroll 4
     for (int j = i + threadIdx.x; j < e; j += kThreads) top = max(top, entry_of(key_of(x[j]), j));
-    for (int d = 1; d < 64; d <<= 1) top = max(top, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(top), d)));
-    if ((threadIdx.x & 63) == 0) sh.s.wave_mass[threadIdx.x / 64] = top;
+    top = wave_top(top);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = top;
     __syncthreads();
-    for (int j = 0; j < kThreads / 64; ++j) top = max(top, sh.s.wave_mass[j]);
-    __syncthreads();
-    return top;
+    return wave_top(waves[threadIdx.x & (kThreads / 64 - 1)]);
+}
+__device__ __forceinline__ uint64_t row_top(const uint64_t* tops, int slices) {
+    uint64_t top = 0;
+    for (int i = threadIdx.x & 63; i < slices; i += 64) top = max(top, tops[i]);
+    return wave_top(top);
 }
 
 // greedy and empty rows, and rows without a candidate: true if there is nothing more to do
@@ -239,217 +297,257 @@ __device__ bool plain_row(const SampleArgs& a, int b, float T, uint64_t top, boo
 }
 
 __device__ void clear_bins(Work& sh) {
-    for (int i = threadIdx.x; i < kBins + 2; i += kThreads) sh.s.mass[i] = 0, sh.s.count[i] = 0;
+    for (int i = threadIdx.x; i <= kBins; i += kThreads) sh.bins.mass[i] = 0, sh.bins.count[i] = 0;
 }
 __device__ void count_slice(const float* x, int i, int e, const Weigher& w, Work& sh) {
+#pragma unroll 4
     for (int j = i + threadIdx.x; j < e; j += kThreads) {
         const double z = w.depth(key_of(x[j]));
         if (!(z < 36.0)) continue;
         const int bin = Weigher::bin(z);
-        atomicAdd(&sh.s.count[bin], 1u);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.s.mass[bin]), static_cast<unsigned long long>(w.units(z)));
+        atomicAdd(&sh.bins.count[bin], 1u);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(z)));
     }
 }
 
 // bins' counts and masses become those of the bins before; the totals stand behind the last
 __device__ void add_up(Work& sh) {
     const int t = threadIdx.x, lane = t & 63, wave = t / 64;
-    uint64_t m = 0;
-    uint32_t n = 0;
+    uint64_t m[kPer], im = 0;
+    uint32_t n[kPer], in = 0;
+#pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = t * kPer + i;
-        if (b < kBins) m += sh.s.mass[b], n += sh.s.count[b];
+        m[i] = b < kBins ? sh.bins.mass[b] : 0, n[i] = b < kBins ? sh.bins.count[b] : 0;
+        im += m[i], in += n[i];
     }
-    uint64_t im = m;
-    uint32_t in = n;
+    const uint64_t sm = im;
+    const uint32_t sn = in;
     for (int d = 1; d < 64; d <<= 1) {
         const uint64_t om = __shfl_up(static_cast<unsigned long long>(im), d);
         const uint32_t on = __shfl_up(in, d);
         if (lane >= d) im += om, in += on;
     }
-    if (lane == 63) sh.s.wave_mass[wave] = im, sh.s.wave_count[wave] = in;
+    if (lane == 63) sh.wave_mass[wave] = im, sh.wave_count[wave] = in;
     __syncthreads();
-    im -= m, in -= n;
-    for (int i = 0; i < wave; ++i) im += sh.s.wave_mass[i], in += sh.s.wave_count[i];
+    im -= sm, in -= sn;
+    for (int i = 0; i < wave; ++i) im += sh.wave_mass[i], in += sh.wave_count[i];
+#pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = t * kPer + i;
-        if (b > kBins) break;
-        const uint64_t bm = sh.s.mass[b];
-        const uint32_t bn = sh.s.count[b];
-        sh.s.mass[b] = im, sh.s.count[b] = in;
-        if (b < kBins) im += bm, in += bn;
+        if (b <= kBins) sh.bins.mass[b] = im, sh.bins.count[b] = in;
+        im += m[i], in += n[i];
     }
     __syncthreads();
 }
 
-// the bin that holds unit x of the mass (x below the total) or candidate x
+// the bin that holds unit x of the mass (x below the total) or candidate x: 64 steps of 72 bins, then one by one
 template <bool BY_MASS>
-__device__ int bin_of(uint64_t x, Work& sh) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-        const uint64_t lo = BY_MASS ? sh.s.mass[b] : sh.s.count[b], hi = BY_MASS ? sh.s.mass[b + 1] : sh.s.count[b + 1];
-        if (lo <= x && x < hi) sh.s.found = b;
-    }
-    __syncthreads();
-    const int b = static_cast<int>(sh.s.found);
-    __syncthreads();
-    return b;
+__device__ int bin_of(uint64_t x, const Work& sh) {
+    static_assert(kBins % 64 == 0 && kBins / 64 <= 128);
+    const int lane = threadIdx.x & 63;
+    const auto before = [&](int b) { return BY_MASS ? sh.bins.mass[b] : static_cast<uint64_t>(sh.bins.count[b]); };
+    const int base = (__popcll(__ballot(before(lane * (kBins / 64)) <= x)) - 1) * (kBins / 64);
+    int n = __popcll(__ballot(before(base + lane) <= x));
+    if (n == 64 && kBins / 64 > 64) n += __popcll(__ballot(lane < kBins / 64 - 64 && before(min(base + 64 + lane, kBins)) <= x));
+    return base + n - 1;
 }
 
-// Bins that are open: up to four ranges [lo, hi], in order, apart.
-struct Open {
-    int lo[4], hi[4], n = 0;
-    __device__ void add(int l, int h) {
-        for (int i = 0; i < n;) {       // ranges that meet become one
-            if (l <= hi[i] + 1 && lo[i] <= h + 1) {
-                l = min(l, lo[i]), h = max(h, hi[i]);
-                --n;
-                for (int j = i; j < n; ++j) lo[j] = lo[j + 1], hi[j] = hi[j + 1];
-            } else {
-                ++i;
-            }
-        }
-        int i = n++;
-        for (; i > 0 && lo[i - 1] > l; --i) lo[i] = lo[i - 1], hi[i] = hi[i - 1];
-        lo[i] = l, hi[i] = h;
-    }
-    __device__ bool holds(int b) const {
-        bool in = false;
-        for (int i = 0; i < n; ++i) in |= lo[i] <= b && b <= hi[i];
-        return in;
-    }
-    // candidates of the open bins before bin b
-    __device__ uint32_t before(int b, const Work& sh) const {
-        uint32_t c = 0;
-        for (int i = 0; i < n; ++i)
-            if (lo[i] < b) c += sh.s.count[min(hi[i] + 1, b)] - sh.s.count[lo[i]];
-        return c;
-    }
-};
-
-// What is asked of a row, and where by its bins the answers may lie.
-struct Question {
-    int k;                              // 0: no top_k that leaves weight out
-    float tp, mp, u;
-    int bk, bm_lo, bm_hi;
-    Open open;
-};
-__device__ Question ask(const SampleArgs& a, int b, Work& sh) {
-    Question q;
+// Makes the plan, once all is counted and added up: one wave.
+__device__ void make_plan(const SampleArgs& a, int b, Work& sh) {
+    Plan& p = sh.plan;
+    const int lane = threadIdx.x & 63;
     const int k = a.top_k ? a.top_k[b] : 0;
-    q.k = k > 0 && static_cast<uint32_t>(k) < sh.s.count[kBins] ? k : 0;
-    q.tp = a.top_p ? a.top_p[b] : 1.0f;
-    q.mp = a.min_p ? a.min_p[b] : 0.0f;
-    q.u = a.u[b];
-    q.bk = q.bm_lo = q.bm_hi = 0;
-    uint64_t lo = sh.s.mass[kBins], hi = lo;  // the total lies within
-    if (q.k) {
-        q.bk = bin_of<false>(q.k - 1, sh);
-        q.open.add(q.bk, q.bk);
-        lo = max(sh.s.mass[q.bk], uint64_t{1}), hi = sh.s.mass[q.bk + 1];
+    const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f, u = a.u[b];
+    const uint64_t all = sh.bins.mass[kBins];
+    uint64_t lo = all, hi = all;        // the total lies within
+    int l[4] = {0, 0, 0, 0}, h[4] = {-1, -1, -1, -1};
+    const bool by_k = k > 0 && static_cast<uint32_t>(k) < sh.bins.count[kBins];
+    if (by_k) {
+        l[0] = h[0] = bin_of<false>(k - 1, sh);
+        lo = max(sh.bins.mass[l[0]], uint64_t{1}), hi = sh.bins.mass[l[0] + 1];
     }
-    if (q.tp < 1.0f) {
-        const int l = bin_of<true>(top_p_place(q.tp, lo), sh), h = bin_of<true>(top_p_place(q.tp, hi), sh);
-        q.open.add(l, h);
-        lo = max(sh.s.mass[l], uint64_t{1}), hi = min(hi, sh.s.mass[h + 1]);
+    if (tp < 1.0f) {
+        l[1] = bin_of<true>(top_p_place(tp, lo), sh), h[1] = bin_of<true>(top_p_place(tp, hi), sh);
+        lo = max(sh.bins.mass[l[1]], uint64_t{1}), hi = min(hi, sh.bins.mass[h[1] + 1]);
     }
-    if (q.mp > 0.0f) {
+    if (mp > 0.0f) {
         // depths next to the border are compared one by one
-        const double z = q.mp < 1.0f ? -log(static_cast<double>(q.mp)) : 0.0;
-        q.bm_lo = Weigher::bin(fmax(z - 1e-6, 0.0)), q.bm_hi = min(Weigher::bin(z + 1e-6), kBins - 1);
-        if (q.bm_lo < kBins) {
-            q.open.add(q.bm_lo, q.bm_hi);
-            lo = min(lo, max(sh.s.mass[q.bm_lo], uint64_t{1})), hi = min(hi, sh.s.mass[q.bm_hi + 1]);
-        } else {
-            q.mp = 0.0f;                // only what has no weight is left out
-        }
+        const double z = mp < 1.0f ? -log(static_cast<double>(mp)) : 0.0;
+        l[2] = Weigher::bin(fmax(z - 1e-6, 0.0)), h[2] = min(Weigher::bin(z + 1e-6), kBins - 1);
+        if (l[2] < kBins) lo = min(lo, max(sh.bins.mass[l[2]], uint64_t{1})), hi = min(hi, sh.bins.mass[h[2] + 1]);
+        else l[2] = 0, h[2] = -1;       // only what has no weight is left out
     }
-    q.open.add(bin_of<true>(drawn_place(q.u, lo), sh), bin_of<true>(drawn_place(q.u, hi), sh));
-    return q;
+    l[3] = bin_of<true>(drawn_place(u, lo), sh), h[3] = bin_of<true>(drawn_place(u, hi), sh);
+    // the ranges in order, those that meet as one
+    const int k_bin = l[0], m_lo = l[2], m_hi = h[2];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (h[j] < l[j] || (h[j + 1] >= l[j + 1] && l[j + 1] < l[j])) {  // empty ones last
+                const int x = l[j], y = h[j];
+                l[j] = l[j + 1], h[j] = h[j + 1], l[j + 1] = x, h[j + 1] = y;
+            }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = i + 1; j < 4; ++j)
+            if (h[i] >= l[i] && h[j] >= l[j] && l[j] <= h[i] + 1) h[i] = max(h[i], h[j]), l[j] = 0, h[j] = -1;
+    uint32_t first = 0, k_first = 0, m_end = 0;
+    int open = 0, k_open = 0, m_open = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (h[i] < l[i]) continue;
+        if (by_k && l[i] <= k_bin && k_bin <= h[i]) {
+            k_open = open + k_bin - l[i];
+            k_first = first + sh.bins.count[k_bin] - sh.bins.count[l[i]];
+        }
+        if (m_lo <= m_hi && l[i] <= m_lo && m_lo <= h[i]) {
+            m_open = open + m_lo - l[i];
+            m_end = first + sh.bins.count[m_hi + 1] - sh.bins.count[l[i]];
+        }
+        for (int bin = l[i] + lane; bin <= h[i] && open + bin - l[i] < kOpen; bin += 64) {
+            auto& e = p.bin[open + bin - l[i]];
+            e.mass = sh.bins.mass[bin], e.end = sh.bins.mass[bin + 1], e.first = first + sh.bins.count[bin] - sh.bins.count[l[i]];
+        }
+        open += h[i] - l[i] + 1;
+        first += sh.bins.count[h[i] + 1] - sh.bins.count[l[i]];
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.lo[i] = l[i], p.hi[i] = h[i];
+        p.ranges = open;
+        p.listed = open <= kOpen ? first : ~0u;
+        p.k_bin = k_open;
+        p.k_at = by_k ? k_first + (k - 1 - sh.bins.count[k_bin]) : ~0u;
+        p.m_bin = m_open;
+        p.m_end = m_end;
+        p.all = all;
+    }
+}
+
+__device__ void copy_plan(Plan& to, const Plan& from) {
+    const int words = static_cast<int>(offsetof(Plan, bin) / 4 + min(from.ranges, kOpen) * (sizeof(from.bin[0]) / 4));
+    for (int i = threadIdx.x; i < words; i += kThreads) reinterpret_cast<uint32_t*>(&to)[i] = reinterpret_cast<const uint32_t*>(&from)[i];
 }
 
 // ids [i, e) of the open bins, to a list
-__device__ void gather(const float* x, int i, int e, const Weigher& w, const Open& open, uint64_t* list, uint32_t* listed) {
+__device__ void gather(const float* x, int i, int e, const Weigher& w, const Plan& p, uint64_t* list, uint32_t* listed) {
+    double lo[4], hi[4];                // in 128ths of depth
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], hi[r] = p.hi[r] + 1;
+#pragma unroll 4
     for (int j = i + threadIdx.x; j < e; j += kThreads) {
         const uint32_t key = key_of(x[j]);
-        const double z = w.depth(key);
-        if (z < 36.0 && open.holds(Weigher::bin(z))) list[atomicAdd(listed, 1u)] = entry_of(key, j);
+        const double z = fmin(w.depth(key), 36.0) * 128.0;
+        bool in = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) in |= z >= lo[r] && z < hi[r];
+        if (in) list[atomicAdd(listed, 1u)] = entry_of(key, j);
     }
 }
 
-// The exact places, from the n candidates of the open bins in sh.s.list.
-__device__ void settle(const SampleArgs& a, int b, int n, const Weigher& w, const Question& q, Work& sh) {
-    const int t = threadIdx.x, lane = t & 63, wave = t / 64;
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + t; i < size; i += kThreads) sh.s.list[i] = 0;
+// The exact places, from the candidates of the open bins in sh.pick.list.
+__device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
     __syncthreads();
-    // bitonic sort, largest first
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int p = t; p < size / 2; p += kThreads) {
-                const int i = 2 * p - (p & (j - 1));
-                const uint64_t x = sh.s.list[i], y = sh.s.list[i + j];
-                if ((x < y) == ((i & k) == 0)) sh.s.list[i] = y, sh.s.list[i + j] = x;
+    const Plan& p = sh.plan;
+    const int t = threadIdx.x, lane = t & 63, wave = t / 64, n = static_cast<int>(p.listed);
+    if (n <= kThreads) {
+        // few: a candidate's rank is the number of larger ones; 1024 / size threads count for one
+        int size = 64;
+        while (size < n) size *= 2;
+        const int parts = kThreads / size, i = t / parts, part = t & (parts - 1);
+        const uint64_t mine = i < n ? sh.pick.list[i] : 0;
+        uint32_t rank = 0;
+        for (int j = part; j < n; j += parts) rank += sh.pick.list[j] > mine;
+        for (int d = 1; d < parts; d <<= 1) rank += __shfl_xor(rank, d);
+        if (i < n && part == 0) sh.pick.sorted[rank] = mine;
+        __syncthreads();
+        if (t < n) sh.pick.list[t] = sh.pick.sorted[t];
+        __syncthreads();
+    } else {
+        for (int i = n + t; i < kList; i += kThreads) sh.pick.list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= kList; k *= 2)  // bitonic, largest first
+            for (int j = k / 2; j > 0; j /= 2) {
+                for (int q = t; q < kList / 2; q += kThreads) {
+                    const int i = 2 * q - (q & (j - 1));
+                    const uint64_t x = sh.pick.list[i], y = sh.pick.list[i + j];
+                    if ((x < y) == ((i & k) == 0)) sh.pick.list[i] = y, sh.pick.list[i + j] = x;
+                }
+                __syncthreads();
             }
-            __syncthreads();
-        }
+    }
     // running masses
     constexpr int kEach = kList / kThreads;
-    uint64_t m[kEach], sum = 0;
+    uint64_t m[kEach], in = 0;
+#pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const int at = t * kEach + i;
-        m[i] = at < n ? w(static_cast<uint32_t>(sh.s.list[at] >> 32)) : 0;
-        sum += m[i];
+        m[i] = at < n ? w(static_cast<uint32_t>(sh.pick.list[at] >> 32)) : 0;
+        in += m[i];
     }
-    uint64_t in = sum;
+    const uint64_t sum = in;
     for (int d = 1; d < 64; d <<= 1) {
         const uint64_t o = __shfl_up(static_cast<unsigned long long>(in), d);
         if (lane >= d) in += o;
     }
-    if (lane == 63) sh.s.wave_mass[wave] = in;
+    if (lane == 63) sh.wave_mass[wave] = in;
     __syncthreads();
     in -= sum;
-    for (int i = 0; i < wave; ++i) in += sh.s.wave_mass[i];
+    for (int i = 0; i < wave; ++i) in += sh.wave_mass[i];
+#pragma unroll
     for (int i = 0; i < kEach; ++i) {
         in += m[i];
-        sh.s.run[t * kEach + i] = in;
+        sh.pick.run[t * kEach + i] = in;
     }
+    if (t == 0) sh.listed = 0;
     __syncthreads();
-    const auto run = [&](uint32_t i) { return i ? sh.s.run[i - 1] : 0; };  // of the first i
-    // the listed candidate that holds unit x of the row's mass
-    const auto holder = [&](uint64_t x) {
-        const int bin = bin_of<true>(x, sh);
-        const uint32_t first = q.open.before(bin, sh);
-        const uint64_t at = x - sh.s.mass[bin] + run(first);
-        for (int i = t; i < n; i += kThreads)
-            if (run(i) <= at && at < run(i + 1)) sh.s.found = i | static_cast<uint64_t>(bin) << 32;
-        __syncthreads();
-        const uint64_t f = sh.s.found;
-        __syncthreads();
-        return f;
-    };
-    const auto up_to = [&](uint32_t i, int bin) { return sh.s.mass[bin] + run(i + 1) - run(q.open.before(bin, sh)); };
-    uint64_t total = sh.s.mass[kBins];
-    if (q.k) total = up_to(q.open.before(q.bk, sh) + (q.k - 1 - sh.s.count[q.bk]), q.bk);
-    if (q.tp < 1.0f) {
-        const uint64_t f = holder(top_p_place(q.tp, total));
-        total = up_to(static_cast<uint32_t>(f), static_cast<int>(f >> 32));
-    }
-    if (q.mp > 0.0f) {
-        const uint32_t first = q.open.before(q.bm_lo, sh), end = q.open.before(q.bm_hi + 1, sh);
-        if (t == 0) sh.s.listed = 0;
-        __syncthreads();
+    const auto run = [&](uint32_t i) { return i ? sh.pick.run[i - 1] : 0; };  // of the first i
+    const float mp = a.min_p ? a.min_p[b] : 0.0f;
+    if (p.m_bin >= 0) {                 // how many of those bins' candidates min_p leaves
         uint32_t c = 0;
-        for (uint32_t i = first + t; i < end; i += kThreads) c += w.share(static_cast<uint32_t>(sh.s.list[i] >> 32)) >= q.mp;
-        if (c) atomicAdd(&sh.s.listed, c);
+        for (uint32_t i = p.bin[p.m_bin].first + t; i < p.m_end; i += kThreads)
+            c += w.share(static_cast<uint32_t>(sh.pick.list[i] >> 32)) >= mp;
+        if (c) atomicAdd(&sh.listed, c);
         __syncthreads();
-        const uint64_t most = sh.s.mass[q.bm_lo] + run(first + sh.s.listed) - run(first);
+    }
+    if (wave) return;
+    // the listed candidate that holds unit x of the row's mass, and its bin: one wave
+    int bin = 0;
+    const auto holder = [&](uint64_t x) -> uint32_t {
+        for (int i = 0; i < p.ranges; i += 64) {
+            const bool in_it = i + lane < p.ranges && p.bin[min(i + lane, kOpen - 1)].mass <= x && x < p.bin[min(i + lane, kOpen - 1)].end;
+            if (const uint64_t v = __ballot(in_it)) bin = i + __ffsll(static_cast<unsigned long long>(v)) - 1;
+        }
+        const uint64_t at = x - p.bin[bin].mass + run(p.bin[bin].first);
+        uint32_t low = p.bin[bin].first, count = n - low;  // the first i with run(i + 1) > at
+        while (count > 0) {
+            const uint32_t step = (count + 63) / 64;
+            const uint32_t i = low + (lane + 1) * step;  // candidates [low, i) end at or before `at`
+            const uint32_t k = __popcll(__ballot(i <= low + count && run(i) <= at));
+            low += k * step;
+            count = step == 1 ? 0 : min(step, count - min(count, k * step));
+        }
+        return low;
+    };
+    const auto up_to = [&](uint32_t i) { return p.bin[bin].mass + run(i + 1) - run(p.bin[bin].first); };
+    uint64_t total = p.all;
+    if (p.k_at != ~0u) bin = p.k_bin, total = up_to(p.k_at);
+    const float tp = a.top_p ? a.top_p[b] : 1.0f;
+    if (tp < 1.0f) {
+        const uint32_t i = holder(top_p_place(tp, total));
+        total = up_to(i);
+    }
+    if (p.m_bin >= 0) {
+        const uint32_t first = p.bin[p.m_bin].first;
+        const uint64_t most = p.bin[p.m_bin].mass + run(first + sh.listed) - run(first);
         total = min(total, max(most, static_cast<uint64_t>(w.unit)));  // the first place stays
     }
-    const uint32_t at = static_cast<uint32_t>(holder(drawn_place(q.u, total)));
-    if (t == 0) {
-        const uint64_t e = sh.s.list[at];
-        a.token[b] = static_cast<int>(~static_cast<uint32_t>(e));
+    const uint32_t at = holder(drawn_place(a.u[b], total));
+    if (lane == 0) {
+        a.token[b] = static_cast<int>(~static_cast<uint32_t>(sh.pick.list[at]));
         if (a.prob) a.prob[b] = static_cast<float>(static_cast<double>(run(at + 1) - run(at)) / static_cast<double>(total));
     }
 }
@@ -457,40 +555,55 @@ __device__ void settle(const SampleArgs& a, int b, int n, const Weigher& w, cons
 __device__ __forceinline__ int slice_begin(int V, int slices, int i) { return static_cast<int>(static_cast<int64_t>(V) * i / slices); }
 
 __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, int slices, uint64_t* tops, Row* rows) {
-    __shared__ Work sh;
+    __shared__ uint64_t waves[kThreads / 64];
     const int b = blockIdx.y, s = blockIdx.x;
     Row& r = rows[b];
     for (int i = s * kThreads + threadIdx.x; i < kBins; i += slices * kThreads) r.mass[i] = 0, r.count[i] = 0;
-    if (s == 0 && threadIdx.x == 0) r.listed = 0, r.done = 0;
+    if (s == 0 && threadIdx.x == 0) r.listed = 0, r.counted = 0, r.gathered = 0;
     if (!(a.temperature[b] >= 0.0f)) return;  // an empty place
-    const uint64_t top = slice_top(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), sh);
+    const uint64_t top = slice_top(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), waves);
     if (threadIdx.x == 0) tops[b * slices + s] = top;
 }
 
-__device__ uint64_t row_top(const uint64_t* tops, int slices) {
-    uint64_t top = 0;
-    for (int i = 0; i < slices; ++i) top = max(top, tops[i]);
-    return top;
+// Whether this workgroup is the last of the row's to come here; it sees what the others have written. (One
+// wave's fences do for all of them, behind a barrier and before one: each writes back or drops a whole cache.)
+__device__ bool last_of(uint32_t* ticket, int slices, Work& sh) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        sh.last = atomicAdd(ticket, 1u) == static_cast<uint32_t>(slices) - 1;
+        if (sh.last) __threadfence();
+    }
+    __syncthreads();
+    return sh.last;
 }
 
 __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, double unit, int slices, const uint64_t* tops, Row* rows) {
     __shared__ Work sh;
     const int b = blockIdx.y, s = blockIdx.x;
     const float T = a.temperature[b];
-    if (!(T > 0.0f)) return;
+    if (!(T >= 0.0f)) return;
     const uint64_t top = row_top(tops + b * slices, slices);
-    if (plain_row(a, b, T, top, false)) return;
-    const Weigher w(static_cast<uint32_t>(top >> 32), T, unit);
+    if (plain_row(a, b, T, top, s == 0 && threadIdx.x == 0)) return;
+    const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
+    sh.exp.fill();
     clear_bins(sh);
     __syncthreads();
     count_slice(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, sh);
     __syncthreads();
     Row& r = rows[b];
     for (int i = threadIdx.x; i < kBins; i += kThreads)
-        if (sh.s.count[i]) {
-            atomicAdd(&r.count[i], sh.s.count[i]);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&r.mass[i]), static_cast<unsigned long long>(sh.s.mass[i]));
+        if (sh.bins.count[i]) {
+            atomicAdd(&r.count[i], sh.bins.count[i]);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&r.mass[i]), static_cast<unsigned long long>(sh.bins.mass[i]));
         }
+    if (!last_of(&r.counted, slices, sh)) return;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins.mass[i] = r.mass[i], sh.bins.count[i] = r.count[i];
+    __syncthreads();
+    add_up(sh);
+    if (threadIdx.x < 64) make_plan(a, b, sh);
+    __syncthreads();
+    copy_plan(r.plan, sh.plan);
 }
 
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, double unit, int slices, const uint64_t* tops, Row* rows) {
@@ -499,29 +612,21 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, dou
     const float T = a.temperature[b];
     if (!(T >= 0.0f)) return;
     const uint64_t top = row_top(tops + b * slices, slices);
-    if (plain_row(a, b, T, top, s == 0 && threadIdx.x == 0)) return;
-    const Weigher w(static_cast<uint32_t>(top >> 32), T, unit);
+    if (plain_row(a, b, T, top, false)) return;
+    const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
+    sh.exp.fill();
     Row& r = rows[b];
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.s.mass[i] = r.mass[i], sh.s.count[i] = r.count[i];
+    const uint32_t n = r.plan.listed;
+    if (n <= kList) gather(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, r.plan, r.list, &r.listed);
+    if (!last_of(&r.gathered, slices, sh)) return;
     __syncthreads();
-    add_up(sh);
-    const Question q = ask(a, b, sh);
-    const uint32_t n = q.open.before(kBins, sh);
-    if (n <= kList) gather(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, q.open, r.list, &r.listed);
-    // the workgroup that is done last sees what all have listed
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) sh.s.last = atomicAdd(&r.done, 1u) == static_cast<uint32_t>(slices) - 1;
-    __syncthreads();
-    if (!sh.s.last) return;
-    __threadfence();
     if (n > kList) {
-        __syncthreads();
         sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
         return;
     }
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.s.list[i] = r.list[i];
-    settle(a, b, n, w, q, sh);
+    copy_plan(sh.plan, r.plan);
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.pick.list[i] = r.list[i];
+    settle(a, b, w, sh);
 }
 
 // a row of one slice
@@ -532,24 +637,22 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
     if (!(T >= 0.0f)) return;
     const float* x = a.logits + b * a.ld;
     clear_bins(sh);
-    const uint64_t top = slice_top(x, 0, a.V, sh);
+    sh.exp.fill();
+    const uint64_t top = slice_top(x, 0, a.V, sh.wave_mass);
     if (plain_row(a, b, T, top, threadIdx.x == 0)) return;
-    const Weigher w(static_cast<uint32_t>(top >> 32), T, unit);
+    const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
     count_slice(x, 0, a.V, w, sh);
     __syncthreads();
     add_up(sh);
-    const Question q = ask(a, b, sh);
-    const uint32_t n = q.open.before(kBins, sh);
-    if (n > kList) {
-        __syncthreads();
+    if (threadIdx.x < 64) make_plan(a, b, sh);
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    if (sh.plan.listed > kList) {
         sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
         return;
     }
-    if (threadIdx.x == 0) sh.s.listed = 0;
-    __syncthreads();
-    gather(x, 0, a.V, w, q.open, sh.s.list, &sh.s.listed);
-    __syncthreads();
-    settle(a, b, n, w, q, sh);
+    gather(x, 0, a.V, w, sh.plan, sh.pick.list, &sh.listed);
+    settle(a, b, w, sh);
 }
 
 int sample_slices(int B, int V) { return std::max(1, std::min((V + 4095) / 4096, 512 / std::min(B, 512))); }
