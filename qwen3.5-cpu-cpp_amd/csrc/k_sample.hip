@@ -63,13 +63,12 @@ struct Weigher {
     bool inf;
     __device__ Weigher(uint32_t key, float T, double unit_, const ExpTable& e)
         : top(of_key(key)), rt(1.0 / static_cast<double>(T)), unit(unit_), table(e), inf(key == kKeyInf) {}
-    // (max - l) / T
-    __device__ double depth(uint32_t key) const {
-        if (inf) return key == kKeyInf ? 0.0 : INFINITY;
-        if (key == kKeyNone) return INFINITY;
-        const double d = top - static_cast<double>(of_key(key));
-        return d == 0.0 ? 0.0 : d * rt;
+    // (max - l) / T: infinite or a NaN where a candidate is ruled out
+    __device__ double depth(float l) const {
+        if (inf) return l == INFINITY ? 0.0 : INFINITY;
+        return (top - static_cast<double>(l)) * rt;
     }
+    __device__ double depth(uint32_t key) const { return depth(of_key(key)); }
     static __device__ int bin(double depth) { return static_cast<int>(fmin(depth * 128.0, static_cast<double>(kBins))); }
     // the weight in 64 bits, of the largest
     __device__ double share(uint32_t key) const {
@@ -217,6 +216,7 @@ __device__ void sample_by_descent(const SampleArgs& a, int b, uint32_t top, cons
 // ---- by bins
 constexpr int kList = 2048;             // candidates of the open bins
 constexpr int kOpen = 512;              // open bins
+constexpr int kBuckets = kThreads;
 constexpr int kPer = (kBins + kThreads) / kThreads;
 
 // a candidate in the ranking's order: larger ones first
@@ -253,7 +253,8 @@ struct Work {
             uint32_t count[kBins + 1];
         } bins;
         struct {
-            uint64_t list[kList], run[kList], sorted[kThreads];
+            uint64_t list[kList], run[kList];
+            uint32_t at[kBuckets];
         } pick;
         Shared descent;
     };
@@ -269,11 +270,18 @@ __device__ __forceinline__ uint64_t wave_top(uint64_t v) {
     for (int d = 1; d < 64; d <<= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), d)));
     return v;
 }
-// largest entry of ids [i, e)
-__device__ uint64_t slice_top(const float* x, int i, int e, uint64_t* waves) {
+// The largest entry of ids [i, e); where the temperature is not 0 only its key matters.
+__device__ uint64_t slice_top(const float* x, int i, int e, bool greedy, uint64_t* waves) {
     uint64_t top = 0;
+    if (greedy) {
 #pragma unroll 4
-    for (int j = i + threadIdx.x; j < e; j += kThreads) top = max(top, entry_of(key_of(x[j]), j));
+        for (int j = i + threadIdx.x; j < e; j += kThreads) top = max(top, entry_of(key_of(x[j]), j));
+    } else {
+        float m = -INFINITY;            // fmaxf passes over a NaN
+#pragma unroll 8
+        for (int j = i + threadIdx.x; j < e; j += kThreads) m = fmaxf(m, x[j]);
+        top = entry_of(key_of(m), 0);
+    }
     top = wave_top(top);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = top;
     __syncthreads();
@@ -302,9 +310,9 @@ __device__ void clear_bins(Work& sh) {
 __device__ void count_slice(const float* x, int i, int e, const Weigher& w, Work& sh) {
 #pragma unroll 4
     for (int j = i + threadIdx.x; j < e; j += kThreads) {
-        const double z = w.depth(key_of(x[j]));
+        const double z = w.depth(x[j]);
         if (!(z < 36.0)) continue;
-        const int bin = Weigher::bin(z);
+        const int bin = static_cast<int>(z * 128.0);
         atomicAdd(&sh.bins.count[bin], 1u);
         atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(z)));
     }
@@ -439,12 +447,11 @@ __device__ void gather(const float* x, int i, int e, const Weigher& w, const Pla
     for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], hi[r] = p.hi[r] + 1;
 #pragma unroll 4
     for (int j = i + threadIdx.x; j < e; j += kThreads) {
-        const uint32_t key = key_of(x[j]);
-        const double z = fmin(w.depth(key), 36.0) * 128.0;
+        const double z = w.depth(x[j]) * 128.0;
         bool in = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) in |= z >= lo[r] && z < hi[r];
-        if (in) list[atomicAdd(listed, 1u)] = entry_of(key, j);
+        if (in) list[atomicAdd(listed, 1u)] = entry_of(key_of(x[j]), j);
     }
 }
 
@@ -453,34 +460,58 @@ __device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
     __syncthreads();
     const Plan& p = sh.plan;
     const int t = threadIdx.x, lane = t & 63, wave = t / 64, n = static_cast<int>(p.listed);
-    if (n <= kThreads) {
-        // few: a candidate's rank is the number of larger ones; 1024 / size threads count for one
-        int size = 64;
-        while (size < n) size *= 2;
-        const int parts = kThreads / size, i = t / parts, part = t & (parts - 1);
-        const uint64_t mine = i < n ? sh.pick.list[i] : 0;
-        uint32_t rank = 0;
-        for (int j = part; j < n; j += parts) rank += sh.pick.list[j] > mine;
-        for (int d = 1; d < parts; d <<= 1) rank += __shfl_xor(rank, d);
-        if (i < n && part == 0) sh.pick.sorted[rank] = mine;
-        __syncthreads();
-        if (t < n) sh.pick.list[t] = sh.pick.sorted[t];
-        __syncthreads();
-    } else {
-        for (int i = n + t; i < kList; i += kThreads) sh.pick.list[i] = 0;
-        __syncthreads();
-        for (int k = 2; k <= kList; k *= 2)  // bitonic, largest first
-            for (int j = k / 2; j > 0; j /= 2) {
-                for (int q = t; q < kList / 2; q += kThreads) {
-                    const int i = 2 * q - (q & (j - 1));
-                    const uint64_t x = sh.pick.list[i], y = sh.pick.list[i + j];
-                    if ((x < y) == ((i & k) == 0)) sh.pick.list[i] = y, sh.pick.list[i + j] = x;
-                }
-                __syncthreads();
-            }
-    }
-    // running masses
+    // Sorted by buckets of equal width in depth, a few candidates each, and within one by counting.
+    for (int i = t; i < kBuckets; i += kThreads) sh.pick.at[i] = 0;
+    __syncthreads();
+    const double width = static_cast<double>(kBuckets) / p.ranges;
+    const auto bucket = [&](uint64_t e) {
+        const double z = w.depth(static_cast<uint32_t>(e >> 32)) * 128.0;
+        double before = 0.0;            // open bins before it
+#pragma unroll
+        for (int r = 0; r < 4; ++r) before += fmin(fmax(z - p.lo[r], 0.0), static_cast<double>(p.hi[r] + 1 - p.lo[r]));
+        return min(static_cast<int>(before * width), kBuckets - 1);
+    };
     constexpr int kEach = kList / kThreads;
+    uint64_t mine[kEach];
+    int of[kEach];
+    uint32_t place[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        mine[i] = t + i * kThreads < n ? sh.pick.list[t + i * kThreads] : 0;
+        of[i] = mine[i] ? bucket(mine[i]) : -1;
+        place[i] = mine[i] ? atomicAdd(&sh.pick.at[of[i]], 1u) : 0;
+    }
+    __syncthreads();
+    static_assert(kBuckets == kThreads);
+    const uint32_t held = sh.pick.at[t];
+    uint32_t begin = held;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(begin, d);
+        if (lane >= d) begin += o;
+    }
+    if (lane == 63) sh.wave_count[wave] = begin;
+    __syncthreads();
+    begin -= held;
+    for (int i = 0; i < wave; ++i) begin += sh.wave_count[i];
+    sh.pick.at[t] = begin;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (mine[i]) sh.pick.list[sh.pick.at[of[i]] + place[i]] = mine[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (!mine[i]) continue;
+        const uint32_t first = sh.pick.at[of[i]], end = of[i] + 1 < kBuckets ? sh.pick.at[of[i] + 1] : n;
+        place[i] = first;
+        for (uint32_t j = first; j < end; ++j) place[i] += sh.pick.list[j] > mine[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (mine[i]) sh.pick.list[place[i]] = mine[i];
+    __syncthreads();
+    // running masses
     uint64_t m[kEach], in = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -561,7 +592,7 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, int 
     for (int i = s * kThreads + threadIdx.x; i < kBins; i += slices * kThreads) r.mass[i] = 0, r.count[i] = 0;
     if (s == 0 && threadIdx.x == 0) r.listed = 0, r.counted = 0, r.gathered = 0;
     if (!(a.temperature[b] >= 0.0f)) return;  // an empty place
-    const uint64_t top = slice_top(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), waves);
+    const uint64_t top = slice_top(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), a.temperature[b] == 0.0f, waves);
     if (threadIdx.x == 0) tops[b * slices + s] = top;
 }
 
@@ -638,7 +669,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
     const float* x = a.logits + b * a.ld;
     clear_bins(sh);
     sh.exp.fill();
-    const uint64_t top = slice_top(x, 0, a.V, sh.wave_mass);
+    const uint64_t top = slice_top(x, 0, a.V, T == 0.0f, sh.wave_mass);
     if (plain_row(a, b, T, top, threadIdx.x == 0)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
     count_slice(x, 0, a.V, w, sh);
