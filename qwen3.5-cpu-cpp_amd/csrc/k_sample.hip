@@ -214,27 +214,33 @@ __device__ void sample_by_descent(const SampleArgs& a, int b, uint32_t top, cons
 }
 
 // ---- by bins
-constexpr int kList = 2048;             // candidates of the open bins
-constexpr int kOpen = 512;              // open bins
+constexpr int kList = 2048;             // candidates that can be listed
+constexpr int kMostK = 1024;            // top_k up to this: every candidate that it may leave is listed
 constexpr int kBuckets = kThreads;
 constexpr int kPer = (kBins + kThreads) / kThreads;
 
 // a candidate in the ranking's order: larger ones first
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) { return static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~id); }
 
-// What is asked of a row, and the bins its answers lie in: up to four ranges of bins, apart and in order.
+// What is asked of a row.
+struct Question {
+    int k;                              // 0: all
+    float p, m, u;
+    bool few;                           // a small top_k: counts alone lead to its candidates
+    __device__ Question(const SampleArgs& a, int b)
+        : k(a.top_k ? max(a.top_k[b], 0) : 0), p(a.top_p ? a.top_p[b] : 1.0f), m(a.min_p ? a.min_p[b] : 0.0f), u(a.u[b]),
+          few(k > 0 && k <= kMostK) {}
+};
+
+// The open bins, in up to four ranges, apart and in order (empty ones have hi < lo): all their candidates are
+// listed.
 struct Plan {
-    int lo[4], hi[4], ranges;
-    uint32_t listed;                    // candidates of all open bins; more than kList: by descent
-    int k_bin;                          // the open bin of the last candidate of top_k, and its place in the list
-    uint32_t k_at;                      // ~0: top_k leaves out nothing that has weight
-    int m_bin;                          // the first open bin that min_p may part, -1: none
-    uint32_t m_end;                     // the candidates of those bins end here in the list
+    int lo[4], hi[4];
+    uint64_t mass[4], end[4];           // mass before the range, and with it
     uint64_t all;                       // mass of the row
-    struct {
-        uint64_t mass, end;             // mass before the bin, and with it
-        uint32_t first;                 // candidates of open bins before it
-    } bin[kOpen];
+    int k_range, m_range;               // where the last candidate of top_k and the first that min_p may leave out
+                                        // are; -1: they leave out nothing that has weight
+    uint32_t k_at, reserved;            // the place of the former in its range
 };
 
 // What a row's workgroups share, in the workspace. Cleared by the first launch.
@@ -262,8 +268,8 @@ struct Work {
     ExpTable exp;
     uint64_t wave_mass[kThreads / 64];
     uint32_t wave_count[kThreads / 64];
-    uint64_t found;
-    uint32_t listed, last;
+    uint32_t in_range[4];
+    uint32_t listed, base, last;
 };
 
 __device__ __forceinline__ uint64_t wave_top(uint64_t v) {
@@ -307,14 +313,17 @@ __device__ bool plain_row(const SampleArgs& a, int b, float T, uint64_t top, boo
 __device__ void clear_bins(Work& sh) {
     for (int i = threadIdx.x; i <= kBins; i += kThreads) sh.bins.mass[i] = 0, sh.bins.count[i] = 0;
 }
-__device__ void count_slice(const float* x, int i, int e, const Weigher& w, Work& sh) {
+// Masses by bin, and counts where there is a top_k; counts alone for a small one. (The additions in LDS bound
+// this: one of 64 bits takes more of its time than the weight.)
+__device__ void count_slice(const float* x, int i, int e, const Question& q, const Weigher& w, Work& sh) {
+    const bool counts = q.k > 0, masses = !q.few;
 #pragma unroll 4
     for (int j = i + threadIdx.x; j < e; j += kThreads) {
         const double z = w.depth(x[j]);
         if (!(z < 36.0)) continue;
         const int bin = static_cast<int>(z * 128.0);
-        atomicAdd(&sh.bins.count[bin], 1u);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(z)));
+        if (counts) atomicAdd(&sh.bins.count[bin], 1u);
+        if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(z)));
     }
 }
 
@@ -362,86 +371,73 @@ __device__ int bin_of(uint64_t x, const Work& sh) {
 }
 
 // Makes the plan, once all is counted and added up: one wave.
-__device__ void make_plan(const SampleArgs& a, int b, Work& sh) {
+__device__ void make_plan(const Question& q, Work& sh) {
     Plan& p = sh.plan;
-    const int lane = threadIdx.x & 63;
-    const int k = a.top_k ? a.top_k[b] : 0;
-    const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f, u = a.u[b];
-    const uint64_t all = sh.bins.mass[kBins];
-    uint64_t lo = all, hi = all;        // the total lies within
+    const uint64_t* mass = sh.bins.mass;
+    const uint32_t* count = sh.bins.count;
     int l[4] = {0, 0, 0, 0}, h[4] = {-1, -1, -1, -1};
-    const bool by_k = k > 0 && static_cast<uint32_t>(k) < sh.bins.count[kBins];
-    if (by_k) {
-        l[0] = h[0] = bin_of<false>(k - 1, sh);
-        lo = max(sh.bins.mass[l[0]], uint64_t{1}), hi = sh.bins.mass[l[0] + 1];
-    }
-    if (tp < 1.0f) {
-        l[1] = bin_of<true>(top_p_place(tp, lo), sh), h[1] = bin_of<true>(top_p_place(tp, hi), sh);
-        lo = max(sh.bins.mass[l[1]], uint64_t{1}), hi = min(hi, sh.bins.mass[h[1] + 1]);
-    }
-    if (mp > 0.0f) {
-        // depths next to the border are compared one by one
-        const double z = mp < 1.0f ? -log(static_cast<double>(mp)) : 0.0;
-        l[2] = Weigher::bin(fmax(z - 1e-6, 0.0)), h[2] = min(Weigher::bin(z + 1e-6), kBins - 1);
-        if (l[2] < kBins) lo = min(lo, max(sh.bins.mass[l[2]], uint64_t{1})), hi = min(hi, sh.bins.mass[h[2] + 1]);
-        else l[2] = 0, h[2] = -1;       // only what has no weight is left out
-    }
-    l[3] = bin_of<true>(drawn_place(u, lo), sh), h[3] = bin_of<true>(drawn_place(u, hi), sh);
-    // the ranges in order, those that meet as one
-    const int k_bin = l[0], m_lo = l[2], m_hi = h[2];
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-#pragma unroll
-        for (int j = 0; j < 3; ++j)
-            if (h[j] < l[j] || (h[j + 1] >= l[j + 1] && l[j + 1] < l[j])) {  // empty ones last
-                const int x = l[j], y = h[j];
-                l[j] = l[j + 1], h[j] = h[j + 1], l[j + 1] = x, h[j + 1] = y;
+    int k_range = -1, m_range = -1, k_bin = 0, m_bin = -1;
+    uint64_t lo = mass[kBins], hi = lo; // the total lies within
+    if (q.few) {
+        // all that top_k may leave; what is behind a rank of kBins bins has no weight
+        h[0] = static_cast<uint32_t>(q.k) < count[kBins] ? bin_of<false>(q.k - 1, sh) : kBins - 1;
+        k_range = static_cast<uint32_t>(q.k) < count[kBins] ? 0 : -1;
+        m_range = q.m > 0.0f ? 0 : -1;
+    } else {
+        if (q.k > 0 && static_cast<uint32_t>(q.k) < count[kBins]) {
+            k_range = 0;
+            k_bin = l[0] = h[0] = bin_of<false>(q.k - 1, sh);
+            lo = max(mass[l[0]], uint64_t{1}), hi = mass[l[0] + 1];
+        }
+        if (q.p < 1.0f) {
+            l[1] = h[1] = bin_of<true>(top_p_place(q.p, lo), sh);
+            if (hi != lo) h[1] = bin_of<true>(top_p_place(q.p, hi), sh);
+            lo = max(mass[l[1]], uint64_t{1}), hi = min(hi, mass[h[1] + 1]);
+        }
+        if (q.m > 0.0f) {
+            // depths next to the border are compared one by one
+            const double z = q.m < 1.0f ? -log(static_cast<double>(q.m)) : 0.0;
+            l[2] = Weigher::bin(fmax(z - 1e-6, 0.0)), h[2] = min(Weigher::bin(z + 1e-6), kBins - 1);
+            if (l[2] < kBins) {
+                m_bin = l[2];
+                lo = min(lo, max(mass[l[2]], uint64_t{1})), hi = min(hi, mass[h[2] + 1]);
+            } else {
+                l[2] = 0, h[2] = -1;    // only what has no weight is left out
             }
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-#pragma unroll
-        for (int j = i + 1; j < 4; ++j)
-            if (h[i] >= l[i] && h[j] >= l[j] && l[j] <= h[i] + 1) h[i] = max(h[i], h[j]), l[j] = 0, h[j] = -1;
-    uint32_t first = 0, k_first = 0, m_end = 0;
-    int open = 0, k_open = 0, m_open = -1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (h[i] < l[i]) continue;
-        if (by_k && l[i] <= k_bin && k_bin <= h[i]) {
-            k_open = open + k_bin - l[i];
-            k_first = first + sh.bins.count[k_bin] - sh.bins.count[l[i]];
         }
-        if (m_lo <= m_hi && l[i] <= m_lo && m_lo <= h[i]) {
-            m_open = open + m_lo - l[i];
-            m_end = first + sh.bins.count[m_hi + 1] - sh.bins.count[l[i]];
+        l[3] = h[3] = bin_of<true>(drawn_place(q.u, lo), sh);
+        if (hi != lo) h[3] = bin_of<true>(drawn_place(q.u, hi), sh);
+        // in order, those that meet as one
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (h[j + 1] >= l[j + 1] && (h[j] < l[j] || l[j + 1] < l[j])) {
+                    const int x = l[j], y = h[j];
+                    l[j] = l[j + 1], h[j] = h[j + 1], l[j + 1] = x, h[j + 1] = y;
+                }
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int j = i + 1; j < 4; ++j)
+                if (h[i] >= l[i] && h[j] >= l[j] && l[j] <= h[i] + 1) h[i] = max(h[i], h[j]), l[j] = 0, h[j] = -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (k_range >= 0 && l[i] <= k_bin && k_bin <= h[i]) k_range = i;
+            if (m_bin >= 0 && l[i] <= m_bin && m_bin <= h[i]) m_range = i;
         }
-        for (int bin = l[i] + lane; bin <= h[i] && open + bin - l[i] < kOpen; bin += 64) {
-            auto& e = p.bin[open + bin - l[i]];
-            e.mass = sh.bins.mass[bin], e.end = sh.bins.mass[bin + 1], e.first = first + sh.bins.count[bin] - sh.bins.count[l[i]];
-        }
-        open += h[i] - l[i] + 1;
-        first += sh.bins.count[h[i] + 1] - sh.bins.count[l[i]];
     }
-    if (lane == 0) {
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p.lo[i] = l[i], p.hi[i] = h[i];
-        p.ranges = open;
-        p.listed = open <= kOpen ? first : ~0u;
-        p.k_bin = k_open;
-        p.k_at = by_k ? k_first + (k - 1 - sh.bins.count[k_bin]) : ~0u;
-        p.m_bin = m_open;
-        p.m_end = m_end;
-        p.all = all;
-    }
+        for (int i = 0; i < 4; ++i) p.lo[i] = l[i], p.hi[i] = h[i], p.mass[i] = h[i] < l[i] ? 0 : mass[l[i]], p.end[i] = h[i] < l[i] ? 0 : mass[h[i] + 1];
+        p.all = mass[kBins];
+        p.k_range = k_range, p.m_range = m_range;
+        p.k_at = k_range < 0 ? 0 : q.k - 1 - count[p.lo[k_range]];
+        }
 }
 
-__device__ void copy_plan(Plan& to, const Plan& from) {
-    const int words = static_cast<int>(offsetof(Plan, bin) / 4 + min(from.ranges, kOpen) * (sizeof(from.bin[0]) / 4));
-    for (int i = threadIdx.x; i < words; i += kThreads) reinterpret_cast<uint32_t*>(&to)[i] = reinterpret_cast<const uint32_t*>(&from)[i];
-}
-
-// ids [i, e) of the open bins, to a list
-__device__ void gather(const float* x, int i, int e, const Weigher& w, const Plan& p, uint64_t* list, uint32_t* listed) {
+// Ids [i, e) of the open bins, to the workgroup's list; sh.listed counts on where it is full.
+__device__ void gather(const float* x, int i, int e, const Weigher& w, const Plan& p, Work& sh) {
     double lo[4], hi[4];                // in 128ths of depth
 #pragma unroll
     for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], hi[r] = p.hi[r] + 1;
@@ -451,38 +447,49 @@ __device__ void gather(const float* x, int i, int e, const Weigher& w, const Pla
         bool in = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) in |= z >= lo[r] && z < hi[r];
-        if (in) list[atomicAdd(listed, 1u)] = entry_of(key_of(x[j]), j);
+        if (in) {
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            if (at < kList) sh.pick.list[at] = entry_of(key_of(x[j]), j);
+        }
     }
 }
 
-// The exact places, from the candidates of the open bins in sh.pick.list.
-__device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
-    __syncthreads();
+// The exact places, from the n candidates of the open bins in sh.pick.list.
+__device__ void settle(const SampleArgs& a, int b, const Question& q, int n, const Weigher& w, Work& sh) {
     const Plan& p = sh.plan;
-    const int t = threadIdx.x, lane = t & 63, wave = t / 64, n = static_cast<int>(p.listed);
+    const int t = threadIdx.x, lane = t & 63, wave = t / 64;
     // Sorted by buckets of equal width in depth, a few candidates each, and within one by counting.
-    for (int i = t; i < kBuckets; i += kThreads) sh.pick.at[i] = 0;
+    sh.pick.at[t] = 0;
+    if (t < 4) sh.in_range[t] = 0;
     __syncthreads();
-    const double width = static_cast<double>(kBuckets) / p.ranges;
-    const auto bucket = [&](uint64_t e) {
-        const double z = w.depth(static_cast<uint32_t>(e >> 32)) * 128.0;
-        double before = 0.0;            // open bins before it
+    double width[4], wide = 0.0;        // bins before the range
 #pragma unroll
-        for (int r = 0; r < 4; ++r) before += fmin(fmax(z - p.lo[r], 0.0), static_cast<double>(p.hi[r] + 1 - p.lo[r]));
-        return min(static_cast<int>(before * width), kBuckets - 1);
-    };
+    for (int r = 0; r < 4; ++r) {
+        width[r] = wide;
+        wide += p.hi[r] + 1 - p.lo[r];
+    }
+    const double scale = static_cast<double>(kBuckets) / wide;
     constexpr int kEach = kList / kThreads;
     uint64_t mine[kEach];
     int of[kEach];
     uint32_t place[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        mine[i] = t + i * kThreads < n ? sh.pick.list[t + i * kThreads] : 0;
-        of[i] = mine[i] ? bucket(mine[i]) : -1;
-        place[i] = mine[i] ? atomicAdd(&sh.pick.at[of[i]], 1u) : 0;
+        const bool there = t + i * kThreads < n;
+        mine[i] = there ? sh.pick.list[t + i * kThreads] : 0;
+        const double z = w.depth(static_cast<uint32_t>(mine[i] >> 32)) * 128.0;
+        double before = 0.0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool in = there && z >= p.lo[r] && z < p.hi[r] + 1;
+            if (in) before = width[r] + (z - p.lo[r]);
+            const uint64_t v = __ballot(in);
+            if (v && lane == 0) atomicAdd(&sh.in_range[r], static_cast<uint32_t>(__popcll(v)));
+        }
+        of[i] = min(static_cast<int>(before * scale), kBuckets - 1);
+        place[i] = there ? atomicAdd(&sh.pick.at[of[i]], 1u) : 0;
     }
     __syncthreads();
-    static_assert(kBuckets == kThreads);
     const uint32_t held = sh.pick.at[t];
     uint32_t begin = held;
     for (int d = 1; d < 64; d <<= 1) {
@@ -497,11 +504,11 @@ __device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-        if (mine[i]) sh.pick.list[sh.pick.at[of[i]] + place[i]] = mine[i];
+        if (t + i * kThreads < n) sh.pick.list[sh.pick.at[of[i]] + place[i]] = mine[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        if (!mine[i]) continue;
+        if (t + i * kThreads >= n) continue;
         const uint32_t first = sh.pick.at[of[i]], end = of[i] + 1 < kBuckets ? sh.pick.at[of[i] + 1] : n;
         place[i] = first;
         for (uint32_t j = first; j < end; ++j) place[i] += sh.pick.list[j] > mine[i];
@@ -509,7 +516,7 @@ __device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-        if (mine[i]) sh.pick.list[place[i]] = mine[i];
+        if (t + i * kThreads < n) sh.pick.list[place[i]] = mine[i];
     __syncthreads();
     // running masses
     uint64_t m[kEach], in = 0;
@@ -525,6 +532,7 @@ __device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
         if (lane >= d) in += o;
     }
     if (lane == 63) sh.wave_mass[wave] = in;
+    if (t == 0) sh.listed = 0;
     __syncthreads();
     in -= sum;
     for (int i = 0; i < wave; ++i) in += sh.wave_mass[i];
@@ -533,50 +541,50 @@ __device__ void settle(const SampleArgs& a, int b, const Weigher& w, Work& sh) {
         in += m[i];
         sh.pick.run[t * kEach + i] = in;
     }
-    if (t == 0) sh.listed = 0;
-    __syncthreads();
-    const auto run = [&](uint32_t i) { return i ? sh.pick.run[i - 1] : 0; };  // of the first i
-    const float mp = a.min_p ? a.min_p[b] : 0.0f;
-    if (p.m_bin >= 0) {                 // how many of those bins' candidates min_p leaves
+    const auto first_of = [&](int r) {  // in the list
+        uint32_t f = 0;
+        for (int i = 0; i < r; ++i) f += sh.in_range[i];
+        return f;
+    };
+    if (p.m_range >= 0) {               // how many of that range's candidates min_p leaves
+        const uint32_t first = first_of(p.m_range), end = first + sh.in_range[p.m_range];
         uint32_t c = 0;
-        for (uint32_t i = p.bin[p.m_bin].first + t; i < p.m_end; i += kThreads)
-            c += w.share(static_cast<uint32_t>(sh.pick.list[i] >> 32)) >= mp;
+        for (uint32_t i = first + t; i < end; i += kThreads) c += w.share(static_cast<uint32_t>(sh.pick.list[i] >> 32)) >= q.m;
         if (c) atomicAdd(&sh.listed, c);
-        __syncthreads();
     }
+    __syncthreads();
     if (wave) return;
-    // the listed candidate that holds unit x of the row's mass, and its bin: one wave
-    int bin = 0;
+    const auto run = [&](uint32_t i) { return i ? sh.pick.run[i - 1] : 0; };  // of the first i
+    // mass up to and with candidate i of the list, in range r
+    const auto up_to = [&](uint32_t i, int r) { return p.mass[r] + run(i + 1) - run(first_of(r)); };
+    // the listed candidate that holds unit x of the row's mass, and its range: one wave
+    int range = 0;
     const auto holder = [&](uint64_t x) -> uint32_t {
-        for (int i = 0; i < p.ranges; i += 64) {
-            const bool in_it = i + lane < p.ranges && p.bin[min(i + lane, kOpen - 1)].mass <= x && x < p.bin[min(i + lane, kOpen - 1)].end;
-            if (const uint64_t v = __ballot(in_it)) bin = i + __ffsll(static_cast<unsigned long long>(v)) - 1;
-        }
-        const uint64_t at = x - p.bin[bin].mass + run(p.bin[bin].first);
-        uint32_t low = p.bin[bin].first, count = n - low;  // the first i with run(i + 1) > at
-        while (count > 0) {
+        for (int r = 0; r < 4; ++r)
+            if (q.few ? r == 0 : p.mass[r] <= x && x < p.end[r]) range = r;
+        uint32_t low = first_of(range), count = n - low;
+        const uint64_t at = x - p.mass[range] + run(low);
+        while (count > 0) {             // the first i with run(i + 1) > at, 64 steps at a time
             const uint32_t step = (count + 63) / 64;
-            const uint32_t i = low + (lane + 1) * step;  // candidates [low, i) end at or before `at`
-            const uint32_t k = __popcll(__ballot(i <= low + count && run(i) <= at));
+            const uint32_t i = low + (lane + 1) * step;
+            const uint32_t k = __popcll(__ballot(i <= low + count && run(min(i, static_cast<uint32_t>(n))) <= at));
             low += k * step;
             count = step == 1 ? 0 : min(step, count - min(count, k * step));
         }
         return low;
     };
-    const auto up_to = [&](uint32_t i) { return p.bin[bin].mass + run(i + 1) - run(p.bin[bin].first); };
-    uint64_t total = p.all;
-    if (p.k_at != ~0u) bin = p.k_bin, total = up_to(p.k_at);
-    const float tp = a.top_p ? a.top_p[b] : 1.0f;
-    if (tp < 1.0f) {
-        const uint32_t i = holder(top_p_place(tp, total));
-        total = up_to(i);
+    uint64_t total = q.few ? run(n) : p.all;
+    if (p.k_range >= 0) total = up_to(first_of(p.k_range) + p.k_at, p.k_range);
+    if (q.p < 1.0f) {
+        const uint32_t i = holder(top_p_place(q.p, total));
+        total = up_to(i, range);
     }
-    if (p.m_bin >= 0) {
-        const uint32_t first = p.bin[p.m_bin].first;
-        const uint64_t most = p.bin[p.m_bin].mass + run(first + sh.listed) - run(first);
+    if (p.m_range >= 0) {
+        const uint32_t first = first_of(p.m_range);
+        const uint64_t most = p.mass[p.m_range] + run(first + sh.listed) - run(first);
         total = min(total, max(most, static_cast<uint64_t>(w.unit)));  // the first place stays
     }
-    const uint32_t at = holder(drawn_place(a.u[b], total));
+    const uint32_t at = holder(drawn_place(q.u, total));
     if (lane == 0) {
         a.token[b] = static_cast<int>(~static_cast<uint32_t>(sh.pick.list[at]));
         if (a.prob) a.prob[b] = static_cast<float>(static_cast<double>(run(at + 1) - run(at)) / static_cast<double>(total));
@@ -592,7 +600,8 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, int 
     for (int i = s * kThreads + threadIdx.x; i < kBins; i += slices * kThreads) r.mass[i] = 0, r.count[i] = 0;
     if (s == 0 && threadIdx.x == 0) r.listed = 0, r.counted = 0, r.gathered = 0;
     if (!(a.temperature[b] >= 0.0f)) return;  // an empty place
-    const uint64_t top = slice_top(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), a.temperature[b] == 0.0f, waves);
+    const uint64_t top =
+        slice_top(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), a.temperature[b] == 0.0f, waves);
     if (threadIdx.x == 0) tops[b * slices + s] = top;
 }
 
@@ -614,27 +623,31 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, do
     const int b = blockIdx.y, s = blockIdx.x;
     const float T = a.temperature[b];
     if (!(T >= 0.0f)) return;
+    const Question q(a, b);
+    sh.exp.fill();
+    clear_bins(sh);
     const uint64_t top = row_top(tops + b * slices, slices);
     if (plain_row(a, b, T, top, s == 0 && threadIdx.x == 0)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
-    sh.exp.fill();
-    clear_bins(sh);
     __syncthreads();
-    count_slice(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, sh);
+    count_slice(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), q, w, sh);
     __syncthreads();
     Row& r = rows[b];
-    for (int i = threadIdx.x; i < kBins; i += kThreads)
-        if (sh.bins.count[i]) {
-            atomicAdd(&r.count[i], sh.bins.count[i]);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&r.mass[i]), static_cast<unsigned long long>(sh.bins.mass[i]));
-        }
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        if (sh.bins.count[i]) atomicAdd(&r.count[i], sh.bins.count[i]);
+        if (sh.bins.mass[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&r.mass[i]), static_cast<unsigned long long>(sh.bins.mass[i]));
+    }
     if (!last_of(&r.counted, slices, sh)) return;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins.mass[i] = r.mass[i], sh.bins.count[i] = r.count[i];
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        if (q.k) sh.bins.count[i] = r.count[i];
+        if (!q.few) sh.bins.mass[i] = r.mass[i];
+    }
     __syncthreads();
     add_up(sh);
-    if (threadIdx.x < 64) make_plan(a, b, sh);
-    __syncthreads();
-    copy_plan(r.plan, sh.plan);
+    if (threadIdx.x < 64) {
+        make_plan(q, sh);
+        if (threadIdx.x == 0) r.plan = sh.plan;
+    }
 }
 
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, double unit, int slices, const uint64_t* tops, Row* rows) {
@@ -642,22 +655,29 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, dou
     const int b = blockIdx.y, s = blockIdx.x;
     const float T = a.temperature[b];
     if (!(T >= 0.0f)) return;
+    const Question q(a, b);
+    Row& r = rows[b];
+    sh.exp.fill();
+    if (threadIdx.x < sizeof(Plan) / 4) reinterpret_cast<uint32_t*>(&sh.plan)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&r.plan)[threadIdx.x];
+    if (threadIdx.x == 0) sh.listed = 0;
     const uint64_t top = row_top(tops + b * slices, slices);
     if (plain_row(a, b, T, top, false)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
-    sh.exp.fill();
-    Row& r = rows[b];
-    const uint32_t n = r.plan.listed;
-    if (n <= kList) gather(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, r.plan, r.list, &r.listed);
-    if (!last_of(&r.gathered, slices, sh)) return;
     __syncthreads();
+    gather(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, sh.plan, sh);
+    __syncthreads();
+    const uint32_t own = sh.listed;
+    if (threadIdx.x == 0 && own) sh.base = atomicAdd(&r.listed, own);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < own && sh.base + i < kList; i += kThreads) r.list[sh.base + i] = sh.pick.list[i];
+    if (!last_of(&r.gathered, slices, sh)) return;
+    const uint32_t n = r.listed;
     if (n > kList) {
         sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
         return;
     }
-    copy_plan(sh.plan, r.plan);
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.pick.list[i] = r.list[i];
-    settle(a, b, w, sh);
+    settle(a, b, q, n, w, sh);
 }
 
 // a row of one slice
@@ -666,24 +686,28 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
     const int b = blockIdx.x;
     const float T = a.temperature[b];
     if (!(T >= 0.0f)) return;
+    const Question q(a, b);
     const float* x = a.logits + b * a.ld;
     clear_bins(sh);
     sh.exp.fill();
     const uint64_t top = slice_top(x, 0, a.V, T == 0.0f, sh.wave_mass);
     if (plain_row(a, b, T, top, threadIdx.x == 0)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
-    count_slice(x, 0, a.V, w, sh);
+    count_slice(x, 0, a.V, q, w, sh);
     __syncthreads();
     add_up(sh);
-    if (threadIdx.x < 64) make_plan(a, b, sh);
+    if (threadIdx.x < 64) make_plan(q, sh);
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    if (sh.plan.listed > kList) {
+    gather(x, 0, a.V, w, sh.plan, sh);
+    __syncthreads();
+    const uint32_t n = sh.listed;
+    if (n > kList) {
+        __syncthreads();
         sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
         return;
     }
-    gather(x, 0, a.V, w, sh.plan, sh.pick.list, &sh.listed);
-    settle(a, b, w, sh);
+    settle(a, b, q, n, w, sh);
 }
 
 int sample_slices(int B, int V) { return std::max(1, std::min((V + 4095) / 4096, 512 / std::min(B, 512))); }
