@@ -276,18 +276,27 @@ __device__ __forceinline__ uint64_t wave_top(uint64_t v) {
     for (int d = 1; d < 64; d <<= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), d)));
     return v;
 }
+// f(logit, id) for ids [i, e): eight are on their way at a time, whatever f does.
+template <typename F>
+__device__ __forceinline__ void each_logit(const float* x, int i, int e, const F& f) {
+    constexpr int kBatch = 8;
+    for (int j = i + threadIdx.x; j < e; j += kBatch * kThreads) {
+        float l[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) l[n] = x[min(j + n * kThreads, e - 1)];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n)
+            if (j + n * kThreads < e) f(l[n], j + n * kThreads);
+    }
+}
+
 // The largest entry of ids [i, e); where the temperature is not 0 only its key matters.
 __device__ uint64_t slice_top(const float* x, int i, int e, bool greedy, uint64_t* waves) {
     uint64_t top = 0;
-    if (greedy) {
-#pragma unroll 4
-        for (int j = i + threadIdx.x; j < e; j += kThreads) top = max(top, entry_of(key_of(x[j]), j));
-    } else {
-        float m = -INFINITY;            // fmaxf passes over a NaN
-#pragma unroll 8
-        for (int j = i + threadIdx.x; j < e; j += kThreads) m = fmaxf(m, x[j]);
-        top = entry_of(key_of(m), 0);
-    }
+    float m = -INFINITY;                // fmaxf passes over a NaN
+    if (greedy) each_logit(x, i, e, [&](float l, int j) { top = max(top, entry_of(key_of(l), j)); });
+    else each_logit(x, i, e, [&](float l, int) { m = fmaxf(m, l); });
+    if (!greedy) top = entry_of(key_of(m), 0);
     top = wave_top(top);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = top;
     __syncthreads();
@@ -317,14 +326,13 @@ __device__ void clear_bins(Work& sh) {
 // this: one of 64 bits takes more of its time than the weight.)
 __device__ void count_slice(const float* x, int i, int e, const Question& q, const Weigher& w, Work& sh) {
     const bool counts = q.k > 0, masses = !q.few;
-#pragma unroll 4
-    for (int j = i + threadIdx.x; j < e; j += kThreads) {
-        const double z = w.depth(x[j]);
-        if (!(z < 36.0)) continue;
+    each_logit(x, i, e, [&](float l, int) {
+        const double z = w.depth(l);
+        if (!(z < 36.0)) return;
         const int bin = static_cast<int>(z * 128.0);
         if (counts) atomicAdd(&sh.bins.count[bin], 1u);
         if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(z)));
-    }
+    });
 }
 
 // bins' counts and masses become those of the bins before; the totals stand behind the last
@@ -441,17 +449,16 @@ __device__ void gather(const float* x, int i, int e, const Weigher& w, const Pla
     double lo[4], hi[4];                // in 128ths of depth
 #pragma unroll
     for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], hi[r] = p.hi[r] + 1;
-#pragma unroll 4
-    for (int j = i + threadIdx.x; j < e; j += kThreads) {
-        const double z = w.depth(x[j]) * 128.0;
+    each_logit(x, i, e, [&](float l, int j) {
+        const double z = w.depth(l) * 128.0;
         bool in = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) in |= z >= lo[r] && z < hi[r];
         if (in) {
             const uint32_t at = atomicAdd(&sh.listed, 1u);
-            if (at < kList) sh.pick.list[at] = entry_of(key_of(x[j]), j);
+            if (at < kList) sh.pick.list[at] = entry_of(key_of(l), j);
         }
-    }
+    });
 }
 
 // The exact places, from the n candidates of the open bins in sh.pick.list.
