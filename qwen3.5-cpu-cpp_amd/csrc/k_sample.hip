@@ -43,33 +43,43 @@ struct ExpTable {
     }
 };
 __device__ __forceinline__ double exp_minus(double z, const ExpTable& e) {
-    constexpr double kLn2 = 0.69314718055994530942, kStep = 64.0 / kLn2;
-    // ln 2 / 64 to 32 bits, so that n times it is exact, and the rest of it
+    constexpr double kLn2 = 0.69314718055994530942;
+    // ln 2 / 64 to 33 bits, so that n times it is exact, and the rest of it
     constexpr double kHigh = 0x1.62e42fefp-7, kLow = 0x1.473de6af278edp-40;
-    const double n = rint(z * kStep);
-    const int i = static_cast<int>(n);
-    const double r = fma(-n, kLow, fma(-n, kHigh, z));
+    // n may be one off at a border: r is then that little larger
+    const int i = static_cast<int>(rintf(static_cast<float>(z) * static_cast<float>(64.0 / kLn2)));
+    const double n = i, r = fma(-n, kLow, fma(-n, kHigh, z));
     double p = fma(r, -1.0 / 120.0, 1.0 / 24.0);
     p = fma(-r, p, 1.0 / 6.0);
     p = fma(-r, p, 0.5);
     p = fma(-r, p, 1.0);
     p = fma(-r, p, 1.0);
-    return ldexp(e.t[i & 63] * p, -(i >> 6));
+    // 2^-(n div 64) straight into the exponent: results are above 2^-53
+    return __builtin_bit_cast(double, __builtin_bit_cast(int64_t, e.t[i & 63] * p) - (static_cast<int64_t>(i >> 6) << 52));
 }
+
+constexpr float kLeastT = 1e-36f;  // below this the bins' arithmetic in fp32 would not do
 
 struct Weigher {
     double top, rt, unit;
+    float top32, rt32;
     const ExpTable& table;
     bool inf;
     __device__ Weigher(uint32_t key, float T, double unit_, const ExpTable& e)
-        : top(of_key(key)), rt(1.0 / static_cast<double>(T)), unit(unit_), table(e), inf(key == kKeyInf) {}
+        : top(of_key(key)), rt(1.0 / static_cast<double>(T)), unit(unit_), top32(of_key(key)), rt32(static_cast<float>(128.0 * rt)), table(e),
+          inf(key == kKeyInf) {}
     // (max - l) / T: infinite or a NaN where a candidate is ruled out
     __device__ double depth(float l) const {
         if (inf) return l == INFINITY ? 0.0 : INFINITY;
         return (top - static_cast<double>(l)) * rt;
     }
     __device__ double depth(uint32_t key) const { return depth(of_key(key)); }
-    static __device__ int bin(double depth) { return static_cast<int>(fmin(depth * 128.0, static_cast<double>(kBins))); }
+    // The same in 128ths and fp32, for bins: whatever its rounding, larger logits have no larger ones, and all with
+    // weight are below kBins (a weight ends at 35.4).
+    __device__ float place(float l) const {
+        if (inf) return l == INFINITY ? 0.0f : INFINITY;
+        return l > -INFINITY ? fminf(top32 - l, 3.4e38f) * rt32 : INFINITY;
+    }
     // the weight in 64 bits, of the largest
     __device__ double share(uint32_t key) const {
         const double z = depth(key);
@@ -272,15 +282,84 @@ struct Work {
     uint32_t listed, base, last;
 };
 
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    const auto step = [&](int o) { v = max(v, static_cast<uint32_t>(o)); };
+    step(dpp_i<0xB1>(static_cast<int>(v)));
+    step(dpp_i<0x4E>(static_cast<int>(v)));
+    step(dpp_i<0x141>(static_cast<int>(v)));
+    step(dpp_i<0x140>(static_cast<int>(v)));
+    step(__builtin_amdgcn_ds_swizzle(static_cast<int>(v), 0x401F));
+    return max(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 0)),
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 32)));
+}
 __device__ __forceinline__ uint64_t wave_top(uint64_t v) {
-    for (int d = 1; d < 64; d <<= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), d)));
+    const uint32_t hi = wave_max_u32(static_cast<uint32_t>(v >> 32));
+    const uint32_t lo = wave_max_u32(static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// Sums of the lanes up to and with each: lanes 1, 2, 4, 8 before within a row of 16, then the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+    return static_cast<uint64_t>(moved<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32 | moved<CTRL, ROWS>(static_cast<uint32_t>(v));
+}
+template <typename U>
+__device__ __forceinline__ U wave_scan(U v) {
+    v += moved<0x111, 0xF>(v);
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);
+    v += moved<0x143, 0xC>(v);
     return v;
 }
-// f(logit, id) for ids [i, e): eight are on their way at a time, whatever f does.
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int l) {
+    return static_cast<uint64_t>(lane_of(static_cast<uint32_t>(v >> 32), l)) << 32 | lane_of(static_cast<uint32_t>(v), l);
+}
+// the sum of the threads before this one; `waves` has a place for each wave, one use between barriers
+template <typename U>
+__device__ __forceinline__ U block_scan(U v, U* waves) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const U in = wave_scan(v);
+    if ((threadIdx.x & 63) == 63) waves[wave] = in;
+    __syncthreads();
+    const U sums = wave_scan(waves[threadIdx.x & (kThreads / 64 - 1)]);
+    return in - v + (wave ? lane_of(sums, wave - 1) : U{0});
+}
+
+// What workgroups of one row leave each other within a launch passes through these and atomic additions: they
+// go to where all of them look, past the caches that do not.
+template <typename U>
+__device__ __forceinline__ U shared_load(const U* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename U>
+__device__ __forceinline__ void shared_store(U* p, U v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// f(logit, id) for ids [i, e), i a multiple of four: sixteen are on their way at a time, whatever f does.
 template <typename F>
 __device__ __forceinline__ void each_logit(const float* x, int i, int e, const F& f) {
-    constexpr int kBatch = 8;
-    for (int j = i + threadIdx.x; j < e; j += kBatch * kThreads) {
+    int j = i + 4 * threadIdx.x;
+    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+        constexpr int kBatch = 4;
+        const int last = (e - 4) & ~3;  // the last whole four
+        for (; j <= last; j += 4 * kBatch * kThreads) {
+            float4 l[kBatch];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) l[n] = *reinterpret_cast<const float4*>(x + min(j + 4 * n * kThreads, last));
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const int id = j + 4 * n * kThreads;
+                if (id <= last) f(l[n].x, id), f(l[n].y, id + 1), f(l[n].z, id + 2), f(l[n].w, id + 3);
+            }
+        }
+        j = max(last + 4, i) + threadIdx.x;
+        if (j < e) f(x[j], j);
+        return;
+    }
+    constexpr int kBatch = 16;
+    for (j = i + threadIdx.x; j < e; j += kBatch * kThreads) {
         float l[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) l[n] = x[min(j + n * kThreads, e - 1)];
@@ -327,39 +406,29 @@ __device__ void clear_bins(Work& sh) {
 __device__ void count_slice(const float* x, int i, int e, const Question& q, const Weigher& w, Work& sh) {
     const bool counts = q.k > 0, masses = !q.few;
     each_logit(x, i, e, [&](float l, int) {
-        const double z = w.depth(l);
-        if (!(z < 36.0)) return;
-        const int bin = static_cast<int>(z * 128.0);
+        const float z = w.place(l);
+        if (!(z < kBins)) return;
+        const int bin = static_cast<int>(z);
         if (counts) atomicAdd(&sh.bins.count[bin], 1u);
-        if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(z)));
+        if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(w.depth(l))));
     });
 }
 
 // bins' counts and masses become those of the bins before; the totals stand behind the last
 __device__ void add_up(Work& sh) {
-    const int t = threadIdx.x, lane = t & 63, wave = t / 64;
     uint64_t m[kPer], im = 0;
     uint32_t n[kPer], in = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int b = t * kPer + i;
+        const int b = threadIdx.x * kPer + i;
         m[i] = b < kBins ? sh.bins.mass[b] : 0, n[i] = b < kBins ? sh.bins.count[b] : 0;
         im += m[i], in += n[i];
     }
-    const uint64_t sm = im;
-    const uint32_t sn = in;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t om = __shfl_up(static_cast<unsigned long long>(im), d);
-        const uint32_t on = __shfl_up(in, d);
-        if (lane >= d) im += om, in += on;
-    }
-    if (lane == 63) sh.wave_mass[wave] = im, sh.wave_count[wave] = in;
-    __syncthreads();
-    im -= sm, in -= sn;
-    for (int i = 0; i < wave; ++i) im += sh.wave_mass[i], in += sh.wave_count[i];
+    im = block_scan(im, sh.wave_mass);
+    in = block_scan(in, sh.wave_count);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int b = t * kPer + i;
+        const int b = threadIdx.x * kPer + i;
         if (b <= kBins) sh.bins.mass[b] = im, sh.bins.count[b] = in;
         im += m[i], in += n[i];
     }
@@ -403,9 +472,9 @@ __device__ void make_plan(const Question& q, Work& sh) {
             lo = max(mass[l[1]], uint64_t{1}), hi = min(hi, mass[h[1] + 1]);
         }
         if (q.m > 0.0f) {
-            // depths next to the border are compared one by one
+            // candidates next to the border are compared one by one
             const double z = q.m < 1.0f ? -log(static_cast<double>(q.m)) : 0.0;
-            l[2] = Weigher::bin(fmax(z - 1e-6, 0.0)), h[2] = min(Weigher::bin(z + 1e-6), kBins - 1);
+            l[2] = static_cast<int>(fmax(z - 1e-4, 0.0) * 128.0), h[2] = min(static_cast<int>((z + 1e-4) * 128.0), kBins - 1);
             if (l[2] < kBins) {
                 m_bin = l[2];
                 lo = min(lo, max(mass[l[2]], uint64_t{1})), hi = min(hi, mass[h[2] + 1]);
@@ -446,11 +515,11 @@ __device__ void make_plan(const Question& q, Work& sh) {
 
 // Ids [i, e) of the open bins, to the workgroup's list; sh.listed counts on where it is full.
 __device__ void gather(const float* x, int i, int e, const Weigher& w, const Plan& p, Work& sh) {
-    double lo[4], hi[4];                // in 128ths of depth
+    float lo[4], hi[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], hi[r] = p.hi[r] + 1;
     each_logit(x, i, e, [&](float l, int j) {
-        const double z = w.depth(l) * 128.0;
+        const float z = w.place(l);
         bool in = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) in |= z >= lo[r] && z < hi[r];
@@ -469,13 +538,13 @@ __device__ void settle(const SampleArgs& a, int b, const Question& q, int n, con
     sh.pick.at[t] = 0;
     if (t < 4) sh.in_range[t] = 0;
     __syncthreads();
-    double width[4], wide = 0.0;        // bins before the range
+    float width[4], wide = 0.0f;        // bins before the range
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         width[r] = wide;
         wide += p.hi[r] + 1 - p.lo[r];
     }
-    const double scale = static_cast<double>(kBuckets) / wide;
+    const float scale = static_cast<float>(kBuckets) / wide;
     constexpr int kEach = kList / kThreads;
     uint64_t mine[kEach];
     int of[kEach];
@@ -484,8 +553,8 @@ __device__ void settle(const SampleArgs& a, int b, const Question& q, int n, con
     for (int i = 0; i < kEach; ++i) {
         const bool there = t + i * kThreads < n;
         mine[i] = there ? sh.pick.list[t + i * kThreads] : 0;
-        const double z = w.depth(static_cast<uint32_t>(mine[i] >> 32)) * 128.0;
-        double before = 0.0;
+        const float z = w.place(of_key(static_cast<uint32_t>(mine[i] >> 32)));
+        float before = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const bool in = there && z >= p.lo[r] && z < p.hi[r] + 1;
@@ -497,17 +566,7 @@ __device__ void settle(const SampleArgs& a, int b, const Question& q, int n, con
         place[i] = there ? atomicAdd(&sh.pick.at[of[i]], 1u) : 0;
     }
     __syncthreads();
-    const uint32_t held = sh.pick.at[t];
-    uint32_t begin = held;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(begin, d);
-        if (lane >= d) begin += o;
-    }
-    if (lane == 63) sh.wave_count[wave] = begin;
-    __syncthreads();
-    begin -= held;
-    for (int i = 0; i < wave; ++i) begin += sh.wave_count[i];
-    sh.pick.at[t] = begin;
+    sh.pick.at[t] = block_scan(sh.pick.at[t], sh.wave_count);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
@@ -533,16 +592,8 @@ __device__ void settle(const SampleArgs& a, int b, const Question& q, int n, con
         m[i] = at < n ? w(static_cast<uint32_t>(sh.pick.list[at] >> 32)) : 0;
         in += m[i];
     }
-    const uint64_t sum = in;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(static_cast<unsigned long long>(in), d);
-        if (lane >= d) in += o;
-    }
-    if (lane == 63) sh.wave_mass[wave] = in;
     if (t == 0) sh.listed = 0;
-    __syncthreads();
-    in -= sum;
-    for (int i = 0; i < wave; ++i) in += sh.wave_mass[i];
+    in = block_scan(in, sh.wave_mass);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         in += m[i];
@@ -598,7 +649,9 @@ __device__ void settle(const SampleArgs& a, int b, const Question& q, int n, con
     }
 }
 
-__device__ __forceinline__ int slice_begin(int V, int slices, int i) { return static_cast<int>(static_cast<int64_t>(V) * i / slices); }
+__device__ __forceinline__ int slice_begin(int V, int slices, int i) {
+    return i == slices ? V : static_cast<int>(static_cast<int64_t>(V) * i / slices) & ~3;
+}
 
 __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, int slices, uint64_t* tops, Row* rows) {
     __shared__ uint64_t waves[kThreads / 64];
@@ -612,15 +665,13 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, int 
     if (threadIdx.x == 0) tops[b * slices + s] = top;
 }
 
-// Whether this workgroup is the last of the row's to come here; it sees what the others have written. (One
-// wave's fences do for all of them, behind a barrier and before one: each writes back or drops a whole cache.)
+// Whether this workgroup is the last of the row's to come here. The others' additions and stores are all done:
+// each wave waits for its own before the barrier, behind which the ticket is drawn.
 __device__ bool last_of(uint32_t* ticket, int slices, Work& sh) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vector memory, nothing outstanding
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        sh.last = atomicAdd(ticket, 1u) == static_cast<uint32_t>(slices) - 1;
-        if (sh.last) __threadfence();
-    }
+    if (threadIdx.x == 0)
+        sh.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(slices) - 1;
     __syncthreads();
     return sh.last;
 }
@@ -634,7 +685,7 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, do
     sh.exp.fill();
     clear_bins(sh);
     const uint64_t top = row_top(tops + b * slices, slices);
-    if (plain_row(a, b, T, top, s == 0 && threadIdx.x == 0)) return;
+    if (plain_row(a, b, T, top, s == 0 && threadIdx.x == 0) || T < kLeastT) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
     __syncthreads();
     count_slice(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), q, w, sh);
@@ -646,8 +697,8 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, do
     }
     if (!last_of(&r.counted, slices, sh)) return;
     for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        if (q.k) sh.bins.count[i] = r.count[i];
-        if (!q.few) sh.bins.mass[i] = r.mass[i];
+        if (q.k) sh.bins.count[i] = shared_load(&r.count[i]);
+        if (!q.few) sh.bins.mass[i] = shared_load(&r.mass[i]);
     }
     __syncthreads();
     add_up(sh);
@@ -671,19 +722,23 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, dou
     if (plain_row(a, b, T, top, false)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
     __syncthreads();
+    if (T < kLeastT) {
+        if (s == 0) sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
+        return;
+    }
     gather(a.logits + b * a.ld, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), w, sh.plan, sh);
     __syncthreads();
     const uint32_t own = sh.listed;
     if (threadIdx.x == 0 && own) sh.base = atomicAdd(&r.listed, own);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < own && sh.base + i < kList; i += kThreads) r.list[sh.base + i] = sh.pick.list[i];
+    for (uint32_t i = threadIdx.x; i < own && sh.base + i < kList; i += kThreads) shared_store(&r.list[sh.base + i], sh.pick.list[i]);
     if (!last_of(&r.gathered, slices, sh)) return;
-    const uint32_t n = r.listed;
+    const uint32_t n = shared_load(&r.listed);
     if (n > kList) {
         sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
         return;
     }
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.pick.list[i] = r.list[i];
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.pick.list[i] = shared_load(&r.list[i]);
     settle(a, b, q, n, w, sh);
 }
 
@@ -700,6 +755,11 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
     const uint64_t top = slice_top(x, 0, a.V, T == 0.0f, sh.wave_mass);
     if (plain_row(a, b, T, top, threadIdx.x == 0)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
+    if (T < kLeastT) {
+        __syncthreads();
+        sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
+        return;
+    }
     count_slice(x, 0, a.V, q, w, sh);
     __syncthreads();
     add_up(sh);
@@ -717,7 +777,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
     settle(a, b, q, n, w, sh);
 }
 
-int sample_slices(int B, int V) { return std::max(1, std::min((V + 4095) / 4096, 512 / std::min(B, 512))); }
+int sample_slices(int B, int V) { return std::max(1, std::min((V + 4095) / 4096, 256 / std::min(B, 256))); }
 
 }  // namespace
 
