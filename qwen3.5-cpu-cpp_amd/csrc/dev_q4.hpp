@@ -33,4 +33,8 @@ __device__ __forceinline__ float from_digits(v4i d) {
     return fmaf(static_cast<float>(d[2] * 256 + d[1]), 256.0f, static_cast<float>(d[0]));
 }
 
+// Here the value exists: without it the compiler puts off what follows the products, whose sums (four
+// registers for one value) then outnumber the registers.
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
+
 }  // namespace q35k

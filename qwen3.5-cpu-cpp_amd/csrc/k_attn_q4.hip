@@ -198,9 +198,6 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-// Here the value exists: without it the compiler puts off what follows the products, whose sums (four
-// registers for one value) then outnumber the registers.
-__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
 
 constexpr int kTile = 64;       // keys a wave takes at a time
 constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16;

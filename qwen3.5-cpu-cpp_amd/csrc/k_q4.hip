@@ -54,20 +54,20 @@ __device__ __forceinline__ int group_sum(int v) {
     return v;
 }
 
-// An image of `rows` rows of X over some blocks of 64 k, the operand of the products as it is read: digit d of
-// row r at k 64 b + 16 c + j in byte ((4 b + c) rows + r) 48 + 16 d + j; then the groups' factors [group][rows],
-// floats, or with zero points four words: the sums of the three digits and the factor's bits.
+// An image of R rows of X (fewer may be there) over some blocks of 64 k, the operand of the products as it is
+// read: digit d of row r at k 64 b + 16 c + j in byte ((4 b + c) R + r) 48 + 16 d + j; then the groups' factors
+// [group][R], floats, or with zero points four words: the sums of the three digits and the factor's bits.
 template <int G, bool ZP>
-__host__ __device__ constexpr int meta_bytes(int rows, int k) { return rows * (k / G) * (ZP ? 16 : 4); }
+__host__ __device__ constexpr int meta_bytes(int R, int k) { return R * (k / G) * (ZP ? 16 : 4); }
 
 // Makes the image of k [k0, k0 + kn) (kn a multiple of 256) with the threads first, first + step, ..
-template <int G, bool ZP>
+template <int G, bool ZP, int R>
 __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, int rows, int k0, int kn, uint8_t* img, uint8_t* meta,
                                            int first, int step) {
     const int per = kn / 8;
     const bool wide = (ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(X) & 15) == 0;
     for (int id = first; id < rows * per; id += step) {  // 32 lanes are in or out together
-        const int r = id / per, kk = (id % per) * 8, k = k0 + kk;
+        const int r = R == 1 ? 0 : id / per, kk = (R == 1 ? id : id % per) * 8, k = k0 + kk;
         const float* src = X + r * ldx + k;
         float x[8];
         if (wide && k + 8 <= K) {
@@ -82,10 +82,10 @@ __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, i
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
         float scale;
         const Digits d = digits8(x, group_max<G>(top), scale);
-        uint8_t* at = img + (((kk >> 6) * 4 + (kk >> 4 & 3)) * rows + r) * 48 + (kk & 8);
+        uint8_t* at = img + ((kk >> 4) * R + r) * 48 + (kk & 8);
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(at + 16 * p) = make_uint2(d.d[p][0], d.d[p][1]);
-        const int g = kk / G * rows + r;
+        const int g = kk / G * R + r;
         if constexpr (ZP) {
             int s[3];
 #pragma unroll
@@ -99,12 +99,12 @@ __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, i
     }
 }
 
-// The images of all blocks of rows, in the workspace: block r0 at r0 x (bytes of a row).
-template <int G, bool ZP>
+// The images of all blocks of R rows, in the workspace, then their factors.
+template <int G, bool ZP, int R>
 __global__ __launch_bounds__(256) void q4_image_kernel(const float* X, int64_t ldx, int M, int K, int most, uint8_t* img, uint8_t* meta) {
-    const int r0 = blockIdx.y * most, rows = min(most, M - r0), kp = (K + 255) / 256 * 256;
-    make_image<G, ZP>(X + r0 * ldx, ldx, K, rows, 0, kp, img + static_cast<int64_t>(r0) * 3 * kp,
-                      meta + static_cast<int64_t>(r0) * (kp / G) * (ZP ? 16 : 4), blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    const int r0 = blockIdx.y * most, kp = (K + 255) / 256 * 256;
+    make_image<G, ZP, R>(X + r0 * ldx, ldx, K, min(most, M - r0), 0, kp, img + static_cast<int64_t>(blockIdx.y) * R * 3 * kp,
+                         meta + static_cast<int64_t>(blockIdx.y) * meta_bytes<G, ZP>(R, kp), blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ---- the products
@@ -148,9 +148,10 @@ struct Unit {
     }
 };
 
-template <int G, bool ZP, int QN>
-__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, int rows, int lane, float* acc) {
-    const int c = lane >> 4, m = lane & 15;
+// A block of 256 k: `img` and `meta` are this lane's places in the images of that block.
+template <int G, bool ZP, int R>
+__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, float* acc) {
+    constexpr int QN = (R + 3) / 4;
 #pragma unroll
     for (int g = 0; g < 256 / G; ++g) {
         const float sw = u.scale(g);
@@ -169,25 +170,23 @@ __device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* im
         }
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
-            const int r = min(4 * q + (m >> 2), rows - 1), mine = min(4 * q + c, rows - 1);  // rows beyond the last: whatever
-            const uint8_t* at = img + r * 48 + min(m & 3, 2) * 16;
             float sx;
             v4i d = {0, 0, 0, 0};
             if constexpr (ZP) {
-                const int4 t = reinterpret_cast<const int4*>(meta)[g * rows + mine];
+                const v4i t = *reinterpret_cast<const v4i*>(meta + (g * R + 4 * q) * 16);
                 const int z = -16 * u.zero(g);
-                d = v4i{z * t.x, z * t.y, z * t.z, 0};
-                sx = __int_as_float(t.w);
+                d = v4i{z * t[0], z * t[1], z * t[2], 0};
+                sx = __int_as_float(t[3]);
             } else {
-                sx = reinterpret_cast<const float*>(meta)[g * rows + mine];
+                sx = *reinterpret_cast<const float*>(meta + (g * R + 4 * q) * 4);
             }
             if constexpr (G == 32) {
-                const long a = *reinterpret_cast<const long*>(at + ((g >> 1) * 4 + (g & 1) * 2 + (c >> 1)) * rows * 48 + (c & 1) * 8);
-                d = __builtin_amdgcn_mfma_i32_16x16x32_i8(a, __builtin_bit_cast(long, make_int2(b[0][0], b[0][1])), d, 0, 0, 0);
+                const v2i a = *reinterpret_cast<const v2i*>(img + (g >> 1) * R * 192 + (g & 1) * R * 96 + q * 192);
+                d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a), __builtin_bit_cast(long, v2i{b[0][0], b[0][1]}), d, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int h = 0; h < G / 64; ++h) {
-                    const v4i a = *reinterpret_cast<const v4i*>(at + ((g * (G / 64) + h) * 4 + c) * rows * 48);
+                    const v4i a = *reinterpret_cast<const v4i*>(img + (g * (G / 64) + h) * R * 192 + q * 192);
                     d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[h], d, 0, 0, 0);
                 }
             }
@@ -196,16 +195,35 @@ __device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* im
     }
 }
 
-template <int G, bool ZP, int QN, bool PRE>
+// From memory straight into LDS, a KB a wave at a time: a workgroup's copy of `bytes` (a multiple of 4, `to` 16-byte
+// aligned; the rest behind the last 16 dword by dword).
+__device__ __forceinline__ void copy_to_lds(uint8_t* to, const uint8_t* from, int bytes) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto glob = [](const uint8_t* p) {
+        return reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(p));
+    };
+    const auto local = [](uint8_t* p) { return reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(p)); };
+    const int whole = bytes & ~15;
+    for (int o = wave * 1024; o < whole; o += kWaves * 1024)
+        if (o + 16 * lane < whole) __builtin_amdgcn_global_load_lds(glob(from + o + 16 * lane), local(to + o), 16, 0, 0);
+    if (wave == 0 && 4 * lane < bytes - whole) __builtin_amdgcn_global_load_lds(glob(from + whole + 4 * lane), local(to + whole), 4, 0, 0);
+}
+
+template <int G, bool ZP, int R, bool PRE>
 __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most, int ks, int chunk) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane >> 4, n = lane & 15;
-    const int r0 = blockIdx.y * most, rows = min(most, a.M - r0);
-    const int tiles = (a.N + 15) / 16, blocks = (a.K + 255) / 256, rt = kWaves / ks, part = wave % ks;
-    const int sets = (tiles + rt - 1) / rt;
-    uint8_t* meta = lds + most * 3 * chunk * 256;
-    float* red = reinterpret_cast<float*>(meta + meta_bytes<G, ZP>(most, chunk * 256));
+    constexpr int QN = (R + 3) / 4, kMeta = meta_bytes<G, ZP>(R, 256);
     typedef Unit<G, ZP> U;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
+    const int r0 = blockIdx.y * most, rows = min(most, a.M - r0);
+    const int tiles = (a.N + 15) / 16, blocks = (a.K + 255) / 256, rt = kWaves / ks, part = wave & (ks - 1);
+    const int sets = (tiles + rt - 1) / rt;
+    uint8_t* meta = lds + R * 768 * chunk;
+    float* red = reinterpret_cast<float*>(meta + kMeta * chunk);
+    // this lane's places: rows that are not there hold whatever, as do the sums over them
+    const int digit = min(n & 3, 2), row = min(n >> 2, R - 1);
+    const uint8_t* img_lane = lds + (G == 32 ? ((c >> 1) * R + row) * 48 + (c & 1) * 8 : (c * R + row) * 48) + digit * 16;
+    const uint8_t* meta_lane = meta + min(c, R - 1) * (ZP ? 16 : 4);
     const bool one = chunk >= blocks;   // one image serves all tiles
     bool made = false;
     for (int set = blockIdx.x; set < sets; set += gridDim.x) {
@@ -216,41 +234,45 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
         for (int q = 0; q < QN; ++q) acc[q] = 0.0f;
         for (int b0 = 0; b0 < blocks; b0 += chunk) {
             const int bn = min(chunk, blocks - b0), its = (bn - part + ks - 1) / ks;  // blocks b0 + part + i ks
+            const uint8_t* w = W + static_cast<int64_t>(b0 + part) * U::kBytes;
             U u[kDepth];
 #pragma unroll
             for (int i = 0; i < kDepth; ++i)
-                if (i < its) u[i].load(W + static_cast<int64_t>(b0 + part + i * ks) * U::kBytes, lane);
+                if (i < its) u[i].load(w + i * ks * U::kBytes, lane);
             if (!one || !made) {
                 if (made) lds_barrier();
                 if constexpr (PRE) {
                     const int kp = blocks * 256;
-                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(r0) * 3 * kp +
-                                                                      static_cast<int64_t>(rows) * 3 * b0 * 256);
-                    for (int i = threadIdx.x; i < rows * 3 * bn * 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = src[i];
-                    const uint32_t* ms = reinterpret_cast<const uint32_t*>(
-                        static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(a.M) * 3 * kp + meta_bytes<G, ZP>(r0, kp) + meta_bytes<G, ZP>(rows, b0 * 256));
-                    for (int i = threadIdx.x; i < meta_bytes<G, ZP>(rows, bn * 256) / 4; i += kThreads) reinterpret_cast<uint32_t*>(meta)[i] = ms[i];
+                    const uint8_t *img = static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(blockIdx.y) * R * 3 * kp,
+                                  *factors = static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(gridDim.y) * R * 3 * kp +
+                                             static_cast<int64_t>(blockIdx.y) * kMeta * blocks;
+                    copy_to_lds(lds, img + static_cast<int64_t>(b0) * R * 768, bn * R * 768);
+                    copy_to_lds(meta, factors + static_cast<int64_t>(b0) * kMeta, bn * kMeta);
+                    __builtin_amdgcn_s_waitcnt(0x0f70);  // vector memory, nothing outstanding
                 } else {
-                    make_image<G, ZP>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, threadIdx.x, kThreads);
+                    make_image<G, ZP, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, threadIdx.x, kThreads);
                 }
                 made = true;
                 lds_barrier();
             }
+            const uint8_t *img = img_lane + part * R * 768, *factors = meta_lane + part * kMeta;
             for (int i = 0; i < its; i += kDepth) {
 #pragma unroll
                 for (int j = 0; j < kDepth; ++j)
                     if (i + j < its) {
-                        const int b = part + (i + j) * ks;
-                        multiply<G, ZP, QN>(u[j], lds + b * rows * 768, meta + meta_bytes<G, ZP>(rows, b * 256), rows, lane, acc);
-                        if (i + j + kDepth < its) u[j].load(W + static_cast<int64_t>(b0 + b + kDepth * ks) * U::kBytes, lane);
+                        multiply<G, ZP, R>(u[j], img, factors, acc);
+#pragma unroll
+                        for (int q = 0; q < QN; ++q) pin(acc[q]);
+                        img += ks * R * 768, factors += ks * kMeta;
+                        if (i + j + kDepth < its) u[j].load(w + (i + j + kDepth) * ks * U::kBytes, lane);
                     }
             }
         }
         const auto store = [&](int q, float y) {
             const int r = 4 * q + c, col = tile * 16 + n;
             if (r < rows && tile < tiles && col < a.N) {
-                const int64_t row = r0 + r;
-                a.Y[row * a.ldy + col] = y + (a.R ? a.R[row * a.ldr + col] : 0.0f);
+                const int64_t at = r0 + r;
+                a.Y[at * a.ldy + col] = y + (a.R ? a.R[at * a.ldr + col] : 0.0f);
             }
         };
         if (ks == 1) {
@@ -263,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
         lds_barrier();
 #pragma unroll
         for (int q = 0; q < QN; ++q)
-            if (q % ks == part) {
+            if ((q & (ks - 1)) == part) {
                 float y = 0.0f;
                 for (int i = 0; i < ks; ++i) y += red[((wave - part + i) * QN + q) * 64 + lane];
                 store(q, y);
@@ -350,66 +372,69 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* codes, cons
     reinterpret_cast<uint32_t*>(packed)[id] = out;
 }
 
-// Rows a block, waves a tile, workgroups, blocks of 256 k an image holds, and whether the image is made by
-// a launch of its own.
+// Rows a block and its image's, waves a tile, workgroups, blocks of 256 k an image holds, and whether the images are
+// made by a launch of their own.
 struct Q4Plan {
-    int quads, most, row_blocks, ks, wgs, chunk;
+    int most, image, row_blocks, ks, wgs, chunk;
     bool pre;
     uint32_t lds;
 };
+template <int G, bool ZP>
+void q4_fit(Q4Plan& p, int N, int K) {
+    const int blocks = q4_blocks(K), each = p.image * 768 + meta_bytes<G, ZP>(p.image, 256);
+    const int red = p.ks > 1 ? kWaves * ((p.image + 3) / 4) * 256 : 0;
+    p.chunk = std::min(blocks, std::max(1, (160 * 1024 - red) / each));
+    p.lds = each * p.chunk + red;
+}
 template <int G, bool ZP>
 Q4Plan q4_plan(int M, int N, int K) {
     Q4Plan p{};
     const int blocks = q4_blocks(K), tiles = q4_tiles(N);
     p.row_blocks = (M + 15) / 16;
     p.most = (M + p.row_blocks - 1) / p.row_blocks;
-    p.quads = p.most <= 4 ? 1 : p.most <= 8 ? 2 : 4;
+    p.image = p.most == 1 ? 1 : p.most <= 4 ? 4 : p.most <= 8 ? 8 : 16;
     p.pre = p.most > 4;
     p.ks = 8;
-    while (p.ks > 1 && tiles * p.ks * p.row_blocks >= 2 * kWaves * 512) p.ks /= 2;
+    while (p.ks > 1 && tiles * p.ks * p.row_blocks >= 2 * kWaves * 256) p.ks /= 2;
     while (p.ks > 1 && p.ks / 2 >= blocks) p.ks /= 2;
-    const int budget = 120 * 1024, each = p.most * 3 * 256 + meta_bytes<G, ZP>(p.most, 256);
-    p.chunk = std::min(blocks, std::max(1, budget / each));
     const int rt = kWaves / p.ks, sets = (tiles + rt - 1) / rt;
-    p.wgs = std::min(sets, std::max(1, 512 / p.row_blocks));
-    p.lds = p.most * 3 * p.chunk * 256 + meta_bytes<G, ZP>(p.most, p.chunk * 256) + (p.ks > 1 ? kWaves * p.quads * 64 * 4 : 0);
+    p.wgs = std::min(sets, std::max(1, 256 / p.row_blocks));
+    q4_fit<G, ZP>(p, N, K);
     return p;
 }
 
-template <int G, bool ZP, int QN, bool PRE>
+template <int G, bool ZP, int R, bool PRE>
 hipError_t launch_q4_form(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
     static std::once_flag once;         // LDS beyond the default limit
     static hipError_t limit;
     std::call_once(once, [] {
-        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, QN, PRE>), hipFuncAttributeMaxDynamicSharedMemorySize,
+        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, R, PRE>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                     160 * 1024);
     });
     if (limit != hipSuccess) return limit;
-    klaunch(q4_mul_kernel<G, ZP, QN, PRE>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
+    if constexpr (PRE) {
+        const int kp = q4_blocks(a.K) * 256;
+        uint8_t* ws = static_cast<uint8_t*>(a.ws);
+        klaunch(q4_image_kernel<G, ZP, R>, dim3((p.most * kp / 8 + 255) / 256, p.row_blocks), dim3(256), 0, s, a.X, a.ldx, a.M, a.K, p.most, ws,
+                ws + static_cast<int64_t>(p.row_blocks) * R * 3 * kp);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    klaunch(q4_mul_kernel<G, ZP, R, PRE>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
     return hipGetLastError();
 }
 
 template <int G, bool ZP>
 hipError_t launch_q4_plan(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
-    if (p.pre) {
-        const int kp = q4_blocks(a.K) * 256;
-        uint8_t* ws = static_cast<uint8_t*>(a.ws);
-        klaunch(q4_image_kernel<G, ZP>, dim3((p.most * kp / 8 + 255) / 256, p.row_blocks), dim3(256), 0, s, a.X, a.ldx, a.M, a.K, p.most, ws,
-                ws + static_cast<int64_t>(a.M) * 3 * kp);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    if (!p.pre) return launch_q4_form<G, ZP, 1, false>(a, p, s);
-    if (p.quads == 1) return launch_q4_form<G, ZP, 1, true>(a, p, s);
-    if (p.quads == 2) return launch_q4_form<G, ZP, 2, true>(a, p, s);
-    return launch_q4_form<G, ZP, 4, true>(a, p, s);
+    if (p.pre) return p.image == 4 ? launch_q4_form<G, ZP, 4, true>(a, p, s) : p.image == 8 ? launch_q4_form<G, ZP, 8, true>(a, p, s) : launch_q4_form<G, ZP, 16, true>(a, p, s);
+    return p.image == 1 ? launch_q4_form<G, ZP, 1, false>(a, p, s) : p.image == 4 ? launch_q4_form<G, ZP, 4, false>(a, p, s) : launch_q4_form<G, ZP, 8, false>(a, p, s);
 }
 
 }  // namespace
 
 uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) {
     const uint64_t kp = static_cast<uint64_t>(q4_blocks(K)) * 256;
-    return M * (3 * kp + kp / G * 16);
+    return (M + 15) / 16 * 16 * (3 * kp + kp / G * 16);
 }
 
 hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s) {
