@@ -6,6 +6,7 @@
 namespace q35k {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float half_bits(uint32_t h) {

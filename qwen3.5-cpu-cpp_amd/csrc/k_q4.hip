@@ -56,7 +56,7 @@ __device__ __forceinline__ int group_sum(int v) {
 
 // An image of R rows of X (fewer may be there) over some blocks of 64 k, the operand of the products as it is
 // read: digit d of row r at k 64 b + 16 c + j in byte ((4 b + c) R + r) 48 + 16 d + j; then the groups' factors
-// [group][R], floats, or with zero points four words: the sums of the three digits and the factor's bits.
+// [group][R], floats, or with zero points four: the sums of the three digits and the factor.
 template <int G, bool ZP>
 __host__ __device__ constexpr int meta_bytes(int R, int k) { return R * (k / G) * (ZP ? 16 : 4); }
 
@@ -64,47 +64,51 @@ __host__ __device__ constexpr int meta_bytes(int R, int k) { return R * (k / G) 
 template <int G, bool ZP, int R>
 __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, int rows, int k0, int kn, uint8_t* img, uint8_t* meta,
                                            int first, int step) {
-    const int per = kn / 8;
+    const int per = kn / 8, count = rows * per;
     const bool wide = (ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(X) & 15) == 0;
-    for (int id = first; id < rows * per; id += step) {  // 32 lanes are in or out together
-        const int r = R == 1 ? 0 : id / per, kk = (R == 1 ? id : id % per) * 8, k = k0 + kk;
-        const float* src = X + r * ldx + k;
-        float x[8];
-        if (wide && k + 8 <= K) {
-            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
+    constexpr int kBatch = R == 1 ? 1 : 4;  // requested together
+    for (int id0 = first; id0 < count; id0 += kBatch * step) {
+        float x[kBatch][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = k + i < K ? src[i] : 0.0f;
+        for (int n = 0; n < kBatch; ++n) {
+            const int id = min(id0 + n * step, count - 1), r = R == 1 ? 0 : id / per, k = k0 + (R == 1 ? id : id % per) * 8;
+            const float* src = X + r * ldx + k;
+            if (wide && k + 8 <= K) {
+                const v4f a = reinterpret_cast<const v4f*>(src)[0], b = reinterpret_cast<const v4f*>(src)[1];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[n][i] = a[i], x[n][4 + i] = b[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[n][i] = k + i < K ? src[i] : 0.0f;
+            }
         }
-        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-        float scale;
-        const Digits d = digits8(x, group_max<G>(top), scale);
-        uint8_t* at = img + ((kk >> 4) * R + r) * 48 + (kk & 8);
+        for (int n = 0; n < kBatch; ++n) {
+            const int id = id0 + n * step;
+            if (id >= count) break;     // 32 lanes are in or out together
+            const int r = R == 1 ? 0 : id / per, kk = (R == 1 ? id : id % per) * 8;
+            uint32_t top = 0;
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(at + 16 * p) = make_uint2(d.d[p][0], d.d[p][1]);
-        const int g = kk / G * R + r;
-        if constexpr (ZP) {
-            int s[3];
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
+            float scale;
+            const Digits d = digits8(x[n], group_max<G>(top), scale);
+            uint8_t* at = img + ((kk >> 4) * R + r) * 48 + (kk & 8);
 #pragma unroll
-            for (int p = 0; p < 3; ++p)
-                s[p] = group_sum<G>(__builtin_amdgcn_sdot4(static_cast<int>(d.d[p][1]), 0x01010101,
-                                                           __builtin_amdgcn_sdot4(static_cast<int>(d.d[p][0]), 0x01010101, 0, false), false));
-            if (kk % G == 0) reinterpret_cast<int4*>(meta)[g] = make_int4(s[0], s[1], s[2], __float_as_int(scale));
-        } else {
-            if (kk % G == 0) reinterpret_cast<float*>(meta)[g] = scale;
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(at + 16 * p) = make_uint2(d.d[p][0], d.d[p][1]);
+            const int g = kk / G * R + r;
+            if constexpr (ZP) {
+                int s[3];
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    s[p] = group_sum<G>(__builtin_amdgcn_sdot4(static_cast<int>(d.d[p][1]), 0x01010101,
+                                                               __builtin_amdgcn_sdot4(static_cast<int>(d.d[p][0]), 0x01010101, 0, false), false));
+                if (kk % G == 0)
+                    reinterpret_cast<float4*>(meta)[g] = make_float4(static_cast<float>(s[0]), static_cast<float>(s[1]), static_cast<float>(s[2]), scale);
+            } else {
+                if (kk % G == 0) reinterpret_cast<float*>(meta)[g] = scale;
+            }
         }
     }
-}
-
-// The images of all blocks of R rows, in the workspace, then their factors.
-template <int G, bool ZP, int R>
-__global__ __launch_bounds__(256) void q4_image_kernel(const float* X, int64_t ldx, int M, int K, int most, uint8_t* img, uint8_t* meta) {
-    const int r0 = blockIdx.y * most, kp = (K + 255) / 256 * 256;
-    make_image<G, ZP, R>(X + r0 * ldx, ldx, K, min(most, M - r0), 0, kp, img + static_cast<int64_t>(blockIdx.y) * R * 3 * kp,
-                         meta + static_cast<int64_t>(blockIdx.y) * meta_bytes<G, ZP>(R, kp), blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ---- the products
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(256) void q4_image_kernel(const float* X, int64_t l
 // three digits (the fourth row of each four is never looked at): lane 16 c + n holds the three digits' sums of
 // row c of the four and weight row n side by side, and only there are they put together, scaled and added
 // in fp32. A group is one such product (two for 128, one of depth 32 for 32), so sums are exact until they
-// are scaled. Zero points start the sums at -16 zero x (sum of the digits).
+// are scaled. With zero points -16 zero x (sum of the digits) is added to each digit's first.
 //
 // A workgroup's waves take tiles of 16 weight rows, `ks` waves a tile, which share its k by blocks of 256 and
 // add up in LDS. Weights go from memory to registers kDepth blocks ahead.
@@ -148,68 +152,74 @@ struct Unit {
     }
 };
 
-// A block of 256 k: `img` and `meta` are this lane's places in the images of that block.
+// What a lane reads of the images for one group: digits and factors of its rows.
 template <int G, bool ZP, int R>
-__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, float* acc) {
-    constexpr int QN = (R + 3) / 4;
-#pragma unroll
-    for (int g = 0; g < 256 / G; ++g) {
-        const float sw = u.scale(g);
-        // eight codes a word: bytes of 16 times the low and the high ones
-        v4i b[G == 128 ? 2 : 1];
-        if constexpr (G == 32) {
-            const uint32_t w = u.word(g);
-            b[0] = v4i{static_cast<int>(w << 4 & 0xf0f0f0f0u), static_cast<int>(w & 0xf0f0f0f0u), 0, 0};
-        } else {
-#pragma unroll
-            for (int h = 0; h < G / 64; ++h) {
-                const uint32_t w0 = u.word(2 * (g * (G / 64) + h)), w1 = u.word(2 * (g * (G / 64) + h) + 1);
-                b[h] = v4i{static_cast<int>(w0 << 4 & 0xf0f0f0f0u), static_cast<int>(w0 & 0xf0f0f0f0u),
-                           static_cast<int>(w1 << 4 & 0xf0f0f0f0u), static_cast<int>(w1 & 0xf0f0f0f0u)};
-            }
-        }
+struct Operand {
+    static constexpr int QN = (R + 3) / 4, H = G == 128 ? 2 : 1;
+    v4i a[QN][H];
+    v4f factor[QN];                     // sums of the three digits and the scale, or the scale alone
+    __device__ void load(const uint8_t* img, const uint8_t* meta, int g) {
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
-            float sx;
-            v4i d = {0, 0, 0, 0};
-            if constexpr (ZP) {
-                const v4i t = *reinterpret_cast<const v4i*>(meta + (g * R + 4 * q) * 16);
-                const int z = -16 * u.zero(g);
-                d = v4i{z * t[0], z * t[1], z * t[2], 0};
-                sx = __int_as_float(t[3]);
-            } else {
-                sx = *reinterpret_cast<const float*>(meta + (g * R + 4 * q) * 4);
-            }
             if constexpr (G == 32) {
-                const v2i a = *reinterpret_cast<const v2i*>(img + (g >> 1) * R * 192 + (g & 1) * R * 96 + q * 192);
-                d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a), __builtin_bit_cast(long, v2i{b[0][0], b[0][1]}), d, 0, 0, 0);
+                const v2i x = *reinterpret_cast<const v2i*>(img + (g >> 1) * R * 192 + (g & 1) * R * 96 + q * 192);
+                a[q][0] = v4i{x[0], x[1], 0, 0};
             } else {
 #pragma unroll
-                for (int h = 0; h < G / 64; ++h) {
-                    const v4i a = *reinterpret_cast<const v4i*>(img + (g * (G / 64) + h) * R * 192 + q * 192);
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[h], d, 0, 0, 0);
-                }
+                for (int h = 0; h < H; ++h) a[q][h] = *reinterpret_cast<const v4i*>(img + (g * H + h) * R * 192 + q * 192);
             }
-            acc[q] = fmaf(from_digits(d), sw * sx, acc[q]);
+            if constexpr (ZP) factor[q] = *reinterpret_cast<const v4f*>(meta + (g * R + 4 * q) * 16);
+            else factor[q][3] = *reinterpret_cast<const float*>(meta + (g * R + 4 * q) * 4);
+        }
+    }
+};
+
+// A block of 256 k of a tile: `img` and `meta` are this lane's places in the images of that block. What a
+// group needs from LDS is asked for a group ahead, and its products are all issued before the first is used.
+template <int G, bool ZP, int R>
+__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, float (&acc)[(R + 3) / 4]) {
+    constexpr int QN = (R + 3) / 4, H = G == 128 ? 2 : 1;
+    Operand<G, ZP, R> o[2];
+    o[0].load(img, meta, 0);
+#pragma unroll
+    for (int g = 0; g < 256 / G; ++g) {
+        if (g + 1 < 256 / G) o[(g + 1) & 1].load(img, meta, g + 1);
+        const Operand<G, ZP, R>& x = o[g & 1];
+        v4i d[QN];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            // eight codes a word: bytes of 16 times the low and the high ones
+            const uint32_t w0 = u.word(G == 32 ? g : 2 * (g * H + h)), w1 = G == 32 ? 0 : u.word(2 * (g * H + h) + 1);
+            const v4i b = {static_cast<int>(w0 << 4 & 0xf0f0f0f0u), static_cast<int>(w0 & 0xf0f0f0f0u), static_cast<int>(w1 << 4 & 0xf0f0f0f0u),
+                           static_cast<int>(w1 & 0xf0f0f0f0u)};
+#pragma unroll
+            for (int q = 0; q < QN; ++q) {
+                const v4i c = h ? d[q] : v4i{0, 0, 0, 0};
+                if constexpr (G == 32)
+                    d[q] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, v2i{x.a[q][0][0], x.a[q][0][1]}),
+                                                                 __builtin_bit_cast(long, v2i{b[0], b[1]}), c, 0, 0, 0);
+                else d[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.a[q][h], b, c, 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const float sw = u.scale(g);
+#pragma unroll
+        for (int q = 0; q < QN; ++q) {
+            float f;
+            if constexpr (ZP) {         // zero x sum of digits and a sum of products are whole and below 2^22: exact
+                const float z = static_cast<float>(-16 * u.zero(g));
+                f = fmaf(fmaf(fmaf(z, x.factor[q][2], static_cast<float>(d[q][2])), 256.0f, fmaf(z, x.factor[q][1], static_cast<float>(d[q][1]))),
+                         256.0f, fmaf(z, x.factor[q][0], static_cast<float>(d[q][0])));
+            } else {
+                f = from_digits(d[q]);
+            }
+            acc[q] = fmaf(f, sw * x.factor[q][3], acc[q]);
+            pin(acc[q]);
         }
     }
 }
 
-// From memory straight into LDS, a KB a wave at a time: a workgroup's copy of `bytes` (a multiple of 4, `to` 16-byte
-// aligned; the rest behind the last 16 dword by dword).
-__device__ __forceinline__ void copy_to_lds(uint8_t* to, const uint8_t* from, int bytes) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const auto glob = [](const uint8_t* p) {
-        return reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(p));
-    };
-    const auto local = [](uint8_t* p) { return reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(p)); };
-    const int whole = bytes & ~15;
-    for (int o = wave * 1024; o < whole; o += kWaves * 1024)
-        if (o + 16 * lane < whole) __builtin_amdgcn_global_load_lds(glob(from + o + 16 * lane), local(to + o), 16, 0, 0);
-    if (wave == 0 && 4 * lane < bytes - whole) __builtin_amdgcn_global_load_lds(glob(from + whole + 4 * lane), local(to + whole), 4, 0, 0);
-}
-
-template <int G, bool ZP, int R, bool PRE>
+template <int G, bool ZP, int R>
 __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most, int ks, int chunk) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int QN = (R + 3) / 4, kMeta = meta_bytes<G, ZP>(R, 256);
@@ -226,32 +236,27 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
     const uint8_t* meta_lane = meta + min(c, R - 1) * (ZP ? 16 : 4);
     const bool one = chunk >= blocks;   // one image serves all tiles
     bool made = false;
+    U u[kDepth];
+    // blocks b0 + part, + ks, .. of the set's tile, the first ones
+    const auto load = [&](int set, int b0, int its) {
+        const uint8_t* w = a.W + (static_cast<int64_t>(min(set * rt + wave / ks, tiles - 1)) * blocks + b0 + part) * U::kBytes;
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i)
+            if (i < its) u[i].load(w + i * ks * U::kBytes, lane);
+        return w;
+    };
+    const uint8_t* w = nullptr;
     for (int set = blockIdx.x; set < sets; set += gridDim.x) {
         const int tile = set * rt + wave / ks;
-        const uint8_t* W = a.W + static_cast<int64_t>(min(tile, tiles - 1)) * blocks * U::kBytes;
         float acc[QN];
 #pragma unroll
         for (int q = 0; q < QN; ++q) acc[q] = 0.0f;
         for (int b0 = 0; b0 < blocks; b0 += chunk) {
-            const int bn = min(chunk, blocks - b0), its = (bn - part + ks - 1) / ks;  // blocks b0 + part + i ks
-            const uint8_t* w = W + static_cast<int64_t>(b0 + part) * U::kBytes;
-            U u[kDepth];
-#pragma unroll
-            for (int i = 0; i < kDepth; ++i)
-                if (i < its) u[i].load(w + i * ks * U::kBytes, lane);
+            const int bn = min(chunk, blocks - b0), its = (bn - part + ks - 1) / ks;
             if (!one || !made) {
+                w = load(set, b0, its);
                 if (made) lds_barrier();
-                if constexpr (PRE) {
-                    const int kp = blocks * 256;
-                    const uint8_t *img = static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(blockIdx.y) * R * 3 * kp,
-                                  *factors = static_cast<const uint8_t*>(a.ws) + static_cast<int64_t>(gridDim.y) * R * 3 * kp +
-                                             static_cast<int64_t>(blockIdx.y) * kMeta * blocks;
-                    copy_to_lds(lds, img + static_cast<int64_t>(b0) * R * 768, bn * R * 768);
-                    copy_to_lds(meta, factors + static_cast<int64_t>(b0) * kMeta, bn * kMeta);
-                    __builtin_amdgcn_s_waitcnt(0x0f70);  // vector memory, nothing outstanding
-                } else {
-                    make_image<G, ZP, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, threadIdx.x, kThreads);
-                }
+                make_image<G, ZP, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, threadIdx.x, kThreads);
                 made = true;
                 lds_barrier();
             }
@@ -261,13 +266,13 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
                 for (int j = 0; j < kDepth; ++j)
                     if (i + j < its) {
                         multiply<G, ZP, R>(u[j], img, factors, acc);
-#pragma unroll
-                        for (int q = 0; q < QN; ++q) pin(acc[q]);
                         img += ks * R * 768, factors += ks * kMeta;
                         if (i + j + kDepth < its) u[j].load(w + (i + j + kDepth) * ks * U::kBytes, lane);
                     }
             }
         }
+        // the next set's first blocks, before this one's end
+        if (one && set + static_cast<int>(gridDim.x) < sets) w = load(set + gridDim.x, 0, (blocks - part + ks - 1) / ks);
         const auto store = [&](int q, float y) {
             const int r = 4 * q + c, col = tile * 16 + n;
             if (r < rows && tile < tiles && col < a.N) {
@@ -372,70 +377,59 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* codes, cons
     reinterpret_cast<uint32_t*>(packed)[id] = out;
 }
 
-// Rows a block and its image's, waves a tile, workgroups, blocks of 256 k an image holds, and whether the images are
-// made by a launch of their own.
+// Rows a block and its image's, waves a tile, workgroups a block of rows, blocks of 256 k an image holds.
 struct Q4Plan {
     int most, image, row_blocks, ks, wgs, chunk;
-    bool pre;
     uint32_t lds;
 };
 template <int G, bool ZP>
 void q4_fit(Q4Plan& p, int N, int K) {
     const int blocks = q4_blocks(K), each = p.image * 768 + meta_bytes<G, ZP>(p.image, 256);
     const int red = p.ks > 1 ? kWaves * ((p.image + 3) / 4) * 256 : 0;
-    p.chunk = std::min(blocks, std::max(1, (160 * 1024 - red) / each));
+    p.chunk = std::min(blocks, (160 * 1024 - red) / each);
     p.lds = each * p.chunk + red;
 }
 template <int G, bool ZP>
 Q4Plan q4_plan(int M, int N, int K) {
     Q4Plan p{};
     const int blocks = q4_blocks(K), tiles = q4_tiles(N);
-    p.row_blocks = (M + 15) / 16;
+    // Blocks of four rows fill the chip sooner, of eight read and unpack the weights less often (64 x 2048 x
+    // 2048 in fours 7.1 us, in eights 7.6; 48 x 8224 x 2048 18.1 and 17.4; 8 x 2048 x 2048 5.0 and 6.2).
+    p.image = M == 1 ? 1 : tiles * ((M + 3) / 4) <= 2048 || M <= 4 ? 4 : 8;
+    p.row_blocks = (M + p.image - 1) / p.image;
     p.most = (M + p.row_blocks - 1) / p.row_blocks;
-    p.image = p.most == 1 ? 1 : p.most <= 4 ? 4 : p.most <= 8 ? 8 : 16;
-    p.pre = p.most > 4;
-    p.ks = 8;
-    while (p.ks > 1 && tiles * p.ks * p.row_blocks >= 2 * kWaves * 256) p.ks /= 2;
-    while (p.ks > 1 && p.ks / 2 >= blocks) p.ks /= 2;
+    // Waves share a tile while there are not enough tiles: up to eight waves a compute unit, for one row up to 32
+    // (12288 x 2048, eight waves a tile 5.1 us, two 5.8; the head of 151936 rows, one wave 30.5 us, eight 32).
+    p.ks = kWaves;
+    while (p.ks > 1 && (static_cast<int64_t>(tiles) * p.row_blocks * p.ks > (M == 1 ? 8192 : 2048) || p.ks / 2 >= blocks)) p.ks /= 2;
     const int rt = kWaves / p.ks, sets = (tiles + rt - 1) / rt;
-    p.wgs = std::min(sets, std::max(1, 256 / p.row_blocks));
+    // two workgroups a compute unit go on from tile to tile; one row without shared tiles takes them all at once
+    // (the head: 1187 workgroups 30.5 us, 256 36.6)
+    p.wgs = M == 1 && p.ks == 1 ? sets : std::min(sets, std::max(1, 512 / p.row_blocks));
     q4_fit<G, ZP>(p, N, K);
     return p;
 }
 
-template <int G, bool ZP, int R, bool PRE>
+template <int G, bool ZP, int R>
 hipError_t launch_q4_form(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
     static std::once_flag once;         // LDS beyond the default limit
     static hipError_t limit;
     std::call_once(once, [] {
-        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, R, PRE>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    160 * 1024);
+        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, R>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     });
     if (limit != hipSuccess) return limit;
-    if constexpr (PRE) {
-        const int kp = q4_blocks(a.K) * 256;
-        uint8_t* ws = static_cast<uint8_t*>(a.ws);
-        klaunch(q4_image_kernel<G, ZP, R>, dim3((p.most * kp / 8 + 255) / 256, p.row_blocks), dim3(256), 0, s, a.X, a.ldx, a.M, a.K, p.most, ws,
-                ws + static_cast<int64_t>(p.row_blocks) * R * 3 * kp);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    klaunch(q4_mul_kernel<G, ZP, R, PRE>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
+    klaunch(q4_mul_kernel<G, ZP, R>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
     return hipGetLastError();
 }
 
 template <int G, bool ZP>
 hipError_t launch_q4_plan(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
-    if (p.pre) return p.image == 4 ? launch_q4_form<G, ZP, 4, true>(a, p, s) : p.image == 8 ? launch_q4_form<G, ZP, 8, true>(a, p, s) : launch_q4_form<G, ZP, 16, true>(a, p, s);
-    return p.image == 1 ? launch_q4_form<G, ZP, 1, false>(a, p, s) : p.image == 4 ? launch_q4_form<G, ZP, 4, false>(a, p, s) : launch_q4_form<G, ZP, 8, false>(a, p, s);
+    return p.image == 1 ? launch_q4_form<G, ZP, 1>(a, p, s) : p.image == 4 ? launch_q4_form<G, ZP, 4>(a, p, s) : launch_q4_form<G, ZP, 8>(a, p, s);
 }
 
 }  // namespace
 
-uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) {
-    const uint64_t kp = static_cast<uint64_t>(q4_blocks(K)) * 256;
-    return (M + 15) / 16 * 16 * (3 * kp + kp / G * 16);
-}
+uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) { return 16; }
 
 hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s) {
     const auto go = [&](auto g, auto z) {
