@@ -31,30 +31,35 @@ __device__ __forceinline__ double min16(double v) {
     v = fmin(v, dpp_d<0x141>(v));
     return fmin(v, dpp_d<0x140>(v));
 }
-// over the 16 lanes of a row
-__device__ __forceinline__ uint32_t max16(uint32_t v) {
-    v = max(v, static_cast<uint32_t>(dpp_i<0xB1>(static_cast<int>(v))));
-    v = max(v, static_cast<uint32_t>(dpp_i<0x4E>(static_cast<int>(v))));
-    v = max(v, static_cast<uint32_t>(dpp_i<0x141>(static_cast<int>(v))));
-    return max(v, static_cast<uint32_t>(dpp_i<0x140>(static_cast<int>(v))));
+// Over the 16 lanes of a row; all of them are there, so that a move becomes part of the instruction that uses it.
+template <int CTRL>
+__device__ __forceinline__ int row_i(int x) { return __builtin_amdgcn_mov_dpp(x, CTRL, 0xF, 0xF, true); }
+template <int CTRL>
+__device__ __forceinline__ float row_f(float x) { return __builtin_bit_cast(float, row_i<CTRL>(__builtin_bit_cast(int, x))); }
+__device__ __forceinline__ int max16(int v) {
+    v = max(v, row_i<0xB1>(v));
+    v = max(v, row_i<0x4E>(v));
+    v = max(v, row_i<0x141>(v));
+    return max(v, row_i<0x140>(v));
 }
+// of values that are not negative (a NaN is above all)
+__device__ __forceinline__ float max16_abs(float v) { return __builtin_bit_cast(float, max16(__builtin_bit_cast(int, v))); }
+// by bits in the values' order, as fmaxf takes an instruction more a step
 __device__ __forceinline__ float max16(float v) {
-    v = fmaxf(v, dpp_f<0xB1>(v));
-    v = fmaxf(v, dpp_f<0x4E>(v));
-    v = fmaxf(v, dpp_f<0x141>(v));
-    return fmaxf(v, dpp_f<0x140>(v));
+    const auto order = [](int b) { return b ^ (b >> 31 & 0x7fffffff); };
+    return __builtin_bit_cast(float, order(max16(order(__builtin_bit_cast(int, v)))));
 }
 __device__ __forceinline__ int sum16(int v) {
-    v += dpp_i<0xB1>(v);
-    v += dpp_i<0x4E>(v);
-    v += dpp_i<0x141>(v);
-    return v + dpp_i<0x140>(v);
+    v += row_i<0xB1>(v);
+    v += row_i<0x4E>(v);
+    v += row_i<0x141>(v);
+    return v + row_i<0x140>(v);
 }
 __device__ __forceinline__ float sum16(float v) {
-    v += dpp_f<0xB1>(v);
-    v += dpp_f<0x4E>(v);
-    v += dpp_f<0x141>(v);
-    return v + dpp_f<0x140>(v);
+    v += row_f<0xB1>(v);
+    v += row_f<0x4E>(v);
+    v += row_f<0x141>(v);
+    return v + row_f<0x140>(v);
 }
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int or16(int v) {
@@ -158,7 +163,7 @@ __global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, RopeFre
             f[i] = static_cast<float>(x[i] * kScale);
             top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
         }
-        top = max16(top);
+        top = static_cast<uint32_t>(max16(static_cast<int>(top)));
         const bool ok = top < 0x7f800000u && top != 0;
         const int e = ok ? multiple_exp(__uint_as_float(top)) : 0;
         int sum = 0;
@@ -191,7 +196,11 @@ __global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, RopeFre
     if ((lane & 15) == 0) (is_k ? a.k_scale : a.v_scale)[at * 4 + lane / 16] = scale;
 }
 
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// sixteen codes of two words as bytes: the even nibbles of each, then the odd ones
+__device__ __forceinline__ v4i bytes_of(v2i w) {
+    return v4i{w[0] & 0x0f0f0f0f, static_cast<int>(static_cast<uint32_t>(w[0]) >> 4 & 0x0f0f0f0fu), w[1] & 0x0f0f0f0f,
+               static_cast<int>(static_cast<uint32_t>(w[1]) >> 4 & 0x0f0f0f0fu)};
+}
 
 // What lanes of a wave have written to LDS is there for its other lanes.
 __device__ __forceinline__ void wave_sync() {
@@ -223,7 +232,7 @@ template <int HQ>
 __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4Args a, QueryImage img, int pieces, int piece_len, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int kWaves = attn_q4_waves<HQ>;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane >> 4, n = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
     const int piece = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
     const int len = a.len[b];
     if (len < 0) return;
@@ -252,34 +261,42 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
         reinterpret_cast<uint4*>(qbuf)[i] = reinterpret_cast<const uint4*>(img.digits + bk * HQ * kQuadBytes)[i];
     if (threadIdx.x < HQ * 16) fbuf[threadIdx.x] = img.factors[bk * HQ * 16 + threadIdx.x];
 
-    uint2 k[4][4];
-    uint4 ks[4], vs[4];
+    // A tile's keys, key and value steps, and value rows: whole tiles by constant places of a lane, the last one's
+    // missing rows as copies of the last row (their scores are masked).
+    v2i k[4][4];
+    v4i ks[4], vs[4], v[8];
     const auto load_k = [&](int t0) {
+        const uint8_t *kt = K + static_cast<int64_t>(t0) * kQ4RowBytes, *st = KS + static_cast<int64_t>(t0) * 16;
+        const bool whole = t0 + kTile <= count;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const uint32_t r = min(t0 + 16 * t + n, count - 1);
+            const uint32_t r = whole ? 16 * t + n : min(16 * t + n, count - 1 - t0);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) k[t][g] = *reinterpret_cast<const uint2*>(K + (r * kQ4RowBytes + 8 * c) + 32 * g);
-            ks[t] = *reinterpret_cast<const uint4*>(KS + r * 16);
+            for (int g = 0; g < 4; ++g) k[t][g] = *reinterpret_cast<const v2i*>(kt + (r * kQ4RowBytes + 8 * c) + 32 * g);
+            ks[t] = *reinterpret_cast<const v4i*>(st + r * 16);
+        }
+    };
+    const auto load_v = [&](int t0) {
+        const uint8_t* vt = V + static_cast<int64_t>(t0) * kQ4RowBytes;
+        const bool whole = t0 + kTile <= count;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t r = whole ? 8 * i + (lane >> 3) : min(8 * i + (lane >> 3), count - 1 - t0);
+            v[i] = *reinterpret_cast<const v4i*>(vt + (r * kQ4RowBytes + 16 * (lane & 7)));
         }
     };
     // a row's eight 16-byte pieces lie in LDS in an order that spreads the rows over the banks
-    v4i v[8];
-    const auto load_v = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t r = min(t0 + 8 * i + (lane >> 3), count - 1);
-            v[i] = *reinterpret_cast<const v4i*>(V + (r * kQ4RowBytes + 16 * (lane & 7)));
-        }
-    };
     const auto place_v = [&] {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             *reinterpret_cast<v4i*>(vbuf + (8 * i + (lane >> 3)) * kQ4RowBytes + 16 * ((lane & 7) ^ (lane >> 3))) = v[i];
     };
     const auto load_vs = [&](int t0) {
+        const uint8_t* st = VS + static_cast<int64_t>(t0) * 16;
+        const bool whole = t0 + kTile <= count;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) vs[t] = *reinterpret_cast<const uint4*>(VS + static_cast<uint32_t>(min(t0 + 16 * t + n, count - 1)) * 16);
+        for (int t = 0; t < 4; ++t)
+            vs[t] = *reinterpret_cast<const v4i*>(st + static_cast<uint32_t>(whole ? 16 * t + n : min(16 * t + n, count - 1 - t0)) * 16);
     };
 
     float m[HQ], l[HQ], lo[HQ][4], o[HQ][16];
@@ -319,10 +336,8 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const uint2 w = k[t][g];
-                const v4i kb = {static_cast<int>(w.x & 0x0f0f0f0fu), static_cast<int>(w.x >> 4 & 0x0f0f0f0fu),
-                                static_cast<int>(w.y & 0x0f0f0f0fu), static_cast<int>(w.y >> 4 & 0x0f0f0f0fu)};
-                const uint32_t sc = word(ks[t], g);
+                const v4i kb = bytes_of(k[t][g]);
+                const uint32_t sc = ks[t][g];
                 const float step = step_of(sc), least = least_of(sc);
 #pragma unroll
                 for (int j = 0; j < HQ; ++j) {
@@ -345,8 +360,10 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
         float alpha[HQ], beta[HQ];
 #pragma unroll
         for (int j = 0; j < HQ; ++j) {
+            if (t0 + kTile > count) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) s[j][t] = t0 + 16 * t + n < count ? s[j][t] : -INFINITY;
+                for (int t = 0; t < 4; ++t) s[j][t] = t0 + 16 * t + n < count ? s[j][t] : -INFINITY;
+            }
             const float top = max16(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
             const float ref = top == -INFINITY ? 0.0f : top, mn = fmaxf(m[j], top), mref = mn == -INFINITY ? 0.0f : mn;
             alpha[j] = exp2_f(m[j] - mref);
@@ -366,8 +383,8 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
                 float st[4], le[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    st[t] = step_of(word(vs[t], g));
-                    le[t] = fmaf(st[t], 0.0f, least_of(word(vs[t], g)));  // NaN where the step is
+                    st[t] = step_of(vs[t][g]);
+                    le[t] = fmaf(st[t], 0.0f, least_of(vs[t][g]));  // NaN where the step is
                 }
 #pragma unroll
                 for (int j = j0; j < j0 + JB; ++j) {
@@ -378,7 +395,7 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
                         part_lo = fmaf(s[j][t], le[t], part_lo);
                     }
                     lo[j][g] = fmaf(lo[j][g], alpha[j], beta[j] * part_lo);
-                    const float big = max16(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+                    const float big = max16_abs(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
                     const float inv = big > 1e-30f ? 4190000.0f * __builtin_amdgcn_rcpf(big) : 0.0f;
                     unit[j - j0][g] = beta[j] * big * (1.0f / 4190000.0f);
                     uint32_t y[4];
@@ -386,8 +403,10 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
                     for (int t = 0; t < 4; ++t)  // 1.5 2^23 + i: i in the low bits
                         y[t] = (__float_as_uint(fmaf(x[t], inv, 12582912.0f)) + (0x8080u - 0x4b400000u)) ^ 0x8080u;
                     uint8_t* at = pbuf + (j - j0) * kPBytes + (g * 4 + (n >> 2)) * 192 + c * 48 + 4 * (n & 3);
-                    *reinterpret_cast<uint32_t*>(at) = plane<0>(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint32_t*>(at + 16) = plane<1>(y[0], y[1], y[2], y[3]);
+                    // bytes 0 and 1 of two words each, then of all four
+                    const uint32_t a01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), a23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+                    *reinterpret_cast<uint32_t*>(at) = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+                    *reinterpret_cast<uint32_t*>(at + 16) = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
                     *reinterpret_cast<uint32_t*>(at + 32) = plane<2>(y[0], y[1], y[2], y[3]);
                     pin(lo[j][g]);
                     pin(unit[j - j0][g]);
@@ -412,8 +431,7 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
                     const int d = 4 * g + i;  // dims 16 d .. + 15
                     const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) v2i*>(
                         reinterpret_cast<uintptr_t>(vbuf + key * kQ4RowBytes + 16 * ((d >> 1) ^ (key & 7)) + 8 * (d & 1))));
-                    const v4i vb = {w[0] & 0x0f0f0f0f, static_cast<int>(static_cast<uint32_t>(w[0]) >> 4 & 0x0f0f0f0fu), w[1] & 0x0f0f0f0f,
-                                    static_cast<int>(static_cast<uint32_t>(w[1]) >> 4 & 0x0f0f0f0fu)};
+                    const v4i vb = bytes_of(w);
 #pragma unroll
                     for (int j = 0; j < JB; ++j) {
                         o[j0 + j][d] = fmaf(from_digits(__builtin_amdgcn_mfma_i32_16x16x64_i8(p[j], vb, v4i{0, 0, 0, 0}, 0, 0, 0)),
