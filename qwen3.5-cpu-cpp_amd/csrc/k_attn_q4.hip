@@ -107,93 +107,70 @@ struct RopeFreq {
     double f[kHD / 2];
 };
 
-// What the products read of a query head: the three digits of its rows, by quads of heads: [quad][group of
-// 64 dims][c][head of the quad][digit] 16 bytes, the dims 16 c .. + 15 of the group in the order
-// in which a cache row's nibbles come apart (0 2 4 6 1 3 5 7 8 10 ..); and per head and group (2^-e, 2^-e times the
-// sum of the multiples), which the rows' least values are multiplied by.
-struct QueryImage {
-    uint8_t* digits;                    // [B][NKV][quads][4][4][4][3][16]
-    float2* factors;                    // [B][NKV][4 quads][4]
-};
+// What lanes of a wave have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// What the products read of a query head lies in LDS: the three digits of its row, by quads of heads: [quad][group
+// of 64 dims][c][head of the quad][digit] 16 bytes, the dims 16 c .. + 15 of the group in the order in which a
+// cache row's nibbles come apart (0 2 4 6 1 3 5 7 8 10 ..); and per head and group (2^-e, 2^-e times the sum of the
+// multiples), which the rows' least values are multiplied by.
 constexpr int kQuadBytes = 4 * 4 * 4 * 3 * 16;
 
-// A wave a row: the batch's query rows (normed, rotated, times log2(e) / sqrt(HD), split into digits), then the new
-// key rows (normed, rotated) and value rows, quantized and appended at slot len[b].
-__global__ __launch_bounds__(256) void attn_q4_prep_kernel(AttnQ4Args a, RopeFreq freq, QueryImage img, int quads) {
-    __shared__ double row[4][kHD], cs[4][kHD];
-    const int lane = threadIdx.x & 63, w = threadIdx.x / 64;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + w;
-    const int per = a.NQ + 2 * a.NKV;
-    const int b = static_cast<int>(id / per), r = static_cast<int>(id % per);
-    const int len = b < a.B ? a.len[b] : -1;
-    const bool on = len >= 0 && len < a.cap, is_q = r < a.NQ, is_k = !is_q && r < a.NQ + a.NKV;
-    const int h = is_q ? r : is_k ? r - a.NQ : r - a.NQ - a.NKV;
-    const int half = a.ROT / 2;
-    double x[4] = {0, 0, 0, 0};
-    if (on) {
-        const float* src = is_q ? a.qg + (static_cast<int64_t>(b) * a.NQ + h) * 2 * kHD
-                                : (is_k ? a.k_new : a.v_new) + (static_cast<int64_t>(b) * a.NKV + h) * kHD;
-        const float4 f = reinterpret_cast<const float4*>(src)[lane];
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-        if (is_q || is_k) {
-            const float4 nw = reinterpret_cast<const float4*>(is_q ? a.q_norm : a.k_norm)[lane];
-            for (int i = lane; i < half; i += 64) sincos(static_cast<double>(a.pos[b]) * freq.f[i], &cs[w][128 + i], &cs[w][i]);
-            const double ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-            const double inv = 1.0 / sqrt(ss / kHD + static_cast<double>(a.eps));
-            x[0] *= inv * (1.0 + nw.x), x[1] *= inv * (1.0 + nw.y), x[2] *= inv * (1.0 + nw.z), x[3] *= inv * (1.0 + nw.w);
-            for (int i = 0; i < 4; ++i) row[w][4 * lane + i] = x[i];
-        }
+// A wave norms a row (lane l: dims 4 l .. + 3) and rotates it by the angles in cs (cosines, then sines from 128 on),
+// through 2 KB of LDS of its own.
+__device__ __forceinline__ void norm_rotate(double* x, const float4& w, float eps, int rot, const double* cs, double* row) {
+    const int lane = threadIdx.x & 63, half = rot / 2;
+    const double ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
+    const double inv = 1.0 / sqrt(ss / kHD + static_cast<double>(eps));
+    x[0] *= inv * (1.0 + w.x), x[1] *= inv * (1.0 + w.y), x[2] *= inv * (1.0 + w.z), x[3] *= inv * (1.0 + w.w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[4 * lane + i] = x[i];
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = 4 * lane + i;
+        if (d < half) x[i] = x[i] * cs[d] - row[d + half] * cs[128 + d];
+        else if (d < rot) x[i] = x[i] * cs[d - half] + row[d - half] * cs[128 + d - half];
     }
-    __syncthreads();
-    if (!on) return;
-    if (is_q || is_k) {
+    wave_sync();
+}
+
+// A normed, rotated query row, times log2(e) / sqrt(HD), as digits: head h of the kv head's.
+__device__ __forceinline__ void place_query(const double* x, int h, uint8_t* qbuf, float2* fbuf) {
+    const int lane = threadIdx.x & 63;
+    constexpr double kScale = 0.0625 * 1.4426950408889634;
+    float f[4];
+    uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 4 * lane + i;
-            if (d < half) x[i] = x[i] * cs[w][d] - row[w][d + half] * cs[w][128 + d];
-            else if (d < a.ROT) x[i] = x[i] * cs[w][d - half] + row[w][d - half] * cs[w][128 + d - half];
-        }
+    for (int i = 0; i < 4; ++i) {
+        f[i] = static_cast<float>(x[i] * kScale);
+        top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
     }
-    if (is_q) {
-        constexpr double kScale = 0.0625 * 1.4426950408889634;
-        float f[4];
-        uint32_t top = 0;
+    top = static_cast<uint32_t>(max16(static_cast<int>(top)));
+    const bool ok = top < 0x7f800000u && top != 0;
+    const int e = ok ? multiple_exp(__uint_as_float(top)) : 0;
+    int sum = 0;
+    uint32_t y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[i] = static_cast<float>(x[i] * kScale);
-            top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-        }
-        top = static_cast<uint32_t>(max16(static_cast<int>(top)));
-        const bool ok = top < 0x7f800000u && top != 0;
-        const int e = ok ? multiple_exp(__uint_as_float(top)) : 0;
-        int sum = 0;
-        uint32_t y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int v = ok ? static_cast<int>(rintf(ldexpf(f[i], e))) : 0;
-            sum += v;
-            y[i] = signed_digits(v);
-        }
-        sum = sum16(sum);
-        const int g = lane >> 4, c = lane >> 2 & 3, o = lane & 3, hk = h / a.GRP, hq = h % a.GRP;
-        const int64_t bk = static_cast<int64_t>(b) * a.NKV + hk;
-        uint8_t* at = img.digits + (bk * quads + hq / 4) * kQuadBytes + ((g * 4 + c) * 4 + hq % 4) * 48 + (o >> 1) * 8 + (o & 1) * 2;
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {  // dims 4 o, 4 o + 2 and 4 o + 1, 4 o + 3 of the sixteen
-            *reinterpret_cast<uint16_t*>(at + 16 * p) = static_cast<uint16_t>((y[0] >> (8 * p) & 0xffu) | (y[2] >> (8 * p) & 0xffu) << 8);
-            *reinterpret_cast<uint16_t*>(at + 16 * p + 4) = static_cast<uint16_t>((y[1] >> (8 * p) & 0xffu) | (y[3] >> (8 * p) & 0xffu) << 8);
-        }
-        if ((lane & 15) == 0) {
-            const float s = top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
-            img.factors[(bk * quads * 4 + hq) * 4 + g] = make_float2(s, s * static_cast<float>(sum));
-        }
-        return;
+    for (int i = 0; i < 4; ++i) {
+        const int v = ok ? static_cast<int>(rintf(ldexpf(f[i], e))) : 0;
+        sum += v;
+        y[i] = signed_digits(v);
     }
-    uint32_t scale;
-    const uint32_t c = quantize4(x, scale);
-    const int64_t at = (static_cast<int64_t>(b) * a.NKV + h) * a.cap + len;
-    reinterpret_cast<uint16_t*>(is_k ? a.k : a.v)[at * 64 + lane] = static_cast<uint16_t>(c);
-    if ((lane & 15) == 0) (is_k ? a.k_scale : a.v_scale)[at * 4 + lane / 16] = scale;
+    sum = sum16(sum);
+    const int g = lane >> 4, c = lane >> 2 & 3, o = lane & 3;
+    uint8_t* at = qbuf + (h / 4) * kQuadBytes + ((g * 4 + c) * 4 + h % 4) * 48 + (o >> 1) * 8 + (o & 1) * 2;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {  // dims 4 o, 4 o + 2 and 4 o + 1, 4 o + 3 of the sixteen
+        *reinterpret_cast<uint16_t*>(at + 16 * p) = static_cast<uint16_t>((y[0] >> (8 * p) & 0xffu) | (y[2] >> (8 * p) & 0xffu) << 8);
+        *reinterpret_cast<uint16_t*>(at + 16 * p + 4) = static_cast<uint16_t>((y[1] >> (8 * p) & 0xffu) | (y[3] >> (8 * p) & 0xffu) << 8);
+    }
+    if ((lane & 15) == 0) {
+        const float s = top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
+        fbuf[h * 4 + g] = make_float2(s, s * static_cast<float>(sum));
+    }
 }
 
 // sixteen codes of two words as bytes: the even nibbles of each, then the odd ones
@@ -202,14 +179,16 @@ __device__ __forceinline__ v4i bytes_of(v2i w) {
                static_cast<int>(static_cast<uint32_t>(w[1]) >> 4 & 0x0f0f0f0fu)};
 }
 
-// What lanes of a wave have written to LDS is there for its other lanes.
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 
 constexpr int kTile = 64;       // keys a wave takes at a time
 constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16;
+
+// Rows a piece: a sequence's rows in as many pieces as there are workgroups for its head, each as many rounds of
+// tiles for its waves as that takes.
+__device__ __forceinline__ int attn_q4_piece(int rows, int pieces, int waves) {
+    const int round = waves * kTile;
+    return ((rows + round - 1) / round + pieces - 1) / pieces * round;
+}
 
 struct Partials {
     float* o;                           // [B][NKV][pieces][GRP][HD]
@@ -229,7 +208,7 @@ struct Partials {
 template <int HQ>
 constexpr int attn_q4_waves = HQ > 2 ? 4 : 8;  // with 16 heads a wave holds more than 256 registers
 template <int HQ>
-__global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4Args a, QueryImage img, int pieces, int piece_len, Partials part) {
+__global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int pieces, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int kWaves = attn_q4_waves<HQ>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
@@ -242,24 +221,23 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
                 a.out[(static_cast<int64_t>(b) * a.NQ + hk * a.GRP) * kHD + i] = NAN;
         return;
     }
-    const int rows = len + 1, first = piece * piece_len, end = min(rows, first + piece_len);
+    const int rows = len + 1, piece_len = attn_q4_piece(rows, pieces, kWaves), first = piece * piece_len, end = min(rows, first + piece_len);
     if (first >= rows) return;
     const int64_t bk = static_cast<int64_t>(b) * a.NKV + hk;
+    const bool fresh = end == rows;     // the new row is this piece's
     // the piece's rows; offsets within it stay within 32 bits
     const int count = end - first;
     const int64_t row0 = bk * a.cap + first;
     const uint8_t *K = a.k + row0 * kQ4RowBytes, *V = a.v + row0 * kQ4RowBytes;
     const uint8_t *KS = reinterpret_cast<const uint8_t*>(a.k_scale) + row0 * 16, *VS = reinterpret_cast<const uint8_t*>(a.v_scale) + row0 * 16;
 
-    // the queries, for all waves; each wave's value rows and weights
+    // the queries, for all waves, the angles, and each wave's value rows and weights
     constexpr int JB = HQ < 2 ? HQ : 2;  // quads whose weights lie in LDS at a time
     uint8_t* qbuf = lds;
     float2* fbuf = reinterpret_cast<float2*>(lds + HQ * kQuadBytes);
-    uint8_t* vbuf = lds + HQ * (kQuadBytes + 128) + wave * (kVBytes + JB * kPBytes);
+    double* cs = reinterpret_cast<double*>(lds + HQ * (kQuadBytes + 128));
+    uint8_t* vbuf = lds + HQ * (kQuadBytes + 128) + 2048 + wave * (kVBytes + JB * kPBytes);
     uint8_t* pbuf = vbuf + kVBytes;
-    for (int i = threadIdx.x; i < HQ * kQuadBytes / 16; i += kWaves * 64)
-        reinterpret_cast<uint4*>(qbuf)[i] = reinterpret_cast<const uint4*>(img.digits + bk * HQ * kQuadBytes)[i];
-    if (threadIdx.x < HQ * 16) fbuf[threadIdx.x] = img.factors[bk * HQ * 16 + threadIdx.x];
 
     // A tile's keys, key and value steps, and value rows: whole tiles by constant places of a lane, the last one's
     // missing rows as copies of the last row (their scores are masked).
@@ -312,11 +290,46 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
 
     // nibble n of the transposed 16 keys: which key its place in the operand is
     const int spot = (n & 8) + (n & 1) * 4 + ((n & 7) >> 1), key = 16 * (spot & 3) + 4 * c + (spot >> 2);
+    // What does not depend on the new row is on its way while the queries are made.
     int t0 = wave * kTile;
-    if (t0 < count) {
-        load_k(t0);
-        load_v(t0);
-        load_vs(t0);
+    const auto request = [&] {
+        if (t0 < count) {
+            load_k(t0);
+            load_v(t0);
+            load_vs(t0);
+        }
+    };
+    constexpr int kHeads = (4 * HQ + kWaves - 1) / kWaves;  // query heads a wave makes
+    float4 qx[kHeads];
+    const float4 qw = reinterpret_cast<const float4*>(a.q_norm)[lane];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+        qx[i] = reinterpret_cast<const float4*>(a.qg + (static_cast<int64_t>(b) * a.NQ + hk * a.GRP + min(wave + i * kWaves, a.GRP - 1)) * 2 * kHD)[lane];
+    if (!fresh) request();
+    for (int i = threadIdx.x; i < a.ROT / 2; i += kWaves * 64) sincos(static_cast<double>(a.pos[b]) * freq.f[i], &cs[128 + i], &cs[i]);
+    lds_barrier();
+    double* row = reinterpret_cast<double*>(vbuf);  // before the values are there
+    if (fresh) {
+        if (wave >= kWaves - 2) {
+            const bool is_k = wave == kWaves - 2;
+            const float4 f = reinterpret_cast<const float4*>((is_k ? a.k_new : a.v_new) + bk * kHD)[lane];
+            double x[4] = {f.x, f.y, f.z, f.w};
+            if (is_k) norm_rotate(x, reinterpret_cast<const float4*>(a.k_norm)[lane], a.eps, a.ROT, cs, row);
+            uint32_t scale;
+            const uint32_t code = quantize4(x, scale);
+            const int64_t at = bk * a.cap + len;
+            reinterpret_cast<uint16_t*>(is_k ? a.k : a.v)[at * 64 + lane] = static_cast<uint16_t>(code);
+            if (n == 0) (is_k ? a.k_scale : a.v_scale)[at * 4 + c] = scale;
+        }
+        __syncthreads();                // the row is where the tiles are read from
+        request();
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        if (wave + i * kWaves >= a.GRP) break;
+        double x[4] = {qx[i].x, qx[i].y, qx[i].z, qx[i].w};
+        norm_rotate(x, qw, a.eps, a.ROT, cs, row);
+        place_query(x, wave + i * kWaves, qbuf, fbuf);
     }
     lds_barrier();
     for (; t0 < count; t0 += kWaves * kTile) {
@@ -447,87 +460,103 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
             wave_sync();
         }
     }
+    // The waves' parts: each scaled to the largest maximum of all, then added.
     __syncthreads();
-    // the waves' parts
-    float* wo = reinterpret_cast<float*>(lds);
-    float2* wml = reinterpret_cast<float2*>(lds + kWaves * HQ * 4 * kHD * 4);
+    float2* wml = reinterpret_cast<float2*>(lds);
+    float* wo = reinterpret_cast<float*>(lds + kWaves * HQ * 4 * 8);
 #pragma unroll
     for (int j = 0; j < HQ; ++j) {
         l[j] = sum16(l[j]);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            lo[j][g] = sum16(lo[j][g]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) wo[((wave * HQ + j) * 4 + c) * kHD + 16 * (4 * g + i) + n] = o[j][4 * g + i] + lo[j][g];
-        }
         if (n == 0) wml[wave * HQ * 4 + 4 * j + c] = make_float2(m[j], l[j]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) lo[j][g] = sum16(lo[j][g]);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.GRP * kHD; i += kWaves * 64) {
-        const int h = i / kHD, d = i % kHD;
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < HQ; ++j) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wml[w * HQ * 4 + h].x);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, x = 0.0f;
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wml[w * HQ * 4 + 4 * j + c].x);
+        const float f = exp2_f(m[j] - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float2 ml = wml[w * HQ * 4 + h];
-            const float f = exp2_f(ml.x - ref);
-            sum = fmaf(f, ml.y, sum);
-            x = fmaf(f, wo[(w * HQ * 4 + h) * kHD + d], x);
-        }
-        if (pieces == 1) {
+        for (int d = 0; d < 16; ++d) wo[((wave * HQ + j) * 4 + c) * kHD + 16 * d + n] = f * (o[j][d] + lo[j][d / 4]);
+    }
+    lds_barrier();
+    for (int i = threadIdx.x; i < a.GRP * (kHD / 4); i += kWaves * 64) {
+        const int h = i / (kHD / 4), d = i % (kHD / 4);
+        v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) x += reinterpret_cast<const v4f*>(wo + (w * HQ * 4 + h) * kHD)[d];
+        float m_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, wml[w * HQ * 4 + h].x);
+        const float ref = m_all == -INFINITY ? 0.0f : m_all;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) l_all = fmaf(exp2_f(wml[w * HQ * 4 + h].x - ref), wml[w * HQ * 4 + h].y, l_all);
+        if (rows <= piece_len) {        // all there is
             const int64_t at = static_cast<int64_t>(b) * a.NQ + hk * a.GRP + h;
-            a.out[at * kHD + d] = x / sum * sigmoid_f(a.qg[at * 2 * kHD + kHD + d]);
+            const v4f g = reinterpret_cast<const v4f*>(a.qg + at * 2 * kHD + kHD)[d];
+            reinterpret_cast<v4f*>(a.out + at * kHD)[d] = v4f{x[0] / l_all * sigmoid_f(g[0]), x[1] / l_all * sigmoid_f(g[1]),
+                                                              x[2] / l_all * sigmoid_f(g[2]), x[3] / l_all * sigmoid_f(g[3])};
         } else {
             const int64_t at = (bk * pieces + piece) * a.GRP + h;
-            part.o[at * kHD + d] = x;
-            if (d == 0) part.ml[at] = make_float2(top, sum);
+            reinterpret_cast<v4f*>(part.o + at * kHD)[d] = x;
+            if (d == 0) part.ml[at] = make_float2(m_all, l_all);
         }
     }
 }
 
-// A workgroup a query head: the pieces' parts, four waves taking them in turn, and the gate.
-__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, int pieces, int piece_len, Partials part) {
-    __shared__ float4 ws[4][64];
-    __shared__ float2 wml[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.x, b = blockIdx.y, hk = h / a.GRP;
+// The pieces' parts of a query head, and the gate: four workgroups a head, 64 dims each; sixteen threads of every
+// workgroup take four dims of every 16th piece.
+__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, int waves, int pieces, Partials part) {
+    __shared__ v4f ws[16][16];
+    __shared__ float2 wml[16];
+    const int d = threadIdx.x & 15, s = threadIdx.x >> 4, h = blockIdx.x >> 2, quarter = blockIdx.x & 3, b = blockIdx.y, hk = h / a.GRP;
     const int len = a.len[b];
     if (len < 0 || len >= a.cap) return;
-    const int np = len / piece_len + 1;
-    const int64_t first = (static_cast<int64_t>(b) * a.NKV + hk) * pieces * a.GRP + h % a.GRP;
+    const int piece_len = attn_q4_piece(len + 1, pieces, waves), np = len / piece_len + 1;
+    if (np == 1) return;                // written by the piece
+    const int64_t first = (static_cast<int64_t>(b) * a.NKV + hk) * pieces * a.GRP + h % a.GRP, o = static_cast<int64_t>(b) * a.NQ + h;
+    const v4f g = reinterpret_cast<const v4f*>(a.qg + o * 2 * kHD + kHD)[quarter * 16 + d];
     float m = -INFINITY, l = 0.0f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = wave; i < np; i += 4) {
-        const int64_t at = first + static_cast<int64_t>(i) * a.GRP;
-        const float2 ml = part.ml[at];
-        const float4 v = reinterpret_cast<const float4*>(part.o + at * kHD)[lane];
-        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn, f = exp2_f(m - ref), g = exp2_f(ml.x - ref);
-        m = mn;
-        l = l * f + ml.y * g;
-        x = make_float4(x.x * f + v.x * g, x.y * f + v.y * g, x.z * f + v.z * g, x.w * f + v.w * g);
+    v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kBatch = 4;           // requested together
+    for (int i0 = s; i0 < np; i0 += 16 * kBatch) {
+        float2 ml[kBatch];
+        v4f v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int64_t at = first + static_cast<int64_t>(min(i0 + 16 * k, np - 1)) * a.GRP;
+            ml[k] = part.ml[at];
+            v[k] = reinterpret_cast<const v4f*>(part.o + at * kHD)[quarter * 16 + d];
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (i0 + 16 * k >= np) break;
+            const float mn = fmaxf(m, ml[k].x), ref = mn == -INFINITY ? 0.0f : mn, f = exp2_f(m - ref), e = exp2_f(ml[k].x - ref);
+            m = mn;
+            l = l * f + ml[k].y * e;
+            x = x * f + v[k] * e;
+        }
     }
-    ws[wave][lane] = x;
-    if (lane == 0) wml[wave] = make_float2(m, l);
+    ws[s][d] = x;
+    if (d == 0) wml[s] = make_float2(m, l);
     __syncthreads();
-    if (wave) return;
-    float top = fmaxf(fmaxf(wml[0].x, wml[1].x), fmaxf(wml[2].x, wml[3].x));
+    if (s) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, wml[i].x);
     top = top == -INFINITY ? 0.0f : top;
     l = 0.0f;
-    x = make_float4(0.f, 0.f, 0.f, 0.f);
+    x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 16; ++i) {
         const float f = exp2_f(wml[i].x - top);
-        const float4 v = ws[i][lane];
         l = fmaf(wml[i].y, f, l);
-        x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
+        x += ws[i][d] * f;
     }
-    const int64_t o = static_cast<int64_t>(b) * a.NQ + h;
-    const float4 g = reinterpret_cast<const float4*>(a.qg + o * 2 * kHD + kHD)[lane];
-    reinterpret_cast<float4*>(a.out + o * kHD)[lane] =
-        make_float4(x.x / l * sigmoid_f(g.x), x.y / l * sigmoid_f(g.y), x.z / l * sigmoid_f(g.z), x.w / l * sigmoid_f(g.w));
+    reinterpret_cast<v4f*>(a.out + o * kHD)[quarter * 16 + d] =
+        v4f{x[0] / l * sigmoid_f(g[0]), x[1] / l * sigmoid_f(g[1]), x[2] / l * sigmoid_f(g[2]), x[3] / l * sigmoid_f(g[3])};
 }
 
 // whether rows [i, e) of sequence b are there
@@ -584,61 +613,50 @@ __global__ __launch_bounds__(256) void kv_q4_kernel(KvQ4Args a) {
 namespace {
 
 struct AttnQ4Plan {
-    int quads, pieces, piece_len;
+    int quads, pieces;
 };
 AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     AttnQ4Plan p{};
     p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
     const int64_t round = (p.quads > 2 ? attn_q4_waves<4> : attn_q4_waves<2>) * kTile, heads = static_cast<int64_t>(a.B) * a.NKV;
-    int64_t rounds = 1;
-    while ((a.cap + rounds * round - 1) / (rounds * round) * heads > 1024 && rounds * round < a.cap) ++rounds;
-    p.piece_len = static_cast<int>(rounds * round);
-    p.pieces = static_cast<int>((a.cap + p.piece_len - 1) / p.piece_len);
+    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min((a.cap + round - 1) / round, 512 / heads)));
     return p;
 }
 
 template <int HQ>
-hipError_t launch_attend(const AttnQ4Args& a, const AttnQ4Plan& p, const QueryImage& img, const Partials& part, hipStream_t s) {
+hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, int pieces, const Partials& part, hipStream_t s) {
     constexpr int kWaves = attn_q4_waves<HQ>;
-    const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
+    const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + 2048 + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
     static std::once_flag once;         // LDS beyond the default limit
     static hipError_t limit;
     std::call_once(once, [&] {
         limit = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_q4_kernel<HQ>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     });
     if (limit != hipSuccess) return limit;
-    klaunch(attn_q4_kernel<HQ>, dim3(p.pieces, a.NKV, a.B), dim3(kWaves * 64), lds, s, a, img, p.pieces, p.piece_len, part);
+    klaunch(attn_q4_kernel<HQ>, dim3(pieces, a.NKV, a.B), dim3(kWaves * 64), lds, s, a, freq, pieces, part);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || pieces == 1) return e;
+    klaunch(attn_q4_combine_kernel, dim3(a.NQ * 4, a.B), dim3(256), 0, s, a, kWaves, pieces, part);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t attn_q4_workspace_floats(const AttnQ4Args& a) {
-    const AttnQ4Plan p = attn_q4_plan(a);
-    const int64_t heads = static_cast<int64_t>(a.B) * a.NKV;
-    return heads * p.quads * (kQuadBytes / 4 + 4 * 4 * 2) + (p.pieces > 1 ? heads * p.pieces * a.GRP * (kHD + 2) : 0);
+    const int64_t pieces = attn_q4_plan(a).pieces;
+    return pieces > 1 ? static_cast<int64_t>(a.B) * a.NQ * pieces * (kHD + 2) : 4;
 }
 
 hipError_t launch_attn_q4(const AttnQ4Args& a, hipStream_t s) {
     const AttnQ4Plan p = attn_q4_plan(a);
-    const int64_t heads = static_cast<int64_t>(a.B) * a.NKV, rows = static_cast<int64_t>(a.B) * (a.NQ + 2 * a.NKV);
     RopeFreq freq{};
     for (int i = 0; i < a.ROT / 2; ++i) freq.f[i] = std::pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
-    QueryImage img;
-    img.digits = reinterpret_cast<uint8_t*>(a.ws);
-    img.factors = reinterpret_cast<float2*>(img.digits + heads * p.quads * kQuadBytes);
     Partials part;
-    part.o = reinterpret_cast<float*>(img.factors + heads * p.quads * 16);
-    part.ml = reinterpret_cast<float2*>(part.o + heads * p.pieces * a.GRP * kHD);
-    klaunch(attn_q4_prep_kernel, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, s, a, freq, img, p.quads);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    e = p.quads == 1   ? launch_attend<1>(a, p, img, part, s)
-        : p.quads == 2 ? launch_attend<2>(a, p, img, part, s)
-                       : launch_attend<4>(a, p, img, part, s);
-    if (e != hipSuccess || p.pieces == 1) return e;
-    klaunch(attn_q4_combine_kernel, dim3(a.NQ, a.B), dim3(256), 0, s, a, p.pieces, p.piece_len, part);
-    return hipGetLastError();
+    part.o = a.ws;
+    part.ml = reinterpret_cast<float2*>(a.ws + static_cast<int64_t>(a.B) * a.NQ * p.pieces * kHD);
+    return p.quads == 1   ? launch_attend<1>(a, freq, p.pieces, part, s)
+           : p.quads == 2 ? launch_attend<2>(a, freq, p.pieces, part, s)
+                          : launch_attend<4>(a, freq, p.pieces, part, s);
 }
 
 hipError_t launch_kv_q4(const KvQ4Args& a, bool store, hipStream_t s) {
