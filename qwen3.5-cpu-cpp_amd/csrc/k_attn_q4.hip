@@ -520,7 +520,7 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, int 
     const v4f g = reinterpret_cast<const v4f*>(a.qg + o * 2 * kHD + kHD)[quarter * 16 + d];
     float m = -INFINITY, l = 0.0f;
     v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kBatch = 4;           // requested together
+    constexpr int kBatch = 8;           // requested together
     for (int i0 = s; i0 < np; i0 += 16 * kBatch) {
         float2 ml[kBatch];
         v4f v[kBatch];
@@ -619,7 +619,7 @@ AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     AttnQ4Plan p{};
     p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
     const int64_t round = (p.quads > 2 ? attn_q4_waves<4> : attn_q4_waves<2>) * kTile, heads = static_cast<int64_t>(a.B) * a.NKV;
-    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min((a.cap + round - 1) / round, 512 / heads)));
+    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min((a.cap + round - 1) / round, 256 / heads)));
     return p;
 }
 
