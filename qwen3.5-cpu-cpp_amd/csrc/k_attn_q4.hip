@@ -206,9 +206,9 @@ struct Partials {
 // operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time)
 // in that order. The part of the least values, sum_t p_t least_t, is a sum a head and group.
 template <int HQ>
-constexpr int attn_q4_waves = HQ > 2 ? 4 : 8;  // with 16 heads a wave holds more than 256 registers
+constexpr int attn_q4_waves = 4;  // with 16 heads a wave holds more than 256 registers
 template <int HQ>
-__global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int pieces, Partials part) {
+__global__ __launch_bounds__(attn_q4_waves<HQ> * 64, HQ > 2 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int pieces, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int kWaves = attn_q4_waves<HQ>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
@@ -305,8 +305,13 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64) void attn_q4_kernel(AttnQ4A
 #pragma unroll
     for (int i = 0; i < kHeads; ++i)
         qx[i] = reinterpret_cast<const float4*>(a.qg + (static_cast<int64_t>(b) * a.NQ + hk * a.GRP + min(wave + i * kWaves, a.GRP - 1)) * 2 * kHD)[lane];
+    // (loads come back in order: what is used first is asked for first)
+    const int angle = min(static_cast<int>(threadIdx.x), kHD / 2 - 1);
+    const double f = freq.f[angle];
+    const int pos = a.pos[b];
+    asm volatile("" ::"v"(pos), "v"(f));
     if (!fresh) request();
-    for (int i = threadIdx.x; i < a.ROT / 2; i += kWaves * 64) sincos(static_cast<double>(a.pos[b]) * freq.f[i], &cs[128 + i], &cs[i]);
+    if (static_cast<int>(threadIdx.x) < a.ROT / 2) sincos(static_cast<double>(pos) * f, &cs[128 + angle], &cs[angle]);
     lds_barrier();
     double* row = reinterpret_cast<double*>(vbuf);  // before the values are there
     if (fresh) {
@@ -619,7 +624,7 @@ AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     AttnQ4Plan p{};
     p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
     const int64_t round = (p.quads > 2 ? attn_q4_waves<4> : attn_q4_waves<2>) * kTile, heads = static_cast<int64_t>(a.B) * a.NKV;
-    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min((a.cap + round - 1) / round, 256 / heads)));
+    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min((a.cap + round - 1) / round, 512 / heads)));
     return p;
 }
 
