@@ -1,6 +1,6 @@
 #pragma once
-// Device helpers of the 4-bit operators: fp16 scales, and fp32 values as whole multiples of a power of
-// two in three signed bytes, for exact products on the integer matrix cores.
+// Device helpers of the 4-bit operators: fp16 scales; fp32 values as whole multiples of a power of two in
+// three signed bytes, for exact products on the integer matrix cores; sums over a wave's lanes.
 #include "dev_common.hpp"
 
 namespace q35k {
@@ -37,5 +37,29 @@ __device__ __forceinline__ float from_digits(v4i d) {
 // Here the value exists: without it the compiler puts off what follows the products, whose sums (four
 // registers for one value) then outnumber the registers.
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
+
+// Sums of the lanes up to and with each: lanes 1, 2, 4, 8 before within a row of 16, then the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+    return static_cast<uint64_t>(moved<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32 | moved<CTRL, ROWS>(static_cast<uint32_t>(v));
+}
+template <typename U>
+__device__ __forceinline__ U wave_scan(U v) {
+    v += moved<0x111, 0xF>(v);
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);
+    v += moved<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int l) {
+    return static_cast<uint64_t>(lane_of(static_cast<uint32_t>(v >> 32), l)) << 32 | lane_of(static_cast<uint32_t>(v), l);
+}
 
 }  // namespace q35k

@@ -183,19 +183,65 @@ __device__ __forceinline__ v4i bytes_of(v2i w) {
 constexpr int kTile = 64;       // keys a wave takes at a time
 constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16;
 
-// Rows a piece: a sequence's rows in as many pieces as there are workgroups for its head, each as many rounds of
-// tiles for its waves as that takes.
-__device__ __forceinline__ int attn_q4_piece(int rows, int pieces, int waves) {
-    const int round = waves * kTile;
-    return ((rows + round - 1) / round + pieces - 1) / pieces * round;
+// A workgroup's share: a piece of one head's rows.
+struct Share {
+    int b, head, piece, pieces, first;  // of `pieces` of that head, the first one's workgroup being `first`
+    int rounds;                         // of tiles for all waves, a piece
+};
+constexpr int kMostShared = 512;        // sequences and workgroups up to which rows are shared out
+
+// The batch's rows shared out among `groups` workgroups: pieces of as many rounds as are needed for all to have
+// one, so that long sequences get many and none waits for another's. Every wave finds the same.
+__device__ __forceinline__ Share share_out(const AttnQ4Args& a, int groups, int w, int waves) {
+    constexpr int kEach = kMostShared / 64;
+    const int lane = threadIdx.x & 63, round = waves * kTile, blocks = (a.B + 63) / 64;
+    int rounds[kEach], total = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int b = i * 64 + lane, len = i < blocks && b < a.B ? a.len[b] : -1;
+        rounds[i] = len < 0 ? 0 : len < a.cap ? len / round + 1 : 1;  // one to say that nothing was appended
+        total += rounds[i];
+    }
+    const auto sum = [](int v) { return static_cast<int>(lane_of(wave_scan(static_cast<uint32_t>(v)), 63)); };
+    // whole rounds of all heads stay below 2^31: rows of a cache below 2^30, of a batch below 2^39 / 256
+    int r = max((sum(total) + groups / a.NKV - 1) / (groups / a.NKV), 1);
+    const auto pieces_of = [&](int i) { return (rounds[i] + r - 1) / r; };
+    for (;;) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (i < blocks) n += pieces_of(i);
+        if (sum(n) * a.NKV <= groups) break;
+        r += max(r / 8, 1);             // ends: with r the longest, every head has one
+    }
+    Share s{-1, 0, 0, 0, 0, r};
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (i >= blocks || s.b >= 0) break;
+        const int n = pieces_of(i) * a.NKV, upto = before + static_cast<int>(wave_scan(static_cast<uint32_t>(n)));
+        const uint64_t mine = __ballot(w < upto);
+        if (mine) {
+            const int l = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+            const int np = __builtin_amdgcn_readlane(n, l) / a.NKV, start = __builtin_amdgcn_readlane(upto, l) - np * a.NKV;
+            s.b = i * 64 + l;
+            s.head = (w - start) / np;
+            s.piece = (w - start) % np;
+            s.pieces = np;
+            s.first = start + s.head * np;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return s;
 }
 
 struct Partials {
-    float* o;                           // [B][NKV][pieces][GRP][HD]
-    float2* ml;                         // [B][NKV][pieces][GRP] (max, sum)
+    float* o;                           // [workgroups][GRP][HD]
+    float2* ml;                         // [workgroups][GRP] (max, sum)
+    int2* where;                        // [B][NKV] first workgroup, workgroups
 };
 
-// Eight waves (four with more than 8 heads) a piece of one cache's keys, tiles of 64 keys a wave, for all query heads of the kv head.
+// Four waves a piece of one cache's keys, tiles of 64 keys a wave, for all query heads of the kv head.
 //
 // Scores: a 16 x 16 x 64 integer product takes four heads as four times three digits (the fourth row is never
 // looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
@@ -205,24 +251,25 @@ struct Partials {
 // integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
 // operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time)
 // in that order. The part of the least values, sum_t p_t least_t, is a sum a head and group.
+constexpr int attn_q4_waves = 4;
 template <int HQ>
-constexpr int attn_q4_waves = 4;  // with 16 heads a wave holds more than 256 registers
-template <int HQ>
-__global__ __launch_bounds__(attn_q4_waves<HQ> * 64, HQ > 2 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int pieces, Partials part) {
+__global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int kWaves = attn_q4_waves<HQ>;
+    constexpr int kWaves = attn_q4_waves;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
-    const int piece = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-    const int len = a.len[b];
+    // every head whole, or the rows shared out
+    Share share{static_cast<int>(blockIdx.x) / a.NKV, static_cast<int>(blockIdx.x) % a.NKV, 0, 1, static_cast<int>(blockIdx.x), 0};
+    if (shared) share = share_out(a, shared, blockIdx.x, kWaves);
+    if (share.b < 0) return;            // no share left
+    const int b = share.b, hk = share.head, len = a.len[b];
     if (len < 0) return;
     if (len >= a.cap) {  // nothing was appended
-        if (piece == 0)
-            for (int i = threadIdx.x; i < a.GRP * kHD; i += kWaves * 64)
-                a.out[(static_cast<int64_t>(b) * a.NQ + hk * a.GRP) * kHD + i] = NAN;
+        for (int i = threadIdx.x; i < a.GRP * kHD; i += kWaves * 64) a.out[(static_cast<int64_t>(b) * a.NQ + hk * a.GRP) * kHD + i] = NAN;
+        if (shared && threadIdx.x == 0) part.where[b * a.NKV + hk] = make_int2(0, 1);
         return;
     }
-    const int rows = len + 1, piece_len = attn_q4_piece(rows, pieces, kWaves), first = piece * piece_len, end = min(rows, first + piece_len);
-    if (first >= rows) return;
+    const int rows = len + 1, piece_len = share.rounds * kWaves * kTile, first = share.piece * piece_len;
+    const int end = share.piece + 1 == share.pieces ? rows : first + piece_len;
     const int64_t bk = static_cast<int64_t>(b) * a.NKV + hk;
     const bool fresh = end == rows;     // the new row is this piece's
     // the piece's rows; offsets within it stay within 32 bits
@@ -465,6 +512,7 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64, HQ > 2 ? 1 : 2) void attn_q
             wave_sync();
         }
     }
+    if (shared && share.piece == 0 && threadIdx.x == 0) part.where[bk] = make_int2(share.first, share.pieces);
     // The waves' parts: each scaled to the largest maximum of all, then added.
     __syncthreads();
     float2* wml = reinterpret_cast<float2*>(lds);
@@ -498,13 +546,13 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64, HQ > 2 ? 1 : 2) void attn_q
         const float ref = m_all == -INFINITY ? 0.0f : m_all;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) l_all = fmaf(exp2_f(wml[w * HQ * 4 + h].x - ref), wml[w * HQ * 4 + h].y, l_all);
-        if (rows <= piece_len) {        // all there is
+        if (share.pieces == 1) {        // all there is
             const int64_t at = static_cast<int64_t>(b) * a.NQ + hk * a.GRP + h;
             const v4f g = reinterpret_cast<const v4f*>(a.qg + at * 2 * kHD + kHD)[d];
             reinterpret_cast<v4f*>(a.out + at * kHD)[d] = v4f{x[0] / l_all * sigmoid_f(g[0]), x[1] / l_all * sigmoid_f(g[1]),
                                                               x[2] / l_all * sigmoid_f(g[2]), x[3] / l_all * sigmoid_f(g[3])};
         } else {
-            const int64_t at = (bk * pieces + piece) * a.GRP + h;
+            const int64_t at = static_cast<int64_t>(blockIdx.x) * a.GRP + h;
             reinterpret_cast<v4f*>(part.o + at * kHD)[d] = x;
             if (d == 0) part.ml[at] = make_float2(m_all, l_all);
         }
@@ -513,15 +561,15 @@ __global__ __launch_bounds__(attn_q4_waves<HQ> * 64, HQ > 2 ? 1 : 2) void attn_q
 
 // The pieces' parts of a query head, and the gate: four workgroups a head, 64 dims each; sixteen threads of every
 // workgroup take four dims of every 16th piece.
-__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, int waves, int pieces, Partials part) {
+__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, Partials part) {
     __shared__ v4f ws[16][16];
     __shared__ float2 wml[16];
     const int d = threadIdx.x & 15, s = threadIdx.x >> 4, h = blockIdx.x >> 2, quarter = blockIdx.x & 3, b = blockIdx.y, hk = h / a.GRP;
-    const int len = a.len[b];
-    if (len < 0 || len >= a.cap) return;
-    const int piece_len = attn_q4_piece(len + 1, pieces, waves), np = len / piece_len + 1;
-    if (np == 1) return;                // written by the piece
-    const int64_t first = (static_cast<int64_t>(b) * a.NKV + hk) * pieces * a.GRP + h % a.GRP, o = static_cast<int64_t>(b) * a.NQ + h;
+    if (a.len[b] < 0) return;
+    const int2 where = part.where[static_cast<int64_t>(b) * a.NKV + hk];
+    const int np = where.y;
+    if (np == 1) return;                // written by its workgroup
+    const int64_t first = static_cast<int64_t>(where.x) * a.GRP + h % a.GRP, o = static_cast<int64_t>(b) * a.NQ + h;
     const v4f g = reinterpret_cast<const v4f*>(a.qg + o * 2 * kHD + kHD)[quarter * 16 + d];
     float m = -INFINITY, l = 0.0f;
     v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -617,20 +665,23 @@ __global__ __launch_bounds__(256) void kv_q4_kernel(KvQ4Args a) {
 
 namespace {
 
+// Workgroups: one a head where heads fill the chip or caches take one round of tiles; else 512, two a compute
+// unit, or as many as there can be rounds.
 struct AttnQ4Plan {
-    int quads, pieces;
+    int quads, groups, shared;
 };
 AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     AttnQ4Plan p{};
     p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
-    const int64_t round = (p.quads > 2 ? attn_q4_waves<4> : attn_q4_waves<2>) * kTile, heads = static_cast<int64_t>(a.B) * a.NKV;
-    p.pieces = static_cast<int>(std::max<int64_t>(1, std::min((a.cap + round - 1) / round, 512 / heads)));
+    const int64_t round = attn_q4_waves * kTile, heads = static_cast<int64_t>(a.B) * a.NKV, rounds = (a.cap + round - 1) / round;
+    p.groups = static_cast<int>(heads);
+    if (heads < kMostShared && rounds > 1) p.groups = p.shared = static_cast<int>(std::min<int64_t>(kMostShared / a.NKV, a.B * rounds) * a.NKV);
     return p;
 }
 
 template <int HQ>
-hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, int pieces, const Partials& part, hipStream_t s) {
-    constexpr int kWaves = attn_q4_waves<HQ>;
+hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4Plan& p, const Partials& part, hipStream_t s) {
+    constexpr int kWaves = attn_q4_waves;
     const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + 2048 + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
     static std::once_flag once;         // LDS beyond the default limit
     static hipError_t limit;
@@ -638,18 +689,18 @@ hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, int pieces, 
         limit = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_q4_kernel<HQ>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     });
     if (limit != hipSuccess) return limit;
-    klaunch(attn_q4_kernel<HQ>, dim3(pieces, a.NKV, a.B), dim3(kWaves * 64), lds, s, a, freq, pieces, part);
+    klaunch(attn_q4_kernel<HQ>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || pieces == 1) return e;
-    klaunch(attn_q4_combine_kernel, dim3(a.NQ * 4, a.B), dim3(256), 0, s, a, kWaves, pieces, part);
+    if (e != hipSuccess || !p.shared) return e;
+    klaunch(attn_q4_combine_kernel, dim3(a.NQ * 4, a.B), dim3(256), 0, s, a, part);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t attn_q4_workspace_floats(const AttnQ4Args& a) {
-    const int64_t pieces = attn_q4_plan(a).pieces;
-    return pieces > 1 ? static_cast<int64_t>(a.B) * a.NQ * pieces * (kHD + 2) : 4;
+    const AttnQ4Plan p = attn_q4_plan(a);
+    return p.shared ? static_cast<int64_t>(p.groups) * a.GRP * (kHD + 2) + 2ll * a.B * a.NKV : 4;
 }
 
 hipError_t launch_attn_q4(const AttnQ4Args& a, hipStream_t s) {
@@ -658,10 +709,11 @@ hipError_t launch_attn_q4(const AttnQ4Args& a, hipStream_t s) {
     for (int i = 0; i < a.ROT / 2; ++i) freq.f[i] = std::pow(a.theta, -static_cast<double>(2 * i) / a.ROT);
     Partials part;
     part.o = a.ws;
-    part.ml = reinterpret_cast<float2*>(a.ws + static_cast<int64_t>(a.B) * a.NQ * p.pieces * kHD);
-    return p.quads == 1   ? launch_attend<1>(a, freq, p.pieces, part, s)
-           : p.quads == 2 ? launch_attend<2>(a, freq, p.pieces, part, s)
-                          : launch_attend<4>(a, freq, p.pieces, part, s);
+    part.ml = reinterpret_cast<float2*>(a.ws + static_cast<int64_t>(p.groups) * a.GRP * kHD);
+    part.where = reinterpret_cast<int2*>(part.ml + static_cast<int64_t>(p.groups) * a.GRP);
+    return p.quads == 1   ? launch_attend<1>(a, freq, p, part, s)
+           : p.quads == 2 ? launch_attend<2>(a, freq, p, part, s)
+                          : launch_attend<4>(a, freq, p, part, s);
 }
 
 hipError_t launch_kv_q4(const KvQ4Args& a, bool store, hipStream_t s) {

@@ -13,7 +13,7 @@
 // with a row plans that, or sorts the candidates and finds the exact places. Rows of one slice take one
 // launch. Where the open bins hold more than kList candidates (thousands of equal logits), the places are
 // found by radix descent over the row.
-#include "dev_common.hpp"
+#include "dev_q4.hpp"
 #include "launch_q4.hpp"
 
 namespace q35k {
@@ -296,29 +296,6 @@ __device__ __forceinline__ uint64_t wave_top(uint64_t v) {
     const uint32_t hi = wave_max_u32(static_cast<uint32_t>(v >> 32));
     const uint32_t lo = wave_max_u32(static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
     return static_cast<uint64_t>(hi) << 32 | lo;
-}
-// Sums of the lanes up to and with each: lanes 1, 2, 4, 8 before within a row of 16, then the rows before.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t moved(uint32_t v) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t moved(uint64_t v) {
-    return static_cast<uint64_t>(moved<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32 | moved<CTRL, ROWS>(static_cast<uint32_t>(v));
-}
-template <typename U>
-__device__ __forceinline__ U wave_scan(U v) {
-    v += moved<0x111, 0xF>(v);
-    v += moved<0x112, 0xF>(v);
-    v += moved<0x114, 0xF>(v);
-    v += moved<0x118, 0xF>(v);
-    v += moved<0x142, 0xA>(v);
-    v += moved<0x143, 0xC>(v);
-    return v;
-}
-__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); }
-__device__ __forceinline__ uint64_t lane_of(uint64_t v, int l) {
-    return static_cast<uint64_t>(lane_of(static_cast<uint32_t>(v >> 32), l)) << 32 | lane_of(static_cast<uint32_t>(v), l);
 }
 // the sum of the threads before this one; `waves` has a place for each wave, one use between barriers
 template <typename U>
