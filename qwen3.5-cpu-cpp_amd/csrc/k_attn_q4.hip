@@ -181,7 +181,7 @@ __device__ __forceinline__ v4i bytes_of(v2i w) {
 
 
 constexpr int kTile = 64;       // keys a wave takes at a time
-constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16;
+constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16, kFreshBytes = kQ4RowBytes + 16;
 
 // A workgroup's share: a piece of one head's rows.
 struct Share {
@@ -283,7 +283,8 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
     uint8_t* qbuf = lds;
     float2* fbuf = reinterpret_cast<float2*>(lds + HQ * kQuadBytes);
     double* cs = reinterpret_cast<double*>(lds + HQ * (kQuadBytes + 128));
-    uint8_t* vbuf = lds + HQ * (kQuadBytes + 128) + 2048 + wave * (kVBytes + JB * kPBytes);
+    uint8_t* fresh_row = lds + HQ * (kQuadBytes + 128) + 2048;  // K's and V's: the codes and the steps
+    uint8_t* vbuf = fresh_row + 2 * kFreshBytes + wave * (kVBytes + JB * kPBytes);
     uint8_t* pbuf = vbuf + kVBytes;
 
     // A tile's keys, key and value steps, and value rows: whole tiles by constant places of a lane, the last one's
@@ -337,27 +338,23 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
 
     // nibble n of the transposed 16 keys: which key its place in the operand is
     const int spot = (n & 8) + (n & 1) * 4 + ((n & 7) >> 1), key = 16 * (spot & 3) + 4 * c + (spot >> 2);
-    // What does not depend on the new row is on its way while the queries are made.
     int t0 = wave * kTile;
-    const auto request = [&] {
-        if (t0 < count) {
-            load_k(t0);
-            load_v(t0);
-            load_vs(t0);
-        }
-    };
     constexpr int kHeads = (4 * HQ + kWaves - 1) / kWaves;  // query heads a wave makes
     float4 qx[kHeads];
     const float4 qw = reinterpret_cast<const float4*>(a.q_norm)[lane];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i)
         qx[i] = reinterpret_cast<const float4*>(a.qg + (static_cast<int64_t>(b) * a.NQ + hk * a.GRP + min(wave + i * kWaves, a.GRP - 1)) * 2 * kHD)[lane];
-    // (loads come back in order: what is used first is asked for first)
     const int angle = min(static_cast<int>(threadIdx.x), kHD / 2 - 1);
     const double f = freq.f[angle];
     const int pos = a.pos[b];
-    asm volatile("" ::"v"(pos), "v"(f));
-    if (!fresh) request();
+    __builtin_amdgcn_sched_barrier(0);  // loads come back in order: what is used first is asked for first
+    if (t0 < count) {                   // on its way while the queries are made
+        load_k(t0);
+        load_v(t0);
+        load_vs(t0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (static_cast<int>(threadIdx.x) < a.ROT / 2) sincos(static_cast<double>(pos) * f, &cs[128 + angle], &cs[angle]);
     lds_barrier();
     double* row = reinterpret_cast<double*>(vbuf);  // before the values are there
@@ -370,11 +367,14 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
             uint32_t scale;
             const uint32_t code = quantize4(x, scale);
             const int64_t at = bk * a.cap + len;
+            uint8_t* row = fresh_row + (is_k ? 0 : kFreshBytes);
+            reinterpret_cast<uint16_t*>(row)[lane] = static_cast<uint16_t>(code);
             reinterpret_cast<uint16_t*>(is_k ? a.k : a.v)[at * 64 + lane] = static_cast<uint16_t>(code);
-            if (n == 0) (is_k ? a.k_scale : a.v_scale)[at * 4 + c] = scale;
+            if (n == 0) {
+                reinterpret_cast<uint32_t*>(row + kQ4RowBytes)[c] = scale;
+                (is_k ? a.k_scale : a.v_scale)[at * 4 + c] = scale;
+            }
         }
-        __syncthreads();                // the row is where the tiles are read from
-        request();
     }
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
@@ -385,6 +385,20 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
     }
     lds_barrier();
     for (; t0 < count; t0 += kWaves * kTile) {
+        if (fresh && t0 + kTile >= count) {  // the new row, and its copies, from LDS: in the cache it may not be yet
+            const int last = count - 1 - t0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (16 * t + n < last) continue;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) k[t][g] = *reinterpret_cast<const v2i*>(fresh_row + 8 * c + 32 * g);
+                ks[t] = *reinterpret_cast<const v4i*>(fresh_row + kQ4RowBytes);
+                vs[t] = *reinterpret_cast<const v4i*>(fresh_row + kFreshBytes + kQ4RowBytes);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (8 * i + (lane >> 3) >= last) v[i] = *reinterpret_cast<const v4i*>(fresh_row + kFreshBytes + 16 * (lane & 7));
+        }
         float s[HQ][4];
 #pragma unroll
         for (int j = 0; j < HQ; ++j)
@@ -559,11 +573,12 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
     }
 }
 
-// The pieces' parts of a query head, and the gate: four workgroups a head, 64 dims each; sixteen threads of every
-// workgroup take four dims of every 16th piece.
-__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, Partials part) {
-    __shared__ v4f ws[16][16];
-    __shared__ float2 wml[16];
+// The pieces' parts of a query head, and the gate: four workgroups a head, 64 dims each, in which sixteen threads take
+// four dims each of every kSlots-th piece.
+template <int kSlots>
+__global__ __launch_bounds__(16 * kSlots) void attn_q4_combine_kernel(AttnQ4Args a, Partials part) {
+    __shared__ v4f ws[kSlots][16];
+    __shared__ float2 wml[kSlots];
     const int d = threadIdx.x & 15, s = threadIdx.x >> 4, h = blockIdx.x >> 2, quarter = blockIdx.x & 3, b = blockIdx.y, hk = h / a.GRP;
     if (a.len[b] < 0) return;
     const int2 where = part.where[static_cast<int64_t>(b) * a.NKV + hk];
@@ -574,18 +589,18 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, Part
     float m = -INFINITY, l = 0.0f;
     v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int kBatch = 8;           // requested together
-    for (int i0 = s; i0 < np; i0 += 16 * kBatch) {
+    for (int i0 = s; i0 < np; i0 += kSlots * kBatch) {
         float2 ml[kBatch];
         v4f v[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-            const int64_t at = first + static_cast<int64_t>(min(i0 + 16 * k, np - 1)) * a.GRP;
+            const int64_t at = first + static_cast<int64_t>(min(i0 + kSlots * k, np - 1)) * a.GRP;
             ml[k] = part.ml[at];
             v[k] = reinterpret_cast<const v4f*>(part.o + at * kHD)[quarter * 16 + d];
         }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-            if (i0 + 16 * k >= np) break;
+            if (i0 + kSlots * k >= np) break;
             const float mn = fmaxf(m, ml[k].x), ref = mn == -INFINITY ? 0.0f : mn, f = exp2_f(m - ref), e = exp2_f(ml[k].x - ref);
             m = mn;
             l = l * f + ml[k].y * e;
@@ -598,12 +613,12 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4Args a, Part
     if (s) return;
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, wml[i].x);
+    for (int i = 0; i < kSlots; ++i) top = fmaxf(top, wml[i].x);
     top = top == -INFINITY ? 0.0f : top;
     l = 0.0f;
     x = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
         const float f = exp2_f(wml[i].x - top);
         l = fmaf(wml[i].y, f, l);
         x += ws[i][d] * f;
@@ -682,7 +697,7 @@ AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
 template <int HQ>
 hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4Plan& p, const Partials& part, hipStream_t s) {
     constexpr int kWaves = attn_q4_waves;
-    const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + 2048 + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
+    const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + 2048 + 2 * kFreshBytes + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
     static std::once_flag once;         // LDS beyond the default limit
     static hipError_t limit;
     std::call_once(once, [&] {
@@ -692,7 +707,11 @@ hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4
     klaunch(attn_q4_kernel<HQ>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.shared) return e;
-    klaunch(attn_q4_combine_kernel, dim3(a.NQ * 4, a.B), dim3(256), 0, s, a, part);
+    // Workgroups of 512 where there is at most one for a compute unit (256 pieces of 16 heads: 7.0 us, with 256 9.3),
+    // else of 256 (40 sequences: 5.8 us, with 512 10.1).
+    const dim3 grid(a.NQ * 4, a.B);
+    if (static_cast<int64_t>(a.NQ) * 4 * a.B <= 256) klaunch(attn_q4_combine_kernel<32>, grid, dim3(512), 0, s, a, part);
+    else klaunch(attn_q4_combine_kernel<16>, grid, dim3(256), 0, s, a, part);
     return hipGetLastError();
 }
 
