@@ -187,6 +187,23 @@ q35_status q35_model_generate_greedy(q35_model *m, const int32_t *prompt, int32_
  * with `token`, each next one with the previous argmax. out has n_new ids (the argmax
  * after each step). All steps run back to back on the device with no host round trip. */
 q35_status q35_model_decode_greedy(q35_model *m, int32_t token, int32_t n_new, int32_t *out);
+/* A token drawn from the model's logits by q35_sample (below), in the settings of q35_sampling: of the last
+ * step, or of the last token of a prefill (Q35_ERR_RANGE before there was one). u in [0, 1). prob may be NULL.
+ * The first call makes device arrays of its own (one more device allocation, kept, and made again when the
+ * context has grown). */
+typedef struct q35_sampling {
+    float temperature;     /* 0: the first index of the maximum, as the greedy calls */
+    int32_t top_k;         /* 0: off */
+    float top_p;           /* 1: off */
+    float min_p;           /* 0: off */
+} q35_sampling;
+q35_status q35_model_sample(q35_model *m, const q35_sampling *how, float u, int32_t *token, float *prob);
+/* q35_model_decode_greedy with each token drawn: n_new steps, the first fed with `token`, each next one with the
+ * token drawn from the step before, u [n_new] on the host. out and prob (may be NULL) have n_new entries; an id is
+ * -1 where every logit is ruled out (NaN or -inf), and the next step takes id 0. All steps run back to back on the
+ * device with no host round trip. */
+q35_status q35_model_decode_sampled(q35_model *m, int32_t token, int32_t n_new, const q35_sampling *how, const float *u,
+                                    int32_t *out, float *prob);
 /* Whole-prompt forward (QwenForward::prefill, src/qwen_forward.cpp:154-206): starts from a
  * zero state, runs the chunked GDN and flash attention prefill and leaves the model state
  * (GDN state, conv window, KV rows, pos = n) as n decode steps would. logits_host receives

@@ -19,6 +19,11 @@
 namespace q35k {
 namespace {
 
+__device__ __forceinline__ void put_token(const SampleArgs& a, int b, int token) {
+    a.token[b] = token;
+    if (a.feed) a.feed[b] = max(token, 0);
+}
+
 constexpr int kThreads = 1024;
 
 // ordered bits of a logit: larger logits have larger keys, both zeros one, a NaN counts as -inf
@@ -215,7 +220,7 @@ __device__ void sample_by_descent(const SampleArgs& a, int b, uint32_t top, cons
         }
         before += __popcll(vote & ((1ull << (threadIdx.x & 63)) - 1));
         if (same && before == at.nth) {
-            a.token[b] = i;
+            put_token(a, b, i);
             if (a.prob) a.prob[b] = static_cast<float>(static_cast<double>(w(at.key)) / static_cast<double>(total));
         }
         seen += all;
@@ -369,7 +374,7 @@ __device__ bool plain_row(const SampleArgs& a, int b, float T, uint64_t top, boo
     const uint32_t key = static_cast<uint32_t>(top >> 32);
     if (T > 0.0f && key != kKeyNone) return false;
     if (writes && T >= 0.0f) {
-        a.token[b] = key == kKeyNone ? -1 : static_cast<int>(~static_cast<uint32_t>(top));
+        put_token(a, b, key == kKeyNone ? -1 : static_cast<int>(~static_cast<uint32_t>(top)));
         if (a.prob) a.prob[b] = key == kKeyNone ? 0.0f : 1.0f;
     }
     return true;
@@ -621,7 +626,7 @@ __device__ void settle(const SampleArgs& a, int b, const Question& q, int n, con
     }
     const uint32_t at = holder(drawn_place(q.u, total));
     if (lane == 0) {
-        a.token[b] = static_cast<int>(~static_cast<uint32_t>(sh.pick.list[at]));
+        put_token(a, b, static_cast<int>(~static_cast<uint32_t>(sh.pick.list[at])));
         if (a.prob) a.prob[b] = static_cast<float>(static_cast<double>(run(at + 1) - run(at)) / static_cast<double>(total));
     }
 }

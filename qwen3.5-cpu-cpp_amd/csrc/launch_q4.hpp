@@ -79,6 +79,7 @@ struct SampleArgs {
     int* token;
     float* prob;                        // may be null
     void* ws;
+    int* feed = nullptr;                // may be null: the token for a step to take, 0 where there is none
 };
 uint64_t sample_workspace_bytes(int B, int V);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t s);

@@ -29,6 +29,7 @@
 #include "../host/safetensors_loader.h"
 #include "../host/synth.h"
 #include "launch.hpp"
+#include "launch_q4.hpp"
 
 namespace {
 
@@ -133,6 +134,11 @@ struct q35_model {
     int pf_planned = 0;  // block size planned at creation (0: none)
     int pf_exact = 0;    // prefill GEMMs on three exact bf16 parts (no fp16 weight copies)
     int prefill_head = 0;  // prefill logits: 0 = the step's output head, 1 = the embedding
+
+    // sampling (one hipMalloc, made by the first call that draws): q35_sample's workspace, the settings,
+    // and room for max_context values of u and of the tokens' shares
+    uint8_t* sample_arena = nullptr;
+    int64_t sample_ctx = 0;  // positions it was made for
 
     bool use_graph = true;
     bool graph_valid = false;
@@ -568,6 +574,7 @@ void destroy(q35_model* m) {
     if (m->kv_arena) (void)hipFree(m->kv_arena);
     if (m->scratch) (void)hipFree(m->scratch);
     if (m->pf_arena) (void)hipFree(m->pf_arena);
+    if (m->sample_arena) (void)hipFree(m->sample_arena);
     if (m->stream) (void)hipStreamDestroy(m->stream);
     delete m;
 }
@@ -1467,6 +1474,113 @@ q35_status q35_model_decode_greedy(q35_model* m, int32_t token, int32_t n_new, i
     const q35_status st = run_greedy(m, token, n_new);
     if (st != Q35_OK) return st;
     HIPCHK(hipMemcpyAsync(out, m->ids_dev + p0, static_cast<size_t>(n_new) * 4, hipMemcpyDeviceToHost, m->stream));
+    HIPCHK(hipStreamSynchronize(m->stream));
+    return Q35_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// The model's row of logits for q35_sample, with its arrays in the sampling arena.
+struct Drawing {
+    q35k::SampleArgs a;
+    float *u, *prob;   // a place for each position
+    q35_sampling how;  // stays until the copy to the device has ended
+};
+
+q35_status prepare_drawing(q35_model* m, const q35_sampling& how, Drawing* out) {
+    const int V = m->d.vocab_size;
+    if (V > 1 << 22) return q35::fail(Q35_ERR_UNSUPPORTED, "drawing from %d logits", V);
+    if (!(how.temperature >= 0.0f)) return q35::fail(Q35_ERR_ARG, "temperature %g", static_cast<double>(how.temperature));
+    const size_t ws = align256(q35k::sample_workspace_bytes(1, V)), row = align256(static_cast<size_t>(m->max_ctx) * 4);
+    if (!m->sample_arena || m->sample_ctx != m->max_ctx) {
+        HIPCHK(hipStreamSynchronize(m->stream));
+        if (m->sample_arena) (void)hipFree(m->sample_arena);
+        m->sample_arena = nullptr;
+        void* p = nullptr;
+        HIPCHK(dev_alloc(&p, ws + 256 + 2 * row));
+        m->sample_arena = static_cast<uint8_t*>(p);
+        m->sample_ctx = m->max_ctx;
+    }
+    q35_sampling* set = reinterpret_cast<q35_sampling*>(m->sample_arena + ws);
+    out->u = reinterpret_cast<float*>(m->sample_arena + ws + 256);
+    out->prob = reinterpret_cast<float*>(m->sample_arena + ws + 256 + row);
+    out->how = how;
+    HIPCHK(hipMemcpyAsync(set, &out->how, sizeof(out->how), hipMemcpyHostToDevice, m->stream));
+    q35k::SampleArgs& a = out->a;
+    a.B = 1;
+    a.V = V;
+    a.ld = V;
+    a.logits = m->logits;
+    a.temperature = &set->temperature;
+    a.top_k = &set->top_k;
+    a.top_p = &set->top_p;
+    a.min_p = &set->min_p;
+    a.ws = m->sample_arena;
+    a.feed = m->token_dev;
+    return Q35_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+q35_status q35_model_sample(q35_model* m, const q35_sampling* how, float u, int32_t* token, float* prob) {
+    if (!m || !how || !token) return q35::fail(Q35_ERR_ARG, "null argument");
+    const q35_status nc = need_context(m);
+    if (nc != Q35_OK) return nc;
+    if (m->pos <= 0) return q35::fail(Q35_ERR_RANGE, "no step has left logits to draw from");
+    Drawing d{};
+    const q35_status st = prepare_drawing(m, *how, &d);
+    if (st != Q35_OK) return st;
+    HIPCHK(hipMemcpyAsync(d.u, &u, 4, hipMemcpyHostToDevice, m->stream));
+    d.a.u = d.u;
+    d.a.token = m->ids_dev + m->pos - 1;
+    d.a.prob = d.prob;
+    HIPCHK(q35k::launch_sample(d.a, m->stream));
+    HIPCHK(hipMemcpyAsync(token, d.a.token, 4, hipMemcpyDeviceToHost, m->stream));
+    if (prob) HIPCHK(hipMemcpyAsync(prob, d.prob, 4, hipMemcpyDeviceToHost, m->stream));
+    HIPCHK(hipStreamSynchronize(m->stream));
+    return Q35_OK;
+}
+
+q35_status q35_model_decode_sampled(q35_model* m, int32_t token, int32_t n_new, const q35_sampling* how, const float* u,
+                                    int32_t* out, float* prob) {
+    if (!m || !how || n_new < 0 || (n_new > 0 && (!out || !u))) return q35::fail(Q35_ERR_ARG, "bad argument");
+    if (n_new == 0) return Q35_OK;
+    const q35_status nc = need_context(m);
+    if (nc != Q35_OK) return nc;
+    if (token < 0 || token >= m->embed_rows || token >= m->d.vocab_size)
+        return q35::fail(Q35_ERR_RANGE, "token %d outside [0, %d)", token, m->d.vocab_size);
+    if (m->d.vocab_size > m->embed_rows)
+        return q35::fail(Q35_ERR_UNSUPPORTED, "%d logits of %lld embedding rows", m->d.vocab_size, (long long)m->embed_rows);
+    const int64_t p0 = m->pos;
+    if (p0 + n_new > m->max_ctx)
+        return q35::fail(Q35_ERR_RANGE, "position %lld + %d steps exceeds max_context %lld", (long long)p0, n_new,
+                         (long long)m->max_ctx);
+    Drawing d{};
+    q35_status st = prepare_drawing(m, *how, &d);
+    if (st != Q35_OK) return st;
+    *m->pinned_token = token;
+    HIPCHK(hipMemcpyAsync(m->token_dev, m->pinned_token, 4, hipMemcpyHostToDevice, m->stream));
+    HIPCHK(hipMemcpyAsync(d.u, u, static_cast<size_t>(n_new) * 4, hipMemcpyHostToDevice, m->stream));
+    for (int i = 0; i < n_new && st == Q35_OK; ++i) {
+        st = launch_one_step(m);
+        if (st == Q35_OK) st = collect_timing(m);
+        if (st != Q35_OK) break;
+        d.a.u = d.u + i;
+        d.a.token = m->ids_dev + p0 + i;
+        d.a.prob = d.prob + i;
+        const hipError_t e = q35k::launch_sample(d.a, m->stream);
+        if (e != hipSuccess) st = q35::fail(Q35_ERR_HIP, "drawing a token: %s", hipGetErrorString(e));
+    }
+    if (st != Q35_OK) {
+        (void)hipStreamSynchronize(m->stream);  // the copies from d and u have ended
+        return st;
+    }
+    HIPCHK(hipMemcpyAsync(out, m->ids_dev + p0, static_cast<size_t>(n_new) * 4, hipMemcpyDeviceToHost, m->stream));
+    if (prob) HIPCHK(hipMemcpyAsync(prob, d.prob, static_cast<size_t>(n_new) * 4, hipMemcpyDeviceToHost, m->stream));
     HIPCHK(hipStreamSynchronize(m->stream));
     return Q35_OK;
 }

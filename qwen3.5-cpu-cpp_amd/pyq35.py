@@ -145,6 +145,10 @@ class SampleArgs(C.Structure):
                                   "workspace")] + [("workspace_bytes", C.c_uint64)]
 
 
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built: run __graft_entry__.build() "
@@ -181,6 +185,8 @@ def _load():
         "q35_model_step": (S, [P, I32, P, P]),
         "q35_model_generate_greedy": (S, [P, P, I32, I32, P]),
         "q35_model_decode_greedy": (S, [P, I32, I32, P]),
+        "q35_model_sample": (S, [P, C.POINTER(Sampling), F, P, P]),
+        "q35_model_decode_sampled": (S, [P, I32, I32, C.POINTER(Sampling), P, P, P]),
         "q35_model_prefill": (S, [P, P, I32, P]),
         "q35_model_extend": (S, [P, P, I32, P, P]),
         "q35_model_set_prefill_block": (S, [P, I32]),
@@ -351,6 +357,21 @@ class Model:
         out = np.zeros(max(n_new, 1), np.int32)
         check(lib.q35_model_decode_greedy(self.h, int(token), n_new, ptr(out)))
         return out[:n_new]
+
+    def sample(self, u: float, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """A token drawn from the last logits by one uniform number, and its share."""
+        how = Sampling(temperature, top_k, top_p, min_p)
+        token, prob = C.c_int32(0), C.c_float(0)
+        check(lib.q35_model_sample(self.h, C.byref(how), u, C.addressof(token), C.addressof(prob)))
+        return token.value, prob.value
+
+    def decode_sampled(self, token: int, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """len(u) steps, each token drawn by one of the uniform numbers u: (ids, their shares)."""
+        how = Sampling(temperature, top_k, top_p, min_p)
+        u = np.ascontiguousarray(u, np.float32)
+        out, prob = np.zeros(max(len(u), 1), np.int32), np.zeros(max(len(u), 1), np.float32)
+        check(lib.q35_model_decode_sampled(self.h, int(token), len(u), C.byref(how), ptr(u), ptr(out), ptr(prob)))
+        return out[:len(u)], prob[:len(u)]
 
     @property
     def prefill_logits_width(self) -> int:
