@@ -1,6 +1,9 @@
 // Products with 4-bit weights and group scales: Y[m][n] = R[m][n] + sum_g s[n][g] sum_{k in g}
 // X[m][k] (c[n][k] - z[n][g]), and the kernels that make such weights. The layout of packed weights
 // is in launch_q4.hpp.
+#include <cstdlib>
+#include <cstdint>
+#include <cstdint>
 #include <mutex>
 #include <type_traits>
 
@@ -60,18 +63,20 @@ __device__ __forceinline__ int group_sum(int v) {
 template <int G, bool ZP>
 __host__ __device__ constexpr int meta_bytes(int R, int k) { return R * (k / G) * (ZP ? 16 : 4); }
 
-// Makes the image of k [k0, k0 + kn) (kn a multiple of 256) with the threads first, first + step, ..
+// Makes the image of k [k0, k0 + kn) (kn a multiple of 256). A wave keeps to one row.
 template <int G, bool ZP, int R>
 __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, int rows, int k0, int kn, uint8_t* img, uint8_t* meta,
-                                           int first, int step) {
-    const int per = kn / 8, count = rows * per;
+                                           int lane, int wave) {
+    constexpr int step = kThreads / R;
+    const int count = kn / 8, first = wave / R * 64 + lane, r = wave & (R - 1);
+    if (r >= rows) return;
     const bool wide = (ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(X) & 15) == 0;
     constexpr int kBatch = R == 1 ? 1 : 4;  // requested together
     for (int id0 = first; id0 < count; id0 += kBatch * step) {
         float x[kBatch][8];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
-            const int id = min(id0 + n * step, count - 1), r = R == 1 ? 0 : id / per, k = k0 + (R == 1 ? id : id % per) * 8;
+            const int k = k0 + min(id0 + n * step, count - 1) * 8;
             const float* src = X + r * ldx + k;
             if (wide && k + 8 <= K) {
                 const v4f a = reinterpret_cast<const v4f*>(src)[0], b = reinterpret_cast<const v4f*>(src)[1];
@@ -86,7 +91,7 @@ __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, i
         for (int n = 0; n < kBatch; ++n) {
             const int id = id0 + n * step;
             if (id >= count) break;     // 32 lanes are in or out together
-            const int r = R == 1 ? 0 : id / per, kk = (R == 1 ? id : id % per) * 8;
+            const int kk = id * 8;
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
@@ -256,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
             if (!one || !made) {
                 w = load(set, b0, its);
                 if (made) lds_barrier();
-                make_image<G, ZP, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, threadIdx.x, kThreads);
+                make_image<G, ZP, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, lane, wave);
                 made = true;
                 lds_barrier();
             }
@@ -294,6 +299,230 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
                 float y = 0.0f;
                 for (int i = 0; i < ks; ++i) y += red[((wave - part + i) * QN + q) * 64 + lane];
                 store(q, y);
+            }
+        lds_barrier();
+    }
+}
+
+// ---- the products of many rows
+// Sixteen rows of X against sixteen of weights, 32 k at a time, on the fp16 matrix cores. An entry of X times the power
+// of two that brings its group's largest to [2^14, 2^15) is hi + lo, two fp16 values, to 2^-22 of itself (or 2^-39 of
+// the largest); a code less its zero is an fp16 value; so products are exact, and their sums, of one group, are
+// in fp32. A code becomes fp16 as the last bits of 1024 + code, or of 1024 + 16 code. A group of 64 k costs a tile and 16 rows
+// some 32 instructions and four products; by digits, which are put together for every four rows, 67 and four. 4096 rows
+// of 8224 x 2048 take 350 us (394 TFLOP/s of products by X as it is, twice that of fp16 products); both
+// pipes are busy in turn. Small products are bound by what comes first, X's image, which every workgroup makes.
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+constexpr int kManyRows = 16, kManyBytes = 16 * 1024, kPair = 2, kManyDepth = 2;
+template <int G>
+__host__ __device__ constexpr int many_bytes() { return kManyBytes + 256 / G * kManyRows * 4; }
+
+// The image of a block of 256 k: [8 of 32 k][lo, hi][c] of 16 places of 16 bytes, a row's eight entries in the order in which a
+// word's codes come apart (0 2 4 6 1 3 5 7); then the groups' factors [group][16]. The rows' places are moved on by
+// many_turn, so that of the writers, who hold eights of one row, few meet in a bank; it is the same for c = 0 and 1,
+// and for 2 and 3, whose readers are served together.
+__device__ __forceinline__ int many_turn(int mi, int c) { return 2 * (mi & 3) + 8 * (c >> 1); }
+template <int G>
+__device__ __forceinline__ void make_many(const float* X, int64_t ldx, int K, int rows, int k0, int blocks, uint8_t* img, uint8_t* meta,
+                                          int lane, int wave) {
+    const int count = blocks * 32;
+    const bool wide = (ldx & 3) == 0 && (reinterpret_cast<uintptr_t>(X) & 15) == 0;
+    constexpr int kBatch = 4;           // requested together
+    for (int r = wave; r < rows; r += kWaves)
+        for (int id0 = lane; id0 < count; id0 += kBatch * 64) {
+            float x[kBatch][8];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const int k = k0 + min(id0 + n * 64, count - 1) * 8;
+                const float* src = X + r * ldx + k;
+                if (wide && k + 8 <= K) {
+                    const v4f a = reinterpret_cast<const v4f*>(src)[0], b = reinterpret_cast<const v4f*>(src)[1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[n][i] = a[i], x[n][4 + i] = b[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[n][i] = k + i < K ? src[i] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const int o = id0 + n * 64;
+                if (o >= count) break;  // 32 lanes are in or out together
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
+                top = group_max<G>(top);
+                const bool ok = top < 0x7f800000u && top != 0;
+                const int e = ok ? min(15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 100) : 0;
+                h8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    constexpr int kOrder[8] = {0, 2, 4, 6, 1, 3, 5, 7};
+                    const v2f y = {ok ? ldexpf(x[n][kOrder[i]], e) : 0.0f, ok ? ldexpf(x[n][kOrder[i + 1]], e) : 0.0f};
+                    const h2 a = __builtin_convertvector(y, h2);
+                    const v2f rest = {y[0] - static_cast<float>(a[0]), y[1] - static_cast<float>(a[1])};
+                    const h2 b = __builtin_convertvector(rest, h2);
+                    hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
+                }
+                const int b = o >> 5, w = o & 31;  // the block, the eight in it
+                const int mi = G == 32 ? w >> 2 : w >> 4 << 2 | (w >> 3 & 1) << 1 | (w & 1), c = G == 32 ? w & 3 : w >> 1 & 3;
+                uint8_t* at = img + b * kManyBytes + mi * 2048 + c * 256 + ((r + many_turn(mi, c)) & 15) * 16;
+                *reinterpret_cast<h8*>(at) = lo;
+                *reinterpret_cast<h8*>(at + 1024) = hi;
+                if (w % (G / 8) == 0)
+                    reinterpret_cast<float*>(meta)[(b * (256 / G) + w / (G / 8)) * kManyRows + r] = top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
+            }
+        }
+}
+
+// eight codes less their zero: zero1 = -(1024 + zero), zero16 = -(64 + zero), twice each
+__device__ __forceinline__ h8 less_zero(uint32_t w, h2 zero1, h2 zero16) {
+    const h2 sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    const uint32_t v = w >> 8;
+    const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) ^ 0x64086408u) + zero1;
+    const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00f000f0u) ^ 0x64806480u), sixteenth, zero16);
+    const h2 c = __builtin_bit_cast(h2, (v & 0x000f000fu) ^ 0x64086408u) + zero1;
+    const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & 0x00f000f0u) ^ 0x64806480u), sixteenth, zero16);
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A block of 256 k of two tiles. img: the block's image; place[mi % 4]: this lane's bytes in the part of 32 k.
+template <int G, bool ZP>
+__device__ __forceinline__ void multiply_many(const Unit<G, ZP> (&u)[kPair], const uint8_t* img, const uint8_t* meta, const int (&place)[4],
+                                              float (&acc)[kPair][4]) {
+    constexpr int kEach = G / 32;
+    h8 x[2][kEach][2];
+    v4f factor[2];
+    const auto load = [&](int g) {
+#pragma unroll
+        for (int m = 0; m < kEach; ++m)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                x[g & 1][m][p] = *reinterpret_cast<const h8*>(img + (g * kEach + m) * 2048 + p * 1024 + place[(g * kEach + m) & 3]);
+        factor[g & 1] = *reinterpret_cast<const v4f*>(meta + g * kManyRows * 4);
+    };
+    load(0);
+#pragma unroll
+    for (int g = 0; g < 256 / G; ++g) {
+        if (g + 1 < 256 / G) load(g + 1);
+        h8 w[kPair][kEach];
+        v4f d[kPair];
+#pragma unroll
+        for (int t = 0; t < kPair; ++t) {
+            h2 zero1 = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)}, zero16 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+            if constexpr (ZP) {
+                const _Float16 z = static_cast<_Float16>(static_cast<short>(-u[t].zero(g)));
+                const h2 zz = {z, z};
+                zero1 += zz, zero16 += zz;
+            }
+#pragma unroll
+            for (int m = 0; m < kEach; ++m) w[t][m] = less_zero(u[t].word(g * kEach + m), zero1, zero16);
+        }
+        // the two tiles' in turn: a product waits for the one before of its own
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int m = 0; m < kEach; ++m)
+#pragma unroll
+                for (int t = 0; t < kPair; ++t)
+                    d[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[g & 1][m][p], w[t][m], p || m ? d[t] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < kPair; ++t) {
+            const float sw = u[t].scale(g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] = fmaf(d[t][r], sw * factor[g & 1][r], acc[t][r]);
+        }
+#pragma unroll
+        for (int t = 0; t < kPair; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) pin(acc[t][r]);
+    }
+}
+
+// As q4_mul_kernel, a wave's share being two tiles.
+template <int G, bool ZP>
+__global__ __launch_bounds__(kThreads) void q4_mul_many_kernel(Q4MulArgs a, int most, int ks, int chunk) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr int kMeta = 256 / G * kManyRows * 4;
+    typedef Unit<G, ZP> U;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
+    const int r0 = blockIdx.y * most, rows = min(most, a.M - r0);
+    const int tiles = (a.N + 15) / 16, pairs = (tiles + 1) / 2, blocks = (a.K + 255) / 256, rt = kWaves / ks, part = wave & (ks - 1);
+    const int sets = (pairs + rt - 1) / rt;
+    uint8_t* meta = lds + kManyBytes * chunk;
+    float* red = reinterpret_cast<float*>(meta + kMeta * chunk);
+    // rows that are not there hold whatever, as do the sums over them
+    int place[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) place[i] = c * 256 + ((n + many_turn(i, c)) & 15) * 16;
+    const bool one = chunk >= blocks;   // one image serves all tiles
+    bool made = false;
+    for (int set = blockIdx.x; set < sets; set += gridDim.x) {
+        const int tile = (set * rt + wave / ks) * 2;
+        const uint8_t* w[kPair];
+#pragma unroll
+        for (int t = 0; t < kPair; ++t) w[t] = a.W + static_cast<int64_t>(min(tile + t, tiles - 1)) * blocks * U::kBytes;
+        float acc[kPair][4];
+#pragma unroll
+        for (int t = 0; t < kPair; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] = 0.0f;
+        for (int b0 = 0; b0 < blocks; b0 += chunk) {
+            const int bn = min(chunk, blocks - b0);
+            U u[kManyDepth][kPair];
+#pragma unroll
+            for (int i = 0; i < kManyDepth; ++i)
+                if (part + i * ks < bn) {
+#pragma unroll
+                    for (int t = 0; t < kPair; ++t) u[i][t].load(w[t] + (b0 + part + i * ks) * U::kBytes, lane);
+                }
+            if (!one || !made) {
+                if (made) lds_barrier();
+                make_many<G>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn, lds, meta, lane, wave);
+                made = true;
+                lds_barrier();
+            }
+            for (int b = part; b < bn; b += kManyDepth * ks) {
+#pragma unroll
+                for (int i = 0; i < kManyDepth; ++i) {
+                    const int at = b + i * ks;
+                    if (at < bn) {
+                        multiply_many<G, ZP>(u[i], lds + at * kManyBytes, meta + at * kMeta + c * 16, place, acc);
+                        if (at + kManyDepth * ks < bn) {
+#pragma unroll
+                            for (int t = 0; t < kPair; ++t) u[i][t].load(w[t] + (b0 + at + kManyDepth * ks) * U::kBytes, lane);
+                        }
+                    }
+                }
+            }
+        }
+        const auto store = [&](int t, int r, float y) {
+            const int row = 4 * c + r, col = (tile + t) * 16 + n;
+            if (row < rows && tile + t < tiles && col < a.N) {
+                const int64_t at = r0 + row;
+                a.Y[at * a.ldy + col] = y + (a.R ? a.R[at * a.ldr + col] : 0.0f);
+            }
+        };
+        if (ks == 1) {
+#pragma unroll
+            for (int t = 0; t < kPair; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) store(t, r, acc[t][r]);
+            continue;
+        }
+#pragma unroll
+        for (int t = 0; t < kPair; ++t) reinterpret_cast<v4f*>(red)[(wave * kPair + t) * 64 + lane] = v4f{acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < kPair; ++t)
+            if ((t & (ks - 1)) == part) {
+                v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < ks; ++i) y += reinterpret_cast<const v4f*>(red)[((wave - part + i) * kPair + t) * 64 + lane];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) store(t, r, y[r]);
             }
         lds_barrier();
     }
@@ -384,8 +613,9 @@ struct Q4Plan {
 };
 template <int G, bool ZP>
 void q4_fit(Q4Plan& p, int N, int K) {
-    const int blocks = q4_blocks(K), each = p.image * 768 + meta_bytes<G, ZP>(p.image, 256);
-    const int red = p.ks > 1 ? kWaves * ((p.image + 3) / 4) * 256 : 0;
+    const bool many = p.image == kManyRows;
+    const int blocks = q4_blocks(K), each = many ? many_bytes<G>() : p.image * 768 + meta_bytes<G, ZP>(p.image, 256);
+    const int red = p.ks > 1 ? kWaves * (many ? 4 * kPair : (p.image + 3) / 4) * 256 : 0;
     p.chunk = std::min(blocks, (160 * 1024 - red) / each);
     p.lds = each * p.chunk + red;
 }
@@ -396,6 +626,26 @@ Q4Plan q4_plan(int M, int N, int K) {
     // Blocks of four rows fill the chip sooner, of eight read and unpack the weights less often (64 x 2048 x
     // 2048 in fours 7.1 us, in eights 7.6; 48 x 8224 x 2048 18.1 and 17.4; 8 x 2048 x 2048 5.0 and 6.2).
     p.image = M == 1 ? 1 : tiles * ((M + 3) / 4) <= 2048 || M <= 4 ? 4 : 8;
+    // Sixteen rows on the fp16 cores where rows and tiles are many (48 x 8224 x 2048 13.8 us, by digits 17.9; 32 x 8224
+    // x 2048 13.1 and 16.6; 4096 x 8224 x 2048 350 and 428), else by digits, whose smaller images are made sooner (24 x
+    // 8224 x 2048 11.5 us, on the fp16 cores 12.0; 64 x 2048 x 2048 6.9 and 8.2; 16 x 151936 x 2048 45 and 47).
+    if (M > 16 && static_cast<int64_t>(tiles) * M >= 16384) {
+        p.image = kManyRows;
+        p.row_blocks = (M + p.image - 1) / p.image;
+        p.most = (M + p.row_blocks - 1) / p.row_blocks;
+        // Waves that share a pair of tiles: as many as make the rounds of a workgroup a compute unit, each of so many blocks
+        // of k and half a block's time for joining, least (48 x 8224 x 2048, two 13.8 us, one 18.7, four 16.2; 64
+        // x 8224 x 2048, four 17.9, two 19.0).
+        const int pairs = (tiles + 1) / 2, most_wgs = std::max(1, 256 / p.row_blocks);
+        int64_t best = INT64_MAX;
+        for (int ks = 1; ks <= kWaves && (ks == 1 || ks <= blocks); ks *= 2) {
+            const int sets = (pairs + kWaves / ks - 1) / (kWaves / ks), wgs = std::min(sets, most_wgs);
+            const int64_t cost = static_cast<int64_t>((sets + wgs - 1) / wgs) * (2 * ((blocks + ks - 1) / ks) + (ks > 1));
+            if (cost < best) best = cost, p.ks = ks, p.wgs = wgs;
+        }
+        q4_fit<G, ZP>(p, N, K);
+        return p;
+    }
     p.row_blocks = (M + p.image - 1) / p.image;
     p.most = (M + p.row_blocks - 1) / p.row_blocks;
     // Waves share a tile while there are not enough tiles: up to eight waves a compute unit, for one row up to 32
@@ -423,12 +673,25 @@ hipError_t launch_q4_form(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
 }
 
 template <int G, bool ZP>
+hipError_t launch_q4_many(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
+    static std::once_flag once;
+    static hipError_t limit;
+    std::call_once(once, [] {
+        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_many_kernel<G, ZP>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    });
+    if (limit != hipSuccess) return limit;
+    klaunch(q4_mul_many_kernel<G, ZP>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
+    return hipGetLastError();
+}
+
+template <int G, bool ZP>
 hipError_t launch_q4_plan(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
-    return p.image == 1 ? launch_q4_form<G, ZP, 1>(a, p, s) : p.image == 4 ? launch_q4_form<G, ZP, 4>(a, p, s) : launch_q4_form<G, ZP, 8>(a, p, s);
+    return p.image == kManyRows ? launch_q4_many<G, ZP>(a, p, s) : p.image == 1 ? launch_q4_form<G, ZP, 1>(a, p, s) : p.image == 4 ? launch_q4_form<G, ZP, 4>(a, p, s) : launch_q4_form<G, ZP, 8>(a, p, s);
 }
 
 }  // namespace
 
+// No form needs more than a place: X's images lie in LDS and waves that share a tile add up there.
 uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) { return 16; }
 
 hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s) {
