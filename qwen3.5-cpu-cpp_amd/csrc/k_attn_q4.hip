@@ -204,7 +204,11 @@ __device__ __forceinline__ v4i bytes_of(v2i w) {
     return v4i{w[0] & 0x0f0f0f0f, static_cast<int>(static_cast<uint32_t>(w[0]) >> 4 & 0x0f0f0f0fu), w[1] & 0x0f0f0f0f,
                static_cast<int>(static_cast<uint32_t>(w[1]) >> 4 & 0x0f0f0f0fu)};
 }
-
+// 16 times sixteen signed codes
+__device__ __forceinline__ v4i bytes_of_signed(v2i w) {
+    constexpr int kHigh = static_cast<int>(0xf0f0f0f0u);
+    return v4i{w[0] << 4 & kHigh, w[0] & kHigh, w[1] << 4 & kHigh, w[1] & kHigh};
+}
 
 constexpr int kTile = 64;       // keys a wave takes at a time
 constexpr int kVBytes = kTile * kQ4RowBytes, kPBytes = 4 * 4 * 4 * 3 * 16, kFreshBytes = kQ4RowBytes + 16;
@@ -273,10 +277,16 @@ struct Partials {
 // looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
 //   s = sum_g 2^-e (step_g sum_d i_d code_d + least_g sum_d i_d).
 // Weights: p = 2^(s - tile's largest) <= 1 is multiplied by its value row's step, which differs by group, and becomes
-// multiples of a 4190000th of the tile's largest such product: p step code summed over 64 keys is again one
+// multiples of a 4190000th of the tile's largest such product: p step (code - 8) summed over 64 keys is again one
 // integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
-// operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time)
-// in that order. The part of the least values, sum_t p_t least_t, is a sum a head and group.
+// operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time) in that
+// order. The rest, sum_t p_t (least_t + 8 step_t), is a sum a head and group. (By code - 8 both are means of values of
+// both signs: of 131072 rows the outputs are 6e-7 off, by code and least 3.2e-6.)
+//
+// The matrix cores do the products in passing; what a tile costs is some 1400 instructions around them (5.5k cycles of
+// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 38 MB, takes 31 us, of
+// which 24 are this kernel's: 1.4 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
+// a wave, 2 to join the waves. 40 sequences of up to 8192, 73 MB, take 38 us; 1 x 700 (8/2 heads) 15.
 constexpr int attn_q4_waves = 4;
 template <int HQ>
 __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
@@ -337,11 +347,11 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
             v[i] = *reinterpret_cast<const v4i*>(vt + (r * kQ4RowBytes + 16 * (lane & 7)));
         }
     };
-    // a row's eight 16-byte pieces lie in LDS in an order that spreads the rows over the banks
+    // a row's eight 16-byte pieces lie in LDS in an order that spreads the rows over the banks; its codes as code - 8
     const auto place_v = [&] {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<v4i*>(vbuf + (8 * i + (lane >> 3)) * kQ4RowBytes + 16 * ((lane & 7) ^ (lane >> 3))) = v[i];
+            *reinterpret_cast<v4i*>(vbuf + (8 * i + (lane >> 3)) * kQ4RowBytes + 16 * ((lane & 7) ^ (lane >> 3))) = v[i] ^ static_cast<int>(0x88888888u);
     };
     const auto load_vs = [&](int t0) {
         const uint8_t* st = VS + static_cast<int64_t>(t0) * 16;
@@ -489,7 +499,7 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     st[t] = step_of(vs[t][g]);
-                    le[t] = fmaf(st[t], 0.0f, least_of(vs[t][g]));  // NaN where the step is
+                    le[t] = fmaf(st[t], 8.0f, least_of(vs[t][g]));
                 }
 #pragma unroll
                 for (int j = j0; j < j0 + JB; ++j) {
@@ -502,7 +512,7 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
                     lo[j][g] = fmaf(lo[j][g], alpha[j], beta[j] * part_lo);
                     const float big = max16_abs(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
                     const float inv = big > 1e-30f ? 4190000.0f * __builtin_amdgcn_rcpf(big) : 0.0f;
-                    unit[j - j0][g] = beta[j] * big * (1.0f / 4190000.0f);
+                    unit[j - j0][g] = beta[j] * big * (0.0625f / 4190000.0f);
                     uint32_t y[4];
 #pragma unroll
                     for (int t = 0; t < 4; ++t)  // 1.5 2^23 + i: i in the low bits
@@ -536,7 +546,7 @@ __global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_ke
                     const int d = 4 * g + i;  // dims 16 d .. + 15
                     const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) v2i*>(
                         reinterpret_cast<uintptr_t>(vbuf + key * kQ4RowBytes + 16 * ((d >> 1) ^ (key & 7)) + 8 * (d & 1))));
-                    const v4i vb = bytes_of(w);
+                    const v4i vb = bytes_of_signed(w);
 #pragma unroll
                     for (int j = 0; j < JB; ++j) {
                         o[j0 + j][d] = fmaf(from_digits(__builtin_amdgcn_mfma_i32_16x16x64_i8(p[j], vb, v4i{0, 0, 0, 0}, 0, 0, 0)),
@@ -783,7 +793,7 @@ hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4
 
 int64_t attn_q4_workspace_floats(const AttnQ4Args& a) {
     const AttnQ4Plan p = attn_q4_plan(a);
-    return p.shared ? static_cast<int64_t>(p.groups) * a.GRP * (kHD + 2) + 2ll * a.B * a.NKV : 4;
+    return p.shared ? static_cast<int64_t>(p.groups) * a.GRP * (kHD + 2) + 2ll * a.B * a.NKV : 64;
 }
 
 hipError_t launch_attn_q4(const AttnQ4Args& a, hipStream_t s) {
