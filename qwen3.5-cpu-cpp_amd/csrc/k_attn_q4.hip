@@ -5,7 +5,6 @@
 // round((x - least) / step), all from 64-bit values rounded to fp32 and then fp16: a value next to the
 // border of two codes is on the same side for whoever computes it from the same inputs.
 #include <cmath>
-#include <mutex>
 
 #include "dev_q4.hpp"
 #include "launch_q4.hpp"
@@ -772,14 +771,11 @@ template <int HQ>
 hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4Plan& p, const Partials& part, hipStream_t s) {
     constexpr int kWaves = attn_q4_waves;
     const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + 2048 + 2 * kFreshBytes + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
-    static std::once_flag once;         // LDS beyond the default limit
-    static hipError_t limit;
-    std::call_once(once, [&] {
-        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_q4_kernel<HQ>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    });
-    if (limit != hipSuccess) return limit;
+    static AllowedLds allowed;
+    hipError_t e = allowed(reinterpret_cast<const void*>(attn_q4_kernel<HQ>), static_cast<int>(lds));
+    if (e != hipSuccess) return e;
     klaunch(attn_q4_kernel<HQ>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
-    hipError_t e = hipGetLastError();
+    e = hipGetLastError();
     if (e != hipSuccess || !p.shared) return e;
     // Workgroups of 512 where there is at most one for a compute unit (256 pieces of 16 heads: 7.0 us, with 256 9.3),
     // else of 256 (40 sequences: 5.8 us, with 512 10.1).

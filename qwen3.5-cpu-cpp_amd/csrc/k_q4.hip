@@ -4,7 +4,6 @@
 #include <cstdlib>
 #include <cstdint>
 #include <cstdint>
-#include <mutex>
 #include <type_traits>
 
 #include "dev_q4.hpp"
@@ -662,24 +661,18 @@ Q4Plan q4_plan(int M, int N, int K) {
 
 template <int G, bool ZP, int R>
 hipError_t launch_q4_form(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
-    static std::once_flag once;         // LDS beyond the default limit
-    static hipError_t limit;
-    std::call_once(once, [] {
-        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, R>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    });
-    if (limit != hipSuccess) return limit;
+    static AllowedLds allowed;
+    const hipError_t e = allowed(reinterpret_cast<const void*>(q4_mul_kernel<G, ZP, R>), 160 * 1024);
+    if (e != hipSuccess) return e;
     klaunch(q4_mul_kernel<G, ZP, R>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
     return hipGetLastError();
 }
 
 template <int G, bool ZP>
 hipError_t launch_q4_many(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
-    static std::once_flag once;
-    static hipError_t limit;
-    std::call_once(once, [] {
-        limit = hipFuncSetAttribute(reinterpret_cast<const void*>(q4_mul_many_kernel<G, ZP>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    });
-    if (limit != hipSuccess) return limit;
+    static AllowedLds allowed;
+    const hipError_t e = allowed(reinterpret_cast<const void*>(q4_mul_many_kernel<G, ZP>), 160 * 1024);
+    if (e != hipSuccess) return e;
     klaunch(q4_mul_many_kernel<G, ZP>, dim3(p.wgs, p.row_blocks), dim3(kThreads), p.lds, s, a, p.most, p.ks, p.chunk);
     return hipGetLastError();
 }

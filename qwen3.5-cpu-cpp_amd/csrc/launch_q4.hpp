@@ -2,6 +2,7 @@
 // Host-side launchers of the kernels of a decode step held in 4 bits: products with 4-bit weights
 // (k_q4.hip), attention over a cache of 4-bit rows (k_attn_q4.hip), sampling (k_sample.hip).
 // Shapes are checked by the callers (c_api_q4.hip, runtime.hip) before launching.
+#include <atomic>
 #include "launch.hpp"
 
 namespace q35k {
@@ -83,5 +84,18 @@ struct SampleArgs {
 };
 uint64_t sample_workspace_bytes(int B, int V);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t s);
+
+// Lets a kernel have more LDS than the default limit, once a device.
+struct AllowedLds {
+    std::atomic<uint64_t> devices{0};
+    hipError_t operator()(const void* kernel, int bytes) {
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e != hipSuccess || (dev < 64 && (devices.load() >> dev & 1))) return e;
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess && dev < 64) devices.fetch_or(uint64_t{1} << dev);
+        return e;
+    }
+};
 
 }  // namespace q35k
