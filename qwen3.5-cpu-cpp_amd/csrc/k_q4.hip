@@ -536,8 +536,8 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, 
     const int groups = (K + G - 1) / G, lane = threadIdx.x & 15;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
     if (id >= static_cast<int64_t>(N) * groups) return;  // whole groups of 16 lanes leave
-    const int64_t n = id / groups;
-    const int g = static_cast<int>(id % groups), k0 = g * G + lane * (G / 16), per = G / 16;
+    const int64_t n = static_cast<uint32_t>(id) / groups;  // below 2^27
+    const int g = static_cast<int>(static_cast<uint32_t>(id) % groups), k0 = g * G + lane * (G / 16), per = G / 16;
     const auto entry = [&](int k) -> float {
         if (k >= K) return 0.0f;
         if constexpr (BF16) return bf16_to_f32(static_cast<const uint16_t*>(W)[n * K + k]);
@@ -574,35 +574,41 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, 
     }
 }
 
-// a thread per dword of codes, then per scale
+// A workgroup a unit: a thread per dword of codes (four bytes of them in their order, in one load where rows allow it), then
+// per scale.
 __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int N, int K,
-                                                      int G, int unit, int64_t units, uint8_t* packed) {
+                                                      int G, int unit, uint8_t* packed) {
     const int words = unit / 4, blocks = (K + 255) / 256, groups = (K + G - 1) / G;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (id >= units * words) return;
-    const int64_t u = id / words;
-    const int w = static_cast<int>(id % words), t = static_cast<int>(u / blocks), s = static_cast<int>(u % blocks);
-    uint32_t out = 0;
-    if (w < 512) {
-        const int h = w / 256, l = w / 4 % 64, i = w & 3, c = l / 16;
-        const int n = t * 16 + (l & 15), k = s * 256 + 128 * h + (G == 32 ? 32 * i + 8 * c : 64 * (i / 2) + 16 * c + 8 * (i & 1));
-        if (n < N)
-            for (int j = 0; j < 8; ++j) {
-                if (k + j >= K) break;
-                const uint32_t b = codes[static_cast<int64_t>(n) * ((K + 1) / 2) + (k + j) / 2];
-                out |= (((j & 1 ? b >> 4 : b) & 15u) ^ 8u) << (8 * (j & 3) + (j & 4));
+    const int t = static_cast<int>(blockIdx.x / blocks), s = static_cast<int>(blockIdx.x % blocks);
+    const bool wide = (K & 7) == 0 && (reinterpret_cast<uintptr_t>(codes) & 3) == 0;
+    for (int w = threadIdx.x; w < words; w += 256) {
+        uint32_t out = 0;
+        if (w < 512) {
+            const int h = w / 256, l = w / 4 % 64, i = w & 3, c = l / 16;
+            const int n = t * 16 + (l & 15), k = s * 256 + 128 * h + (G == 32 ? 32 * i + 8 * c : 64 * (i / 2) + 16 * c + 8 * (i & 1));
+            const uint8_t* row = codes + static_cast<int64_t>(n) * ((K + 1) / 2);
+            if (n < N && k < K && wide) {
+                const uint32_t b = *reinterpret_cast<const uint32_t*>(row + k / 2), even = b & 0x0f0f0f0fu, odd = b >> 4 & 0x0f0f0f0fu;
+                out = (__builtin_amdgcn_perm(odd, even, 0x05010400u) | __builtin_amdgcn_perm(odd, even, 0x07030602u) << 4) ^ 0x88888888u;
+            } else if (n < N) {
+                for (int j = 0; j < 8; ++j) {
+                    if (k + j >= K) break;
+                    const uint32_t b = row[(k + j) / 2];
+                    out |= (((j & 1 ? b >> 4 : b) & 15u) ^ 8u) << (8 * (j & 3) + (j & 4));
+                }
             }
-    } else {
-        const int per = 256 / G, e = (w - 512) * (zeros ? 1 : 2);  // first scale of this dword
-        for (int j = 0; j < (zeros ? 1 : 2); ++j) {
-            const int n = t * 16 + (e + j) / per, g = s * per + (e + j) % per;
-            if (n >= N || g >= groups) continue;
-            const int64_t at = static_cast<int64_t>(n) * groups + g;
-            if (zeros) out = scales[at] | static_cast<uint32_t>((zeros[at] & 15) - 8) << 16;
-            else out |= static_cast<uint32_t>(scales[at]) << (16 * j);
+        } else {
+            const int per = 256 / G, e = (w - 512) * (zeros ? 1 : 2);  // first scale of this dword
+            for (int j = 0; j < (zeros ? 1 : 2); ++j) {
+                const int n = t * 16 + (e + j) / per, g = s * per + (e + j) % per;
+                if (n >= N || g >= groups) continue;
+                const int64_t at = static_cast<int64_t>(n) * groups + g;
+                if (zeros) out = scales[at] | static_cast<uint32_t>((zeros[at] & 15) - 8) << 16;
+                else out |= static_cast<uint32_t>(scales[at]) << (16 * j);
+            }
         }
+        reinterpret_cast<uint32_t*>(packed)[static_cast<int64_t>(blockIdx.x) * words + w] = out;
     }
-    reinterpret_cast<uint32_t*>(packed)[id] = out;
 }
 
 // Rows a block and its image's, waves a tile, workgroups a block of rows, blocks of 256 k an image holds.
@@ -710,9 +716,8 @@ hipError_t launch_q4_quantize(const void* W, bool bf16, int N, int K, int G, uin
 hipError_t launch_q4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int N, int K, int G, uint8_t* packed,
                           hipStream_t s) {
     const int unit = q4_unit_bytes(G, zeros != nullptr);
-    const int64_t units = static_cast<int64_t>(q4_tiles(N)) * q4_blocks(K), n = units * (unit / 4);
-    klaunch(q4_pack_kernel, dim3(static_cast<uint32_t>((n + 255) / 256)), dim3(256), 0, s, codes, scales, zeros, N, K, G, unit, units,
-            packed);
+    const int64_t units = static_cast<int64_t>(q4_tiles(N)) * q4_blocks(K);
+    klaunch(q4_pack_kernel, dim3(static_cast<uint32_t>(units)), dim3(256), 0, s, codes, scales, zeros, N, K, G, unit, packed);
     return hipGetLastError();
 }
 

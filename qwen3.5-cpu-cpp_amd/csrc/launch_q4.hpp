@@ -3,6 +3,8 @@
 // (k_q4.hip), attention over a cache of 4-bit rows (k_attn_q4.hip), sampling (k_sample.hip).
 // Shapes are checked by the callers (c_api_q4.hip, runtime.hip) before launching.
 #include <atomic>
+#include <cstdint>
+
 #include "launch.hpp"
 
 namespace q35k {
