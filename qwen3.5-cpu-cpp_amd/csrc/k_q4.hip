@@ -530,26 +530,39 @@ __global__ __launch_bounds__(kThreads) void q4_mul_many_kernel(Q4MulArgs a, int 
 // 16 lanes a group. Without zero points the entry of the largest magnitude becomes code 0, -8 steps:
 // scale = -entry / 8; with them the codes span [min(least, 0), max(largest, 0)]. Scales are rounded to
 // fp16 first and codes chosen by the rounded scale. A group with an infinity or a NaN gets scale NaN.
-template <bool BF16>
-__global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, int K, int G, uint8_t* codes, uint16_t* scales,
-                                                          uint8_t* zeros) {
+template <bool BF16, int G>
+__global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, int K, uint8_t* codes, uint16_t* scales, uint8_t* zeros) {
+    constexpr int per = G / 16, kBytes = per * (BF16 ? 2 : 4);
     const int groups = (K + G - 1) / G, lane = threadIdx.x & 15;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
     if (id >= static_cast<int64_t>(N) * groups) return;  // whole groups of 16 lanes leave
     const int64_t n = static_cast<uint32_t>(id) / groups;  // below 2^27
-    const int g = static_cast<int>(static_cast<uint32_t>(id) % groups), k0 = g * G + lane * (G / 16), per = G / 16;
-    const auto entry = [&](int k) -> float {
-        if (k >= K) return 0.0f;
-        if constexpr (BF16) return bf16_to_f32(static_cast<const uint16_t*>(W)[n * K + k]);
-        else return static_cast<const float*>(W)[n * K + k];
-    };
+    const int g = static_cast<int>(static_cast<uint32_t>(id) % groups), k0 = g * G + lane * per;
+    float x[per];
+    if (k0 + per <= K && K % per == 0 && reinterpret_cast<uintptr_t>(W) % kBytes == 0) {  // in one piece
+        struct alignas(kBytes < 16 ? kBytes : 16) Piece {
+            uint32_t w[kBytes / 4];
+        };
+        const Piece v = *reinterpret_cast<const Piece*>(static_cast<const uint8_t*>(W) + (n * K + k0) * (BF16 ? 2 : 4));
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            if constexpr (BF16) x[i] = i & 1 ? bf16_hi(v.w[i / 2]) : bf16_lo(v.w[i / 2]);
+            else x[i] = __uint_as_float(v.w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            if constexpr (BF16) x[i] = k0 + i < K ? bf16_to_f32(static_cast<const uint16_t*>(W)[n * K + k0 + i]) : 0.0f;
+            else x[i] = k0 + i < K ? static_cast<const float*>(W)[n * K + k0 + i] : 0.0f;
+        }
+    }
     float lo = 0.0f, hi = 0.0f;
     bool bad = false;
+#pragma unroll
     for (int i = 0; i < per; ++i) {
-        const float x = entry(k0 + i);
-        lo = fminf(lo, x);
-        hi = fmaxf(hi, x);
-        bad |= !(fabsf(x) < INFINITY);
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+        bad |= !(fabsf(x[i]) < INFINITY);
     }
     for (int d = 1; d < 16; d <<= 1) {
         lo = fminf(lo, __shfl_xor(lo, d, 16));
@@ -564,12 +577,14 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, 
         scales[id] = sb;
         if (zeros) zeros[id] = static_cast<uint8_t>(zero);
     }
+#pragma unroll
     for (int i = 0; i < per; i += 2) {
         uint32_t c[2];
+#pragma unroll
         for (int j = 0; j < 2; ++j)
             c[j] = k0 + i + j >= K ? 0u
                    : none ? static_cast<uint32_t>(zero)
-                          : static_cast<uint32_t>(fminf(fmaxf(rintf(entry(k0 + i + j) / s) + zero, 0.0f), 15.0f));
+                          : static_cast<uint32_t>(fminf(fmaxf(rintf(x[i + j] / s) + zero, 0.0f), 15.0f));
         if (k0 + i < K) codes[n * ((K + 1) / 2) + (k0 + i) / 2] = static_cast<uint8_t>(c[0] | c[1] << 4);
     }
 }
@@ -707,9 +722,12 @@ hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s) {
 
 hipError_t launch_q4_quantize(const void* W, bool bf16, int N, int K, int G, uint8_t* codes, uint16_t* scales, uint8_t* zeros,
                               hipStream_t s) {
-    const int64_t n = static_cast<int64_t>(N) * ((K + G - 1) / G);
-    klaunch(bf16 ? q4_quantize_kernel<true> : q4_quantize_kernel<false>, dim3(static_cast<uint32_t>((n + 15) / 16)), dim3(256), 0, s, W,
-            N, K, G, codes, scales, zeros);
+    const dim3 grid(static_cast<uint32_t>((static_cast<int64_t>(N) * ((K + G - 1) / G) + 15) / 16));
+    const auto go = [&](auto g) {
+        constexpr int kG = decltype(g)::value;
+        klaunch(bf16 ? q4_quantize_kernel<true, kG> : q4_quantize_kernel<false, kG>, grid, dim3(256), 0, s, W, N, K, codes, scales, zeros);
+    };
+    G == 32 ? go(std::integral_constant<int, 32>()) : G == 64 ? go(std::integral_constant<int, 64>()) : go(std::integral_constant<int, 128>());
     return hipGetLastError();
 }
 
