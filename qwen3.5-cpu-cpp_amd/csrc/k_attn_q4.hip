@@ -217,6 +217,7 @@ struct Share {
     int b, head, piece, pieces, first;  // of `pieces` of that head, the first one's workgroup being `first`
     int rounds;                         // of tiles for all waves, a piece
 };
+constexpr int kSharedWaves = 4;         // of a workgroup then
 constexpr int kMostShared = 512;        // sequences and workgroups up to which rows are shared out
 
 // The batch's rows shared out among `groups` workgroups: pieces of as many rounds as are needed for all to have
@@ -270,7 +271,7 @@ struct Partials {
     int2* where;                        // [B][NKV] first workgroup, workgroups
 };
 
-// Four waves a piece of one cache's keys, tiles of 64 keys a wave, for all query heads of the kv head.
+// Four waves (or eight) a piece of one cache's keys, tiles of 64 keys a wave, for all query heads of the kv head.
 //
 // Scores: a 16 x 16 x 64 integer product takes four heads as four times three digits (the fourth row is never
 // looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
@@ -286,15 +287,13 @@ struct Partials {
 // a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 38 MB, takes 31 us, of
 // which 24 are this kernel's: 1.4 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
 // a wave, 2 to join the waves. 40 sequences of up to 8192, 73 MB, take 38 us; 1 x 700 (8/2 heads) 15.
-constexpr int attn_q4_waves = 4;
-template <int HQ>
-__global__ __launch_bounds__(attn_q4_waves * 64, HQ > 2 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
+template <int HQ, int kWaves>
+__global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int kWaves = attn_q4_waves;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
     // every head whole, or the rows shared out
     Share share{static_cast<int>(blockIdx.x) / a.NKV, static_cast<int>(blockIdx.x) % a.NKV, 0, 1, static_cast<int>(blockIdx.x), 0};
-    if (shared) share = share_out(a, shared, blockIdx.x, kWaves);
+    if (kWaves == kSharedWaves && shared) share = share_out(a, shared, blockIdx.x, kWaves);
     if (share.b < 0) return;            // no share left
     const int b = share.b, hk = share.head, len = a.len[b];
     if (len < 0) return;
@@ -753,28 +752,32 @@ __global__ __launch_bounds__(256) void kv_q4_load_kernel(KvQ4Args a) {
 
 namespace {
 
-// Workgroups: one a head where heads fill the chip or caches take one round of tiles; else 512, two a compute
-// unit, or as many as there can be rounds.
 struct AttnQ4Plan {
-    int quads, groups, shared;
+    int quads, waves, groups, shared;
 };
 AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     AttnQ4Plan p{};
     p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
-    const int64_t round = attn_q4_waves * kTile, heads = static_cast<int64_t>(a.B) * a.NKV, rounds = (a.cap + round - 1) / round;
+    p.waves = kSharedWaves;
+    const int64_t round = kSharedWaves * kTile, heads = static_cast<int64_t>(a.B) * a.NKV, rounds = (a.cap + round - 1) / round;
     p.groups = static_cast<int>(heads);
-    if (heads < kMostShared && rounds > 1) p.groups = p.shared = static_cast<int>(std::min<int64_t>(kMostShared / a.NKV, a.B * rounds) * a.NKV);
+    if (heads >= kMostShared || rounds == 1) return p;  // a workgroup a head
+    // Of eight waves where that is one tile a wave (1 x 300, 8/2 heads 11.3 us, rows shared out 14.5; 40 x 512, 16/2 17.2
+    // and 20.3; 1 x 1024, 8/2 18.6 and 15.9), or two and heads are many (90 x 1024, 16/2 25.5 and 34.3; 40 x up
+    // to 1024 23.4 and 19.8), and their registers allow it.
+    if (p.quads <= 2 && (a.cap <= 8 * kTile || (a.cap <= 16 * kTile && heads >= 128))) p.waves = 8;
+    // Else rows are shared out: 512 workgroups, two a compute unit, or as many as there can be rounds.
+    else p.groups = p.shared = static_cast<int>(std::min<int64_t>(kMostShared / a.NKV, a.B * rounds) * a.NKV);
     return p;
 }
 
-template <int HQ>
+template <int HQ, int kWaves>
 hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4Plan& p, const Partials& part, hipStream_t s) {
-    constexpr int kWaves = attn_q4_waves;
     const uint32_t lds = std::max(HQ * (kQuadBytes + 128) + 2048 + 2 * kFreshBytes + kWaves * (kVBytes + std::min(HQ, 2) * kPBytes), kWaves * HQ * 4 * (kHD * 4 + 8));
     static AllowedLds allowed;
-    hipError_t e = allowed(reinterpret_cast<const void*>(attn_q4_kernel<HQ>), static_cast<int>(lds));
+    hipError_t e = allowed(reinterpret_cast<const void*>(attn_q4_kernel<HQ, kWaves>), static_cast<int>(lds));
     if (e != hipSuccess) return e;
-    klaunch(attn_q4_kernel<HQ>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
+    klaunch(attn_q4_kernel<HQ, kWaves>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
     e = hipGetLastError();
     if (e != hipSuccess || !p.shared) return e;
     // Workgroups of 512 where there is at most one for a compute unit (256 pieces of 16 heads: 7.0 us, with 256 9.3),
@@ -800,9 +803,10 @@ hipError_t launch_attn_q4(const AttnQ4Args& a, hipStream_t s) {
     part.o = a.ws;
     part.ml = reinterpret_cast<float2*>(a.ws + static_cast<int64_t>(p.groups) * a.GRP * kHD);
     part.where = reinterpret_cast<int2*>(part.ml + static_cast<int64_t>(p.groups) * a.GRP);
-    return p.quads == 1   ? launch_attend<1>(a, freq, p, part, s)
-           : p.quads == 2 ? launch_attend<2>(a, freq, p, part, s)
-                          : launch_attend<4>(a, freq, p, part, s);
+    if (p.waves == 8) return p.quads == 1 ? launch_attend<1, 8>(a, freq, p, part, s) : launch_attend<2, 8>(a, freq, p, part, s);
+    return p.quads == 1   ? launch_attend<1, 4>(a, freq, p, part, s)
+           : p.quads == 2 ? launch_attend<2, 4>(a, freq, p, part, s)
+                          : launch_attend<4, 4>(a, freq, p, part, s);
 }
 
 hipError_t launch_kv_q4(const KvQ4Args& a, bool store, hipStream_t s) {
