@@ -7,7 +7,7 @@
 // each other in mass are told apart down to 2^-S of the largest weight.
 //
 // A row is cut into slices, a workgroup each. The first launch finds the largest logit; the second counts
-// candidates and mass by bins of 1/128 of (max - l) / T, down to 36, below which weights are 0; the third
+// candidates and mass by bins of (max - l) / T, down to 36, below which weights are 0; the third
 // gathers the candidates of the bins that the borders and the draw may lie in (a border that is known to a bin
 // leaves the next one open to as much mass, so mostly to a bin as well). The workgroup that is done last
 // with a row plans that, or sorts the candidates and finds the exact places. A small top_k needs no counts: the largest
@@ -42,7 +42,11 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 constexpr uint32_t kKeyNone = 0x007fffffu;  // -inf
 constexpr uint32_t kKeyInf = 0xff800000u;   // +inf
 
-constexpr int kBins = 36 * 128;  // and one for what has no weight
+// Bins of 1/128 down to a depth of 12 and of 1/16 from there to 36: few borders are that deep, and what a launch clears,
+// adds to and reads back is less than half of it.
+constexpr int kFine = 12 * 128, kBins = kFine + 24 * 16;  // and one for what has no weight
+// a depth in 128ths as a place among them; larger ones have no smaller places
+__device__ __forceinline__ float place_of(float z) { return z < kFine ? z : fmaf(z, 0.125f, kFine * 0.875f); }
 
 // e^-z for 0 <= z < 36, to a unit in the last place or two: z = n ln 2 / 64 + r, |r| <= ln 2 / 128, so e^-z =
 // 2^-(n div 64) 2^-(n mod 64 / 64) e^-r, the second factor from a table and the last by five terms of its
@@ -85,11 +89,11 @@ struct Weigher {
         return (top - static_cast<double>(l)) * rt;
     }
     __device__ double depth(uint32_t key) const { return depth(of_key(key)); }
-    // The same in 128ths and fp32, for bins: whatever its rounding, larger logits have no larger ones, and all with
+    // The same in fp32, for bins: whatever its rounding, larger logits have no larger ones, and all with
     // weight are below kBins (a weight ends at 35.4).
     __device__ float place(float l) const {
         if (inf) return l == INFINITY ? 0.0f : INFINITY;
-        return l > -INFINITY ? fminf(top32 - l, 3.4e38f) * rt32 : INFINITY;
+        return l > -INFINITY ? place_of(fminf(top32 - l, 3.4e38f) * rt32) : INFINITY;
     }
     // the weight in 64 bits, of the largest
     __device__ double share(uint32_t key) const {
@@ -437,14 +441,14 @@ __device__ __forceinline__ void add_up(Work& sh) {
     __syncthreads();
 }
 
-// the bin that holds unit x of the mass (x below the total) or candidate x: 64 steps of 72 bins, then one by one
+// the bin that holds unit x of the mass (x below the total) or candidate x: 64 steps of kBins / 64 bins, then one by one
 template <bool BY_MASS>
 __device__ __forceinline__ int bin_of(uint64_t x, const Work& sh) {
     static_assert(kBins % 64 == 0 && kBins / 64 <= 128);
     const int lane = threadIdx.x & 63;
     const auto before = [&](int b) { return BY_MASS ? sh.bins.mass[b] : static_cast<uint64_t>(sh.bins.count[b]); };
     const int base = (__popcll(__ballot(before(lane * (kBins / 64)) <= x)) - 1) * (kBins / 64);
-    int n = __popcll(__ballot(before(base + lane) <= x));
+    int n = __popcll(__ballot(before(min(base + lane, kBins)) <= x));
     if (n == 64 && kBins / 64 > 64) n += __popcll(__ballot(lane < kBins / 64 - 64 && before(min(base + 64 + lane, kBins)) <= x));
     return base + n - 1;
 }
@@ -476,7 +480,8 @@ __device__ __forceinline__ void make_plan(const Question& q, Work& sh) {
         if (q.m > 0.0f) {
             // candidates next to the border are compared one by one
             const double z = q.m < 1.0f ? -log(static_cast<double>(q.m)) : 0.0;
-            l[2] = static_cast<int>(fmax(z - 1e-4, 0.0) * 128.0), h[2] = min(static_cast<int>((z + 1e-4) * 128.0), kBins - 1);
+            const auto bin = [](double depth) { return static_cast<int>(fminf(place_of(static_cast<float>(depth * 128.0)), kBins)); };
+            l[2] = bin(fmax(z - 1e-4, 0.0)), h[2] = min(bin(z + 1e-4), kBins - 1);
             if (l[2] < kBins) {
                 m_bin = l[2];
                 lo = min(lo, max(mass[l[2]], uint64_t{1})), hi = min(hi, mass[h[2] + 1]);
