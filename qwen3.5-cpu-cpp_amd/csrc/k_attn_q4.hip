@@ -291,9 +291,9 @@ struct Partials {
 // both signs: of 131072 rows the outputs are 6e-7 off, by code and least 3.2e-6.)
 //
 // The matrix cores do the products in passing; what a tile costs is some 1400 instructions around them (5.5k cycles of
-// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 38 MB, takes 31 us, of
-// which 24 are this kernel's: 1.4 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
-// a wave, 2 to join the waves. 40 sequences of up to 8192, 73 MB, take 38 us; 1 x 700 (8/2 heads) 15.
+// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 73 MB, takes 31 us, of
+// which 24 are this kernel's: 1 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
+// a wave, 2 to join the waves. 40 sequences of up to 8192, 94 MB, take 39 us; 1 x 700 (8/2 heads) 14.5.
 template <int HQ, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];

@@ -15,10 +15,10 @@
 // them and draws. Rows of one slice take one launch. Where the open bins hold more than kList candidates (thousands
 // of equal logits), the places are found by radix descent over the row.
 //
-// One row of 151936 with a top_k of 20 takes 16.5 us (by counts 22.5), 48 with settings of all kinds 45 us. The logits
-// are read two or three times, 29 MB of 48 rows in about 5 us each from the caches; the rest is one workgroup's
-// chain of steps at the end of each launch (settling 64 candidates takes 3.5 us, 2048 5) and, of many rows, the weights:
-// some 17 instructions in 64 bits each, and two additions in LDS.
+// One row of 151936 with a top_k of 20 takes 16.5 us (by counts 22.5), 48 with settings of all kinds 43 us. The logits
+// are read two or three times, 29 MB of 48 rows in about 5 us each; the rest is one workgroup's chain of steps at the end
+// of each launch (settling 64 candidates takes 3.5 us, 2048 5) and, of many rows, the weights: 12 instructions in
+// 64 bits each and an addition of 64 bits in LDS (together 6 us), and the listing of those in open bins (3 us).
 #include "dev_q4.hpp"
 #include "launch_q4.hpp"
 
@@ -48,29 +48,26 @@ constexpr int kFine = 12 * 128, kBins = kFine + 24 * 16;  // and one for what ha
 // a depth in 128ths as a place among them; larger ones have no smaller places
 __device__ __forceinline__ float place_of(float z) { return z < kFine ? z : fmaf(z, 0.125f, kFine * 0.875f); }
 
-// e^-z for 0 <= z < 36, to a unit in the last place or two: z = n ln 2 / 64 + r, |r| <= ln 2 / 128, so e^-z =
-// 2^-(n div 64) 2^-(n mod 64 / 64) e^-r, the second factor from a table and the last by five terms of its
-// series (the sixth is below 2^-54).
+// 2^(-y / 512) for 0 <= y < 2^15: y = n + f, |f| <= 1/2, so it is 2^-(n div 512) 2^-(n mod 512 / 512) 2^(-f / 512), the second
+// factor from a table and the last by four terms of its series (the fifth is below 2^-55).
 struct ExpTable {
-    double t[64];
+    double t[512];
     __device__ __forceinline__ void fill() {
-        if (threadIdx.x < 64) t[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+        if (threadIdx.x < 512) t[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 512.0);
     }
 };
-__device__ __forceinline__ double exp_minus(double z, const ExpTable& e) {
-    constexpr double kLn2 = 0.69314718055994530942;
-    // ln 2 / 64 to 33 bits, so that n times it is exact, and the rest of it
-    constexpr double kHigh = 0x1.62e42fefp-7, kLow = 0x1.473de6af278edp-40;
-    // n may be one off at a border: r is then that little larger
-    const int i = static_cast<int>(rintf(static_cast<float>(z) * static_cast<float>(64.0 / kLn2)));
-    const double n = i, r = fma(-n, kLow, fma(-n, kHigh, z));
-    double p = fma(r, -1.0 / 120.0, 1.0 / 24.0);
-    p = fma(-r, p, 1.0 / 6.0);
-    p = fma(-r, p, 0.5);
-    p = fma(-r, p, 1.0);
-    p = fma(-r, p, 1.0);
-    // 2^-(n div 64) straight into the exponent: results are above 2^-53
-    return __builtin_bit_cast(double, __builtin_bit_cast(int64_t, e.t[i & 63] * p) - (static_cast<int64_t>(i >> 6) << 52));
+constexpr double kLn2 = 0.69314718055994530942;
+__device__ __forceinline__ double exp2_minus(double y, const ExpTable& e) {
+    constexpr double kWhole = 0x1.8p52, kStep = kLn2 / 512.0;
+    const double m = y + kWhole, f = y - (m - kWhole);  // n in the last bits of m
+    const int n = static_cast<int>(__builtin_bit_cast(uint64_t, m));
+    double p = fma(f, kStep * kStep * kStep * kStep / 24.0, -kStep * kStep * kStep / 6.0);
+    p = fma(f, p, kStep * kStep / 2.0);
+    p = fma(f, p, -kStep);
+    p = fma(f, p, 1.0);
+    // 2^-(n div 512) straight into the exponent
+    const uint64_t r = __builtin_bit_cast(uint64_t, e.t[n & 511] * p);
+    return __builtin_bit_cast(double, r - (static_cast<uint64_t>(static_cast<uint32_t>(n >> 9) << 20) << 32));
 }
 
 constexpr float kLeastT = 1e-36f;  // below this the bins' arithmetic in fp32 would not do
@@ -81,9 +78,9 @@ struct Weigher {
     const ExpTable& table;
     bool inf;
     __device__ __forceinline__ Weigher(uint32_t key, float T, double unit_, const ExpTable& e)
-        : top(of_key(key)), rt(1.0 / static_cast<double>(T)), unit(unit_), top32(of_key(key)), rt32(static_cast<float>(128.0 * rt)), table(e),
-          inf(key == kKeyInf) {}
-    // (max - l) / T: infinite or a NaN where a candidate is ruled out
+        : top(of_key(key)), rt(512.0 / kLn2 / static_cast<double>(T)), unit(unit_), top32(of_key(key)),
+          rt32(static_cast<float>(128.0 / static_cast<double>(T))), table(e), inf(key == kKeyInf) {}
+    // (max - l) / T in units of ln 2 / 512: infinite or a NaN where a candidate is ruled out
     __device__ double depth(float l) const {
         if (inf) return l == INFINITY ? 0.0 : INFINITY;
         return (top - static_cast<double>(l)) * rt;
@@ -95,15 +92,17 @@ struct Weigher {
         if (inf) return l == INFINITY ? 0.0f : INFINITY;
         return l > -INFINITY ? place_of(fminf(top32 - l, 3.4e38f) * rt32) : INFINITY;
     }
+    static constexpr double kDeepest = 36.0 * 512.0 / kLn2;
     // the weight in 64 bits, of the largest
     __device__ double share(uint32_t key) const {
-        const double z = depth(key);
-        return z < 36.0 ? exp_minus(z, table) : 0.0;
+        const double y = depth(key);
+        return y < kDeepest ? exp2_minus(y, table) : 0.0;
     }
-    __device__ uint64_t units(double depth) const {
-        // rounded to a whole number by what 2^52 more leaves of it
-        return depth < 36.0 ? __builtin_bit_cast(uint64_t, fma(exp_minus(depth, table), unit, 0x1p52)) & 0xfffffffffffffull : 0;
+    // a whole number of units: rounded by what 2^52 more leaves of it
+    __device__ uint64_t units_within(double depth) const {
+        return __builtin_bit_cast(uint64_t, fma(exp2_minus(depth, table), unit, 0x1p52)) & 0xfffffffffffffull;
     }
+    __device__ uint64_t units(double depth) const { return depth < kDeepest ? units_within(depth) : 0; }
     __device__ uint64_t operator()(uint32_t key) const { return units(depth(key)); }
 };
 
@@ -416,7 +415,7 @@ __device__ __forceinline__ void count_slice(const float* x, int i, int e, const 
         if (!(z < kBins)) return;
         const int bin = static_cast<int>(z);
         if (counts) atomicAdd(&sh.bins.count[bin], 1u);
-        if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units(w.depth(l))));
+        if (masses) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[bin]), static_cast<unsigned long long>(w.units_within(w.depth(l))));
     });
 }
 
@@ -522,14 +521,14 @@ __device__ __forceinline__ void make_plan(const Question& q, Work& sh) {
 
 // Ids [i, e) of the open bins, to the workgroup's list; sh.listed counts on where it is full.
 __device__ __forceinline__ void gather(const float* x, int i, int e, const Weigher& w, const Plan& p, Work& sh) {
-    float lo[4], hi[4];
+    uint32_t lo[4], bins[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], hi[r] = p.hi[r] + 1;
+    for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], bins[r] = p.hi[r] + 1 - p.lo[r];
     each_logit(x, i, e, [&](float l, int j) {
-        const float z = w.place(l);
+        const uint32_t bin = static_cast<uint32_t>(w.place(l));  // the largest number where there is no weight
         bool in = false;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) in |= z >= lo[r] && z < hi[r];
+        for (int r = 0; r < 4; ++r) in |= bin - lo[r] < bins[r];
         if (in) {
             const uint32_t at = atomicAdd(&sh.listed, 1u);
             if (at < kList) sh.pick.list[at] = entry_of(key_of(l), j);
@@ -666,7 +665,7 @@ __device__ __forceinline__ void settle_wave(const SampleArgs& a, int b, const Qu
     if (lane < n) sh.pick.list[before] = mine;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    mine = sh.pick.list[min(lane, n - 1)];
+    mine = sh.pick.list[min(lane, max(n - 1, 0))];
     const uint32_t key = static_cast<uint32_t>(mine >> 32);
     const uint64_t sums = wave_scan(lane < n ? w(key) : uint64_t{0});
     const auto run = [&](int i) { return i ? lane_of(sums, i - 1) : uint64_t{0}; };  // of the first i
