@@ -79,7 +79,7 @@ struct Weigher {
     bool inf;
     __device__ __forceinline__ Weigher(uint32_t key, float T, double unit_, const ExpTable& e)
         : top(of_key(key)), rt(512.0 / kLn2 / static_cast<double>(T)), unit(unit_), top32(of_key(key)),
-          rt32(static_cast<float>(128.0 / static_cast<double>(T))), table(e), inf(key == kKeyInf) {}
+          rt32(static_cast<float>(rt * (kLn2 / 4.0))), table(e), inf(key == kKeyInf) {}
     // (max - l) / T in units of ln 2 / 512: infinite or a NaN where a candidate is ruled out
     __device__ double depth(float l) const {
         if (inf) return l == INFINITY ? 0.0 : INFINITY;
@@ -761,13 +761,12 @@ __device__ __forceinline__ bool plan_by_parts(const Question& q, uint32_t key, c
     if (wave == 0) {
 #pragma unroll
         for (int i = 1; i < kThreads / 64; ++i) key = max(key, sh.part[i][lane]);
-        int before = 0;
-        for (int i = 0; i < 64; ++i) {
-            const uint32_t other = lane_of(key, i);
-            before += other > key || (other == key && i < lane);
-        }
-        if (before == q.k - 1) {
-            const float z = w.place(of_key(key));
+        // the first bits of the k-th, bit by bit
+        uint32_t bound = 0;
+        for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
+            if (__popcll(__ballot(key >= (bound | bit))) >= q.k) bound |= bit;
+        if (lane == 0) {
+            const float z = w.place(of_key(bound));
             Plan& p = sh.plan;
             for (int r = 0; r < 4; ++r) p.lo[r] = 0, p.hi[r] = -1, p.mass[r] = 0, p.end[r] = 0;
             p.hi[0] = z < kBins ? static_cast<int>(z) : -1;
