@@ -15,7 +15,7 @@
 // them and draws. Rows of one slice take one launch. Where the open bins hold more than kList candidates (thousands
 // of equal logits), the places are found by radix descent over the row.
 //
-// One row of 151936 with a top_k of 20 takes 16.5 us (by counts 22.5), 48 with settings of all kinds 43 us. The logits
+// One row of 151936 with a top_k of 20 takes 15.5 us (by counts 22.5), 48 with settings of all kinds 43 us. The logits
 // are read two or three times, 29 MB of 48 rows in about 5 us each; the rest is one workgroup's chain of steps at the end
 // of each launch (settling 64 candidates takes 3.5 us, 2048 5) and, of many rows, the weights: 12 instructions in
 // 64 bits each and an addition of 64 bits in LDS (together 6 us), and the listing of those in open bins (3 us).
@@ -386,10 +386,11 @@ __device__ __forceinline__ uint64_t slice_top(const float* x, int i, int e, bool
     __syncthreads();
     return wave_top(waves[threadIdx.x & (kThreads / 64 - 1)]);
 }
-__device__ __forceinline__ uint64_t row_top(const uint64_t* tops, int slices) {
+// a lane's of the slices' tops; the row's is the wave_top of these
+__device__ __forceinline__ uint64_t lane_top(const uint64_t* tops, int slices) {
     uint64_t top = 0;
     for (int i = threadIdx.x & 63; i < slices; i += 64) top = max(top, tops[i]);
-    return wave_top(top);
+    return top;
 }
 
 // greedy and empty rows, and rows without a candidate: true if there is nothing more to do
@@ -783,24 +784,23 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, do
                                                                 Row* rows) {
     __shared__ Work sh;
     const int b = blockIdx.y, s = blockIdx.x;
+    // all that is read is asked for before the first of it is used (an empty row's may be anything)
     const float T = a.temperature[b];
-    if (!(T >= 0.0f)) return;
     const Question q(a, b);
+    uint64_t top = lane_top(tops + b * slices, slices);
+    uint32_t part_key = kKeyNone;       // this thread's of the parts
+    const uint32_t* own = parts + static_cast<int64_t>(b) * slices * kParts;
+    for (int i = threadIdx.x / kParts; i < slices; i += kThreads / kParts) part_key = max(part_key, own[i * kParts + (threadIdx.x & (kParts - 1))]);
     sh.exp.fill();
-    // this thread's keys of the parts, if they matter
-    uint32_t part_key = kKeyNone;
+    if (!(T >= 0.0f)) return;
     const bool by_parts = q.k > 0 && q.k <= kParts;
-    if (by_parts) {
-        const uint32_t* own = parts + static_cast<int64_t>(b) * slices * kParts;
-        for (int i = threadIdx.x / kParts; i < slices; i += kThreads / kParts) part_key = max(part_key, own[i * kParts + (threadIdx.x & (kParts - 1))]);
-    }
-    const uint64_t top = row_top(tops + b * slices, slices);
+    top = wave_top(top);
     if (plain_row(a, b, T, top, s == 0 && threadIdx.x == 0) || T < kLeastT) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
     __syncthreads();
     Row& r = rows[b];
     const int begin = slice_begin(a.V, slices, s), end = slice_begin(a.V, slices, s + 1);
-    // (one row of 151936, top_k 20: 16.5 us in all, by counts 22.5)
+    // (one row of 151936, top_k 20: 15.5 us in all, by counts 22.5)
     if (by_parts) {
         if (plan_by_parts(q, part_key, w, sh)) {
             const bool many = gather_and_settle(a, b, begin, end, slices, q, w, r, sh);
@@ -833,16 +833,19 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, do
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, double unit, int slices, const uint64_t* tops, Row* rows) {
     __shared__ Work sh;
     const int b = blockIdx.y, s = blockIdx.x;
-    const float T = a.temperature[b];
-    if (!(T >= 0.0f)) return;
-    const Question q(a, b);
     Row& r = rows[b];
     const uint32_t done = r.done;
     if (done == 1) return;
+    // all that is read is asked for before the first of it is used (an empty row's may be anything)
+    const float T = a.temperature[b];
+    const Question q(a, b);
+    const uint32_t plan = threadIdx.x < sizeof(Plan) / 4 ? reinterpret_cast<const uint32_t*>(&r.plan)[threadIdx.x] : 0;
+    uint64_t top = lane_top(tops + b * slices, slices);
     sh.exp.fill();
-    if (threadIdx.x < sizeof(Plan) / 4) reinterpret_cast<uint32_t*>(&sh.plan)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&r.plan)[threadIdx.x];
+    if (!(T >= 0.0f)) return;
+    if (threadIdx.x < sizeof(Plan) / 4) reinterpret_cast<uint32_t*>(&sh.plan)[threadIdx.x] = plan;
     if (threadIdx.x == 0) sh.listed = 0;
-    const uint64_t top = row_top(tops + b * slices, slices);
+    top = wave_top(top);
     if (plain_row(a, b, T, top, false)) return;
     const Weigher w(static_cast<uint32_t>(top >> 32), T, unit, sh.exp);
     __syncthreads();
