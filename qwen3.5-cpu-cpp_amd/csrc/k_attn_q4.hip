@@ -621,12 +621,14 @@ __global__ __launch_bounds__(16 * kSlots) void attn_q4_combine_kernel(AttnQ4Args
     __shared__ v4f ws[kSlots][16];
     __shared__ float2 wml[kSlots];
     const int d = threadIdx.x & 15, s = threadIdx.x >> 4, h = blockIdx.x >> 2, quarter = blockIdx.x & 3, b = blockIdx.y, hk = h / a.GRP;
-    if (a.len[b] < 0) return;
+    // asked for together (an empty place's may be anything)
+    const int len = a.len[b];
     const int2 where = part.where[static_cast<int64_t>(b) * a.NKV + hk];
-    const int np = where.y;
-    if (np == 1) return;                // written by its workgroup
-    const int64_t first = static_cast<int64_t>(where.x) * a.GRP + h % a.GRP, o = static_cast<int64_t>(b) * a.NQ + h;
+    const int64_t o = static_cast<int64_t>(b) * a.NQ + h;
     const v4f g = reinterpret_cast<const v4f*>(a.qg + o * 2 * kHD + kHD)[quarter * 16 + d];
+    const int np = where.y;
+    if (len < 0 || np == 1) return;     // one: written by its workgroup
+    const int64_t first = static_cast<int64_t>(where.x) * a.GRP + h % a.GRP;
     float m = -INFINITY, l = 0.0f;
     v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int kBatch = 8;           // requested together
