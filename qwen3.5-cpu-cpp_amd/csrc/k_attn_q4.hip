@@ -217,14 +217,13 @@ struct Share {
     int b, head, piece, pieces, first;  // of `pieces` of that head, the first one's workgroup being `first`
     int rounds;                         // of tiles for all waves, a piece
 };
-constexpr int kSharedWaves = 4;         // of a workgroup then
 constexpr int kMostShared = 512;        // sequences and workgroups up to which rows are shared out
 
 // The batch's rows shared out among `groups` workgroups: pieces of as many rounds as are needed for all to have
 // one, so that long sequences get many and none waits for another's. Every wave finds the same.
 __device__ __forceinline__ Share share_out(const AttnQ4Args& a, int groups, int w, int waves) {
     constexpr int kEach = kMostShared / 64;
-    if (a.B == 1) {                     // the same without the sums (1 x 131072 30.7 us, with them 32.1)
+    if (a.B == 1) {                     // the same without the sums (1 x 131072 30.7 us by workgroups of four waves, with them 32.1)
         const int len = a.len[0], all = len < 0 ? 0 : len < a.cap ? len / (waves * kTile) + 1 : 1, per = static_cast<uint32_t>(groups) / a.NKV;
         const int r = max(static_cast<int>((static_cast<uint32_t>(all) + per - 1) / per), 1), np = (static_cast<uint32_t>(all) + r - 1) / r;
         if (w >= np * a.NKV) return {-1, 0, 0, 0, 0, r};
@@ -291,16 +290,16 @@ struct Partials {
 // both signs: of 131072 rows the outputs are 6e-7 off, by code and least 3.2e-6.)
 //
 // The matrix cores do the products in passing; what a tile costs is some 1400 instructions around them (5.5k cycles of
-// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 73 MB, takes 31 us, of
+// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 73 MB, takes 29 us, of
 // which 24 are this kernel's: 1 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
-// a wave, 2 to join the waves. 40 sequences of up to 8192, 94 MB, take 39 us; 1 x 700 (8/2 heads) 14.5.
+// a wave, 2 to join the waves. 40 sequences of up to 8192, 94 MB, take 39 us; 1 x 700 (8/2 heads) 14.3.
 template <int HQ, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
     // every head whole, or the rows shared out
     Share share{static_cast<int>(blockIdx.x) / a.NKV, static_cast<int>(blockIdx.x) % a.NKV, 0, 1, static_cast<int>(blockIdx.x), 0};
-    if (kWaves == kSharedWaves && shared) share = share_out(a, shared, blockIdx.x, kWaves);
+    if (shared) share = share_out(a, shared, blockIdx.x, kWaves);
     if (share.b < 0) return;            // no share left
     const int b = share.b, hk = share.head, len = a.len[b];
     if (len < 0) return;
@@ -767,16 +766,25 @@ struct AttnQ4Plan {
 AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     AttnQ4Plan p{};
     p.quads = a.GRP <= 4 ? 1 : a.GRP <= 8 ? 2 : 4;
-    p.waves = kSharedWaves;
-    const int64_t round = kSharedWaves * kTile, heads = static_cast<int64_t>(a.B) * a.NKV, rounds = (a.cap + round - 1) / round;
+    p.waves = 4;
+    const int64_t heads = static_cast<int64_t>(a.B) * a.NKV;
     p.groups = static_cast<int>(heads);
-    if (heads >= kMostShared || rounds == 1) return p;  // a workgroup a head
-    // Of eight waves where that is one tile a wave (1 x 300, 8/2 heads 11.3 us, rows shared out 14.5; 40 x 512, 16/2 17.2
-    // and 20.3; 1 x 1024, 8/2 18.6 and 15.9), or two and heads are many (90 x 1024, 16/2 25.5 and 34.3; 40 x up
-    // to 1024 23.4 and 19.8), and their registers allow it.
-    if (p.quads <= 2 && (a.cap <= 8 * kTile || (a.cap <= 16 * kTile && heads >= 128))) p.waves = 8;
-    // Else rows are shared out: 512 workgroups, two a compute unit, or as many as there can be rounds.
-    else p.groups = p.shared = static_cast<int>(std::min<int64_t>(kMostShared / a.NKV, a.B * rounds) * a.NKV);
+    if (heads >= kMostShared || a.cap <= 4 * kTile) return p;  // a workgroup a head
+    const bool eight = p.quads <= 2;    // their registers allow it
+    // A workgroup a head of eight waves where that is one tile a wave (1 x 300, 8/2 heads 11.3 us, rows shared out 14.5;
+    // 40 x 512, 16/2 17.2 and 20.3; 1 x 1024, 8/2 18.6 and 15.9), or two and heads are many (90 x 1024, 16/2 25.5 and
+    // 34.3; 40 x up to 1024 23.4 and 19.8).
+    if (eight && (a.cap <= 8 * kTile || (a.cap <= 16 * kTile && heads >= 128))) {
+        p.waves = 8;
+        return p;
+    }
+    // Else rows are shared out: eight waves a compute unit, or as many workgroups as there can be rounds. Two
+    // workgroups of four waves, or one of eight, half as many to be merged, where sequences are few and one round of
+    // all of them may not do (1 x 131072, 16/2 30.1 us, by fours 32.3; 20 x up to 8192 29.1 and 30.3; 1 x 16384 20.5 and
+    // 18.4; 40 x up to 8192 45.7 and 40.4).
+    if (eight && heads <= 40 && heads * a.cap >= kMostShared * 4 * kTile) p.waves = 8;
+    const int64_t each = p.waves * kTile, most = kMostShared * 4 / p.waves;  // most >= heads: every head has a workgroup
+    p.groups = p.shared = static_cast<int>(std::min<int64_t>(most / a.NKV, a.B * ((a.cap + each - 1) / each)) * a.NKV);
     return p;
 }
 
@@ -789,8 +797,8 @@ hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4
     klaunch(attn_q4_kernel<HQ, kWaves>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
     e = hipGetLastError();
     if (e != hipSuccess || !p.shared) return e;
-    // Workgroups of 512 where there is at most one for a compute unit (256 pieces of 16 heads: 7.0 us, with 256 9.3),
-    // else of 256 (40 sequences: 5.8 us, with 512 10.1).
+    // Workgroups of 512 threads where there is at most one for a compute unit (256 pieces of 16 heads: 7.0 us, with 256
+    // threads 9.3), else of 256 (40 sequences: 5.8 us, with 512 10.1).
     const dim3 grid(a.NQ * 4, a.B);
     if (static_cast<int64_t>(a.NQ) * 4 * a.B <= 256) klaunch(attn_q4_combine_kernel<32>, grid, dim3(512), 0, s, a, part);
     else klaunch(attn_q4_combine_kernel<16>, grid, dim3(256), 0, s, a, part);
