@@ -630,7 +630,8 @@ q35_status q35_matmul_q4(const float *X, int64_t ldx, const void *packed, int32_
  *   out [batch][NQ][HD]
  * workspace (16-byte aligned): q35_attn_q4_workspace_bytes() bytes; that depends on the sizes, never on the
  * lengths. Results do not depend on the order in which workgroups run.
- * Requires HD == 256, NQ / NKV at most 16, an even rotary_dim, 16-byte aligned arrays. */
+ * What is written may overlap no other array. Requires HD == 256, NQ / NKV at most 16, an even rotary_dim, 16-byte
+ * aligned arrays. */
 typedef struct q35_attn_q4_args {
     int32_t batch, q_heads, kv_heads, head_dim, rotary_dim;
     int32_t reserved;
@@ -685,7 +686,8 @@ q35_status q35_kv_q4_load(const q35_kv_q4_args *args, q35_stream s);
  *   u (device) [batch]: in [0, 1) (values outside count as the nearest of it, a NaN as 0)
  *   token [batch]: the id, -1 where every candidate is ruled out
  *   prob [batch], may be NULL: the share of the token in the weight that is left (0 with token -1)
- * workspace (16-byte aligned): q35_sample_workspace_bytes() bytes. vocab is at most 2^22. */
+ * workspace (16-byte aligned): q35_sample_workspace_bytes() bytes. What is written may overlap no other array. vocab
+ * is at most 2^22. */
 typedef struct q35_sample_args {
     int32_t batch, vocab;
     int64_t ld_logits;

@@ -20,6 +20,20 @@ bool overlap(const void* p, uint64_t n, const void* q, uint64_t m) {
     return n && m && x < y + m && y < x + n;
 }
 
+// An array of a call. What is written may overlap nothing else (what is read may be the same array twice).
+struct Part {
+    const void* p;
+    uint64_t n;
+    bool out;
+};
+template <int N>
+bool written_overlaps(const Part (&part)[N]) {
+    for (int i = 0; i < N; ++i)
+        for (int j = i + 1; j < N; ++j)
+            if ((part[i].out || part[j].out) && overlap(part[i].p, part[i].n, part[j].p, part[j].n)) return true;
+    return false;
+}
+
 // The kernels run on the current device: a stream of another one is refused.
 q35_status check_stream(hipStream_t s, const char* who) {
     if (!s) return Q35_OK;
@@ -87,14 +101,10 @@ q35_status kv_q4(const q35_kv_q4_args* args, bool store, q35_stream s, const cha
         return q35::fail(Q35_ERR_ARG, "%s: caches must be 16-byte aligned", who);
     const uint64_t heads = static_cast<uint64_t>(g.batch) * g.kv_heads, n = heads * g.capacity;
     const uint64_t wide = (g.shared_rows ? g.kv_heads : heads) * g.rows_capacity * 256 * (g.kv_dtype ? 2 : 4);
-    // what is written may overlap nothing else (what is read may be the same array twice)
-    const struct { const void* p; uint64_t n; bool out; } part[] = {
-        {g.k_rows, wide, !store}, {g.v_rows, wide, !store}, {g.k, n * 128, store}, {g.v, n * 128, store},
-        {g.k_scale, n * 16, store}, {g.v_scale, n * 16, store}};
-    for (int i = 0; i < 6; ++i)
-        for (int j = i + 1; j < 6; ++j)
-            if ((part[i].out || part[j].out) && overlap(part[i].p, part[i].n, part[j].p, part[j].n))
-                return q35::fail(Q35_ERR_ARG, "%s: an output overlaps another array", who);
+    const uint64_t batch = g.batch * 4ull;
+    const Part part[] = {{g.k_rows, wide, !store}, {g.v_rows, wide, !store}, {g.k, n * 128, store}, {g.v, n * 128, store},
+                         {g.k_scale, n * 16, store}, {g.v_scale, n * 16, store}, {g.begin, g.begin ? batch : 0, false}, {g.end, batch, false}};
+    if (written_overlaps(part)) return q35::fail(Q35_ERR_ARG, "%s: an output overlaps another array", who);
     const q35_status st = check_stream(static_cast<hipStream_t>(s), who);
     if (st != Q35_OK) return st;
     q35k::KvQ4Args a{};
@@ -234,11 +244,13 @@ q35_status q35_attn_q4(const q35_attn_q4_args *args, q35_stream s) {
                           static_cast<const void*>(g.out), static_cast<const void*>(g.workspace)})
         if (!aligned(p, 16)) return q35::fail(Q35_ERR_ARG, "%s: rows, caches and workspace must be 16-byte aligned", who);
     const uint64_t n = static_cast<uint64_t>(g.batch) * g.kv_heads * g.capacity;
-    const struct { const void* p; uint64_t n; } part[] = {{g.k, n * 128}, {g.v, n * 128}, {g.k_scale, n * 16}, {g.v_scale, n * 16}};
-    for (int i = 0; i < 4; ++i)
-        for (int j = i + 1; j < 4; ++j)
-            if (overlap(part[i].p, part[i].n, part[j].p, part[j].n)) return q35::fail(Q35_ERR_ARG, "%s: caches overlap", who);
     const uint64_t need = static_cast<uint64_t>(q35k::attn_q4_workspace_floats(a)) * 4;
+    const uint64_t batch = g.batch * 4ull, row = 256 * batch;
+    const Part part[] = {{g.k, n * 128, true}, {g.v, n * 128, true}, {g.k_scale, n * 16, true}, {g.v_scale, n * 16, true},
+                         {g.out, row * g.q_heads, true}, {g.workspace, need, true}, {g.qg, row * g.q_heads * 2, false},
+                         {g.k_new, row * g.kv_heads, false}, {g.v_new, row * g.kv_heads, false}, {g.q_norm, 1024, false},
+                         {g.k_norm, 1024, false}, {g.len, batch, false}, {g.pos, batch, false}};
+    if (written_overlaps(part)) return q35::fail(Q35_ERR_ARG, "%s: an output overlaps another array", who);
     if (g.workspace_bytes < need)
         return q35::fail(Q35_ERR_ARG, "%s: workspace of %llu bytes, needs %llu", who,
                          static_cast<unsigned long long>(g.workspace_bytes), static_cast<unsigned long long>(need));
@@ -290,6 +302,12 @@ q35_status q35_sample(const q35_sample_args *args, q35_stream s) {
     if (g.workspace_bytes < need)
         return q35::fail(Q35_ERR_ARG, "%s: workspace of %llu bytes, needs %llu", who,
                          static_cast<unsigned long long>(g.workspace_bytes), static_cast<unsigned long long>(need));
+    const uint64_t batch = g.batch * 4ull;
+    const auto settings = [&](const void* p) { return Part{p, p ? batch : 0, false}; };
+    const Part part[] = {{g.logits, static_cast<uint64_t>((g.batch - 1) * g.ld_logits + g.vocab) * 4, false}, settings(g.temperature),
+                         settings(g.top_k), settings(g.top_p), settings(g.min_p), settings(g.u), {g.token, batch, true},
+                         {g.prob, g.prob ? batch : 0, true}, {g.workspace, need, true}};
+    if (written_overlaps(part)) return q35::fail(Q35_ERR_ARG, "%s: an output overlaps another array", who);
     st = check_stream(static_cast<hipStream_t>(s), who);
     if (st != Q35_OK) return st;
     q35k::SampleArgs a{};

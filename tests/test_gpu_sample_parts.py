@@ -1,13 +1,15 @@
 """q35_sample for a small top_k, whose candidates are found by the largest logits of parts of the row: orders in which the
 largest stand together, equal logits by the thousand, rows with fewer candidates than top_k, infinities, and
 lists next to what one wave settles."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import pyq35
 from batch_ref import Buffers, Graph
 from q4_ref import sample_args
-from test_gpu_sample import check, settings
+from test_gpu_sample import check, run, settings
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +115,26 @@ def test_graph(hip):
                 assert np.array_equal(first[0], bufs.get("token")) and np.array_equal(first[1], bufs.get("prob")) and (first[0] >= 0).all()
         finally:
             g.close()
+
+
+def test_two_calls_at_once(hip):
+    rng = np.random.default_rng(8)
+    B, V = 6, 60000
+    x = settings(B, rng, k=[0, 20, 300], t=[0.7, 1.5], p=[0.9, 1.0])
+    x["logits"] = rows(rng, B, V, "any")
+    y = dict(x, logits=rows(rng, B, V, "heap"), u=rng.random(B, dtype=np.float32))
+    want = [run(hip, x), run(hip, y)]
+    out = dict(token=np.zeros(B, np.int32), prob=np.zeros(B, np.float32))
+    with Buffers(hip, **x, **out) as p, Buffers(hip, **y, **out) as q:
+        s = [C.c_void_p(), C.c_void_p()]
+        for i in s:
+            hip._ck(hip.rt.hipStreamCreate(C.byref(i)), "hipStreamCreate")
+        a, b = sample_args(p, B, V, V), sample_args(q, B, V, V)
+        for _ in range(5):
+            pyq35.check(pyq35.lib.q35_sample(a, s[0]))
+            pyq35.check(pyq35.lib.q35_sample(b, s[1]))
+        hip.sync()
+        for d, w in ((p, want[0]), (q, want[1])):
+            assert np.array_equal(d.get("token"), w[0]) and np.array_equal(d.get("prob"), w[1])
+        for i in s:
+            hip._ck(hip.rt.hipStreamDestroy(i), "hipStreamDestroy")

@@ -156,3 +156,32 @@ def test_sample_null():
     assert status(lib.q35_sample, None, None) == ARG and lib.q35_sample_workspace_bytes(None) == 0
     need = lib.q35_sample_workspace_bytes(sample())
     assert need > 0 and status(lib.q35_sample, sample(workspace_bytes=need - 1), None) == ARG
+
+
+@pytest.mark.parametrize("out", ["k", "v", "k_scale", "v_scale", "out", "workspace"])
+@pytest.mark.parametrize("other", [n for n in ATTN])
+def test_attn_overlap(out, other):
+    """What is written shares a byte with another array's end, or ends where that begins."""
+    if out == other:
+        return
+    sizes = {"len": 12, "pos": 12, "qg": 3 * 8 * 2048, "k_new": 3 * 2 * 1024, "v_new": 3 * 2 * 1024, "q_norm": 1024, "k_norm": 1024,
+             "k": 600 * 128, "v": 600 * 128, "k_scale": 600 * 16, "v_scale": 600 * 16, "out": 3 * 8 * 1024}
+    if other != "workspace":
+        at = (sizes[other] - 1) // 16 * 16
+        assert status(lib.q35_attn_q4, attn(**{other: BASE, out: BASE + at}), None) == ARG
+    if out != "workspace":
+        at = sizes[out] - 16
+        assert status(lib.q35_attn_q4, attn(**{out: BASE, other: BASE + at}), None) == ARG
+
+
+@pytest.mark.parametrize("out", ["token", "prob", "workspace"])
+@pytest.mark.parametrize("other", SAMPLE)
+def test_sample_overlap(out, other):
+    if out == other:
+        return
+    if other != "workspace":
+        last = {"logits": 3000}.get(other, 3) * 4 - 4
+        at = last // 16 * 16 if out == "workspace" else last
+        assert status(lib.q35_sample, sample(**{other: BASE, out: BASE + at}), None) == ARG
+    if out != "workspace":
+        assert status(lib.q35_sample, sample(**{out: BASE, other: BASE}), None) == ARG
