@@ -139,8 +139,8 @@ __device__ __forceinline__ void wave_sync() {
 }
 // What the products read of a query head lies in LDS: the three digits of its row, by quads of heads: [quad][group
 // of 64 dims][c][head of the quad][digit] 16 bytes, the dims 16 c .. + 15 of the group in the order in which a
-// cache row's nibbles come apart (0 2 4 6 1 3 5 7 8 10 ..); and per head and group (2^-e, 2^-e times the sum of the
-// multiples), which the rows' least values are multiplied by.
+// cache row's nibbles come apart (0 2 4 6 1 3 5 7 8 10 ..); and per head and group (2^-e, which is the row's, and the
+// sum of the group's multiples, which the rows' least values are multiplied by).
 constexpr int kQuadBytes = 4 * 4 * 4 * 3 * 16;
 
 // A wave norms a row (lane l: dims 4 l .. + 3) and rotates it by the angles in cs (cosines, then sines from 128 on),
@@ -174,6 +174,8 @@ __device__ __forceinline__ void place_query(const double* x, int h, uint8_t* qbu
         top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
     }
     top = static_cast<uint32_t>(max16(static_cast<int>(top)));
+    const auto row_top = [&](int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(top), l)); };
+    top = max(max(row_top(0), row_top(16)), max(row_top(32), row_top(48)));
     const bool ok = top < 0x7f800000u && top != 0;
     const int e = ok ? multiple_exp(__uint_as_float(top)) : 0;
     int sum = 0;
@@ -194,7 +196,7 @@ __device__ __forceinline__ void place_query(const double* x, int h, uint8_t* qbu
     }
     if ((lane & 15) == 0) {
         const float s = top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
-        fbuf[h * 4 + g] = make_float2(s, s * static_cast<float>(sum));
+        fbuf[h * 4 + g] = make_float2(s, static_cast<float>(sum));
     }
 }
 
@@ -281,7 +283,7 @@ struct Partials {
 //
 // Scores: a 16 x 16 x 64 integer product takes four heads as four times three digits (the fourth row is never
 // looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
-//   s = sum_g 2^-e (step_g sum_d i_d code_d + least_g sum_d i_d).
+//   s = 2^-e sum_g (step_g sum_d i_d code_d + least_g sum_d i_d).
 // Weights: p = 2^(s - tile's largest) <= 1 is multiplied by its value row's step, which differs by group, and becomes
 // multiples of a 4190000th of the tile's largest such product: p step (code - 8) summed over 64 keys is again one
 // integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
@@ -447,11 +449,11 @@ __global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void att
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             v4i q[HQ];
-            float2 f[HQ];
+            float f[HQ];
 #pragma unroll
             for (int j = 0; j < HQ; ++j) {
                 q[j] = *reinterpret_cast<const v4i*>(qbuf + j * kQuadBytes + ((g * 4 + c) * 4 + (n >> 2)) * 48 + min(n & 3, 2) * 16);
-                f[j] = fbuf[(j * 4 + c) * 4 + g];
+                f[j] = fbuf[(j * 4 + c) * 4 + g].y;
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -461,7 +463,7 @@ __global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void att
 #pragma unroll
                 for (int j = 0; j < HQ; ++j) {
                     const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[j], kb, v4i{0, 0, 0, 0}, 0, 0, 0);
-                    s[j][t] = fmaf(from_digits(d), step * f[j].x, fmaf(least, f[j].y, s[j][t]));
+                    s[j][t] = fmaf(from_digits(d), step, fmaf(least, f[j], s[j][t]));
                     if constexpr (HQ > 2) pin(s[j][t]);
                 }
             }
@@ -469,6 +471,12 @@ __global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void att
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int j = 0; j < HQ; ++j) pin(s[j][t]);
+        }
+#pragma unroll
+        for (int j = 0; j < HQ; ++j) {
+            const float unit = fbuf[(j * 4 + c) * 4].x;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[j][t] *= unit;
         }
         const int next = t0 + kWaves * kTile;
         place_v();
