@@ -291,7 +291,7 @@ struct Partials {
 // order. The rest, sum_t p_t (least_t + 8 step_t), is a sum a head and group. (By code - 8 both are means of values of
 // both signs: of 131072 rows the outputs are 6e-7 off, by code and least 3.2e-6.)
 //
-// The matrix cores do the products in passing; what a tile costs is some 1400 instructions around them (5.5k cycles of
+// The matrix cores do the products in passing; what a tile costs is some 1200 instructions around them (5k cycles of
 // a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 73 MB, takes 29 us, of
 // which 24 are this kernel's: 1 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
 // a wave, 2 to join the waves. 40 sequences of up to 8192, 94 MB, take 39 us; 1 x 700 (8/2 heads) 14.3.
