@@ -188,7 +188,10 @@ q35_status q35_model_generate_greedy(q35_model *m, const int32_t *prompt, int32_
  * after each step). All steps run back to back on the device with no host round trip. */
 q35_status q35_model_decode_greedy(q35_model *m, int32_t token, int32_t n_new, int32_t *out);
 /* A token drawn from the model's logits by q35_sample (below), in the settings of q35_sampling: of the last
- * step, or of the last token of a prefill (Q35_ERR_RANGE before there was one). u in [0, 1). prob may be NULL.
+ * step, or of the last token of a prefill. Q35_ERR_RANGE where none of these was the last to give the model its
+ * state: before the first, and until the next after q35_model_reset, q35_model_set_position (to the position at
+ * hand as well), q35_model_write_gdn_state / _conv_state / _kv, q35_model_fill_synthetic and
+ * q35_model_reserve_context. u in [0, 1). prob may be NULL.
  * The first call makes device arrays of its own (one more device allocation, kept, and made again when the
  * context has grown). */
 typedef struct q35_sampling {

@@ -139,6 +139,7 @@ struct q35_model {
     // and room for max_context values of u and of the tokens' shares
     uint8_t* sample_arena = nullptr;
     int64_t sample_ctx = 0;  // positions it was made for
+    bool has_logits = false;  // `logits` are of the state at hand: a step or a prompt left them and nothing since took their place
 
     bool use_graph = true;
     bool graph_valid = false;
@@ -543,6 +544,7 @@ q35_status launch_steps(q35_model* m, int steps) {
         HIPCHK(hipGraphLaunch(steps == kGraphRun ? m->exec_run : m->exec, m->stream));
     }
     m->pos += steps;
+    m->has_logits = true;
     return Q35_OK;
 }
 
@@ -643,6 +645,7 @@ void release_context(q35_model* m) {
     m->kv_bytes = 0;
     m->scratch_bytes = 0;
     m->pos = 0;
+    m->has_logits = false;
 }
 
 // The KV cache and scratch arenas exist (a failed q35_model_reserve_context that could not
@@ -718,6 +721,7 @@ q35_status install_context(q35_model* m, int64_t max_ctx, void* kv, void* sc) {
     HIPCHK(q35k::launch_rope_table(m->rope_cs, max_ctx, rot_dims(d), d.rope_theta, m->stream));
     HIPCHK(hipStreamSynchronize(m->stream));
     m->pos = 0;
+    m->has_logits = false;
     m->budget.kv_cache_bytes = m->kv_bytes;
     m->budget.activation_bytes = m->scratch_bytes;
     return Q35_OK;
@@ -1307,6 +1311,7 @@ q35_status extend(q35_model* m, const int32_t* ids, int32_t n, float* logits_hos
     float* F = reinterpret_cast<float*>(m->pf_arena);
     const hipStream_t s = m->stream;
     const int64_t start = m->pos;
+    m->has_logits = false;
     for (int64_t r0 = 0; r0 < n; r0 += p.tb) {
         const int T = static_cast<int>(std::min<int64_t>(p.tb, n - r0));
         // the previous block's kernels read the ids buffer: order the upload after them
@@ -1331,6 +1336,7 @@ q35_status extend(q35_model* m, const int32_t* ids, int32_t n, float* logits_hos
     HIPCHK(q35k::launch_argmax(m->logits, d.vocab_size, m->argmax_part, m->token_dev, m->ids_dev, m->pos_dev, s));
     HIPCHK(hipStreamSynchronize(s));
     m->pos = start + n;
+    m->has_logits = true;
     return Q35_OK;
 }
 
@@ -1405,6 +1411,7 @@ q35_status q35_model_synchronize(q35_model* m) {
 q35_status q35_model_reset(q35_model* m) {
     const q35_status nc = need_context(m);
     if (nc != Q35_OK) return nc;
+    m->has_logits = false;
     HIPCHK(q35k::launch_fill_f32(m->state_arena, static_cast<int64_t>(m->state_bytes / 4), 0.0f, m->stream));
     HIPCHK(q35k::launch_fill_f32(m->kv_arena, static_cast<int64_t>(m->kv_bytes / 4), 0.0f, m->stream));
     HIPCHK(q35k::launch_set_int(m->pos_dev, 0, m->stream));
@@ -1530,7 +1537,7 @@ q35_status q35_model_sample(q35_model* m, const q35_sampling* how, float u, int3
     if (!m || !how || !token) return q35::fail(Q35_ERR_ARG, "null argument");
     const q35_status nc = need_context(m);
     if (nc != Q35_OK) return nc;
-    if (m->pos <= 0) return q35::fail(Q35_ERR_RANGE, "no step has left logits to draw from");
+    if (!m->has_logits) return q35::fail(Q35_ERR_RANGE, "no step has left logits of this state to draw from");
     Drawing d{};
     const q35_status st = prepare_drawing(m, *how, &d);
     if (st != Q35_OK) return st;
@@ -1683,6 +1690,7 @@ q35_status q35_model_read_gdn_state(q35_model* m, int32_t layer, float* host) {
 q35_status q35_model_write_gdn_state(q35_model* m, int32_t layer, const float* host) {
     if (!m || !host || layer < 0 || layer >= m->d.n_layers_gdn) return q35::fail(Q35_ERR_ARG, "bad argument");
     const size_t n = static_cast<size_t>(m->d.gdn_v_heads) * 128 * 128;
+    m->has_logits = false;
     HIPCHK(hipMemcpyAsync(m->gdn_state + layer * n, host, n * 4, hipMemcpyHostToDevice, m->stream));
     HIPCHK(hipStreamSynchronize(m->stream));
     return Q35_OK;
@@ -1706,6 +1714,7 @@ q35_status q35_model_write_conv_state(q35_model* m, int32_t layer, const float* 
     std::vector<float> ring(static_cast<size_t>(4 * conv), 0.0f);
     for (int64_t c = 0; c < conv; ++c)
         for (int k = 0; k < 3; ++k) ring[static_cast<size_t>(ring_slot(m->pos, k) * conv + c)] = host[c * 3 + k];
+    m->has_logits = false;
     HIPCHK(hipMemcpyAsync(m->conv_ring + layer * 4 * conv, ring.data(), ring.size() * 4, hipMemcpyHostToDevice,
                           m->stream));
     HIPCHK(hipStreamSynchronize(m->stream));
@@ -1745,6 +1754,7 @@ q35_status q35_model_write_kv(q35_model* m, int32_t layer, int64_t pos0, int64_t
     if (need_context(m) != Q35_OK) return Q35_ERR_RANGE;
     const int NKV = m->d.attn_kv_heads, HD = m->d.attn_head_dim, E = m->kv_elem;
     std::vector<uint16_t> tmp(m->kv_elem == 2 ? static_cast<size_t>(n) * NKV * HD : 0);
+    m->has_logits = false;
     for (int which = 0; which < 2; ++which) {
         const float* src = which == 0 ? k_host : v_host;
         if (!src) continue;
@@ -1766,6 +1776,7 @@ q35_status q35_model_write_kv(q35_model* m, int32_t layer, int64_t pos0, int64_t
 q35_status q35_model_set_position(q35_model* m, int64_t pos) {
     if (!m || pos < 0 || pos > m->max_ctx) return q35::fail(Q35_ERR_RANGE, "bad position");
     if (need_context(m) != Q35_OK) return Q35_ERR_RANGE;
+    m->has_logits = false;
     HIPCHK(q35k::launch_set_int(m->pos_dev, static_cast<int>(pos), m->stream));
     HIPCHK(hipStreamSynchronize(m->stream));
     m->pos = pos;
@@ -1775,6 +1786,7 @@ q35_status q35_model_set_position(q35_model* m, int64_t pos) {
 q35_status q35_model_fill_synthetic(q35_model* m, int64_t pos, uint64_t seed, float state_std) {
     if (!m || pos < 0 || pos > m->max_ctx) return q35::fail(Q35_ERR_RANGE, "bad position");
     if (need_context(m) != Q35_OK) return Q35_ERR_RANGE;
+    m->has_logits = false;
     const int NKV = m->d.attn_kv_heads, HD = m->d.attn_head_dim;
     for (int l = 0; l < m->d.n_layers_attn; ++l)
         for (int which = 0; which < 2; ++which)
