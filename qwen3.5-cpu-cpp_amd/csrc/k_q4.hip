@@ -1,8 +1,6 @@
 // Products with 4-bit weights and group scales: Y[m][n] = R[m][n] + sum_g s[n][g] sum_{k in g}
 // X[m][k] (c[n][k] - z[n][g]), and the kernels that make such weights. The layout of packed weights
 // is in launch_q4.hpp.
-#include <cstdlib>
-#include <cstdint>
 #include <cstdint>
 #include <type_traits>
 
@@ -14,31 +12,16 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = 8;
 
-// ---- rows of X as whole numbers
-// A group of a row's entries becomes multiples of a power of two, each three signed bytes: integer products
-// with 4-bit codes are exact.
-struct Digits {
-    uint32_t d[3][2];                   // eight entries: plane, four bytes each
-};
-// the multiples of eight entries whose group's largest magnitude has the bits `top`, and 2^-e / 16 (codes are
-// multiplied as 16 times themselves); NaN for a group with an infinity or a NaN
-__device__ __forceinline__ Digits digits8(const float* x, uint32_t top, float& scale) {
-    const float m = __uint_as_float(top);
-    const int e = multiple_exp(m);
-    const bool ok = top < 0x7f800000u && top != 0;
-    scale = top >= 0x7f800000u ? NAN : ldexpf(0.0625f, ok ? -e : 0);
-    uint32_t y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = signed_digits(ok ? static_cast<int>(rintf(ldexpf(x[i], e))) : 0);
-    Digits r;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        r.d[0][h] = plane<0>(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
-        r.d[1][h] = plane<1>(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
-        r.d[2][h] = plane<2>(y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
-    }
-    return r;
-}
+// ---- rows of X as pairs of fp16 values
+// An entry of X times the power of two that brings its group's largest to [2^14, 2^15) is hi + lo, two fp16 values, to 2^-22
+// of itself (or 2^-39 of the largest); a code less its zero is an fp16 value; so products on the fp16 matrix cores are
+// exact, and their sums, of one group, are in fp32. An entry keeps its bits beside one that is far larger: where one a group
+// of 64 is 10^4 times the others and its weights are 0, outputs of 2048 k are off by 4e-8 of their norm. (As 24-bit multiples
+// of a unit of the largest, for the integer cores, by 7e-4, for a tenth less time where weights are all there is to read.)
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
 template <int G>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {  // over the G / 8 lanes that hold a group
     v = max(v, static_cast<uint32_t>(dpp_i<0xB1>(static_cast<int>(v))));
@@ -47,23 +30,71 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {  // over the G / 8 l
     if constexpr (G >= 128) v = max(v, static_cast<uint32_t>(dpp_i<0x140>(static_cast<int>(v))));
     return v;
 }
+// Eight entries of a group, whose other lanes hold the rest, as pairs in the order in which a word's codes come apart (0 2 4
+// 6 1 3 5 7); returns what undoes the power of two, a NaN for a group with an infinity or a NaN.
 template <int G>
-__device__ __forceinline__ int group_sum(int v) {
-    v += dpp_i<0xB1>(v);
-    v += dpp_i<0x4E>(v);
-    if constexpr (G >= 64) v += dpp_i<0x141>(v);
-    if constexpr (G >= 128) v += dpp_i<0x140>(v);
-    return v;
+__device__ __forceinline__ float split8(const float (&x)[8], h8& hi, h8& lo) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = group_max<G>(top);
+    const bool ok = top < 0x7f800000u && top != 0;
+    const int e = ok ? min(15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 100) : 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        constexpr int kOrder[8] = {0, 2, 4, 6, 1, 3, 5, 7};
+        const v2f y = {ok ? ldexpf(x[kOrder[i]], e) : 0.0f, ok ? ldexpf(x[kOrder[i + 1]], e) : 0.0f};
+        const h2 a = __builtin_convertvector(y, h2);
+        const v2f rest = {y[0] - static_cast<float>(a[0]), y[1] - static_cast<float>(a[1])};
+        const h2 b = __builtin_convertvector(rest, h2);
+        hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
+    }
+    return top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
+}
+// the eight of a row that is in a block of 256 k: the part of 32 k, and the lanes c, that they belong to
+template <int G>
+__device__ __forceinline__ void place8(int eight, int& mi, int& c) {
+    if constexpr (G == 32) mi = eight >> 2, c = eight & 3;
+    else mi = eight >> 4 << 2 | (eight >> 3 & 1) << 1 | (eight & 1), c = eight >> 1 & 3;
 }
 
-// An image of R rows of X (fewer may be there) over some blocks of 64 k, the operand of the products as it is
-// read: digit d of row r at k 64 b + 16 c + j in byte ((4 b + c) R + r) 48 + 16 d + j; then the groups' factors
-// [group][R], floats, or with zero points four: the sums of the three digits and the factor.
-template <int G, bool ZP>
-__host__ __device__ constexpr int meta_bytes(int R, int k) { return R * (k / G) * (ZP ? 16 : 4); }
+// eight codes less their zero: zero1 = -(1024 + zero), zero16 = -(64 + zero), twice each. A code becomes fp16 as the
+// last bits of 1024 + code, or of 1024 + 16 code.
+__device__ __forceinline__ h8 less_zero(uint32_t w, h2 zero1, h2 zero16) {
+    const h2 sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    const uint32_t v = w >> 8;
+    const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) ^ 0x64086408u) + zero1;
+    const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00f000f0u) ^ 0x64806480u), sixteenth, zero16);
+    const h2 c = __builtin_bit_cast(h2, (v & 0x000f000fu) ^ 0x64086408u) + zero1;
+    const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & 0x00f000f0u) ^ 0x64806480u), sixteenth, zero16);
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// eight entries of a row from k on, 0 behind its end
+__device__ __forceinline__ void load8(const float* row, int k, int K, bool wide, float (&x)[8]) {
+    const float* src = row + k;
+    if (wide && k + 8 <= K) {
+        const v4f a = reinterpret_cast<const v4f*>(src)[0], b = reinterpret_cast<const v4f*>(src)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = k + i < K ? src[i] : 0.0f;
+    }
+}
+
+// An image of R rows of X (fewer may be there) over some blocks of 256 k, the operand of the products as it is read: [block][8 of
+// 32 k][c] of 2 R places of 16 bytes, a row's eight entries' first parts and second ones in turn; then the groups' factors
+// [group][R]. The places are moved on by image_turn, so that of the writers, who hold eights of one row, few
+// meet in a bank; it is the same for c = 0 and 1, and for 2 and 3, whose readers are served together.
+__host__ __device__ constexpr int image_bytes(int R) { return R * 1024; }
+template <int G>
+__host__ __device__ constexpr int meta_bytes(int R) { return R * (256 / G) * 4; }
+template <int R>
+__device__ __forceinline__ int image_turn(int mi, int c) { return R == 1 ? 0 : 2 * (mi & 3) + R * (c >> 1); }
 
 // Makes the image of k [k0, k0 + kn) (kn a multiple of 256). A wave keeps to one row.
-template <int G, bool ZP, int R>
+template <int G, int R>
 __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, int rows, int k0, int kn, uint8_t* img, uint8_t* meta,
                                            int lane, int wave) {
     constexpr int step = kThreads / R;
@@ -74,57 +105,35 @@ __device__ __forceinline__ void make_image(const float* X, int64_t ldx, int K, i
     for (int id0 = first; id0 < count; id0 += kBatch * step) {
         float x[kBatch][8];
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-            const int k = k0 + min(id0 + n * step, count - 1) * 8;
-            const float* src = X + r * ldx + k;
-            if (wide && k + 8 <= K) {
-                const v4f a = reinterpret_cast<const v4f*>(src)[0], b = reinterpret_cast<const v4f*>(src)[1];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] = a[i], x[n][4 + i] = b[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[n][i] = k + i < K ? src[i] : 0.0f;
-            }
-        }
+        for (int n = 0; n < kBatch; ++n) load8(X + r * ldx, k0 + min(id0 + n * step, count - 1) * 8, K, wide, x[n]);
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
             const int id = id0 + n * step;
             if (id >= count) break;     // 32 lanes are in or out together
-            const int kk = id * 8;
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
-            float scale;
-            const Digits d = digits8(x[n], group_max<G>(top), scale);
-            uint8_t* at = img + ((kk >> 4) * R + r) * 48 + (kk & 8);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2*>(at + 16 * p) = make_uint2(d.d[p][0], d.d[p][1]);
-            const int g = kk / G * R + r;
-            if constexpr (ZP) {
-                int s[3];
-#pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    s[p] = group_sum<G>(__builtin_amdgcn_sdot4(static_cast<int>(d.d[p][1]), 0x01010101,
-                                                               __builtin_amdgcn_sdot4(static_cast<int>(d.d[p][0]), 0x01010101, 0, false), false));
-                if (kk % G == 0)
-                    reinterpret_cast<float4*>(meta)[g] = make_float4(static_cast<float>(s[0]), static_cast<float>(s[1]), static_cast<float>(s[2]), scale);
-            } else {
-                if (kk % G == 0) reinterpret_cast<float*>(meta)[g] = scale;
-            }
+            h8 hi, lo;
+            const float factor = split8<G>(x[n], hi, lo);
+            const int b = id >> 5, w = id & 31;  // the block, the eight in it
+            int mi, c;
+            place8<G>(w, mi, c);
+            const int at = 2 * r + image_turn<R>(mi, c);
+            uint8_t* to = img + b * image_bytes(R) + (mi * 4 + c) * R * 32;
+            *reinterpret_cast<h8*>(to + (at & (2 * R - 1)) * 16) = hi;
+            *reinterpret_cast<h8*>(to + ((at + 1) & (2 * R - 1)) * 16) = lo;
+            if (w % (G / 8) == 0) reinterpret_cast<float*>(meta)[(b * (256 / G) + w / (G / 8)) * R + r] = factor;
         }
     }
 }
 
 // ---- the products
-// A 16 x 16 x 64 integer product takes 16 rows of weights and, on its other side, four rows of X as four times
-// three digits (the fourth row of each four is never looked at): lane 16 c + n holds the three digits' sums of
-// row c of the four and weight row n side by side, and only there are they put together, scaled and added
-// in fp32. A group is one such product (two for 128, one of depth 32 for 32), so sums are exact until they
-// are scaled. With zero points -16 zero x (sum of the digits) is added to each digit's first.
+// A 16 x 16 x 32 fp16 product takes 16 rows of weights and, on its other side, up to eight rows of X as two parts each: lane
+// 16 c + n holds, side by side, the two parts' sums of row c (of four rows; of eight, of rows 2 c and 2 c + 1; of one, of
+// that row in every c) and weight row n, and only there are they added, scaled and added up in fp32. A group is one such
+// product for every 32 k.
 //
 // A workgroup's waves take tiles of 16 weight rows, `ks` waves a tile, which share its k by blocks of 256 and
-// add up in LDS. Weights go from memory to registers kDepth blocks ahead.
-constexpr int kDepth = 4;
+// add up in LDS. Weights go from memory to registers kDepth blocks ahead: with two, three workgroups' registers fit a
+// compute unit (the head of 151936 rows 33.7 us, four ahead 38.0).
+constexpr int kDepth = 2;
 
 template <int G, bool ZP>
 struct Unit {
@@ -156,88 +165,77 @@ struct Unit {
     }
 };
 
-// What a lane reads of the images for one group: digits and factors of its rows.
-template <int G, bool ZP, int R>
+// the zero points of a group as less_zero takes them
+template <bool ZP, typename U>
+__device__ __forceinline__ void zeros_of(const U& u, int g, h2& zero1, h2& zero16) {
+    zero1 = h2{static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+    zero16 = h2{static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+    if constexpr (ZP) {
+        const _Float16 z = static_cast<_Float16>(static_cast<short>(-u.zero(g)));
+        const h2 zz = {z, z};
+        zero1 += zz, zero16 += zz;
+    }
+}
+
+// What a lane reads of the images for one group: the parts that it holds of the operand and its rows' factors.
+template <int G, int R>
 struct Operand {
-    static constexpr int QN = (R + 3) / 4, H = G == 128 ? 2 : 1;
-    v4i a[QN][H];
-    v4f factor[QN];                     // sums of the three digits and the scale, or the scale alone
-    __device__ void load(const uint8_t* img, const uint8_t* meta, int g) {
+    static constexpr int kEach = G / 32, kRows = R == 8 ? 2 : 1;
+    h8 x[kEach];
+    float factor[kRows];
+    __device__ void load(const uint8_t* img, const uint8_t* meta, const int (&place)[4], int g) {
 #pragma unroll
-        for (int q = 0; q < QN; ++q) {
-            if constexpr (G == 32) {
-                const v2i x = *reinterpret_cast<const v2i*>(img + (g >> 1) * R * 192 + (g & 1) * R * 96 + q * 192);
-                a[q][0] = v4i{x[0], x[1], 0, 0};
-            } else {
-#pragma unroll
-                for (int h = 0; h < H; ++h) a[q][h] = *reinterpret_cast<const v4i*>(img + (g * H + h) * R * 192 + q * 192);
-            }
-            if constexpr (ZP) factor[q] = *reinterpret_cast<const v4f*>(meta + (g * R + 4 * q) * 16);
-            else factor[q][3] = *reinterpret_cast<const float*>(meta + (g * R + 4 * q) * 4);
+        for (int m = 0; m < kEach; ++m) x[m] = *reinterpret_cast<const h8*>(img + (g * kEach + m) * R * 128 + place[(g * kEach + m) & 3]);
+        if constexpr (kRows == 2) {
+            const v2f f = *reinterpret_cast<const v2f*>(meta + g * R * 4);
+            factor[0] = f[0], factor[1] = f[1];
+        } else {
+            factor[0] = *reinterpret_cast<const float*>(meta + g * R * 4);
         }
     }
 };
 
-// A block of 256 k of a tile: `img` and `meta` are this lane's places in the images of that block. What a
-// group needs from LDS is asked for a group ahead, and its products are all issued before the first is used.
+// A block of 256 k of a tile: img: the block's image; place[mi % 4]: this lane's bytes in the part of 32 k; meta: its place in
+// the block's factors. What a group needs from LDS is asked for a group ahead.
 template <int G, bool ZP, int R>
-__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, float (&acc)[(R + 3) / 4]) {
-    constexpr int QN = (R + 3) / 4, H = G == 128 ? 2 : 1;
-    Operand<G, ZP, R> o[2];
-    o[0].load(img, meta, 0);
+__device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* img, const uint8_t* meta, const int (&place)[4],
+                                         float (&acc)[R == 8 ? 2 : 1]) {
+    typedef Operand<G, R> O;
+    O o[2];
+    o[0].load(img, meta, place, 0);
 #pragma unroll
     for (int g = 0; g < 256 / G; ++g) {
-        if (g + 1 < 256 / G) o[(g + 1) & 1].load(img, meta, g + 1);
-        const Operand<G, ZP, R>& x = o[g & 1];
-        v4i d[QN];
+        if (g + 1 < 256 / G) o[(g + 1) & 1].load(img, meta, place, g + 1);
+        const O& x = o[g & 1];
+        h2 zero1, zero16;
+        zeros_of<ZP>(u, g, zero1, zero16);
+        v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            // eight codes a word: bytes of 16 times the low and the high ones
-            const uint32_t w0 = u.word(G == 32 ? g : 2 * (g * H + h)), w1 = G == 32 ? 0 : u.word(2 * (g * H + h) + 1);
-            const v4i b = {static_cast<int>(w0 << 4 & 0xf0f0f0f0u), static_cast<int>(w0 & 0xf0f0f0f0u), static_cast<int>(w1 << 4 & 0xf0f0f0f0u),
-                           static_cast<int>(w1 & 0xf0f0f0f0u)};
-#pragma unroll
-            for (int q = 0; q < QN; ++q) {
-                const v4i c = h ? d[q] : v4i{0, 0, 0, 0};
-                if constexpr (G == 32)
-                    d[q] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, v2i{x.a[q][0][0], x.a[q][0][1]}),
-                                                                 __builtin_bit_cast(long, v2i{b[0], b[1]}), c, 0, 0, 0);
-                else d[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.a[q][h], b, c, 0, 0, 0);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int m = 0; m < O::kEach; ++m)
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.x[m], less_zero(u.word(g * O::kEach + m), zero1, zero16), d, 0, 0, 0);
         const float sw = u.scale(g);
 #pragma unroll
-        for (int q = 0; q < QN; ++q) {
-            float f;
-            if constexpr (ZP) {         // zero x sum of digits and a sum of products are whole and below 2^22: exact
-                const float z = static_cast<float>(-16 * u.zero(g));
-                f = fmaf(fmaf(fmaf(z, x.factor[q][2], static_cast<float>(d[q][2])), 256.0f, fmaf(z, x.factor[q][1], static_cast<float>(d[q][1]))),
-                         256.0f, fmaf(z, x.factor[q][0], static_cast<float>(d[q][0])));
-            } else {
-                f = from_digits(d[q]);
-            }
-            acc[q] = fmaf(f, sw * x.factor[q][3], acc[q]);
-            pin(acc[q]);
-        }
+        for (int j = 0; j < O::kRows; ++j) acc[j] = fmaf((d[2 * j] + d[2 * j + 1]) * sw, x.factor[j], acc[j]);
     }
 }
 
 template <int G, bool ZP, int R>
 __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most, int ks, int chunk) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int QN = (R + 3) / 4, kMeta = meta_bytes<G, ZP>(R, 256);
+    constexpr int kRows = R == 8 ? 2 : 1, kImage = image_bytes(R), kMeta = meta_bytes<G>(R);
     typedef Unit<G, ZP> U;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, n = lane & 15;
     const int r0 = blockIdx.y * most, rows = min(most, a.M - r0);
     const int tiles = (a.N + 15) / 16, blocks = (a.K + 255) / 256, rt = kWaves / ks, part = wave & (ks - 1);
     const int sets = (tiles + rt - 1) / rt;
-    uint8_t* meta = lds + R * 768 * chunk;
+    uint8_t* meta = lds + kImage * chunk;
     float* red = reinterpret_cast<float*>(meta + kMeta * chunk);
     // this lane's places: rows that are not there hold whatever, as do the sums over them
-    const int digit = min(n & 3, 2), row = min(n >> 2, R - 1);
-    const uint8_t* img_lane = lds + (G == 32 ? ((c >> 1) * R + row) * 48 + (c & 1) * 8 : (c * R + row) * 48) + digit * 16;
-    const uint8_t* meta_lane = meta + min(c, R - 1) * (ZP ? 16 : 4);
+    const int part_of = 2 * (R == 8 ? n >> 1 : R == 4 ? n >> 2 : 0) + (n & 1);
+    int place[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) place[i] = c * R * 32 + ((part_of + image_turn<R>(i, c)) & (2 * R - 1)) * 16;
+    const uint8_t* meta_lane = meta + (R == 8 ? c * 8 : R == 4 ? c * 4 : 0);
     const bool one = chunk >= blocks;   // one image serves all tiles
     bool made = false;
     U u[kDepth];
@@ -252,33 +250,33 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
     const uint8_t* w = nullptr;
     for (int set = blockIdx.x; set < sets; set += gridDim.x) {
         const int tile = set * rt + wave / ks;
-        float acc[QN];
+        float acc[kRows];
 #pragma unroll
-        for (int q = 0; q < QN; ++q) acc[q] = 0.0f;
+        for (int j = 0; j < kRows; ++j) acc[j] = 0.0f;
         for (int b0 = 0; b0 < blocks; b0 += chunk) {
             const int bn = min(chunk, blocks - b0), its = (bn - part + ks - 1) / ks;
             if (!one || !made) {
                 w = load(set, b0, its);
                 if (made) lds_barrier();
-                make_image<G, ZP, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, lane, wave);
+                make_image<G, R>(a.X + r0 * a.ldx, a.ldx, a.K, rows, b0 * 256, bn * 256, lds, meta, lane, wave);
                 made = true;
                 lds_barrier();
             }
-            const uint8_t *img = img_lane + part * R * 768, *factors = meta_lane + part * kMeta;
+            const uint8_t *img = lds + part * kImage, *factors = meta_lane + part * kMeta;
             for (int i = 0; i < its; i += kDepth) {
 #pragma unroll
                 for (int j = 0; j < kDepth; ++j)
                     if (i + j < its) {
-                        multiply<G, ZP, R>(u[j], img, factors, acc);
-                        img += ks * R * 768, factors += ks * kMeta;
+                        multiply<G, ZP, R>(u[j], img, factors, place, acc);
+                        img += ks * kImage, factors += ks * kMeta;
                         if (i + j + kDepth < its) u[j].load(w + (i + j + kDepth) * ks * U::kBytes, lane);
                     }
             }
         }
         // the next set's first blocks, before this one's end
         if (one && set + static_cast<int>(gridDim.x) < sets) w = load(set + gridDim.x, 0, (blocks - part + ks - 1) / ks);
-        const auto store = [&](int q, float y) {
-            const int r = 4 * q + c, col = tile * 16 + n;
+        const auto store = [&](int j, float y) {
+            const int r = kRows * c + j, col = tile * 16 + n;
             if (r < rows && tile < tiles && col < a.N) {
                 const int64_t at = r0 + r;
                 a.Y[at * a.ldy + col] = y + (a.R ? a.R[at * a.ldr + col] : 0.0f);
@@ -286,42 +284,34 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
         };
         if (ks == 1) {
 #pragma unroll
-            for (int q = 0; q < QN; ++q) store(q, acc[q]);
+            for (int j = 0; j < kRows; ++j) store(j, acc[j]);
             continue;
         }
 #pragma unroll
-        for (int q = 0; q < QN; ++q) red[(wave * QN + q) * 64 + lane] = acc[q];
+        for (int j = 0; j < kRows; ++j) red[(wave * kRows + j) * 64 + lane] = acc[j];
         lds_barrier();
 #pragma unroll
-        for (int q = 0; q < QN; ++q)
-            if ((q & (ks - 1)) == part) {
+        for (int j = 0; j < kRows; ++j)
+            if ((j & (ks - 1)) == part) {
                 float y = 0.0f;
-                for (int i = 0; i < ks; ++i) y += red[((wave - part + i) * QN + q) * 64 + lane];
-                store(q, y);
+                for (int i = 0; i < ks; ++i) y += red[((wave - part + i) * kRows + j) * 64 + lane];
+                store(j, y);
             }
         lds_barrier();
     }
 }
 
 // ---- the products of many rows
-// Sixteen rows of X against sixteen of weights, 32 k at a time, on the fp16 matrix cores. An entry of X times the power
-// of two that brings its group's largest to [2^14, 2^15) is hi + lo, two fp16 values, to 2^-22 of itself (or 2^-39 of
-// the largest); a code less its zero is an fp16 value; so products are exact, and their sums, of one group, are
-// in fp32. A code becomes fp16 as the last bits of 1024 + code, or of 1024 + 16 code. A group of 64 k costs a tile and 16 rows
-// some 32 instructions and four products; by digits, which are put together for every four rows, 67 and four. 4096 rows
-// of 8224 x 2048 take 350 us (394 TFLOP/s of products by X as it is, twice that of fp16 products); both
-// pipes are busy in turn. Small products are bound by what comes first, X's image, which every workgroup makes.
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float v2f __attribute__((ext_vector_type(2)));
+// Sixteen rows of X against sixteen of weights, 32 k at a time, each of their two parts a product. A group of 64 k costs a
+// tile and 16 rows some 32 instructions and four products. 4096 rows of 8224 x 2048 take 395 us (349 TFLOP/s of products
+// by X as it is, twice that of fp16 products); both pipes are busy in turn. Small products are bound by what comes first,
+// X's image, which every workgroup makes.
 constexpr int kManyRows = 16, kManyBytes = 16 * 1024, kPair = 2, kManyDepth = 2;
 template <int G>
 __host__ __device__ constexpr int many_bytes() { return kManyBytes + 256 / G * kManyRows * 4; }
 
-// The image of a block of 256 k: [8 of 32 k][lo, hi][c] of 16 places of 16 bytes, a row's eight entries in the order in which a
-// word's codes come apart (0 2 4 6 1 3 5 7); then the groups' factors [group][16]. The rows' places are moved on by
-// many_turn, so that of the writers, who hold eights of one row, few meet in a bank; it is the same for c = 0 and 1,
-// and for 2 and 3, whose readers are served together.
+// The image of a block of 256 k: [8 of 32 k][lo, hi][c] of 16 places of 16 bytes, a row's eight entries, moved on by many_turn
+// as above; then the groups' factors [group][16].
 __device__ __forceinline__ int many_turn(int mi, int c) { return 2 * (mi & 3) + 8 * (c >> 1); }
 template <int G>
 __device__ __forceinline__ void make_many(const float* X, int64_t ldx, int K, int rows, int k0, int blocks, uint8_t* img, uint8_t* meta,
@@ -333,58 +323,22 @@ __device__ __forceinline__ void make_many(const float* X, int64_t ldx, int K, in
         for (int id0 = lane; id0 < count; id0 += kBatch * 64) {
             float x[kBatch][8];
 #pragma unroll
-            for (int n = 0; n < kBatch; ++n) {
-                const int k = k0 + min(id0 + n * 64, count - 1) * 8;
-                const float* src = X + r * ldx + k;
-                if (wide && k + 8 <= K) {
-                    const v4f a = reinterpret_cast<const v4f*>(src)[0], b = reinterpret_cast<const v4f*>(src)[1];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[n][i] = a[i], x[n][4 + i] = b[i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[n][i] = k + i < K ? src[i] : 0.0f;
-                }
-            }
+            for (int n = 0; n < kBatch; ++n) load8(X + r * ldx, k0 + min(id0 + n * 64, count - 1) * 8, K, wide, x[n]);
 #pragma unroll
             for (int n = 0; n < kBatch; ++n) {
                 const int o = id0 + n * 64;
                 if (o >= count) break;  // 32 lanes are in or out together
-                uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
-                top = group_max<G>(top);
-                const bool ok = top < 0x7f800000u && top != 0;
-                const int e = ok ? min(15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 100) : 0;
                 h8 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    constexpr int kOrder[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-                    const v2f y = {ok ? ldexpf(x[n][kOrder[i]], e) : 0.0f, ok ? ldexpf(x[n][kOrder[i + 1]], e) : 0.0f};
-                    const h2 a = __builtin_convertvector(y, h2);
-                    const v2f rest = {y[0] - static_cast<float>(a[0]), y[1] - static_cast<float>(a[1])};
-                    const h2 b = __builtin_convertvector(rest, h2);
-                    hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
-                }
+                const float factor = split8<G>(x[n], hi, lo);
                 const int b = o >> 5, w = o & 31;  // the block, the eight in it
-                const int mi = G == 32 ? w >> 2 : w >> 4 << 2 | (w >> 3 & 1) << 1 | (w & 1), c = G == 32 ? w & 3 : w >> 1 & 3;
+                int mi, c;
+                place8<G>(w, mi, c);
                 uint8_t* at = img + b * kManyBytes + mi * 2048 + c * 256 + ((r + many_turn(mi, c)) & 15) * 16;
                 *reinterpret_cast<h8*>(at) = lo;
                 *reinterpret_cast<h8*>(at + 1024) = hi;
-                if (w % (G / 8) == 0)
-                    reinterpret_cast<float*>(meta)[(b * (256 / G) + w / (G / 8)) * kManyRows + r] = top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
+                if (w % (G / 8) == 0) reinterpret_cast<float*>(meta)[(b * (256 / G) + w / (G / 8)) * kManyRows + r] = factor;
             }
         }
-}
-
-// eight codes less their zero: zero1 = -(1024 + zero), zero16 = -(64 + zero), twice each
-__device__ __forceinline__ h8 less_zero(uint32_t w, h2 zero1, h2 zero16) {
-    const h2 sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-    const uint32_t v = w >> 8;
-    const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) ^ 0x64086408u) + zero1;
-    const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00f000f0u) ^ 0x64806480u), sixteenth, zero16);
-    const h2 c = __builtin_bit_cast(h2, (v & 0x000f000fu) ^ 0x64086408u) + zero1;
-    const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & 0x00f000f0u) ^ 0x64806480u), sixteenth, zero16);
-    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // A block of 256 k of two tiles. img: the block's image; place[mi % 4]: this lane's bytes in the part of 32 k.
@@ -410,12 +364,8 @@ __device__ __forceinline__ void multiply_many(const Unit<G, ZP> (&u)[kPair], con
         v4f d[kPair];
 #pragma unroll
         for (int t = 0; t < kPair; ++t) {
-            h2 zero1 = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)}, zero16 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
-            if constexpr (ZP) {
-                const _Float16 z = static_cast<_Float16>(static_cast<short>(-u[t].zero(g)));
-                const h2 zz = {z, z};
-                zero1 += zz, zero16 += zz;
-            }
+            h2 zero1, zero16;
+            zeros_of<ZP>(u[t], g, zero1, zero16);
 #pragma unroll
             for (int m = 0; m < kEach; ++m) w[t][m] = less_zero(u[t].word(g * kEach + m), zero1, zero16);
         }
@@ -634,8 +584,8 @@ struct Q4Plan {
 template <int G, bool ZP>
 void q4_fit(Q4Plan& p, int N, int K) {
     const bool many = p.image == kManyRows;
-    const int blocks = q4_blocks(K), each = many ? many_bytes<G>() : p.image * 768 + meta_bytes<G, ZP>(p.image, 256);
-    const int red = p.ks > 1 ? kWaves * (many ? 4 * kPair : (p.image + 3) / 4) * 256 : 0;
+    const int blocks = q4_blocks(K), each = many ? many_bytes<G>() : image_bytes(p.image) + meta_bytes<G>(p.image);
+    const int red = p.ks > 1 ? kWaves * (many ? 4 * kPair : p.image == 8 ? 2 : 1) * 256 : 0;
     p.chunk = std::min(blocks, (160 * 1024 - red) / each);
     p.lds = each * p.chunk + red;
 }
@@ -643,19 +593,20 @@ template <int G, bool ZP>
 Q4Plan q4_plan(int M, int N, int K) {
     Q4Plan p{};
     const int blocks = q4_blocks(K), tiles = q4_tiles(N);
-    // Blocks of four rows fill the chip sooner, of eight read and unpack the weights less often (64 x 2048 x
-    // 2048 in fours 7.1 us, in eights 7.6; 48 x 8224 x 2048 18.1 and 17.4; 8 x 2048 x 2048 5.0 and 6.2).
-    p.image = M == 1 ? 1 : tiles * ((M + 3) / 4) <= 2048 || M <= 4 ? 4 : 8;
-    // Sixteen rows on the fp16 cores where rows and tiles are many (48 x 8224 x 2048 13.8 us, by digits 17.9; 32 x 8224
-    // x 2048 13.1 and 16.6; 4096 x 8224 x 2048 350 and 428), else by digits, whose smaller images are made sooner (24 x
-    // 8224 x 2048 11.5 us, on the fp16 cores 12.0; 64 x 2048 x 2048 6.9 and 8.2; 16 x 151936 x 2048 45 and 47).
-    if (M > 16 && static_cast<int64_t>(tiles) * M >= 16384) {
+    // Blocks of four rows fill the chip sooner, of eight read and unpack the weights less often (K 2048: 64 x 2048 in
+    // fours 7.9 us, in eights 6.9; 8 x 8224 8.9 and 7.1; 32 x 2048 6.2 and 6.1; 12 x 2048 5.1 and 5.2; 8 x 2048 4.6 and 5.1;
+    // 16 x 2048 x 6144 9.4 and 11.1).
+    p.image = M == 1 ? 1 : tiles * ((M + 3) / 4) <= 1024 || M <= 4 ? 4 : 8;
+    // Sixteen rows, and two tiles a wave, where rows and tiles are many (48 x 8224 x 2048 13.7 us, by eights 15.7; 32 x
+    // 8224 13.0 and 14.7; 16 x 151936 54 and 62; 12 x 50000 18.8 and 23.8), else by fewer, whose smaller images are made
+    // sooner (24 x 8224 10.7 us, by sixteens 12.4; 16 x 12288 10.1 and 11.0; 64 x 2048 6.9 and 8.3; 8 x 151936 39.5 and 51.7).
+    if (M > 8 && static_cast<int64_t>(tiles) * M >= 16384) {
         p.image = kManyRows;
         p.row_blocks = (M + p.image - 1) / p.image;
         p.most = (M + p.row_blocks - 1) / p.row_blocks;
         // Waves that share a pair of tiles: as many as make the rounds of a workgroup a compute unit, each of so many blocks
-        // of k and half a block's time for joining, least (48 x 8224 x 2048, two 13.8 us, one 18.7, four 16.2; 64
-        // x 8224 x 2048, four 17.9, two 19.0).
+        // of k and half a block's time for joining, least (48 x 8224 x 2048, two 13.7 us, one 18.4, four 16.0; 64 x 8224 x
+        // 2048, four 17.9, two 18.7; 1024 x 8224 x 2048, one 107, two 116).
         const int pairs = (tiles + 1) / 2, most_wgs = std::max(1, 256 / p.row_blocks);
         int64_t best = INT64_MAX;
         for (int ks = 1; ks <= kWaves && (ks == 1 || ks <= blocks); ks *= 2) {
@@ -669,13 +620,13 @@ Q4Plan q4_plan(int M, int N, int K) {
     p.row_blocks = (M + p.image - 1) / p.image;
     p.most = (M + p.row_blocks - 1) / p.row_blocks;
     // Waves share a tile while there are not enough tiles: up to eight waves a compute unit, for one row up to 32
-    // (12288 x 2048, eight waves a tile 5.1 us, two 5.8; the head of 151936 rows, one wave 30.5 us, eight 32).
+    // (1 x 12288 x 2048, eight waves a tile 5.8 us, two 6.1, one 7.8; 1 x 151936, one 33.9, two 36.2, eight 40.6; 8 x 8224,
+    // two 7.2, eight 7.4, one 9.4).
     p.ks = kWaves;
     while (p.ks > 1 && (static_cast<int64_t>(tiles) * p.row_blocks * p.ks > (M == 1 ? 8192 : 2048) || p.ks / 2 >= blocks)) p.ks /= 2;
     const int rt = kWaves / p.ks, sets = (tiles + rt - 1) / rt;
-    // two workgroups a compute unit go on from tile to tile; one row without shared tiles takes them all at once
-    // (the head: 1187 workgroups 30.5 us, 256 36.6)
-    p.wgs = M == 1 && p.ks == 1 ? sets : std::min(sets, std::max(1, 512 / p.row_blocks));
+    // two workgroups a compute unit go on from tile to tile (the head of 151936 rows: 33.5 us, by one 39.6, by all at once 34.2)
+    p.wgs = std::min(sets, std::max(1, 512 / p.row_blocks));
     q4_fit<G, ZP>(p, N, K);
     return p;
 }
