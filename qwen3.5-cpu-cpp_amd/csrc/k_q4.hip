@@ -31,25 +31,26 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {  // over the G / 8 l
     return v;
 }
 // Eight entries of a group, whose other lanes hold the rest, as pairs in the order in which a word's codes come apart (0 2 4
-// 6 1 3 5 7); returns what undoes the power of two, a NaN for a group with an infinity or a NaN.
+// 6 1 3 5 7); returns what undoes the power of two. An infinity or a NaN is its own first part, with a second of 0, beside
+// which the group's finite entries do not matter: they are brought below 2^15 whatever they are.
 template <int G>
 __device__ __forceinline__ float split8(const float (&x)[8], h8& hi, h8& lo) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
     top = group_max<G>(top);
-    const bool ok = top < 0x7f800000u && top != 0;
-    const int e = ok ? min(15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 100) : 0;
+    const bool finite = top < 0x7f800000u;
+    const int e = top == 0 ? 0 : finite ? min(15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 100) : 15 - 128;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         constexpr int kOrder[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-        const v2f y = {ok ? ldexpf(x[kOrder[i]], e) : 0.0f, ok ? ldexpf(x[kOrder[i + 1]], e) : 0.0f};
+        const v2f y = {ldexpf(x[kOrder[i]], e), ldexpf(x[kOrder[i + 1]], e)};
         const h2 a = __builtin_convertvector(y, h2);
-        const v2f rest = {y[0] - static_cast<float>(a[0]), y[1] - static_cast<float>(a[1])};
+        const v2f rest = {finite ? y[0] - static_cast<float>(a[0]) : 0.0f, finite ? y[1] - static_cast<float>(a[1]) : 0.0f};
         const h2 b = __builtin_convertvector(rest, h2);
         hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
     }
-    return top >= 0x7f800000u ? NAN : ldexpf(1.0f, -e);
+    return ldexpf(1.0f, -e);
 }
 // the eight of a row that is in a block of 256 k: the part of 32 k, and the lanes c, that they belong to
 template <int G>
