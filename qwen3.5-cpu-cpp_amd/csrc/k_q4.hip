@@ -30,8 +30,10 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {  // over the G / 8 l
     if constexpr (G >= 128) v = max(v, static_cast<uint32_t>(dpp_i<0x140>(static_cast<int>(v))));
     return v;
 }
+// Sums over groups are in units of this, so that the largest scale times the largest factor, 2^16 2^113, stays below 2^128.
+constexpr float kUnit = 4.0f;
 // Eight entries of a group, whose other lanes hold the rest, as pairs in the order in which a word's codes come apart (0 2 4
-// 6 1 3 5 7); returns what undoes the power of two. An infinity or a NaN is its own first part, with a second of 0, beside
+// 6 1 3 5 7); returns what undoes the power of two, over kUnit. An infinity or a NaN is its own first part, with a second of 0, beside
 // which the group's finite entries do not matter: they are brought below 2^15 whatever they are.
 template <int G>
 __device__ __forceinline__ float split8(const float (&x)[8], h8& hi, h8& lo) {
@@ -50,7 +52,7 @@ __device__ __forceinline__ float split8(const float (&x)[8], h8& hi, h8& lo) {
         const h2 b = __builtin_convertvector(rest, h2);
         hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
     }
-    return ldexpf(1.0f, -e);
+    return ldexpf(1.0f / kUnit, -e);
 }
 // the eight of a row that is in a block of 256 k: the part of 32 k, and the lanes c, that they belong to
 template <int G>
@@ -216,7 +218,7 @@ __device__ __forceinline__ void multiply(const Unit<G, ZP>& u, const uint8_t* im
             d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.x[m], less_zero(u.word(g * O::kEach + m), zero1, zero16), d, 0, 0, 0);
         const float sw = u.scale(g);
 #pragma unroll
-        for (int j = 0; j < O::kRows; ++j) acc[j] = fmaf((d[2 * j] + d[2 * j + 1]) * sw, x.factor[j], acc[j]);
+        for (int j = 0; j < O::kRows; ++j) acc[j] = fmaf(d[2 * j] + d[2 * j + 1], sw * x.factor[j], acc[j]);
     }
 }
 
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void q4_mul_kernel(Q4MulArgs a, int most,
             const int r = kRows * c + j, col = tile * 16 + n;
             if (r < rows && tile < tiles && col < a.N) {
                 const int64_t at = r0 + r;
-                a.Y[at * a.ldy + col] = y + (a.R ? a.R[at * a.ldr + col] : 0.0f);
+                a.Y[at * a.ldy + col] = fmaf(y, kUnit, a.R ? a.R[at * a.ldr + col] : 0.0f);
             }
         };
         if (ks == 1) {
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void q4_mul_many_kernel(Q4MulArgs a, int 
             const int row = 4 * c + r, col = (tile + t) * 16 + n;
             if (row < rows && tile + t < tiles && col < a.N) {
                 const int64_t at = r0 + row;
-                a.Y[at * a.ldy + col] = y + (a.R ? a.R[at * a.ldr + col] : 0.0f);
+                a.Y[at * a.ldy + col] = fmaf(y, kUnit, a.R ? a.R[at * a.ldr + col] : 0.0f);
             }
         };
         if (ks == 1) {

@@ -1,9 +1,10 @@
-"""q35_matmul_q4 with infinities and NaN in X: outputs are what the formula's products and sums give."""
+"""q35_matmul_q4 with infinities and NaN in X, and with entries and scales next to the largest that there are: outputs are what
+the formula's products and sums give."""
 import numpy as np
 import pytest
 
 import pyq35
-from q4_ref import weights64
+from q4_ref import bytes_of, nibbles, weights64
 from test_gpu_matmul_q4 import make
 from test_gpu_matmul_q4_outliers import bound, multiply
 
@@ -41,3 +42,18 @@ def test_infinities_and_nan(hip, M, N, K, G, zeros, bad):
     y = dict(x, X=x["X"][rest])
     exact = y["X"][:, :K].astype(np.float64) @ w.T
     assert (np.abs(got[rest] - exact) <= bound(y, w, exact)).all()
+
+
+@pytest.mark.parametrize("M,N,K,G,zeros", FORMS)
+def test_largest_entries_and_scales(hip, M, N, K, G, zeros):
+    """An entry of 3e38 meets weights of 0 in groups of scale 60000: what it leaves of the others is finite."""
+    x = make(M, N, K, G, zeros, M + N)
+    c = nibbles(x["codes"])[:, :K].copy()
+    x["X"][:, 9] = np.float32(3e38)
+    c[:, 9] = 8 if x["zeros"] is None else x["zeros"][:, 0] & 15
+    x["codes"] = bytes_of(c)
+    x["scales"][:, 0] = np.float16(60000.0).view(np.uint16)
+    w = weights64(x["codes"], x["scales"], x["zeros"], K, G)
+    want = x["X"][:, :K].astype(np.float64) @ w.T
+    got = multiply(hip, x)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound(x, w, want)).all()
