@@ -596,7 +596,8 @@ q35_status q35_gdn_batch(const q35_gdn_batch_args *args, q35_stream s);
  * of a group that is largest in magnitude becomes code 0: scale = fp16(-entry / 8) (it may be negative). With
  * zeros a group's codes span [min(least, 0), max(largest, 0)]: scale = fp16(span / 15), zero =
  * round(-least / scale). code = round(w / scale) + zero, kept within 0 .. 15; fp32 arithmetic, halves to
- * even. A group with an infinity or a NaN gets scale NaN, one whose scale rounds to 0 the value 0.
+ * even. A group with an infinity or a NaN, or whose scale exceeds fp16, gets scale NaN, one whose scale rounds to 0
+ * the value 0.
  * q35_q4_pack lays such weights out for q35_matmul_q4, once: q35_q4_packed_bytes() bytes, 16-byte aligned,
  * of tiles of 16 rows by 256 k with their scales (0 for refused sizes). N * K, padded to such tiles, is at
  * most 2^32. */

@@ -482,7 +482,8 @@ __global__ __launch_bounds__(kThreads) void q4_mul_many_kernel(Q4MulArgs a, int 
 
 // 16 lanes a group. Without zero points the entry of the largest magnitude becomes code 0, -8 steps:
 // scale = -entry / 8; with them the codes span [min(least, 0), max(largest, 0)]. Scales are rounded to
-// fp16 first and codes chosen by the rounded scale. A group with an infinity or a NaN gets scale NaN.
+// fp16 first and codes chosen by the rounded scale. A group with an infinity or a NaN, or whose scale fp16 does not
+// hold, gets scale NaN.
 template <bool BF16, int G>
 __global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, int K, uint8_t* codes, uint16_t* scales, uint8_t* zeros) {
     constexpr int per = G / 16, kBytes = per * (BF16 ? 2 : 4);
@@ -522,7 +523,8 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const void* W, int N, 
         hi = fmaxf(hi, __shfl_xor(hi, d, 16));
         bad |= static_cast<bool>(__shfl_xor(static_cast<int>(bad), d, 16));
     }
-    const uint16_t sb = bad ? 0x7e00 : bits_half(zeros ? (hi - lo) / 15.0f : (hi > -lo ? hi : lo) * -0.125f);
+    uint16_t sb = bits_half(zeros ? (hi - lo) / 15.0f : (hi > -lo ? hi : lo) * -0.125f);
+    if (bad || (sb & 0x7fff) >= 0x7c00) bad = true, sb = 0x7e00;
     const float s = half_bits(sb);
     const bool none = bad || s == 0.0f;
     const float zero = !zeros || none ? 8.0f : fminf(fmaxf(rintf(-lo / s), 0.0f), 15.0f);
