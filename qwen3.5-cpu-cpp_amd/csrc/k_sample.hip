@@ -526,7 +526,7 @@ __device__ __forceinline__ void gather(const float* x, int i, int e, const Weigh
 #pragma unroll
     for (int r = 0; r < 4; ++r) lo[r] = p.lo[r], bins[r] = p.hi[r] + 1 - p.lo[r];
     each_logit(x, i, e, [&](float l, int j) {
-        const uint32_t bin = static_cast<uint32_t>(w.place(l));  // the largest number where there is no weight
+        const uint32_t bin = static_cast<uint32_t>(fminf(w.place(l), kBins));  // kBins where there is no weight: no range's
         bool in = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) in |= bin - lo[r] < bins[r];
