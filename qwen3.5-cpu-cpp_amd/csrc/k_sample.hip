@@ -12,8 +12,8 @@
 // leaves the next one open to as much mass, so mostly to a bin as well). The workgroup that is done last
 // with a row plans that, or sorts the candidates and finds the exact places. A small top_k needs no counts: the largest
 // logits of 64 parts of the row, which the first launch leaves, bound its candidates, and the second launch gathers
-// them and draws. Rows of one slice take one launch. Where the open bins hold more than kList candidates (thousands
-// of equal logits), the places are found by radix descent over the row.
+// them and draws. Rows of one slice take one launch. Where the open bins hold more than kList candidates (thousands of
+// equal logits, or whole rows within one or two temperatures), the places are found by radix descent over the row.
 //
 // One row of 151936 with a top_k of 20 takes 15.5 us (by counts 22.5), 48 with settings of all kinds 43 us. The logits
 // are read two or three times, 29 MB of 48 rows in about 5 us each; the rest is one workgroup's chain of steps at the end
@@ -42,11 +42,9 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 constexpr uint32_t kKeyNone = 0x007fffffu;  // -inf
 constexpr uint32_t kKeyInf = 0xff800000u;   // +inf
 
-// Bins of 1/128 down to a depth of 12 and of 1/16 from there to 36: few borders are that deep, and what a launch clears,
-// adds to and reads back is less than half of it.
-constexpr int kFine = 12 * 128, kBins = kFine + 24 * 16;  // and one for what has no weight
-// a depth in 128ths as a place among them; larger ones have no smaller places
-__device__ __forceinline__ float place_of(float z) { return z < kFine ? z : fmaf(z, 0.125f, kFine * 0.875f); }
+// Bins of 1/128 of a depth, down to 36. (Wider ones below 12 cost a batch 1 us less, but there lies the bulk of a row with one
+// token far above it, thousands of candidates a bin.)
+constexpr int kBins = 36 * 128;         // and one for what has no weight
 
 // 2^(-y / 512) for 0 <= y < 2^15: y = n + f, |f| <= 1/2, so it is 2^-(n div 512) 2^-(n mod 512 / 512) 2^(-f / 512), the second
 // factor from a table and the last by four terms of its series (the fifth is below 2^-55).
@@ -90,7 +88,7 @@ struct Weigher {
     // weight are below kBins (a weight ends at 35.4).
     __device__ float place(float l) const {
         if (inf) return l == INFINITY ? 0.0f : INFINITY;
-        return l > -INFINITY ? place_of(fminf(top32 - l, 3.4e38f) * rt32) : INFINITY;
+        return l > -INFINITY ? fminf(top32 - l, 3.4e38f) * rt32 : INFINITY;
     }
     static constexpr double kDeepest = 36.0 * 512.0 / kLn2;
     // the weight in 64 bits, of the largest
@@ -480,7 +478,7 @@ __device__ __forceinline__ void make_plan(const Question& q, Work& sh) {
         if (q.m > 0.0f) {
             // candidates next to the border are compared one by one
             const double z = q.m < 1.0f ? -log(static_cast<double>(q.m)) : 0.0;
-            const auto bin = [](double depth) { return static_cast<int>(fminf(place_of(static_cast<float>(depth * 128.0)), kBins)); };
+            const auto bin = [](double depth) { return static_cast<int>(fminf(static_cast<float>(depth * 128.0), kBins)); };
             l[2] = bin(fmax(z - 1e-4, 0.0)), h[2] = min(bin(z + 1e-4), kBins - 1);
             if (l[2] < kBins) {
                 m_bin = l[2];
