@@ -12,13 +12,14 @@
 // leaves the next one open to as much mass, so mostly to a bin as well). The workgroup that is done last
 // with a row plans that, or sorts the candidates and finds the exact places. A small top_k needs no counts: the largest
 // logits of 64 parts of the row, which the first launch leaves, bound its candidates, and the second launch gathers
-// them and draws. Rows of one slice take one launch. Where the open bins hold more than kList candidates (thousands of
-// equal logits, or whole rows within one or two temperatures), the places are found by radix descent over the row.
+// them and draws. Rows of one slice take one launch. Where the open bins hold more than kList candidates (that many equal
+// logits, or a whole row within less than a temperature), the places are found by radix descent over the row.
 //
-// One row of 151936 with a top_k of 20 takes 15.5 us (by counts 22.5), 48 with settings of all kinds 43 us. The logits
+// One row of 151936 with a top_k of 20 takes 15.5 us (by counts 22.5), 48 with settings of all kinds 46 us. The logits
 // are read two or three times, 29 MB of 48 rows in about 5 us each; the rest is one workgroup's chain of steps at the end
 // of each launch (settling 64 candidates takes 3.5 us, 2048 5) and, of many rows, the weights: 12 instructions in
-// 64 bits each and an addition of 64 bits in LDS (together 6 us), and the listing of those in open bins (3 us).
+// 64 bits each and an addition of 64 bits in LDS (together 6 us), and the listing of those in open bins (3 us). Flat
+// rows have longer lists (one of 151936 at a temperature of 5, top_p 0.95: 41 us; 2000 equal logits on top 47, 8000 105).
 #include "dev_q4.hpp"
 #include "launch_q4.hpp"
 
@@ -113,133 +114,13 @@ __device__ __forceinline__ uint64_t drawn_place(float u, uint64_t total) {
     return min(static_cast<uint64_t>(floor(static_cast<double>(u > 0.0f ? fminf(u, 1.0f) : 0.0f) * static_cast<double>(total))), total - 1);
 }
 
-// A place in the ranking: the candidates with larger keys, and `nth` with the same key, are before it.
-struct Place {
-    uint32_t key;
-    uint32_t nth;
-    uint64_t count, mass;  // of the larger keys
-};
-
-struct Shared {
-    uint32_t count[256];
-    uint64_t mass[256];
-    uint64_t red[kThreads / 64];
-    Place place;
-    uint64_t left;
-    uint32_t prefix;
-};
-
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, Shared& sh) {
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x / 64] = v;
-    __syncthreads();
-    uint64_t t = 0;
-    for (int i = 0; i < kThreads / 64; ++i) t += sh.red[i];
-    return t;
-}
-
-// The place that holds unit `at` of the mass (BY_MASS) or has `at` candidates before it. There is one.
-template <bool BY_MASS>
-__device__ __forceinline__ Place find(const float* x, int V, const Weigher& w, uint64_t at, Shared& sh) {
-    uint32_t prefix = 0;
-    Place p{0, 0, 0, 0};
-    uint64_t left = at;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (threadIdx.x < 256) sh.count[threadIdx.x] = 0, sh.mass[threadIdx.x] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < V; i += kThreads) {
-            const uint32_t k = key_of(x[i]);
-            if (shift < 24 && (k >> (shift + 8)) != prefix) continue;
-            atomicAdd(&sh.count[k >> shift & 255], 1u);
-            const uint64_t m = w(k);
-            if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[k >> shift & 255]), static_cast<unsigned long long>(m));
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int d = 255;
-            for (; d > 0; --d) {
-                const uint64_t n = BY_MASS ? sh.mass[d] : sh.count[d];
-                if (left < n) break;
-                left -= n;
-                p.count += sh.count[d];
-                p.mass += sh.mass[d];
-            }
-            sh.place = p;
-            sh.left = left;
-            sh.prefix = prefix << 8 | static_cast<uint32_t>(d);
-        }
-        __syncthreads();
-        p = sh.place;
-        left = sh.left;
-        prefix = sh.prefix;
-    }
-    p.key = prefix;
-    const uint64_t each = BY_MASS ? w(prefix) : 1;
-    p.nth = static_cast<uint32_t>(each ? left / each : 0);
-    return p;
-}
-
-// The places by descent over the whole row: for rows whose open bins hold too many candidates.
-__device__ __forceinline__ void sample_by_descent(const SampleArgs& a, int b, uint32_t top, const Weigher& w, Shared& sh) {
-    const float* x = a.logits + b * a.ld;
-    uint64_t total;
-    const int k = a.top_k ? a.top_k[b] : 0;
-    const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f;
-    uint32_t last = kKeyNone;  // the last key that is kept
-    if (k > 0 && k < a.V) {
-        const Place p = find<false>(x, a.V, w, k - 1, sh);
-        last = p.key;
-        total = p.mass + (p.nth + 1ull) * w(p.key);
-    } else {
-        uint64_t s = 0;
-        for (int i = threadIdx.x; i < a.V; i += kThreads) s += w(key_of(x[i]));
-        total = block_sum_u64(s, sh);
-    }
-    if (tp < 1.0f) {
-        const Place p = find<true>(x, a.V, w, top_p_place(tp, total), sh);
-        last = p.key;
-        total = p.mass + (p.nth + 1ull) * w(p.key);
-    }
-    if (mp > 0.0f && !(w.share(last) >= mp)) {
-        uint64_t s = 0;
-        for (int i = threadIdx.x; i < a.V; i += kThreads) {
-            const uint32_t key = key_of(x[i]);
-            if (w.share(key) >= mp) s += w(key);
-        }
-        total = max(block_sum_u64(s, sh), w(top));  // the first place stays
-    }
-    const Place at = find<true>(x, a.V, w, drawn_place(a.u[b], total), sh);
-    // the nth candidate with that key
-    uint32_t seen = 0;
-    for (int i0 = 0; i0 < a.V; i0 += kThreads) {
-        const int i = i0 + threadIdx.x;
-        const bool same = i < a.V && key_of(x[i]) == at.key;
-        const uint64_t vote = __ballot(same);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x / 64] = __popcll(vote);
-        __syncthreads();
-        uint32_t before = seen, all = 0;
-        for (int j = 0; j < kThreads / 64; ++j) {
-            if (j < static_cast<int>(threadIdx.x / 64)) before += static_cast<uint32_t>(sh.red[j]);
-            all += static_cast<uint32_t>(sh.red[j]);
-        }
-        before += __popcll(vote & ((1ull << (threadIdx.x & 63)) - 1));
-        if (same && before == at.nth) {
-            put_token(a, b, i);
-            if (a.prob) a.prob[b] = static_cast<float>(static_cast<double>(w(at.key)) / static_cast<double>(total));
-        }
-        seen += all;
-        if (seen > at.nth) return;  // the same for every thread
-    }
-}
-
 // ---- by bins
 constexpr int kParts = 64;              // of a row, every slice having some of each
-constexpr int kList = 2048;             // candidates that can be listed
+constexpr int kFew = 2048;              // most lists are shorter
+constexpr int kList = 8192;             // candidates that can be listed: some bins of a flat row (by descent it takes ten times as long)
 constexpr int kMostK = 1024;            // top_k up to this: every candidate that it may leave is listed
 constexpr int kBuckets = kThreads;
+constexpr uint32_t kCrowd = 64;         // candidates of one bucket up to which counting sorts it
 constexpr int kPer = (kBins + kThreads) / kThreads;
 
 // a candidate in the ranking's order: larger ones first
@@ -286,7 +167,6 @@ struct Work {
             uint32_t at[kBuckets];
         } pick;
         uint32_t part[kThreads / 64][kParts];
-        Shared descent;
     };
     Plan plan;
     ExpTable exp;
@@ -535,11 +415,30 @@ __device__ __forceinline__ void gather(const float* x, int i, int e, const Weigh
     });
 }
 
-// The exact places, from the n candidates of the open bins in sh.pick.list.
+// sh.pick.list's first n entries in their order, by a bitonic network.
+__device__ __forceinline__ void sort_list(int n, Work& sh) {
+    int N = 64;
+    while (N < n) N *= 2;
+    for (int i = n + threadIdx.x; i < N; i += kThreads) sh.pick.list[i] = 0;
+    for (int run = 2; run <= N; run *= 2)
+        for (int d = run / 2; d > 0; d /= 2) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < N / 2; i += kThreads) {
+                const int at = 2 * i - (i & (d - 1));
+                const uint64_t x = sh.pick.list[at], y = sh.pick.list[at + d];
+                if ((x < y) == ((at & run) == 0)) sh.pick.list[at] = y, sh.pick.list[at + d] = x;
+            }
+        }
+    __syncthreads();
+}
+
+// The exact places, from the n <= kEach kThreads candidates of the open bins in sh.pick.list.
+template <int kEach>
 __device__ __forceinline__ void settle(const SampleArgs& a, int b, const Question& q, int n, const Weigher& w, Work& sh) {
     const Plan& p = sh.plan;
     const int t = threadIdx.x, lane = t & 63, wave = t / 64;
-    // Sorted by buckets of equal width in depth, a few candidates each, and within one by counting.
+    // Sorted by buckets of equal width in depth, a few candidates each, and within one by counting; where one holds many, by
+    // comparing all (2000 equal ones: 47 us in all, by counting 219).
     sh.pick.at[t] = 0;
     if (t < 4) sh.in_range[t] = 0;
     __syncthreads();
@@ -550,10 +449,10 @@ __device__ __forceinline__ void settle(const SampleArgs& a, int b, const Questio
         wide += p.hi[r] + 1 - p.lo[r];
     }
     const float scale = static_cast<float>(kBuckets) / wide;
-    constexpr int kEach = kList / kThreads;
     uint64_t mine[kEach];
     int of[kEach];
     uint32_t place[kEach];
+    bool crowded = false;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const bool there = t + i * kThreads < n;
@@ -569,26 +468,30 @@ __device__ __forceinline__ void settle(const SampleArgs& a, int b, const Questio
         }
         of[i] = min(static_cast<int>(before * scale), kBuckets - 1);
         place[i] = there ? atomicAdd(&sh.pick.at[of[i]], 1u) : 0;
+        crowded |= place[i] >= kCrowd;
     }
-    __syncthreads();
-    sh.pick.at[t] = block_scan(sh.pick.at[t], sh.wave_count);
-    __syncthreads();
+    if (__syncthreads_or(crowded)) {
+        sort_list(n, sh);
+    } else {
+        sh.pick.at[t] = block_scan(sh.pick.at[t], sh.wave_count);
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        if (t + i * kThreads < n) sh.pick.list[sh.pick.at[of[i]] + place[i]] = mine[i];
-    __syncthreads();
+        for (int i = 0; i < kEach; ++i)
+            if (t + i * kThreads < n) sh.pick.list[sh.pick.at[of[i]] + place[i]] = mine[i];
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        if (t + i * kThreads >= n) continue;
-        const uint32_t first = sh.pick.at[of[i]], end = of[i] + 1 < kBuckets ? sh.pick.at[of[i] + 1] : n;
-        place[i] = first;
-        for (uint32_t j = first; j < end; ++j) place[i] += sh.pick.list[j] > mine[i];
+        for (int i = 0; i < kEach; ++i) {
+            if (t + i * kThreads >= n) continue;
+            const uint32_t first = sh.pick.at[of[i]], end = of[i] + 1 < kBuckets ? sh.pick.at[of[i] + 1] : n;
+            place[i] = first;
+            for (uint32_t j = first; j < end; ++j) place[i] += sh.pick.list[j] > mine[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (t + i * kThreads < n) sh.pick.list[place[i]] = mine[i];
+        __syncthreads();
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        if (t + i * kThreads < n) sh.pick.list[place[i]] = mine[i];
-    __syncthreads();
     // running masses
     uint64_t m[kEach], in = 0;
 #pragma unroll
@@ -699,6 +602,134 @@ __device__ __forceinline__ void settle_wave(const SampleArgs& a, int b, const Qu
     }
 }
 
+// ---- by descent
+// f(logit) for the whole row, with few copies of f: the next four are on their way while f has these.
+template <typename F>
+__device__ __forceinline__ void each_of_row(const float* x, int V, const F& f) {
+    constexpr int kBatch = 4;
+    float l[2][kBatch];
+    const auto load = [&](float (&to)[kBatch], int j) {
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) to[n] = x[min(j + n * kThreads, V - 1)];
+    };
+    load(l[0], threadIdx.x);
+#pragma unroll 1
+    for (int j = threadIdx.x; j < V; j += kBatch * kThreads) {
+        load(l[1], j + kBatch * kThreads);
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n)
+            if (j + n * kThreads < V) f(l[0][n]);
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) l[0][n] = l[1][n];
+    }
+}
+
+// A place in the ranking: the candidates with larger keys, and `nth` with the same key, are before it.
+struct Place {
+    uint32_t key, nth;
+    uint64_t mass;                      // of the larger keys
+};
+// The place that holds unit `left` of the mass (by_mass) or has `left` candidates before it. There is one. The key's first
+// twelve bits, the next, and the last eight, each by counts and masses of what agrees so far; a thread adds
+// those of equal bits in a row at once, as a row of equal logits would wait for one place.
+__device__ __forceinline__ Place find(const float* x, int V, const Weigher& w, uint64_t left, bool by_mass, Work& sh) {
+    static_assert(kBins >= 4096);
+    Place p{0, 0, 0};
+#pragma unroll 1
+    for (int shift = 20; shift >= 0; shift = shift == 20 ? 8 : shift - 8) {
+        const int bits = shift ? 12 : 8;
+        const uint32_t last = (1u << bits) - 1, all = shift == 20 ? 0 : ~0u;
+        __syncthreads();
+        clear_bins(sh);
+        __syncthreads();
+        uint32_t place = 0, n = 0;      // of the candidates not yet added
+        uint64_t m = 0;
+        const auto add = [&] {
+            if (n) atomicAdd(&sh.bins.count[place], n);
+            if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[place]), static_cast<unsigned long long>(m));
+        };
+        each_of_row(x, V, [&](float l) {
+            const uint32_t k = key_of(l);
+            if ((k >> shift >> bits & all) != p.key) return;
+            const uint32_t to = last - (k >> shift & last);  // larger keys first
+            if (to != place) {
+                add();
+                place = to, n = 0, m = 0;
+            }
+            ++n, m += w(k);
+        });
+        add();
+        __syncthreads();
+        add_up(sh);
+        const int bin = by_mass ? bin_of<true>(left, sh) : bin_of<false>(left, sh);
+        left -= by_mass ? sh.bins.mass[bin] : sh.bins.count[bin];
+        p.mass += sh.bins.mass[bin];
+        p.key = p.key << bits | (last - bin);
+    }
+    const uint64_t each = by_mass ? w(p.key) : 1;
+    p.nth = static_cast<uint32_t>(each ? left / each : 0);
+    return p;
+}
+
+// The places by descent, for rows whose open bins hold too many candidates, or next to temperature 0. One workgroup reads the
+// row three times a place (one of 151936, top_p 0.95: at a temperature of 100 410 us, all equal 510).
+__device__ __forceinline__ void sample_by_descent(const SampleArgs& a, int b, const Question& q, const Weigher& w, Work& sh) {
+    const float* x = a.logits + b * a.ld;
+    // the mass of those that have at least `least` of the largest weight
+    const auto mass_of = [&](float least) {
+        uint64_t s = 0;
+        each_of_row(x, a.V, [&](float l) {
+            const uint32_t key = key_of(l);
+            if (w.share(key) >= least) s += w(key);
+        });
+        s = wave_scan(s);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) sh.wave_mass[threadIdx.x / 64] = s;
+        __syncthreads();
+        return lane_of(wave_scan(sh.wave_mass[threadIdx.x & (kThreads / 64 - 1)]), kThreads / 64 - 1);
+    };
+    const bool by_k = q.k > 0 && q.k < a.V;
+    uint64_t total = by_k ? 0 : mass_of(0.0f);
+    Place at{};
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {  // the last of top_k, of top_p, the drawn one
+        if (step == 0 ? !by_k : step == 1 && !(q.p < 1.0f)) continue;
+        if (step == 2 && q.m > 0.0f) total = min(total, max(mass_of(q.m), static_cast<uint64_t>(w.unit)));  // the first place stays
+        at = find(x, a.V, w, step == 0 ? q.k - 1 : step == 1 ? top_p_place(q.p, total) : drawn_place(q.u, total), step > 0, sh);
+        if (step < 2) total = at.mass + (at.nth + 1ull) * w(at.key);
+    }
+    // the nth candidate with that key: every wave counts those of a stretch, and the one that has it looks again
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    constexpr int kBatch = 8, kWaves = kThreads / 64;
+    const int stretch = ((a.V + kWaves - 1) / kWaves + 63) & ~63, begin = wave * stretch, end = min(begin + stretch, a.V);
+    const auto each_vote = [&](const auto& f) {
+        for (int i = begin; i < end; i += 64 * kBatch) {
+            float l[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) l[j] = x[min(i + 64 * j + lane, end - 1)];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (f(i + 64 * j, __ballot(i + 64 * j + lane < end && key_of(l[j]) == at.key))) return;
+        }
+    };
+    uint32_t n = 0;
+    each_vote([&](int, uint64_t vote) { return n += __popcll(vote), false; });
+    if (lane == 0) sh.wave_count[wave] = n;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int i = 0; i < wave; ++i) before += sh.wave_count[i];
+    if (at.nth < before || at.nth >= before + n) return;
+    each_vote([&](int i, uint64_t vote) {
+        const uint32_t c = __popcll(vote);
+        if (at.nth >= before + c) return before += c, false;
+        if ((vote >> lane & 1) && before + __popcll(vote & ((1ull << lane) - 1)) == at.nth) {
+            put_token(a, b, i + lane);
+            if (a.prob) a.prob[b] = static_cast<float>(static_cast<double>(w(at.key)) / static_cast<double>(total));
+        }
+        return true;
+    });
+}
+
 __device__ __forceinline__ int slice_begin(int V, int slices, int i) {
     return i == slices ? V : static_cast<int>(static_cast<int64_t>(V) * i / slices) & ~3;
 }
@@ -746,7 +777,7 @@ __device__ __forceinline__ bool gather_and_settle(const SampleArgs& a, int b, in
         return false;
     }
     for (uint32_t j = threadIdx.x; j < n; j += kThreads) sh.pick.list[j] = shared_load(&r.list[j]);
-    settle(a, b, q, n, w, sh);
+    n <= kFew ? settle<kFew / kThreads>(a, b, q, n, w, sh) : settle<kList / kThreads>(a, b, q, n, w, sh);
     return false;
 }
 
@@ -780,7 +811,8 @@ __device__ __forceinline__ bool plan_by_parts(const Question& q, uint32_t key, c
 
 __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, double unit, int slices, const uint64_t* tops, const uint32_t* parts,
                                                                 Row* rows) {
-    __shared__ Work sh;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    Work& sh = *reinterpret_cast<Work*>(lds);
     const int b = blockIdx.y, s = blockIdx.x;
     // all that is read is asked for before the first of it is used (an empty row's may be anything)
     const float T = a.temperature[b];
@@ -829,7 +861,8 @@ __global__ __launch_bounds__(kThreads) void sample_count_kernel(SampleArgs a, do
 }
 
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, double unit, int slices, const uint64_t* tops, Row* rows) {
-    __shared__ Work sh;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    Work& sh = *reinterpret_cast<Work*>(lds);
     const int b = blockIdx.y, s = blockIdx.x;
     Row& r = rows[b];
     const uint32_t done = r.done;
@@ -850,12 +883,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, dou
     // by descent where the open bins hold too many (done is 2 where that is known), and next to temperature 0
     bool descend = (T < kLeastT || done) && s == 0;
     if (T >= kLeastT && !done) descend = gather_and_settle(a, b, slice_begin(a.V, slices, s), slice_begin(a.V, slices, s + 1), slices, q, w, r, sh);
-    if (descend) sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
+    if (descend) sample_by_descent(a, b, q, w, sh);
 }
 
 // a row of one slice
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, double unit) {
-    __shared__ Work sh;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    Work& sh = *reinterpret_cast<Work*>(lds);
     const int b = blockIdx.x;
     const float T = a.temperature[b];
     if (!(T >= 0.0f)) return;
@@ -883,12 +917,12 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
             return;
         }
         if (n <= kList) {
-            settle(a, b, q, n, w, sh);
+            n <= kFew ? settle<kFew / kThreads>(a, b, q, n, w, sh) : settle<kList / kThreads>(a, b, q, n, w, sh);
             return;
         }
         __syncthreads();
     }
-    sample_by_descent(a, b, static_cast<uint32_t>(top >> 32), w, sh.descent);
+    sample_by_descent(a, b, q, w, sh);
 }
 
 int sample_slices(int B, int V) { return std::max(1, std::min((V + 4095) / 4096, 256 / std::min(B, 256))); }
@@ -905,22 +939,28 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t s) {
     while ((1ll << bits) < a.V) ++bits;
     const double unit = ldexp(1.0, std::min(62 - bits, 50));
     const int slices = sample_slices(a.B, a.V);
+    static AllowedLds allowed_row, allowed_count, allowed_draw;
     if (slices == 1) {
-        klaunch(sample_row_kernel, dim3(a.B), dim3(kThreads), 0, s, a, unit);
+        const hipError_t e = allowed_row(reinterpret_cast<const void*>(sample_row_kernel), sizeof(Work));
+        if (e != hipSuccess) return e;
+        klaunch(sample_row_kernel, dim3(a.B), dim3(kThreads), sizeof(Work), s, a, unit);
         return hipGetLastError();
     }
+    hipError_t e = allowed_count(reinterpret_cast<const void*>(sample_count_kernel), sizeof(Work));
+    if (e == hipSuccess) e = allowed_draw(reinterpret_cast<const void*>(sample_draw_kernel), sizeof(Work));
+    if (e != hipSuccess) return e;
     Row* rows = static_cast<Row*>(a.ws);
     uint64_t* tops = reinterpret_cast<uint64_t*>(rows + a.B);
     uint32_t* parts = reinterpret_cast<uint32_t*>(tops + static_cast<int64_t>(a.B) * slices);
     const dim3 grid(slices, a.B);
     klaunch(sample_top_kernel, grid, dim3(kThreads), 0, s, a, slices, tops, parts, rows);
-    hipError_t e = hipGetLastError();
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
-    klaunch(sample_count_kernel, grid, dim3(kThreads), 0, s, a, unit, slices, static_cast<const uint64_t*>(tops),
+    klaunch(sample_count_kernel, grid, dim3(kThreads), sizeof(Work), s, a, unit, slices, static_cast<const uint64_t*>(tops),
             static_cast<const uint32_t*>(parts), rows);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    klaunch(sample_draw_kernel, grid, dim3(kThreads), 0, s, a, unit, slices, static_cast<const uint64_t*>(tops), rows);
+    klaunch(sample_draw_kernel, grid, dim3(kThreads), sizeof(Work), s, a, unit, slices, static_cast<const uint64_t*>(tops), rows);
     return hipGetLastError();
 }
 

@@ -1,5 +1,5 @@
 """q35_sample on rows whose borders lie among thousands of candidates of nearly one weight: a token far above a bulk that still
-holds much of the mass, flat rows at high temperatures, bulks deep below the largest; large batches of a full vocabulary."""
+holds much of the mass, flat rows at high temperatures, bulks deep below the largest, equal logits by the thousand; large batches of a full vocabulary."""
 import time
 
 import numpy as np
@@ -48,6 +48,20 @@ def test_many_rows_of_a_full_vocabulary(hip):
     check(hip, x, most_open=0.1)
 
 
+@pytest.mark.parametrize("n", [64, 65, 66, 300, 1025, 2047, 2049, 3000, 8000, 8191, 8192, 8193, 9000])
+@pytest.mark.parametrize("B,V", [(4, 151936), (130, 9100)])
+def test_equal_ones_on_top(hip, B, V, n):
+    """n equal logits far above the others, next to what a bucket, a wave and a list hold, with some of their own above them."""
+    rng = np.random.default_rng(n)
+    x = dict(logits=(rng.standard_normal((B, V)) - 50).astype(np.float32), **settings(B, rng, t=1.0, k=[0, 0, 40, 2000], p=[1.0, 0.9, 0.3], m=0.0))
+    for b in range(B):
+        at = rng.permutation(V)
+        x["logits"][b, at[:n]] = 1.0
+        x["logits"][b, at[n - 3:n]] = np.float32(1.0) + np.arange(3, dtype=np.float32) * np.float32(2.0 ** -20)
+    # top_p of equal candidates: the border may fall within 2^-24 of a whole one
+    check(hip, x, most_open=0.5)
+
+
 def call_time(hip, x):
     """Seconds a call, the least of some runs of 20."""
     B, V = x["logits"].shape
@@ -74,3 +88,13 @@ def test_a_confident_row_is_no_slower(hip, spread, t, above):
     row = np.float32(spread) * row
     row[0, 77] += np.float32(above)
     assert call_time(hip, dict(off, logits=row)) < 5 * ordinary
+
+
+@pytest.mark.parametrize("t,equal", [(3.0, 0), (5.0, 0), (1.0, 2000), (1.0, 5000)])
+def test_a_flat_row_is_little_slower(hip, t, equal):
+    """Some thousand candidates beside the borders are listed and sorted, not counted one against the other or by descent."""
+    rng = np.random.default_rng(7)
+    row = rng.standard_normal((1, 151936)).astype(np.float32)
+    ordinary = call_time(hip, dict(settings(1, rng, t=1.0, k=0, p=0.95, m=0.0, u=0.999), logits=2 * row))
+    row[0, rng.permutation(151936)[:equal]] = 20.0
+    assert call_time(hip, dict(settings(1, rng, t=t, k=0, p=0.95, m=0.0, u=0.7), logits=row)) < 6 * ordinary
