@@ -611,7 +611,8 @@ q35_status q35_q4_pack(const uint8_t *codes, const uint16_t *scales, const uint8
  * were packed. R may be Y itself. An entry of X counts as two fp16 values, to 2^-22 of itself or to 2^-39 of the
  * largest of its group of k (below 2^-100 it may count as 0), whatever the number of rows; its products with codes
  * less zeros are exact, sums are in fp32. Infinities and NaN of X, of scales and of R go into the outputs as products and
- * sums take them. workspace (16-byte aligned): q35_matmul_q4_workspace_bytes() bytes.
+ * sums take them. Y, from its first entry to its last, overlaps no input but an R that is Y itself. workspace (16-byte
+ * aligned): q35_matmul_q4_workspace_bytes() bytes; the kernels of today leave it alone, so calls may share it.
  * Meant for the rows of a decode step (one to some dozens); M is at most Q35_MATMUL_Q4_MOST_ROWS. */
 #define Q35_MATMUL_Q4_MOST_ROWS 4096
 uint64_t q35_matmul_q4_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t group);

@@ -731,7 +731,7 @@ __global__ __launch_bounds__(256) void kv_q4_load_kernel(KvQ4Args a) {
         const int b = static_cast<int>(id / 2 / a.NKV), h = static_cast<int>(id / 2 % a.NKV), v = static_cast<int>(id & 1);
         int i, e;
         if (!range_of(a, b, i, e)) continue;
-        const int64_t to = (static_cast<int64_t>(a.shared ? 0 : b) * a.NKV + h) * a.rows_cap, from = (id / 2) * a.cap;
+        const int64_t to = (static_cast<int64_t>(b) * a.NKV + h) * a.rows_cap, from = (id / 2) * a.cap;
         for (int64_t t = i + (blockIdx.x * 4 + threadIdx.x / 64) * kTake; t < e; t += gridDim.x * 4 * kTake) {
             uint32_t code[kKvRows], sc[kKvRows];
 #pragma unroll

@@ -661,9 +661,6 @@ hipError_t launch_q4_plan(const Q4MulArgs& a, const Q4Plan& p, hipStream_t s) {
 
 }  // namespace
 
-// No form needs more than a place: X's images lie in LDS and waves that share a tile add up there.
-uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G) { return 16; }
-
 hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s) {
     const auto go = [&](auto g, auto z) {
         constexpr int G = decltype(g)::value;

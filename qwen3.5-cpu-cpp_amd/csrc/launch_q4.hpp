@@ -27,12 +27,10 @@ struct Q4MulArgs {
     const uint8_t* W;                   // packed
     const float* R;                     // may be null, may be Y
     float* Y;
-    void* ws;
     int64_t ldx, ldr, ldy;
     int M, N, K, G;
     bool zeros;
 };
-uint64_t q4_mul_workspace_bytes(int M, int N, int K, int G);
 hipError_t launch_q4_mul(const Q4MulArgs& a, hipStream_t s);
 // bf16 or fp32 W [N][K] -> codes [N][(K + 1) / 2], scales and (zeros not null) zeros [N][groups]
 hipError_t launch_q4_quantize(const void* W, bool bf16, int N, int K, int G, uint8_t* codes, uint16_t* scales, uint8_t* zeros,
