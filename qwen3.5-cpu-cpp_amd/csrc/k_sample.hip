@@ -144,7 +144,7 @@ struct Plan {
     uint64_t all;                       // mass of the row
     int k_range, m_range;               // where the last candidate of top_k and the first that min_p may leave out
                                         // are; -1: they leave out nothing that has weight
-    uint32_t k_at, reserved;            // the place of the former in its range
+    uint32_t k_at;                      // the place of the former in its range
 };
 
 // What a row's workgroups share, in the workspace. Cleared by the first launch.
@@ -748,8 +748,11 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, int 
     if (threadIdx.x == 0) tops[b * slices + s] = top;
 }
 
-// Whether this workgroup is the last of the row's to come here. The others' additions and stores are all done:
-// each wave waits for its own before the barrier, behind which the ticket is drawn.
+// Whether this workgroup is the last of the row's to come here. What the workgroups leave each other are atomic additions
+// and shared_store's alone, which are done, where all look, once their wave has waited for them; every wave does before
+// the barrier, behind which the ticket is drawn. So a workgroup that draws the last ticket finds, by atomic reads
+// (shared_load), all of the others', and the ticket needs no release or acquire, which would write back and drop the
+// whole second cache. Plain stores and loads would need them: those of a row's plan go to the next launch.
 __device__ __forceinline__ bool last_of(uint32_t* ticket, int slices, Work& sh) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vector memory, nothing outstanding
     __syncthreads();
