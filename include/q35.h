@@ -638,6 +638,9 @@ q35_status q35_matmul_q4(const float *X, int64_t ldx, const void *packed, int32_
  *   out [batch][NQ][HD]
  * workspace (16-byte aligned): q35_attn_q4_workspace_bytes() bytes; that depends on the sizes, never on the
  * lengths. Results do not depend on the order in which workgroups run.
+ * A normed, rotated query row's entries are held to 2^-23 of its largest, a softmax weight times its value row's step to
+ * 2^-23 of the largest such product of 64 rows and 64 dims; the rest is fp32. Where batch * NKV comes near 512 or
+ * above, a sequence far longer than the others is better in a call of its own: each head has a workgroup or two.
  * What is written may overlap no other array. Requires HD == 256, NQ / NKV at most 16, an even rotary_dim, 16-byte
  * aligned arrays. */
 typedef struct q35_attn_q4_args {
