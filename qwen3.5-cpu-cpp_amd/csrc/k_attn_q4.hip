@@ -162,7 +162,8 @@ __device__ __forceinline__ void norm_rotate(double* x, const float4& w, float ep
     wave_sync();
 }
 
-// A normed, rotated query row, times log2(e) / sqrt(HD), as digits: head h of the kv head's.
+// A normed, rotated query row, times log2(e) / sqrt(HD), as digits: head h of the kv head's. One unit serves the row (a unit
+// for each 64 dims took 1.5% more of a batch's time): an entry is off by 2^-23 of the largest of all 256.
 __device__ __forceinline__ void place_query(const double* x, int h, uint8_t* qbuf, float2* fbuf) {
     const int lane = threadIdx.x & 63;
     constexpr double kScale = 0.0625 * 1.4426950408889634;
@@ -225,7 +226,7 @@ constexpr int kMostShared = 512;        // sequences and workgroups up to which 
 // one, so that long sequences get many and none waits for another's. Every wave finds the same.
 __device__ __forceinline__ Share share_out(const AttnQ4Args& a, int groups, int w, int waves) {
     constexpr int kEach = kMostShared / 64;
-    if (a.B == 1) {                     // the same without the sums (1 x 131072 30.7 us by workgroups of four waves, with them 32.1)
+    if (a.B == 1) {                     // the same without the sums (1 x 700 14.3 us, with them 15.3; 1 x 131072 30.3 and 32.0)
         const int len = a.len[0], all = len < 0 ? 0 : len < a.cap ? len / (waves * kTile) + 1 : 1, per = static_cast<uint32_t>(groups) / a.NKV;
         const int r = max(static_cast<int>((static_cast<uint32_t>(all) + per - 1) / per), 1), np = (static_cast<uint32_t>(all) + r - 1) / r;
         if (w >= np * a.NKV) return {-1, 0, 0, 0, 0, r};
@@ -285,16 +286,17 @@ struct Partials {
 // looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
 //   s = 2^-e sum_g (step_g sum_d i_d code_d + least_g sum_d i_d).
 // Weights: p = 2^(s - tile's largest) <= 1 is multiplied by its value row's step, which differs by group, and becomes
-// multiples of a 4190000th of the tile's largest such product: p step (code - 8) summed over 64 keys is again one
+// multiples of a 4190000th of the tile's largest such product (of one below 1e-30, 0): p step (code - 8) summed over 64 keys is again one
 // integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
 // operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time) in that
 // order. The rest, sum_t p_t (least_t + 8 step_t), is a sum a head and group. (By code - 8 both are means of values of
 // both signs: of 131072 rows the outputs are 6e-7 off, by code and least 3.2e-6.)
 //
 // The matrix cores do the products in passing; what a tile costs is some 1200 instructions around them (5k cycles of
-// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 73 MB, takes 29 us, of
+// a wave), and what a call costs is mostly that workgroups are short: 1 x 131072 (16/2 heads), 73 MB, takes 30 us, of
 // which 24 are this kernel's: 1 to share the rows out, 3 to request what it reads, 4 for its queries, 12 for two tiles
-// a wave, 2 to join the waves. 40 sequences of up to 8192, 94 MB, take 39 us; 1 x 700 (8/2 heads) 14.3.
+// a wave, 2 to join the waves. 40 sequences of up to 8192, 94 MB, take 41 us; 1 x 700 (8/2 heads) 14.3. (Figures here and
+// below: calls replayed from a graph, over three sets of inputs, all of one run.)
 template <int HQ, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, HQ > 2 || kWaves > 4 ? 1 : 2) void attn_q4_kernel(AttnQ4Args a, RopeFreq freq, int shared, Partials part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -777,19 +779,21 @@ AttnQ4Plan attn_q4_plan(const AttnQ4Args& a) {
     p.waves = 4;
     const int64_t heads = static_cast<int64_t>(a.B) * a.NKV;
     p.groups = static_cast<int>(heads);
-    if (heads >= kMostShared || a.cap <= 4 * kTile) return p;  // a workgroup a head
+    // A workgroup a head. (Of 512 heads and more, and by the few pieces left of nearly as many, a sequence that is far longer than
+    // the others takes its own time: 255 x 16/2 of up to 2000 rows, one of 131072, 981 us, 256 1880, where one alone takes 30.)
+    if (heads >= kMostShared || a.cap <= 4 * kTile) return p;
     const bool eight = p.quads <= 2;    // their registers allow it
-    // A workgroup a head of eight waves where that is one tile a wave (1 x 300, 8/2 heads 11.3 us, rows shared out 14.5;
-    // 40 x 512, 16/2 17.2 and 20.3; 1 x 1024, 8/2 18.6 and 15.9), or two and heads are many (90 x 1024, 16/2 25.5 and
-    // 34.3; 40 x up to 1024 23.4 and 19.8).
+    // A workgroup a head of eight waves where that is one tile a wave (1 x 300, 8/2 heads 11.4 us, rows shared out 13.4;
+    // 40 x 512, 16/2 17.7 and 21.3; 1 x 1024, 8/2 18.8 and 14.7), or two and heads are many (90 x 1024, 16/2 25.7 and
+    // 34.6; 40 x up to 1024 24.4 and 21.5).
     if (eight && (a.cap <= 8 * kTile || (a.cap <= 16 * kTile && heads >= 128))) {
         p.waves = 8;
         return p;
     }
     // Else rows are shared out: eight waves a compute unit, or as many workgroups as there can be rounds. Two
     // workgroups of four waves, or one of eight, half as many to be merged, where sequences are few and one round of
-    // all of them may not do (1 x 131072, 16/2 30.1 us, by fours 32.3; 20 x up to 8192 29.1 and 30.3; 1 x 16384 20.5 and
-    // 18.4; 40 x up to 8192 45.7 and 40.4).
+    // all of them may not do (1 x 131072, 16/2 30.9 us, by fours 31.5; 20 x up to 8192 29.8 and 31.2; 1 x 16384 19.7 and
+    // 18.2; 40 x up to 8192 44.1 and 41.0).
     if (eight && heads <= 40 && heads * a.cap >= kMostShared * 4 * kTile) p.waves = 8;
     const int64_t each = p.waves * kTile, most = kMostShared * 4 / p.waves;  // most >= heads: every head has a workgroup
     p.groups = p.shared = static_cast<int>(std::min<int64_t>(most / a.NKV, a.B * ((a.cap + each - 1) / each)) * a.NKV);
@@ -805,8 +809,8 @@ hipError_t launch_attend(const AttnQ4Args& a, const RopeFreq& freq, const AttnQ4
     klaunch(attn_q4_kernel<HQ, kWaves>, dim3(p.groups), dim3(kWaves * 64), lds, s, a, freq, p.shared, part);
     e = hipGetLastError();
     if (e != hipSuccess || !p.shared) return e;
-    // Workgroups of 512 threads where there is at most one for a compute unit (256 pieces of 16 heads: 7.0 us, with 256
-    // threads 9.3), else of 256 (40 sequences: 5.8 us, with 512 10.1).
+    // Workgroups of 512 threads where there is at most one for a compute unit (256 pieces of 16 heads 30.9 us in all, with
+    // 256 threads 31.9; three pieces of 8 heads 14.3 and 13.8), else of 256 (40 sequences 42.0, with 512 46.0).
     const dim3 grid(a.NQ * 4, a.B);
     if (static_cast<int64_t>(a.NQ) * 4 * a.B <= 256) klaunch(attn_q4_combine_kernel<32>, grid, dim3(512), 0, s, a, part);
     else klaunch(attn_q4_combine_kernel<16>, grid, dim3(256), 0, s, a, part);
