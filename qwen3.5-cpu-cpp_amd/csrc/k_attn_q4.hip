@@ -286,8 +286,8 @@ struct Partials {
 // looked at) and 16 keys over a group of 64 dims; lane 16 c + n then holds head c's three sums for key n, and
 //   s = 2^-e sum_g (step_g sum_d i_d code_d + least_g sum_d i_d).
 // Weights: p = 2^(s - tile's largest) <= 1 is multiplied by its value row's step, which differs by group, and becomes
-// multiples of a 4190000th of the tile's largest such product (of one below 1e-30, 0): p step (code - 8) summed over 64 keys is again one
-// integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
+// multiples of a 4190000th of the tile's largest such product (of one below 1e-30, 0): p step (code - 8) summed over 64
+// keys is again one integer product, heads and digits by 16 dims. A lane's four weights (of keys n, n + 16, ..) are one word of that
 // operand, so P's order of keys is theirs, and value rows are read transposed (16 x 16 nibbles at a time) in that
 // order. The rest, sum_t p_t (least_t + 8 step_t), is a sum a head and group. (By code - 8 both are means of values of
 // both signs: of 131072 rows the outputs are 6e-7 off, by code and least 3.2e-6.)

@@ -928,6 +928,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a, doub
     sample_by_descent(a, b, q, w, sh);
 }
 
+// Workgroups a row: one for each 4096 logits, up to 256 in all. From 129 rows on each has one, and one launch (in graphs, top_p
+// 0.95 of 151936: 128 rows 79 us, 129 95, 256 109).
 int sample_slices(int B, int V) { return std::max(1, std::min((V + 4095) / 4096, 256 / std::min(B, 256))); }
 
 }  // namespace
