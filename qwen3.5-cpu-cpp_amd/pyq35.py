@@ -359,7 +359,8 @@ class Model:
         return out[:n_new]
 
     def sample(self, u: float, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-        """A token drawn from the last logits by one uniform number, and its share."""
+        """A token drawn from the last logits by one uniform number, and its share. Refused (Q35_ERR_RANGE) where a reset,
+        a position or a written state has taken the place of the state that they belong to."""
         how = Sampling(temperature, top_k, top_p, min_p)
         token, prob = C.c_int32(0), C.c_float(0)
         check(lib.q35_model_sample(self.h, C.byref(how), u, C.addressof(token), C.addressof(prob)))

@@ -17,7 +17,7 @@ def hip():
 
 
 FORMS = [(1, 90, 300, 64, False), (1, 70, 256, 128, True), (5, 60, 515, 32, True), (8, 8300, 130, 64, False), (21, 12600, 128, 128, True),
-         (19, 14000, 100, 32, False)]
+         (19, 14000, 100, 32, False), (12, 22000, 100, 64, False), (7, 8400, 200, 32, True)]
 
 
 @pytest.mark.parametrize("M,N,K,G,zeros", FORMS)

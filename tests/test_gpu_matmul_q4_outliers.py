@@ -54,7 +54,8 @@ def multiply(hip, x):
 @pytest.mark.parametrize("size", [1e2, 1e4, 1e6])
 @pytest.mark.parametrize("M,N,K,G,zeros", [
     (1, 300, 2048, 64, False), (1, 64, 1000, 128, True), (1, 40, 511, 32, False), (3, 100, 2048, 64, True), (4, 33, 640, 32, True),
-    (8, 8300, 256, 64, False), (13, 64, 6144, 32, False), (16, 9000, 513, 128, True), (24, 11000, 512, 64, True), (70, 50, 700, 64, False)])
+    (8, 8300, 256, 64, False), (13, 64, 6144, 32, False), (16, 9000, 513, 128, True), (24, 11000, 512, 64, True), (70, 50, 700, 64, False),
+    (9, 30000, 130, 64, True), (12, 22000, 300, 128, False), (16, 16500, 260, 32, False), (6, 9000, 300, 128, True), (40, 5000, 640, 64, True)])
 def test_beside_an_outlier(hip, M, N, K, G, zeros, size):
     rng = np.random.default_rng(M + K)
     x = outliers(make(M, N, K, G, zeros, M + N + K), size, rng)
