@@ -117,10 +117,12 @@ __device__ __forceinline__ uint64_t drawn_place(float u, uint64_t total) {
 // ---- by bins
 constexpr int kParts = 64;              // of a row, every slice having some of each
 constexpr int kFew = 2048;              // most lists are shorter
-constexpr int kList = 8192;             // candidates that can be listed: some bins of a flat row (by descent it takes ten times as long)
+constexpr int kList = 8192;             // candidates that can be listed: some bins of a flat row
 constexpr int kMostK = 1024;            // top_k up to this: every candidate that it may leave is listed
 constexpr int kBuckets = kThreads;
-constexpr uint32_t kCrowd = 64;         // candidates of one bucket up to which counting sorts it
+// Candidates of one bucket up to which counting sorts it (of one row, 100 equal ones by counting 32.3 us in all, by comparing all
+// 31.6; 500 51.5 and 36).
+constexpr uint32_t kCrowd = 64;
 constexpr int kPer = (kBins + kThreads) / kThreads;
 
 // a candidate in the ranking's order: larger ones first
